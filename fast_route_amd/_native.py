@@ -58,6 +58,15 @@ SIGNATURES = {
                                         c_void_p, c_void_p, c_void_p]),
     "fr_fused_moe_fp8": (c_int, [c_void_p, c_int, c_void_p, c_void_p, c_void_p, c_void_p, c_void_p, c_int, c_int64,
                                  c_int64, c_int64, c_int, c_int, c_int, c_void_p, c_void_p, c_int64, c_void_p]),
+    "fr_quant_mxfp4_rows": (c_int, [c_void_p, c_int, c_int64, c_int64, c_int64, c_void_p, c_void_p, c_void_p]),
+    "fr_dequant_mxfp4_rows": (c_int, [c_void_p, c_void_p, c_int64, c_int64, c_int, c_void_p, c_void_p]),
+    "fr_mxfp4_tiled_bytes": (c_int64, [c_int64, c_int64, c_int64]),
+    "fr_mxfp4_tile_weights": (c_int, [c_void_p, c_void_p, c_int64, c_int64, c_int64, c_int, c_void_p, c_void_p]),
+    "fr_linear_mxfp4_workspace_bytes": (c_int64, [c_int64, c_int64, c_int64]),
+    "fr_linear_mxfp4": (c_int, [c_void_p, c_int, c_int64, c_int64, c_int64, c_void_p, c_int64, c_void_p, c_void_p, c_int64, c_void_p]),
+    "fr_moe_mxfp4_workspace_bytes": (c_int64, [c_int64, c_int64, c_int64, c_int, c_int]),
+    "fr_fused_moe_mxfp4": (c_int, [c_void_p, c_int, c_void_p, c_void_p, c_void_p, c_int, c_int64, c_int64, c_int64, c_int, c_int,
+                                   c_int, c_void_p, c_void_p, c_int64, c_void_p]),
     "fr_fused_moe_noalloc": (c_int, [c_void_p, c_void_p, c_void_p, c_void_p, c_int, c_int64, c_int64, c_int64, c_int, c_int,
                                      c_int, c_int, c_void_p, c_void_p]),
     "fr_probe_mfma_stream": (c_int, [c_int, c_int, c_int, c_void_p, c_void_p, c_void_p, c_void_p]),

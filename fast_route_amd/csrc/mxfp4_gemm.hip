@@ -1,0 +1,408 @@
+// Products of MXFP4 operands on gfx950: a matrix (linear) and the two grouped products of the mixture-of-experts layer.
+//
+//   C[m, f] = sum_k X[m, k] W[f, k],   both operands e2m1 codes with a power-of-two scale per 32 elements of k, fp32 sums.
+//
+// A workgroup of four wavefronts computes a token tile of up to kMxMaxUnits row groups (32 rows each) x 256 weight rows: a
+// wavefront holds two units of weight rows against all token rows.
+#include "mxfp4_core.h"
+
+namespace fr {
+namespace {
+
+constexpr int kMxThreads = 256;
+enum { MX_LINEAR = 0, MX_SILU = 1, MX_DOWN = 2 };
+
+struct MxArgs {
+  const unsigned char* x;  // operand of the token rows
+  const unsigned char* w;  // operand(s) of the weights
+  int64_t w_stride;        // bytes of an expert's weights
+  int k_tiles;
+  int w_groups;            // row groups of an expert's weights
+  int f_tiles;             // tiles of eight weight row groups
+  // grouped: the tile list; else tiles of most_units row groups out of x_groups
+  const int* tile_count;
+  const MxTile* tiles;
+  int x_groups;
+  // MX_SILU: operand of the activated rows, its tiles along K, blocks of 32 activated features
+  unsigned char* act;
+  int act_tiles, act_blocks;
+  // MX_DOWN: rows of the pairs
+  const int32_t* sorted;
+  const float* topk_w;
+  int n_pairs;
+  float* rows;
+  // MX_LINEAR
+  void* out;
+  int64_t ldo;
+  int64_t M;
+  int N;               // columns of rows / out
+};
+
+__device__ __forceinline__ float mx_silu_mul(float g, float u) { return g / (1.f + __expf(-g)) * u; }
+
+template <typename T, int EPI, int U>
+__device__ __forceinline__ void mx_tile(const MxArgs& a, const MxTile& t, int f) {
+  const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const int wg = (f * 4 + wave) * 2;  // first of the wavefront's two weight row groups
+  f32x16 acc[U][2];
+#pragma unroll
+  for (int u = 0; u < U; ++u)
+#pragma unroll
+    for (int j = 0; j < 2; ++j)
+#pragma unroll
+      for (int r = 0; r < 16; ++r) acc[u][j][r] = 0.f;
+  if (wg < a.w_groups) {
+    const int64_t pitch = static_cast<int64_t>(a.k_tiles) * kMxUnit;
+    const unsigned char* w0 = a.w + t.expert * a.w_stride + wg * pitch;
+    const unsigned char* w1 = w0 + (wg + 1 < a.w_groups ? pitch : 0);
+    const unsigned char* x0 = a.x + t.group * pitch;
+    for (int k = 0; k < a.k_tiles; ++k) {
+      mx_frag wf[2][4];
+      int ws[2];
+#pragma unroll
+      for (int s = 0; s < 4; ++s) {
+        wf[0][s] = *reinterpret_cast<const mx_frag*>(w0 + k * kMxUnit + s * 1024 + lane * 16);
+        wf[1][s] = *reinterpret_cast<const mx_frag*>(w1 + k * kMxUnit + s * 1024 + lane * 16);
+      }
+      ws[0] = *reinterpret_cast<const int*>(w0 + k * kMxUnit + kMxScales + lane * 4);
+      ws[1] = *reinterpret_cast<const int*>(w1 + k * kMxUnit + kMxScales + lane * 4);
+#pragma unroll
+      for (int u = 0; u < U; ++u) {
+        const unsigned char* xu = x0 + u * pitch + k * kMxUnit;
+        const int xs = *reinterpret_cast<const int*>(xu + kMxScales + lane * 4);
+        mx_each<0, 4>([&](auto S) {
+          constexpr int s = decltype(S)::value;
+          const mx_frag xf = *reinterpret_cast<const mx_frag*>(xu + s * 1024 + lane * 16);
+          acc[u][0] = mx_mfma<s>(wf[0][s], ws[0], xf, xs, acc[u][0]);
+          acc[u][1] = mx_mfma<s>(wf[1][s], ws[1], xf, xs, acc[u][1]);
+        });
+      }
+    }
+  }
+  // the lane's 16 consecutive features of token row col
+  const int col = lane & 31, half = lane >> 5;
+  if constexpr (EPI == MX_SILU) {
+    const int blk = f * 4 + wave;  // of 32 activated features
+    if (blk >= a.act_tiles * 8) return;
+#pragma unroll
+    for (int u = 0; u < U; ++u) {
+      float v[16];
+      unsigned amax = 0;
+#pragma unroll
+      for (int r = 0; r < 16; ++r) {
+        v[r] = mx_silu_mul(acc[u][0][r], acc[u][1][r]);
+        const unsigned m = magnitude(v[r]);
+        amax = amax > m ? amax : m;
+      }
+      const unsigned byte = mx_scale_byte(mx_pair_max(amax));
+      unsigned char* unit = a.act + (static_cast<int64_t>(t.group + u) * a.act_tiles + (blk >> 3)) * kMxUnit;
+      const uint2 o = {mx_pack8(v, byte), mx_pack8(v + 8, byte)};
+      *reinterpret_cast<uint2*>(unit + mx_code_at(col, blk & 7) + half * 8) = o;
+      if (half == 0) unit[mx_scale_at(col, blk & 7)] = static_cast<unsigned char>(byte);
+    }
+  } else {
+#pragma unroll
+    for (int u = 0; u < U; ++u) {
+      const int64_t slot = static_cast<int64_t>(t.group + u) * kMxRows + col;
+      if constexpr (EPI == MX_DOWN) {
+        const int pair = a.sorted[slot];
+        if (pair < a.n_pairs) {
+          const float s = a.topk_w[pair];
+#pragma unroll
+          for (int j = 0; j < 2; ++j) {
+            const int c = (wg + j) * 32 + half * 16;  // N is a multiple of 32
+            if (c < a.N) {
+              float* row = a.rows + static_cast<int64_t>(pair) * a.N + c;
+#pragma unroll
+              for (int r = 0; r < 16; r += 4)
+                *reinterpret_cast<f32x4*>(row + r) = f32x4{acc[u][j][r] * s, acc[u][j][r + 1] * s, acc[u][j][r + 2] * s, acc[u][j][r + 3] * s};
+            }
+          }
+        }
+      } else if (slot < a.M) {
+#pragma unroll
+        for (int j = 0; j < 2; ++j) {
+          const int c = (wg + j) * 32 + half * 16;
+          T* row = static_cast<T*>(a.out) + slot * a.ldo + c;
+          if (c + 16 <= a.N && (a.ldo & 7) == 0) {
+            typedef T vec8 __attribute__((ext_vector_type(8)));
+#pragma unroll
+            for (int r = 0; r < 16; r += 8) {
+              vec8 o;
+#pragma unroll
+              for (int i = 0; i < 8; ++i) o[i] = static_cast<T>(acc[u][j][r + i]);
+              *reinterpret_cast<vec8*>(row + r) = o;
+            }
+          } else {
+#pragma unroll
+            for (int r = 0; r < 16; ++r)
+              if (c + r < a.N) row[r] = static_cast<T>(acc[u][j][r]);
+          }
+        }
+      }
+    }
+  }
+}
+
+// MOST: row groups of a tile, at most.
+template <typename T, int EPI, int MOST>
+__global__ __launch_bounds__(kMxThreads, 1) void mx_gemm_kernel(MxArgs a) {
+  // workgroups b, b + 8, .. share an XCD and its L2: an XCD takes a consecutive part of the walk
+  const int tiles = EPI == MX_LINEAR ? (a.x_groups + MOST - 1) / MOST : a.tile_count[0];
+  const int total = tiles * a.f_tiles, per = (total + 7) / 8;
+  const int i = blockIdx.x >> 3, lin = (blockIdx.x & 7) * per + i;
+  if (i >= per || lin >= total) return;
+  MxTile t;
+  int n, t0;
+  const int guess = lin / a.f_tiles;  // a tile of the chunk that lin belongs to
+  if constexpr (EPI == MX_LINEAR) {
+    t0 = guess / kMxChunk * kMxChunk;
+    n = min(kMxChunk, tiles - t0);
+  } else {
+    t0 = a.tiles[guess].chunk0;
+    n = a.tiles[guess].chunk_n;
+  }
+  const int q = lin - t0 * a.f_tiles, f = q / n, index = t0 + q - f * n;
+  if constexpr (EPI == MX_LINEAR) t = MxTile{index * MOST, min(MOST, a.x_groups - index * MOST), 0, 0, 0};
+  else t = a.tiles[index];
+  if constexpr (MOST >= 8) {
+    if (t.units == 8) return mx_tile<T, EPI, 8>(a, t, f);
+    if (t.units == 7) return mx_tile<T, EPI, 7>(a, t, f);
+    if (t.units == 6) return mx_tile<T, EPI, 6>(a, t, f);
+    if (t.units == 5) return mx_tile<T, EPI, 5>(a, t, f);
+  }
+  if constexpr (MOST >= 4) {
+    if (t.units == 4) return mx_tile<T, EPI, 4>(a, t, f);
+    if (t.units == 3) return mx_tile<T, EPI, 3>(a, t, f);
+  }
+  if constexpr (MOST >= 2) {
+    if (t.units == 2) return mx_tile<T, EPI, 2>(a, t, f);
+  }
+  mx_tile<T, EPI, 1>(a, t, f);
+}
+
+template <typename T, int EPI>
+int launch_mx_gemm(const MxArgs& a, int most, int64_t tiles, hipStream_t st) {
+  const int64_t wgs = 8 * ceil_div(tiles * a.f_tiles, int64_t(8));
+  FR_REQUIRE(wgs < (int64_t(1) << 31), FR_E_SHAPE, "mxfp4 product: %lld workgroups", (long long)wgs);
+  const dim3 grid(static_cast<unsigned>(wgs)), block(kMxThreads);
+  switch (most) {
+    case 8: hipLaunchKernelGGL((mx_gemm_kernel<T, EPI, 8>), grid, block, 0, st, a); break;
+    case 4: hipLaunchKernelGGL((mx_gemm_kernel<T, EPI, 4>), grid, block, 0, st, a); break;
+    case 2: hipLaunchKernelGGL((mx_gemm_kernel<T, EPI, 2>), grid, block, 0, st, a); break;
+    default: hipLaunchKernelGGL((mx_gemm_kernel<T, EPI, 1>), grid, block, 0, st, a); break;
+  }
+  return check_launch("mx_gemm_kernel");
+}
+
+// Row groups per tile, at most, for `rows` token rows per weight matrix on average.
+int most_units(int64_t rows) { return rows > 128 ? 8 : rows > 64 ? 4 : rows > 32 ? 2 : 1; }
+
+// out[m, :] = sum over the token's pairs, in order, of their weighted rows; a pair without an expert (a token row of NaN
+// logits) has no row.
+template <typename T>
+__global__ __launch_bounds__(kMxThreads) void mx_combine_kernel(const float* __restrict__ rows, const int32_t* __restrict__ ids, int E, int topk,
+                                                                int64_t M, int H, T* __restrict__ out) {
+  typedef T vec8 __attribute__((ext_vector_type(8)));
+  const int per = H / 8;
+  const int64_t i = static_cast<int64_t>(blockIdx.x) * kMxThreads + threadIdx.x;
+  if (i >= M * per) return;
+  const int64_t m = i / per;
+  const int c = static_cast<int>(i - m * per) * 8;
+  float s[8] = {};
+  for (int j = 0; j < topk; ++j) {
+    const int64_t p = m * topk + j;
+    if (static_cast<unsigned>(ids[p]) >= static_cast<unsigned>(E)) continue;
+    const f32x4 lo = *reinterpret_cast<const f32x4*>(rows + p * H + c), hi = *reinterpret_cast<const f32x4*>(rows + p * H + c + 4);
+#pragma unroll
+    for (int r = 0; r < 4; ++r) {
+      s[r] += lo[r];
+      s[4 + r] += hi[r];
+    }
+  }
+  vec8 o;
+#pragma unroll
+  for (int r = 0; r < 8; ++r) o[r] = static_cast<T>(s[r]);
+  *reinterpret_cast<vec8*>(out + m * H + c) = o;
+}
+
+// ---- workspaces ------------------------------------------------------------------------------------------------
+struct Bump {
+  unsigned char* base;
+  int64_t at = 0;
+  template <typename T>
+  T* take(int64_t count) {
+    T* p = reinterpret_cast<T*>(base + at);
+    at = round_up(at + count * static_cast<int64_t>(sizeof(T)), 256);
+    return p;
+  }
+};
+
+struct MxLayer {
+  float* topk_w;
+  int32_t *topk_ids, *sorted, *expert_ids, *npost;
+  void* align_ws;
+  int64_t align_bytes, groups, tile_limit, bytes;
+  int most;
+  int* tile_count;
+  MxTile* tiles;
+  unsigned char *x, *act;
+  float* rows;
+};
+
+MxLayer mx_layer(void* ws, int64_t M, int64_t H, int64_t F, int E, int topk) {
+  MxLayer l;
+  Bump b{static_cast<unsigned char*>(ws)};
+  const int64_t n = M * topk;
+  l.most = most_units(ceil_div(n, static_cast<int64_t>(E)));
+  // groups of 32 slots: each holds a pair, and every expert fills up one at most
+  l.groups = n < (n + int64_t(E) * (kMxRows - 1)) / kMxRows ? n : (n + int64_t(E) * (kMxRows - 1)) / kMxRows;
+  const int64_t experts = n < E ? n : E;
+  l.tile_limit = l.groups / l.most + experts;  // an expert has a lower tile than the limit at most once
+  l.topk_w = b.take<float>(n);
+  l.topk_ids = b.take<int32_t>(n);
+  l.sorted = b.take<int32_t>(n + int64_t(E) * (kMxRows - 1));
+  l.expert_ids = b.take<int32_t>(n + E);
+  l.npost = b.take<int32_t>(1);
+  l.align_bytes = fr_moe_align_workspace_bytes(n, E);
+  l.align_ws = b.take<unsigned char>(l.align_bytes);
+  l.tile_count = b.take<int>(1);
+  l.tiles = b.take<MxTile>(l.tile_limit);
+  l.x = b.take<unsigned char>(l.groups * mx_tiles(H) * kMxUnit);
+  l.act = b.take<unsigned char>(l.groups * mx_tiles(F) * kMxUnit);
+  l.rows = b.take<float>(n * H);
+  l.bytes = b.at;
+  return l;
+}
+
+int check_mx_layer(const char* who, int64_t M, int64_t H, int64_t F, int E, int topk) {
+  FR_REQUIRE(M >= 0 && M <= (int64_t(1) << 24), FR_E_SHAPE, "%s: M=%lld outside [0, 2^24]", who, (long long)M);
+  FR_REQUIRE(H >= 32 && F >= 32 && H % 32 == 0 && F % 32 == 0 && H <= (1 << 20) && F <= (1 << 20), FR_E_SHAPE,
+             "%s: H=%lld and F=%lld must be multiples of 32 up to 2^20", who, (long long)H, (long long)F);
+  FR_REQUIRE(E >= 1 && E <= 256, FR_E_SHAPE, "%s: E=%d outside [1, 256]", who, E);
+  FR_REQUIRE(topk >= 1 && topk <= E, FR_E_SHAPE, "%s: topk=%d outside [1, E=%d]", who, topk, E);
+  FR_REQUIRE(M * topk <= (int64_t(1) << 24), FR_E_SHAPE, "%s: M*topk=%lld above 2^24", who, (long long)(M * topk));
+  return FR_OK;
+}
+
+}  // namespace
+}  // namespace fr
+
+extern "C" int64_t fr_linear_mxfp4_workspace_bytes(int64_t M, int64_t N, int64_t K) {
+  using namespace fr;
+  if (M < 0 || N < 1 || K < 0 || M > (int64_t(1) << 24) || N > (int64_t(1) << 24) || K > (int64_t(1) << 20)) return -1;
+  return mx_groups(M) * mx_tiles(K) * kMxUnit;
+}
+
+extern "C" int fr_linear_mxfp4(const void* x, int dtype, int64_t M, int64_t K, int64_t ldx, const void* w_tiled, int64_t N, void* out,
+                               void* workspace, int64_t workspace_bytes, void* stream) {
+  using namespace fr;
+  FR_REQUIRE(M >= 0 && M <= (int64_t(1) << 24), FR_E_SHAPE, "fr_linear_mxfp4: M=%lld outside [0, 2^24]", (long long)M);
+  FR_REQUIRE(K >= 32 && K % 32 == 0 && K <= (1 << 20), FR_E_SHAPE, "fr_linear_mxfp4: K=%lld must be a multiple of 32 up to 2^20", (long long)K);
+  FR_REQUIRE(N >= 1 && N <= (1 << 24), FR_E_SHAPE, "fr_linear_mxfp4: N=%lld outside [1, 2^24]", (long long)N);
+  FR_REQUIRE(dtype == FR_BF16 || dtype == FR_F16, FR_E_DTYPE, "fr_linear_mxfp4: dtype %d not in {f16, bf16}", dtype);
+  if (M == 0) return FR_OK;
+  FR_REQUIRE(x && w_tiled && out, FR_E_NULL, "fr_linear_mxfp4: null pointer");
+  FR_REQUIRE(ldx >= K && ldx % 8 == 0 && aligned16(x) && aligned16(w_tiled) && aligned16(out), FR_E_ALIGN,
+             "fr_linear_mxfp4: 16-byte alignment, ldx %% 8 == 0, ldx >= K");
+  const int64_t need = fr_linear_mxfp4_workspace_bytes(M, N, K);
+  FR_REQUIRE(workspace && workspace_bytes >= need, FR_E_WORKSPACE, "fr_linear_mxfp4: workspace %lld < %lld bytes", (long long)workspace_bytes, (long long)need);
+  FR_REQUIRE((reinterpret_cast<uintptr_t>(workspace) & 255u) == 0, FR_E_ALIGN, "fr_linear_mxfp4: workspace must be 256-byte aligned");
+  hipStream_t st = static_cast<hipStream_t>(stream);
+  const int64_t groups = mx_groups(M);
+  int rc = mx_quant_tiled(x, dtype, M, K, ldx, groups, MxGather{}, workspace, st);
+  if (rc != FR_OK) return rc;
+  MxArgs a = {};
+  a.x = static_cast<const unsigned char*>(workspace);
+  a.w = static_cast<const unsigned char*>(w_tiled);
+  a.k_tiles = static_cast<int>(mx_tiles(K));
+  a.w_groups = static_cast<int>(mx_groups(N));
+  a.f_tiles = static_cast<int>(ceil_div(static_cast<int64_t>(a.w_groups), int64_t(8)));
+  a.x_groups = static_cast<int>(groups);
+  a.out = out;
+  a.ldo = N;
+  a.M = M;
+  a.N = static_cast<int>(N);
+  const int most = most_units(M);
+  return dtype == FR_BF16 ? launch_mx_gemm<bf16_t, MX_LINEAR>(a, most, ceil_div(groups, int64_t(most)), st)
+                          : launch_mx_gemm<f16_t, MX_LINEAR>(a, most, ceil_div(groups, int64_t(most)), st);
+}
+
+extern "C" int64_t fr_moe_mxfp4_workspace_bytes(int64_t M, int64_t H, int64_t F, int E, int topk) {
+  using namespace fr;
+  if (check_mx_layer("fr_moe_mxfp4_workspace_bytes", M, H, F, E, topk) != FR_OK) return -1;
+  return mx_layer(nullptr, M, H, F, E, topk).bytes;
+}
+
+extern "C" int fr_fused_moe_mxfp4(const void* x, int dtype, const void* w1_tiled, const void* w2_tiled, const void* logits, int logits_dtype,
+                                  int64_t M, int64_t H, int64_t F, int E, int topk, int renormalize, void* out, void* workspace,
+                                  int64_t workspace_bytes, void* stream) {
+  using namespace fr;
+  int rc = check_mx_layer("fr_fused_moe_mxfp4", M, H, F, E, topk);
+  if (rc != FR_OK) return rc;
+  FR_REQUIRE(dtype == FR_BF16 || dtype == FR_F16, FR_E_DTYPE, "fr_fused_moe_mxfp4: dtype %d not in {f16, bf16}", dtype);
+  FR_REQUIRE(logits_dtype == FR_F32 || logits_dtype == FR_BF16 || logits_dtype == FR_F16, FR_E_DTYPE,
+             "fr_fused_moe_mxfp4: logits dtype %d not in {f32, f16, bf16}", logits_dtype);
+  if (M == 0) return FR_OK;
+  FR_REQUIRE(x && w1_tiled && w2_tiled && logits && out, FR_E_NULL, "fr_fused_moe_mxfp4: null pointer");
+  FR_REQUIRE(aligned16(x) && aligned16(w1_tiled) && aligned16(w2_tiled) && aligned16(out), FR_E_ALIGN, "fr_fused_moe_mxfp4: 16-byte alignment");
+  const MxLayer l = mx_layer(workspace, M, H, F, E, topk);
+  FR_REQUIRE(workspace && workspace_bytes >= l.bytes, FR_E_WORKSPACE, "fr_fused_moe_mxfp4: workspace %lld < %lld bytes", (long long)workspace_bytes, (long long)l.bytes);
+  FR_REQUIRE((reinterpret_cast<uintptr_t>(workspace) & 255u) == 0, FR_E_ALIGN, "fr_fused_moe_mxfp4: workspace must be 256-byte aligned");
+  hipStream_t st = static_cast<hipStream_t>(stream);
+  const int64_t n = M * topk;
+  if (route_align_fits(M, E, topk, false)) {
+    rc = route_align_small(logits, logits_dtype, M, E, topk, renormalize, kMxRows, l.topk_w, l.topk_ids, l.sorted, l.expert_ids, l.npost, nullptr, 0,
+                           nullptr, nullptr, st);
+  } else {
+    rc = fr_gating_topk(logits, logits_dtype, M, E, E, topk, renormalize, l.topk_w, l.topk_ids, stream);
+    if (rc == FR_OK) rc = fr_moe_align(l.topk_ids, FR_I32, n, E, kMxRows, l.sorted, l.expert_ids, l.npost, l.align_ws, l.align_bytes, stream);
+  }
+  if (rc != FR_OK) return rc;
+  MxGather g;
+  g.sorted = l.sorted;
+  g.expert_ids = l.expert_ids;
+  g.npost = l.npost;
+  g.topk = topk;
+  g.E = E;
+  g.most_units = l.most;
+  g.tile_count = l.tile_count;
+  g.tiles = l.tiles;
+  rc = mx_quant_tiled(x, dtype, n, H, H, l.groups, g, l.x, st);
+  if (rc != FR_OK) return rc;
+  MxArgs a = {};
+  a.tile_count = l.tile_count;
+  a.tiles = l.tiles;
+  a.sorted = l.sorted;
+  a.topk_w = l.topk_w;
+  a.n_pairs = static_cast<int>(n);
+  a.act_tiles = static_cast<int>(mx_tiles(F));
+  a.act_blocks = static_cast<int>(F / kMxBlock);
+  // gate and up
+  a.x = l.x;
+  a.act = l.act;
+  a.w = static_cast<const unsigned char*>(w1_tiled);
+  a.k_tiles = static_cast<int>(mx_tiles(H));
+  a.w_groups = static_cast<int>(2 * F / kMxRows);
+  a.w_stride = static_cast<int64_t>(a.w_groups) * a.k_tiles * kMxUnit;
+  a.f_tiles = 2 * a.act_tiles;  // whole units of activated features: the last ones are filled up with zeros
+  rc = launch_mx_gemm<bf16_t, MX_SILU>(a, l.most, l.tile_limit, st);
+  if (rc != FR_OK) return rc;
+  // down
+  a.x = l.act;
+  a.w = static_cast<const unsigned char*>(w2_tiled);
+  a.k_tiles = a.act_tiles;
+  a.w_groups = static_cast<int>(H / kMxRows);
+  a.w_stride = static_cast<int64_t>(a.w_groups) * a.k_tiles * kMxUnit;
+  a.f_tiles = static_cast<int>(ceil_div(static_cast<int64_t>(a.w_groups), int64_t(8)));
+  a.rows = l.rows;
+  a.N = static_cast<int>(H);
+  rc = launch_mx_gemm<bf16_t, MX_DOWN>(a, l.most, l.tile_limit, st);
+  if (rc != FR_OK) return rc;
+  const dim3 grid(static_cast<unsigned>(ceil_div(M * (H / 8), int64_t(kMxThreads))));
+  if (dtype == FR_BF16)
+    hipLaunchKernelGGL((mx_combine_kernel<bf16_t>), grid, dim3(kMxThreads), 0, st, l.rows, l.topk_ids, E, topk, M, (int)H, static_cast<bf16_t*>(out));
+  else
+    hipLaunchKernelGGL((mx_combine_kernel<f16_t>), grid, dim3(kMxThreads), 0, st, l.rows, l.topk_ids, E, topk, M, (int)H, static_cast<f16_t*>(out));
+  return check_launch("mx_combine_kernel");
+}

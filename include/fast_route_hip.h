@@ -312,6 +312,47 @@ int fr_fused_moe_fp8(const void* x, int x_dtype, const void* w1q, const float* w
                      int64_t F, int E, int topk, int renormalize, void* out, void* workspace,
                      int64_t workspace_bytes, void* stream);
 
+/* ---- MXFP4 path -------------------------------------------------------------
+ * No counterpart in the reference.  Rows in the OCP microscaling format with 4-bit elements: 32 consecutive
+ * elements share a scale 2^(b - 127) held in a byte, an element is e2m1 (0, 1/2, 1, 3/2, 2, 3, 4, 6, sign in the
+ * top bit), two to a byte, the even element in the low half.  K % 32 == 0 throughout.
+ *
+ * Quantisation: b = floor(log2(max|x|)) - 2 + 127 over the block, at least 0 (127 for a block of zeros); elements to the nearest
+ * value of x / 2^(b - 127), ties to the even code, magnitudes above 6 become 6.  A block that holds an infinity or a NaN
+ * gets b = 255 and zero codes: all its elements are read back as NaN, and so is every product they enter.
+ * x is f16 / bf16 [rows, K], row stride ldx (a multiple of 8); codes_out uint8 [rows, K / 2], scales_out uint8 [rows, K / 32];
+ * x and codes_out 16-byte aligned. */
+int fr_quant_mxfp4_rows(const void* x, int dtype, int64_t rows, int64_t K, int64_t ldx, void* codes_out, void* scales_out,
+                        void* stream);
+/* The way back, to f16 (rounded to nearest, overflow to infinity), bf16 or f32 [rows, K] dense; codes and out 16-byte aligned. */
+int fr_dequant_mxfp4_rows(const void* codes, const void* scales, int64_t rows, int64_t K, int out_dtype, void* out, void* stream);
+
+/* Weights in the layout that the products below read (units of 32 rows x 256 elements of K, codes and scales together, rows and K
+ * filled up with zeros): codes [matrices, rows, K / 2] and scales [matrices, rows, K / 32] into `out`
+ * (fr_mxfp4_tiled_bytes bytes, -1: too large).  gate_up != 0: rows are F gate rows and then F up rows
+ * (the w1 of the layer, rows = 2 F).  codes and out 16-byte aligned. */
+int64_t fr_mxfp4_tiled_bytes(int64_t matrices, int64_t rows, int64_t K);
+int fr_mxfp4_tile_weights(const void* codes, const void* scales, int64_t matrices, int64_t rows, int64_t K, int gate_up, void* out,
+                          void* stream);
+
+/* out[M, N] = q(x)[M, K] @ w[N, K]^T: x (f16 / bf16, row stride ldx, a multiple of 8) quantised to MXFP4 on the way, w laid out by
+ * fr_mxfp4_tile_weights(.., 1, N, K, 0, ..), fp32 accumulation, out dense in x's type.  M and N any size;
+ * `workspace`: 256-byte aligned, fr_linear_mxfp4_workspace_bytes(M, N, K) bytes. */
+int64_t fr_linear_mxfp4_workspace_bytes(int64_t M, int64_t N, int64_t K);
+int fr_linear_mxfp4(const void* x, int dtype, int64_t M, int64_t K, int64_t ldx, const void* w_tiled, int64_t N, void* out,
+                    void* workspace, int64_t workspace_bytes, void* stream);
+
+/* Whole layer with MXFP4 weights from f16 / bf16 activations and router logits[M, E] (dense): gating, routing, x quantised per
+ * block, gate/up product + SiLU*up, the activated rows quantised from their fp32 values, down product, routed weight and
+ * top-k sum in fp32, rounded once to `dtype`.  w1_tiled / w2_tiled: fr_mxfp4_tile_weights of [E, 2F, H] (gate_up = 1)
+ * and [E, H, F] (gate_up = 0).  `out` may alias `x`.  H and F multiples of 32, E <= 256, M * topk <= 2^24.
+ * `workspace`: 256-byte aligned, fr_moe_mxfp4_workspace_bytes bytes (-1: sizes outside the limits); two
+ * calls that may overlap in time need one each. */
+int64_t fr_moe_mxfp4_workspace_bytes(int64_t M, int64_t H, int64_t F, int E, int topk);
+int fr_fused_moe_mxfp4(const void* x, int dtype, const void* w1_tiled, const void* w2_tiled, const void* logits, int logits_dtype,
+                       int64_t M, int64_t H, int64_t F, int E, int topk, int renormalize, void* out, void* workspace,
+                       int64_t workspace_bytes, void* stream);
+
 /* ---- measurement aid -------------------------------------------------------
  * A pure stream of bf16 MFMAs (no loads, no LDS) on every CU: `iters` rounds over 256 accumulator
  * registers per lane and SIMD, `shape` 32 = v_mfma_f32_32x32x16_bf16, 16 = v_mfma_f32_16x16x32_bf16,

@@ -23,3 +23,11 @@ from .moe_oracle import (  # noqa: F401
     make_inputs,
     zipf_logits,
 )
+from .mxfp4_oracle import (  # noqa: F401
+    fused_moe_mxfp4,
+    mxfp4_doubt,
+    mxfp4_held,
+    mxfp4_quant_rows,
+    mxfp4_round,
+    mxfp4_values,
+)
