@@ -85,6 +85,24 @@ __device__ __forceinline__ f32x16 mx_mfma(mx_frag w, int ws, mx_frag x, int xs, 
   return __builtin_amdgcn_mfma_scale_f32_32x32x64_f8f6f4(a, b, acc, 4, 4, S, ws, S, xs);  // 4: e2m1
 }
 
+// The same written out, for accumulators that fill the accumulation half of the register file (tiles above four row groups): left to
+// the compiler, they wander through ordinary registers around the K loop and operands are spilled inside it.  What the compiler sees to for
+// MFMAs of its own, and not for these: no vector instruction may write an operand right before one (operands come from memory and are waited
+// for), and a result may be read by another instruction 18 wait states after the last MFMA on it.
+template <int S>
+__device__ __forceinline__ void mx_mfma_held(mx_frag w, int ws, mx_frag x, int xs, f32x16& acc) {
+#if defined(__HIP_DEVICE_COMPILE__)
+#define FR_MX_MFMA(lo_, hi_) \
+  asm volatile("v_mfma_scale_f32_32x32x64_f8f6f4 %0, %1, %2, %0, %3, %4 op_sel:[" lo_ "," lo_ ",0] op_sel_hi:[" hi_ "," hi_ ",0] cbsz:4 blgp:4" \
+               : "+a"(acc) : "v"(w), "v"(x), "v"(ws), "v"(xs))
+  if constexpr (S == 0) FR_MX_MFMA("0", "0");
+  else if constexpr (S == 1) FR_MX_MFMA("1", "0");
+  else if constexpr (S == 2) FR_MX_MFMA("0", "1");
+  else FR_MX_MFMA("1", "1");
+#undef FR_MX_MFMA
+#endif
+}
+
 // largest |v| bits over the 32 elements of a block held by a lane and its partner in the other half of the wavefront
 __device__ __forceinline__ unsigned mx_pair_max(unsigned v) {
   const unsigned o = static_cast<unsigned>(partner_i32<32>(static_cast<int>(v)));

@@ -40,6 +40,27 @@ struct MxArgs {
 
 __device__ __forceinline__ float mx_silu_mul(float g, float u) { return g / (1.f + __expf(-g)) * u; }
 
+// An accumulator's registers copied to ordinary ones here and now.  Left to itself the register allocator fetches the accumulators of a
+// tall tile (256 registers, all of the accumulation half) early, and spills addresses inside the K loop for them.
+template <bool HELD>
+__device__ __forceinline__ f32x16 mx_fetch(const f32x16& v) {
+  f32x16 o = v;
+#if defined(__HIP_DEVICE_COMPILE__)
+  if constexpr (HELD) {
+#pragma unroll
+    for (int r = 0; r < 16; r += 4)
+      asm volatile("v_accvgpr_read_b32 %0, %4\n\tv_accvgpr_read_b32 %1, %5\n\tv_accvgpr_read_b32 %2, %6\n\tv_accvgpr_read_b32 %3, %7"
+                   : "=v"(o[r]), "=v"(o[r + 1]), "=v"(o[r + 2]), "=v"(o[r + 3])
+                   : "a"(v[r]), "a"(v[r + 1]), "a"(v[r + 2]), "a"(v[r + 3]));
+  }
+#endif
+  return o;
+}
+
+template <typename T, int EPI, int U>
+__device__ __forceinline__ void mx_epilogue(const MxArgs& a, const MxTile& t, int f, int wave, int lane, f32x16 (&acc)[U][2]);
+
+// Fragments from memory to registers.
 template <typename T, int EPI, int U>
 __device__ __forceinline__ void mx_tile(const MxArgs& a, const MxTile& t, int f) {
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
@@ -79,26 +100,141 @@ __device__ __forceinline__ void mx_tile(const MxArgs& a, const MxTile& t, int f)
       }
     }
   }
-  // the lane's 16 consecutive features of token row col
-  const int col = lane & 31, half = lane >> 5;
+  mx_epilogue<T, EPI, U>(a, t, f, wave, lane, acc);
+}
+
+// Token rows through LDS (every wavefront reads all of them), weights from memory to registers (nobody else reads them).
+template <typename T, int EPI, int U>
+__device__ __forceinline__ void mx_tile_lds(const MxArgs& a, const MxTile& t, int f, unsigned char* lds) {
+#if defined(__HIP_DEVICE_COMPILE__)
+  typedef __attribute__((address_space(3))) void* lptr_t;
+  constexpr int QS = (U + 3) / 4, SLOT = U * 4096 + QS * 1024;
+  const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const int wg = min((f * 4 + wave) * 2, a.w_groups - 1), wg1 = min(wg + 1, a.w_groups - 1);
+  const int pitch = a.k_tiles * kMxUnit, last = a.k_tiles - 1;
+  const unsigned char* const w0 = a.w + t.expert * a.w_stride + static_cast<int64_t>(wg) * pitch;
+  const unsigned char* const w1 = a.w + t.expert * a.w_stride + static_cast<int64_t>(wg1) * pitch;
+  const __amdgpu_buffer_rsrc_t xr = 
+      __builtin_amdgcn_make_buffer_rsrc(const_cast<unsigned char*>(a.x + static_cast<int64_t>(t.group) * pitch), 0, -1, 0x00020000);
+  const int q = wave % QS, su = min(q * 4 + (lane >> 4), U - 1);
+  const int code_off = lane * 16, scale_off = su * pitch + kMxScales + (lane & 15) * 16;
+  f32x16 acc[U][2];
+#pragma unroll
+  for (int u = 0; u < U; ++u)
+#pragma unroll
+    for (int j = 0; j < 2; ++j)
+#pragma unroll
+      for (int r = 0; r < 16; ++r) acc[u][j][r] = 0.f;
+  mx_frag wf[2][4], xf[2][U];
+  int ws[2][2], xs[2][U];  // of K tile k in half k & 1
+  auto load_x = [&](int k) {  // K tile k into slot k & 1
+    const int kc = min(k, last);
+    unsigned char* slot = lds + (k & 1) * SLOT;
+#pragma unroll
+    for (int u = 0; u < U; ++u)
+      __builtin_amdgcn_raw_ptr_buffer_load_lds(xr, (lptr_t)(slot + u * 4096 + wave * 1024), 16, code_off, u * pitch + kc * kMxUnit + wave * 1024, 0, 0);
+    __builtin_amdgcn_raw_ptr_buffer_load_lds(xr, (lptr_t)(slot + U * 4096 + q * 1024), 16, scale_off, kc * kMxUnit, 0, 0);
+  };
+  auto load_w = [&](int k, int s) {
+    const int kc = min(k, last);
+    wf[0][s] = *reinterpret_cast<const mx_frag*>(w0 + kc * kMxUnit + s * 1024 + lane * 16);
+    wf[1][s] = *reinterpret_cast<const mx_frag*>(w1 + kc * kMxUnit + s * 1024 + lane * 16);
+  };
+  auto load_ws = [&](int k, int (&to)[2]) {
+    const int kc = min(k, last);
+    to[0] = *reinterpret_cast<const int*>(w0 + kc * kMxUnit + kMxScales + lane * 4);
+    to[1] = *reinterpret_cast<const int*>(w1 + kc * kMxUnit + kMxScales + lane * 4);
+  };
+  auto read_x = [&](int k, int s, int u) {
+    return *reinterpret_cast<const mx_frag*>(lds + (k & 1) * SLOT + u * 4096 + s * 1024 + lane * 16);
+  };
+  auto read_xs = [&](int k, int u) { return *reinterpret_cast<const int*>(lds + (k & 1) * SLOT + U * 4096 + u * 256 + lane * 4); };
+  load_x(0);
+  for (int s = 0; s < 4; ++s) load_w(0, s);
+  load_ws(0, ws[0]);
+  asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+  __builtin_amdgcn_s_barrier();
+  load_x(1);
+  load_ws(1, ws[1]);
+#pragma unroll
+  for (int u = 0; u < U; ++u) {
+    xf[0][u] = read_x(0, 0, u);
+    xs[0][u] = read_xs(0, u);
+  }
+  if constexpr (U > 4) {
+#pragma unroll
+    for (int u = 0; u < U; ++u)
+#pragma unroll
+      for (int j = 0; j < 2; ++j) asm volatile("s_nop 3" : "+a"(acc[u][j]));
+  }
+  for (int k0 = 0; k0 <= last; k0 += 2) {
+#pragma unroll
+    for (int p = 0; p < 2; ++p) {
+      const int k = k0 + p;
+      if (p == 0 || k <= last) {
+        mx_each<0, 4>([&](auto S) {
+          constexpr int s = decltype(S)::value;
+          if constexpr (s == 3) {
+            // the next K tile has landed (the loads issued behind it are ten, the six newest this K tile's) and this one's
+            // has been read, by everybody behind the barrier
+            asm volatile("s_waitcnt vmcnt(6) lgkmcnt(0)" ::: "memory");
+            __builtin_amdgcn_s_barrier();
+            load_x(k + 2);
+            __builtin_amdgcn_sched_barrier(0);
+          }
+#pragma unroll
+          for (int u = 0; u < U; ++u) {
+#pragma unroll
+            for (int j = 0; j < 2; ++j) {
+              if constexpr (U > 4) mx_mfma_held<s>(wf[j][s], ws[p][j], xf[s & 1][u], xs[p][u], acc[u][j]);
+              else acc[u][j] = mx_mfma<s>(wf[j][s], ws[p][j], xf[s & 1][u], xs[p][u], acc[u][j]);
+            }
+            if constexpr (s < 3) xf[(s + 1) & 1][u] = read_x(k, s + 1, u);
+            else {
+              xf[0][u] = read_x(k + 1, 0, u);
+              xs[p ^ 1][u] = read_xs(k + 1, u);
+            }
+            __builtin_amdgcn_sched_barrier(0);
+          }
+          load_w(k + 1, s);
+          if constexpr (s == 3) load_ws(k + 2, ws[p]);
+          __builtin_amdgcn_sched_barrier(0);
+        });
+      }
+    }
+  }
+  asm volatile("s_waitcnt vmcnt(0)\n\ts_nop 15\n\ts_nop 15" ::: "memory");  // no load of this workgroup's is under way to LDS; the last MFMAs are done
+  __builtin_amdgcn_sched_barrier(0);
+  mx_epilogue<T, EPI, U>(a, t, f, wave, lane, acc);
+#endif
+}
+
+// acc[u][j]: the lane's 16 consecutive features of token row `lane % 32` of row group u.
+template <typename T, int EPI, int U>
+__device__ __forceinline__ void mx_epilogue(const MxArgs& a, const MxTile& t, int f, int wave, int lane, f32x16 (&acc)[U][2]) {
+  constexpr bool HELD = U > 4;
+  const int wg = (f * 4 + wave) * 2, col = lane & 31, half = lane >> 5;
   if constexpr (EPI == MX_SILU) {
-    const int blk = f * 4 + wave;  // of 32 activated features
-    if (blk >= a.act_tiles * 8) return;
+    const int blk = f * 4 + wave;  // of 32 activated features; the operand's last K tile is filled up with zeros
+    const bool pad = blk >= a.act_blocks;
+    unsigned char* unit = a.act + (static_cast<int64_t>(t.group) * a.act_tiles + (blk >> 3)) * kMxUnit;
 #pragma unroll
     for (int u = 0; u < U; ++u) {
+      const f32x16 g = mx_fetch<HELD>(acc[u][0]), up = mx_fetch<HELD>(acc[u][1]);
       float v[16];
       unsigned amax = 0;
 #pragma unroll
       for (int r = 0; r < 16; ++r) {
-        v[r] = mx_silu_mul(acc[u][0][r], acc[u][1][r]);
+        v[r] = pad ? 0.f : mx_silu_mul(g[r], up[r]);
         const unsigned m = magnitude(v[r]);
         amax = amax > m ? amax : m;
       }
       const unsigned byte = mx_scale_byte(mx_pair_max(amax));
-      unsigned char* unit = a.act + (static_cast<int64_t>(t.group + u) * a.act_tiles + (blk >> 3)) * kMxUnit;
       const uint2 o = {mx_pack8(v, byte), mx_pack8(v + 8, byte)};
       *reinterpret_cast<uint2*>(unit + mx_code_at(col, blk & 7) + half * 8) = o;
       if (half == 0) unit[mx_scale_at(col, blk & 7)] = static_cast<unsigned char>(byte);
+      unit += static_cast<int64_t>(a.act_tiles) * kMxUnit;
+      if (HELD) __builtin_amdgcn_sched_barrier(0);
     }
   } else {
 #pragma unroll
@@ -106,38 +242,40 @@ __device__ __forceinline__ void mx_tile(const MxArgs& a, const MxTile& t, int f)
       const int64_t slot = static_cast<int64_t>(t.group + u) * kMxRows + col;
       if constexpr (EPI == MX_DOWN) {
         const int pair = a.sorted[slot];
-        if (pair < a.n_pairs) {
-          const float s = a.topk_w[pair];
-#pragma unroll
-          for (int j = 0; j < 2; ++j) {
-            const int c = (wg + j) * 32 + half * 16;  // N is a multiple of 32
-            if (c < a.N) {
-              float* row = a.rows + static_cast<int64_t>(pair) * a.N + c;
-#pragma unroll
-              for (int r = 0; r < 16; r += 4)
-                *reinterpret_cast<f32x4*>(row + r) = f32x4{acc[u][j][r] * s, acc[u][j][r + 1] * s, acc[u][j][r + 2] * s, acc[u][j][r + 3] * s};
-            }
-          }
-        }
-      } else if (slot < a.M) {
+        const bool live = pair < a.n_pairs;
+        const float s = live ? a.topk_w[pair] : 0.f;
 #pragma unroll
         for (int j = 0; j < 2; ++j) {
-          const int c = (wg + j) * 32 + half * 16;
-          T* row = static_cast<T*>(a.out) + slot * a.ldo + c;
-          if (c + 16 <= a.N && (a.ldo & 7) == 0) {
-            typedef T vec8 __attribute__((ext_vector_type(8)));
+          const f32x16 v = mx_fetch<HELD>(acc[u][j]);
+          const int c = (wg + j) * 32 + half * 16;  // N is a multiple of 32
+          if (live && c < a.N) {
+            float* row = a.rows + static_cast<int64_t>(pair) * a.N + c;
 #pragma unroll
-            for (int r = 0; r < 16; r += 8) {
-              vec8 o;
-#pragma unroll
-              for (int i = 0; i < 8; ++i) o[i] = static_cast<T>(acc[u][j][r + i]);
-              *reinterpret_cast<vec8*>(row + r) = o;
-            }
-          } else {
-#pragma unroll
-            for (int r = 0; r < 16; ++r)
-              if (c + r < a.N) row[r] = static_cast<T>(acc[u][j][r]);
+            for (int r = 0; r < 16; r += 4) *reinterpret_cast<f32x4*>(row + r) = f32x4{v[r] * s, v[r + 1] * s, v[r + 2] * s, v[r + 3] * s};
           }
+          if (HELD) __builtin_amdgcn_sched_barrier(0);
+        }
+      } else {
+        typedef T vec8 __attribute__((ext_vector_type(8)));
+#pragma unroll
+        for (int j = 0; j < 2; ++j) {
+          const f32x16 v = mx_fetch<HELD>(acc[u][j]);
+          const int c = (wg + j) * 32 + half * 16;
+          vec8 o[2];
+#pragma unroll
+          for (int r = 0; r < 16; ++r) o[r >> 3][r & 7] = static_cast<T>(v[r]);
+          if (slot < a.M) {
+            T* row = static_cast<T*>(a.out) + slot * a.ldo + c;
+            if (c + 16 <= a.N && (a.ldo & 7) == 0) {
+              *reinterpret_cast<vec8*>(row) = o[0];
+              *reinterpret_cast<vec8*>(row + 8) = o[1];
+            } else {
+#pragma unroll
+              for (int r = 0; r < 16; ++r)
+                if (c + r < a.N) row[r] = o[r >> 3][r & 7];
+            }
+          }
+          if (HELD) __builtin_amdgcn_sched_barrier(0);
         }
       }
     }
@@ -146,7 +284,8 @@ __device__ __forceinline__ void mx_tile(const MxArgs& a, const MxTile& t, int f)
 
 // MOST: row groups of a tile, at most.
 template <typename T, int EPI, int MOST>
-__global__ __launch_bounds__(kMxThreads, 1) void mx_gemm_kernel(MxArgs a) {
+__global__ __launch_bounds__(kMxThreads, MOST == 8 ? 1 : 2) void mx_gemm_kernel(MxArgs a) {
+  extern __shared__ __attribute__((aligned(16))) unsigned char mx_lds[];
   // workgroups b, b + 8, .. share an XCD and its L2: an XCD takes a consecutive part of the walk
   const int tiles = EPI == MX_LINEAR ? (a.x_groups + MOST - 1) / MOST : a.tile_count[0];
   const int total = tiles * a.f_tiles, per = (total + 7) / 8;
@@ -166,19 +305,40 @@ __global__ __launch_bounds__(kMxThreads, 1) void mx_gemm_kernel(MxArgs a) {
   if constexpr (EPI == MX_LINEAR) t = MxTile{index * MOST, min(MOST, a.x_groups - index * MOST), 0, 0, 0};
   else t = a.tiles[index];
   if constexpr (MOST >= 8) {
-    if (t.units == 8) return mx_tile<T, EPI, 8>(a, t, f);
-    if (t.units == 7) return mx_tile<T, EPI, 7>(a, t, f);
-    if (t.units == 6) return mx_tile<T, EPI, 6>(a, t, f);
-    if (t.units == 5) return mx_tile<T, EPI, 5>(a, t, f);
+    if (t.units == 8) return mx_tile_lds<T, EPI, 8>(a, t, f, mx_lds);
+    if (t.units == 7) return mx_tile_lds<T, EPI, 7>(a, t, f, mx_lds);
+    if (t.units == 6) return mx_tile_lds<T, EPI, 6>(a, t, f, mx_lds);
+    if (t.units == 5) return mx_tile_lds<T, EPI, 5>(a, t, f, mx_lds);
   }
   if constexpr (MOST >= 4) {
-    if (t.units == 4) return mx_tile<T, EPI, 4>(a, t, f);
-    if (t.units == 3) return mx_tile<T, EPI, 3>(a, t, f);
+    if (t.units == 4) return mx_tile_lds<T, EPI, 4>(a, t, f, mx_lds);
+    if (t.units == 3) return mx_tile_lds<T, EPI, 3>(a, t, f, mx_lds);
   }
   if constexpr (MOST >= 2) {
     if (t.units == 2) return mx_tile<T, EPI, 2>(a, t, f);
   }
   mx_tile<T, EPI, 1>(a, t, f);
+}
+
+constexpr int mx_lds_bytes(int most) { return 2 * (most * 4096 + (most + 3) / 4 * 1024); }
+
+// More than 64 KB of LDS needs the kernel's limit raised, once per device (a set-up call, not stream work).
+template <typename T, int EPI, int MOST>
+int mx_allow_lds() {
+  if (mx_lds_bytes(MOST) <= 65536) return FR_OK;
+  constexpr int kMaxDevices = 64;
+  static bool set[kMaxDevices] = {};  // a race between threads sets the same limit twice
+  int dev = 0;
+  hipError_t e = hipGetDevice(&dev);
+  if (e != hipSuccess || dev < 0 || dev >= kMaxDevices) return fail(FR_E_LAUNCH, "mxfp4 product: device %d (%s)", dev, hipGetErrorString(e));
+  if (set[dev]) return FR_OK;
+  e = hipFuncSetAttribute(reinterpret_cast<const void*>(&mx_gemm_kernel<T, EPI, MOST>), hipFuncAttributeMaxDynamicSharedMemorySize, mx_lds_bytes(MOST));
+  if (e != hipSuccess) {
+    (void)hipGetLastError();
+    return fail(FR_E_LAUNCH, "mxfp4 product: %d bytes of LDS: %s", mx_lds_bytes(MOST), hipGetErrorString(e));
+  }
+  set[dev] = true;
+  return FR_OK;
 }
 
 template <typename T, int EPI>
@@ -187,8 +347,13 @@ int launch_mx_gemm(const MxArgs& a, int most, int64_t tiles, hipStream_t st) {
   FR_REQUIRE(wgs < (int64_t(1) << 31), FR_E_SHAPE, "mxfp4 product: %lld workgroups", (long long)wgs);
   const dim3 grid(static_cast<unsigned>(wgs)), block(kMxThreads);
   switch (most) {
-    case 8: hipLaunchKernelGGL((mx_gemm_kernel<T, EPI, 8>), grid, block, 0, st, a); break;
-    case 4: hipLaunchKernelGGL((mx_gemm_kernel<T, EPI, 4>), grid, block, 0, st, a); break;
+    case 8: {
+      const int rc = mx_allow_lds<T, EPI, 8>();
+      if (rc != FR_OK) return rc;
+      hipLaunchKernelGGL((mx_gemm_kernel<T, EPI, 8>), grid, block, mx_lds_bytes(8), st, a);
+      break;
+    }
+    case 4: hipLaunchKernelGGL((mx_gemm_kernel<T, EPI, 4>), grid, block, mx_lds_bytes(4), st, a); break;
     case 2: hipLaunchKernelGGL((mx_gemm_kernel<T, EPI, 2>), grid, block, 0, st, a); break;
     default: hipLaunchKernelGGL((mx_gemm_kernel<T, EPI, 1>), grid, block, 0, st, a); break;
   }
