@@ -85,28 +85,24 @@ __device__ __forceinline__ f32x16 mx_mfma(mx_frag w, int ws, mx_frag x, int xs, 
   return __builtin_amdgcn_mfma_scale_f32_32x32x64_f8f6f4(a, b, acc, 4, 4, S, ws, S, xs);  // 4: e2m1
 }
 
-// The same written out, for accumulators that fill the accumulation half of the register file (tiles above four row groups): left to
-// the compiler, they wander through ordinary registers around the K loop and operands are spilled inside it.  What the compiler sees to for
-// MFMAs of its own, and not for these: no vector instruction may write an operand right before one (operands come from memory and are waited
-// for), and a result may be read by another instruction 18 wait states after the last MFMA on it.
-template <int S>
-__device__ __forceinline__ void mx_mfma_held(mx_frag w, int ws, mx_frag x, int xs, f32x16& acc) {
-#if defined(__HIP_DEVICE_COMPILE__)
-#define FR_MX_MFMA(lo_, hi_) \
-  asm volatile("v_mfma_scale_f32_32x32x64_f8f6f4 %0, %1, %2, %0, %3, %4 op_sel:[" lo_ "," lo_ ",0] op_sel_hi:[" hi_ "," hi_ ",0] cbsz:4 blgp:4" \
-               : "+a"(acc) : "v"(w), "v"(x), "v"(ws), "v"(xs))
-  if constexpr (S == 0) FR_MX_MFMA("0", "0");
-  else if constexpr (S == 1) FR_MX_MFMA("1", "0");
-  else if constexpr (S == 2) FR_MX_MFMA("0", "1");
-  else FR_MX_MFMA("1", "1");
-#undef FR_MX_MFMA
-#endif
-}
-
 // largest |v| bits over the 32 elements of a block held by a lane and its partner in the other half of the wavefront
 __device__ __forceinline__ unsigned mx_pair_max(unsigned v) {
   const unsigned o = static_cast<unsigned>(partner_i32<32>(static_cast<int>(v)));
   return v > o ? v : o;
+}
+
+// A pair's weighted row between the down product and the sum over a token's pairs: 16 consecutive values as 16-bit integers times a shared
+// step, |q| <= 32766.  A value is off by at most half a step, 2^-15 of the largest of its 16 (1e-5 of a row's values on average, a
+// twentieth of the last rounding to fp16), in little more than half the bytes of fp32.  An infinity is +-32767, a NaN -32768.
+constexpr int kMxRowBlock = 16;
+constexpr float kMxRowMagic = 12582912.f;  // 3 2^22: the low bits of a sum with it are the integer nearest to the other summand
+// exponent byte k + 127 of a block whose largest finite magnitude, in [2^k, 2^(k + 1)), has these bits; below 2^-112 the step no longer shrinks
+__device__ __forceinline__ unsigned mx_row_byte(unsigned amax) { return max(amax >> 23, 15u); }
+__device__ __forceinline__ float mx_row_factor(unsigned byte) { return __uint_as_float((127 + 14 + 127 - byte) << 23) * (1.f - 0x1p-14f); }
+__device__ __forceinline__ float mx_row_step(unsigned byte) { return __uint_as_float((byte - 14) << 23) * (1.f / (1.f - 0x1p-14f)); }
+__device__ __forceinline__ float mx_row_value(int q, float step) {
+  const float v = static_cast<float>(q) * step;
+  return q == 32767 ? __builtin_inff() : q > -32767 ? v : q == -32768 ? __builtin_nanf("") : -__builtin_inff();
 }
 
 // A token tile of the grouped product: `units` row groups from `group` on, of one expert; the tiles chunk0 .. chunk0 + chunk_n - 1 are
@@ -115,7 +111,7 @@ struct MxTile {
   int group, units, expert, chunk0, chunk_n;
 };
 constexpr int kMxChunk = 8;      // tiles walked together, at most
-constexpr int kMxMaxUnits = 8;   // row groups of a tile, at most
+constexpr int kMxMaxUnits = 4;   // row groups of a tile, at most
 
 // ---- launches (mxfp4_quant.hip, mxfp4_gemm.hip) ----------------------------------------------------------------
 

@@ -30,7 +30,9 @@ struct MxArgs {
   const int32_t* sorted;
   const float* topk_w;
   int n_pairs;
-  float* rows;
+  uint4* rows;             // [n_pairs, N] integers, eight to an element
+  unsigned char* row_exps; // [n_pairs, exp_pitch]: blocks 4 i + (0, 1, 2, 3) at 4 i + (0, 2, 1, 3)
+  int exp_pitch;
   // MX_LINEAR
   void* out;
   int64_t ldo;
@@ -39,23 +41,6 @@ struct MxArgs {
 };
 
 __device__ __forceinline__ float mx_silu_mul(float g, float u) { return g / (1.f + __expf(-g)) * u; }
-
-// An accumulator's registers copied to ordinary ones here and now.  Left to itself the register allocator fetches the accumulators of a
-// tall tile (256 registers, all of the accumulation half) early, and spills addresses inside the K loop for them.
-template <bool HELD>
-__device__ __forceinline__ f32x16 mx_fetch(const f32x16& v) {
-  f32x16 o = v;
-#if defined(__HIP_DEVICE_COMPILE__)
-  if constexpr (HELD) {
-#pragma unroll
-    for (int r = 0; r < 16; r += 4)
-      asm volatile("v_accvgpr_read_b32 %0, %4\n\tv_accvgpr_read_b32 %1, %5\n\tv_accvgpr_read_b32 %2, %6\n\tv_accvgpr_read_b32 %3, %7"
-                   : "=v"(o[r]), "=v"(o[r + 1]), "=v"(o[r + 2]), "=v"(o[r + 3])
-                   : "a"(v[r]), "a"(v[r + 1]), "a"(v[r + 2]), "a"(v[r + 3]));
-  }
-#endif
-  return o;
-}
 
 template <typename T, int EPI, int U>
 __device__ __forceinline__ void mx_epilogue(const MxArgs& a, const MxTile& t, int f, int wave, int lane, f32x16 (&acc)[U][2]);
@@ -103,21 +88,29 @@ __device__ __forceinline__ void mx_tile(const MxArgs& a, const MxTile& t, int f)
   mx_epilogue<T, EPI, U>(a, t, f, wave, lane, acc);
 }
 
-// Token rows through LDS (every wavefront reads all of them), weights from memory to registers (nobody else reads them).
+// Token rows through LDS (every wavefront reads all of them), weights from memory to registers (no other wavefront reads them).  A
+// ring of kMxSlots K tiles of token rows and two of weights are under way.  All loads are spread between the MFMAs, a row
+// group's two at a time: issued in one run per K tile they held up the MFMAs behind them (8 experts, H = 4096, F = 14336, 16384 tokens: gate/up
+// 1966 -> 1830 us, down 1048 -> 1003).
+//
+// 128 x 256 outputs and two workgroups per CU, whose prologues and epilogues meet the other's MFMAs.  256 x 256 by one workgroup
+// of four wavefronts moves a third less through L1 but stalls more: 2098 / 1039 us.  A stream of these MFMAs alone reaches 6.4 PFLOP/s (the
+// part lowers its clock to 1.67 GHz for it); without any load, on data that is there, this loop reaches 5.1 to 5.5.
+constexpr int kMxSlots = 4;
 template <typename T, int EPI, int U>
 __device__ __forceinline__ void mx_tile_lds(const MxArgs& a, const MxTile& t, int f, unsigned char* lds) {
 #if defined(__HIP_DEVICE_COMPILE__)
   typedef __attribute__((address_space(3))) void* lptr_t;
-  constexpr int QS = (U + 3) / 4, SLOT = U * 4096 + QS * 1024;
+  constexpr int SLOT = U * 4096 + 1024;
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int wg = min((f * 4 + wave) * 2, a.w_groups - 1), wg1 = min(wg + 1, a.w_groups - 1);
   const int pitch = a.k_tiles * kMxUnit, last = a.k_tiles - 1;
   const unsigned char* const w0 = a.w + t.expert * a.w_stride + static_cast<int64_t>(wg) * pitch;
   const unsigned char* const w1 = a.w + t.expert * a.w_stride + static_cast<int64_t>(wg1) * pitch;
-  const __amdgpu_buffer_rsrc_t xr = 
+  const __amdgpu_buffer_rsrc_t xr =
       __builtin_amdgcn_make_buffer_rsrc(const_cast<unsigned char*>(a.x + static_cast<int64_t>(t.group) * pitch), 0, -1, 0x00020000);
-  const int q = wave % QS, su = min(q * 4 + (lane >> 4), U - 1);
-  const int code_off = lane * 16, scale_off = su * pitch + kMxScales + (lane & 15) * 16;
+  // a K tile of token rows: wavefront w takes fragment w of every row group and a copy of all their scales
+  const int code_off = lane * 16, scale_off = min(lane >> 4, U - 1) * pitch + kMxScales + (lane & 15) * 16;
   f32x16 acc[U][2];
 #pragma unroll
   for (int u = 0; u < U; ++u)
@@ -125,47 +118,49 @@ __device__ __forceinline__ void mx_tile_lds(const MxArgs& a, const MxTile& t, in
     for (int j = 0; j < 2; ++j)
 #pragma unroll
       for (int r = 0; r < 16; ++r) acc[u][j][r] = 0.f;
-  mx_frag wf[2][4], xf[2][U];
-  int ws[2][2], xs[2][U];  // of K tile k in half k & 1
-  auto load_x = [&](int k) {  // K tile k into slot k & 1
+  mx_frag wf[2][2][4], xf[U];  // weights of K tile k in half k & 1
+  int ws[2][2], xs[2][U];
+  auto load_x1 = [&](int k, int u) {  // u == U: the scales
     const int kc = min(k, last);
-    unsigned char* slot = lds + (k & 1) * SLOT;
+    unsigned char* slot = lds + (k & (kMxSlots - 1)) * SLOT;
+    if (u < U) __builtin_amdgcn_raw_ptr_buffer_load_lds(xr, (lptr_t)(slot + u * 4096 + wave * 1024), 16, code_off, u * pitch + kc * kMxUnit + wave * 1024, 0, 0);
+    else __builtin_amdgcn_raw_ptr_buffer_load_lds(xr, (lptr_t)(slot + U * 4096), 16, scale_off, kc * kMxUnit, 0, 0);
+    __builtin_amdgcn_sched_barrier(0);
+  };
+  auto load_x = [&](int k) {
 #pragma unroll
-    for (int u = 0; u < U; ++u)
-      __builtin_amdgcn_raw_ptr_buffer_load_lds(xr, (lptr_t)(slot + u * 4096 + wave * 1024), 16, code_off, u * pitch + kc * kMxUnit + wave * 1024, 0, 0);
-    __builtin_amdgcn_raw_ptr_buffer_load_lds(xr, (lptr_t)(slot + U * 4096 + q * 1024), 16, scale_off, kc * kMxUnit, 0, 0);
+    for (int u = 0; u <= U; ++u) load_x1(k, u);
   };
-  auto load_w = [&](int k, int s) {
+  const __amdgpu_buffer_rsrc_t r0 = __builtin_amdgcn_make_buffer_rsrc(const_cast<unsigned char*>(w0), 0, -1, 0x00020000);
+  const int d01 = (wg1 - wg) * pitch;
+  auto load_w1 = [&](int k, int s, int p, int j) {
     const int kc = min(k, last);
-    wf[0][s] = *reinterpret_cast<const mx_frag*>(w0 + kc * kMxUnit + s * 1024 + lane * 16);
-    wf[1][s] = *reinterpret_cast<const mx_frag*>(w1 + kc * kMxUnit + s * 1024 + lane * 16);
+    wf[p][j][s] = __builtin_bit_cast(mx_frag, __builtin_amdgcn_raw_buffer_load_b128(r0, lane * 16 + s * 1024, (j ? d01 : 0) + kc * kMxUnit, 0));
   };
-  auto load_ws = [&](int k, int (&to)[2]) {
+  auto load_w = [&](int k, int s, int p) { load_w1(k, s, p, 0); load_w1(k, s, p, 1); };
+  auto load_ws = [&](int k, int p) {
     const int kc = min(k, last);
-    to[0] = *reinterpret_cast<const int*>(w0 + kc * kMxUnit + kMxScales + lane * 4);
-    to[1] = *reinterpret_cast<const int*>(w1 + kc * kMxUnit + kMxScales + lane * 4);
+    ws[p][0] = __builtin_amdgcn_raw_buffer_load_b32(r0, lane * 4 + kMxScales, kc * kMxUnit, 0);
+    ws[p][1] = __builtin_amdgcn_raw_buffer_load_b32(r0, lane * 4 + kMxScales, d01 + kc * kMxUnit, 0);
   };
   auto read_x = [&](int k, int s, int u) {
-    return *reinterpret_cast<const mx_frag*>(lds + (k & 1) * SLOT + u * 4096 + s * 1024 + lane * 16);
+    return *reinterpret_cast<const mx_frag*>(lds + (k & (kMxSlots - 1)) * SLOT + u * 4096 + s * 1024 + lane * 16);
   };
-  auto read_xs = [&](int k, int u) { return *reinterpret_cast<const int*>(lds + (k & 1) * SLOT + U * 4096 + u * 256 + lane * 4); };
+  auto read_xs = [&](int k, int u) { return *reinterpret_cast<const int*>(lds + (k & (kMxSlots - 1)) * SLOT + U * 4096 + u * 256 + lane * 4); };
   load_x(0);
-  for (int s = 0; s < 4; ++s) load_w(0, s);
-  load_ws(0, ws[0]);
-  asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
-  __builtin_amdgcn_s_barrier();
   load_x(1);
-  load_ws(1, ws[1]);
+  load_x(2);
+  load_ws(0, 0);
+#pragma unroll
+  for (int s = 0; s < 7; ++s) load_w(s >> 2, s & 3, s >> 2);
+  __builtin_amdgcn_sched_barrier(0);
+  // K tile 0 of the token rows has landed: 2 (U + 1) + 16 loads are newer
+  asm volatile("s_waitcnt vmcnt(%0)" ::"n"(2 * (U + 1) + 14) : "memory");
+  __builtin_amdgcn_s_barrier();
 #pragma unroll
   for (int u = 0; u < U; ++u) {
-    xf[0][u] = read_x(0, 0, u);
+    xf[u] = read_x(0, 0, u);
     xs[0][u] = read_xs(0, u);
-  }
-  if constexpr (U > 4) {
-#pragma unroll
-    for (int u = 0; u < U; ++u)
-#pragma unroll
-      for (int j = 0; j < 2; ++j) asm volatile("s_nop 3" : "+a"(acc[u][j]));
   }
   for (int k0 = 0; k0 <= last; k0 += 2) {
 #pragma unroll
@@ -175,36 +170,40 @@ __device__ __forceinline__ void mx_tile_lds(const MxArgs& a, const MxTile& t, in
         mx_each<0, 4>([&](auto S) {
           constexpr int s = decltype(S)::value;
           if constexpr (s == 3) {
-            // the next K tile has landed (the loads issued behind it are ten, the six newest this K tile's) and this one's
-            // has been read, by everybody behind the barrier
-            asm volatile("s_waitcnt vmcnt(6) lgkmcnt(0)" ::: "memory");
+            // K tile k + 1 of the token rows has landed, everybody's loads of it behind the barrier (this wavefront has issued U + 1 of
+            // k + 2 and 18 of weights since); and slot (k + 3) & 3, that of k - 1, has been read by everybody.
+            asm volatile("s_waitcnt vmcnt(%0)" ::"n"(U + 1 + 14) : "memory");
             __builtin_amdgcn_s_barrier();
-            load_x(k + 2);
-            __builtin_amdgcn_sched_barrier(0);
           }
 #pragma unroll
           for (int u = 0; u < U; ++u) {
 #pragma unroll
-            for (int j = 0; j < 2; ++j) {
-              if constexpr (U > 4) mx_mfma_held<s>(wf[j][s], ws[p][j], xf[s & 1][u], xs[p][u], acc[u][j]);
-              else acc[u][j] = mx_mfma<s>(wf[j][s], ws[p][j], xf[s & 1][u], xs[p][u], acc[u][j]);
-            }
-            if constexpr (s < 3) xf[(s + 1) & 1][u] = read_x(k, s + 1, u);
+            for (int j = 0; j < 2; ++j) acc[u][j] = mx_mfma<s>(wf[p][j][s], ws[p][j], xf[u], xs[p][u], acc[u][j]);
+            __builtin_amdgcn_sched_barrier(0);
+            if constexpr (s < 3) xf[u] = read_x(k, s + 1, u);
             else {
-              xf[0][u] = read_x(k + 1, 0, u);
+              xf[u] = read_x(k + 1, 0, u);
               xs[p ^ 1][u] = read_xs(k + 1, u);
+              load_x1(k + 3, u);
+            }
+            // weights of the step before: its fragments are free
+            if constexpr (s > 0) {
+              if (u < 2) load_w1(k + 2, s - 1, p, u);
+            } else {
+              if (u < 2) {
+                load_w1(k + 1, 3, p ^ 1, u);
+                if (u == 1) load_ws(k + 1, p ^ 1);
+              }
             }
             __builtin_amdgcn_sched_barrier(0);
           }
-          load_w(k + 1, s);
-          if constexpr (s == 3) load_ws(k + 2, ws[p]);
+          if constexpr (s == 3) load_x1(k + 3, U);
           __builtin_amdgcn_sched_barrier(0);
         });
       }
     }
   }
-  asm volatile("s_waitcnt vmcnt(0)\n\ts_nop 15\n\ts_nop 15" ::: "memory");  // no load of this workgroup's is under way to LDS; the last MFMAs are done
-  __builtin_amdgcn_sched_barrier(0);
+  asm volatile("s_waitcnt vmcnt(0)" ::: "memory");  // no load of this workgroup's is under way to LDS
   mx_epilogue<T, EPI, U>(a, t, f, wave, lane, acc);
 #endif
 }
@@ -212,7 +211,6 @@ __device__ __forceinline__ void mx_tile_lds(const MxArgs& a, const MxTile& t, in
 // acc[u][j]: the lane's 16 consecutive features of token row `lane % 32` of row group u.
 template <typename T, int EPI, int U>
 __device__ __forceinline__ void mx_epilogue(const MxArgs& a, const MxTile& t, int f, int wave, int lane, f32x16 (&acc)[U][2]) {
-  constexpr bool HELD = U > 4;
   const int wg = (f * 4 + wave) * 2, col = lane & 31, half = lane >> 5;
   if constexpr (EPI == MX_SILU) {
     const int blk = f * 4 + wave;  // of 32 activated features; the operand's last K tile is filled up with zeros
@@ -220,7 +218,7 @@ __device__ __forceinline__ void mx_epilogue(const MxArgs& a, const MxTile& t, in
     unsigned char* unit = a.act + (static_cast<int64_t>(t.group) * a.act_tiles + (blk >> 3)) * kMxUnit;
 #pragma unroll
     for (int u = 0; u < U; ++u) {
-      const f32x16 g = mx_fetch<HELD>(acc[u][0]), up = mx_fetch<HELD>(acc[u][1]);
+      const f32x16 g = acc[u][0], up = acc[u][1];
       float v[16];
       unsigned amax = 0;
 #pragma unroll
@@ -234,7 +232,6 @@ __device__ __forceinline__ void mx_epilogue(const MxArgs& a, const MxTile& t, in
       *reinterpret_cast<uint2*>(unit + mx_code_at(col, blk & 7) + half * 8) = o;
       if (half == 0) unit[mx_scale_at(col, blk & 7)] = static_cast<unsigned char>(byte);
       unit += static_cast<int64_t>(a.act_tiles) * kMxUnit;
-      if (HELD) __builtin_amdgcn_sched_barrier(0);
     }
   } else {
 #pragma unroll
@@ -244,22 +241,53 @@ __device__ __forceinline__ void mx_epilogue(const MxArgs& a, const MxTile& t, in
         const int pair = a.sorted[slot];
         const bool live = pair < a.n_pairs;
         const float s = live ? a.topk_w[pair] : 0.f;
+        if (live && wg < a.w_groups) {
+          unsigned bytes[2];
 #pragma unroll
-        for (int j = 0; j < 2; ++j) {
-          const f32x16 v = mx_fetch<HELD>(acc[u][j]);
-          const int c = (wg + j) * 32 + half * 16;  // N is a multiple of 32
-          if (live && c < a.N) {
-            float* row = a.rows + static_cast<int64_t>(pair) * a.N + c;
+          for (int j = 0; j < 2; ++j) {
+            float v[16];
+            unsigned amax = 0;
 #pragma unroll
-            for (int r = 0; r < 16; r += 4) *reinterpret_cast<f32x4*>(row + r) = f32x4{v[r] * s, v[r + 1] * s, v[r + 2] * s, v[r + 3] * s};
+            for (int r = 0; r < 16; ++r) {
+              v[r] = acc[u][j][r] * s;
+              const unsigned m = magnitude(v[r]);
+              amax = amax > m ? amax : m;
+            }
+            const bool odd = amax >= 0x7F800000u;
+            if (odd) {
+              amax = 0;
+#pragma unroll
+              for (int r = 0; r < 16; ++r) {
+                const unsigned m = magnitude(v[r]);
+                amax = m < 0x7F800000u && m > amax ? m : amax;
+              }
+            }
+            bytes[j] = mx_row_byte(amax);
+            const float factor = mx_row_factor(bytes[j]);
+            unsigned q[16];
+#pragma unroll
+            for (int r = 0; r < 16; ++r) q[r] = __float_as_uint(__builtin_fmaf(v[r], factor, kMxRowMagic));
+            if (odd) {
+#pragma unroll
+              for (int r = 0; r < 16; ++r)
+                if (magnitude(v[r]) >= 0x7F800000u) q[r] = v[r] != v[r] ? 0x8000u : v[r] > 0.f ? 0x7FFFu : 0x8001u;
+            }
+            if (wg + j < a.w_groups) {
+              uint4* row = a.rows + (static_cast<int64_t>(pair) * a.N + (wg + j) * 32 + half * 16) / 8;
+#pragma unroll
+              for (int r = 0; r < 16; r += 8)
+                row[r / 8] = uint4{__builtin_amdgcn_perm(q[r + 1], q[r], 0x05040100u), __builtin_amdgcn_perm(q[r + 3], q[r + 2], 0x05040100u),
+                                   __builtin_amdgcn_perm(q[r + 5], q[r + 4], 0x05040100u), __builtin_amdgcn_perm(q[r + 7], q[r + 6], 0x05040100u)};
+            }
           }
-          if (HELD) __builtin_amdgcn_sched_barrier(0);
+          *reinterpret_cast<unsigned short*>(a.row_exps + static_cast<int64_t>(pair) * a.exp_pitch + wg * 2 + half * 2) =
+              static_cast<unsigned short>(bytes[0] | bytes[1] << 8);
         }
       } else {
         typedef T vec8 __attribute__((ext_vector_type(8)));
 #pragma unroll
         for (int j = 0; j < 2; ++j) {
-          const f32x16 v = mx_fetch<HELD>(acc[u][j]);
+          const f32x16 v = acc[u][j];
           const int c = (wg + j) * 32 + half * 16;
           vec8 o[2];
 #pragma unroll
@@ -275,7 +303,6 @@ __device__ __forceinline__ void mx_epilogue(const MxArgs& a, const MxTile& t, in
                 if (c + r < a.N) row[r] = o[r >> 3][r & 7];
             }
           }
-          if (HELD) __builtin_amdgcn_sched_barrier(0);
         }
       }
     }
@@ -284,7 +311,7 @@ __device__ __forceinline__ void mx_epilogue(const MxArgs& a, const MxTile& t, in
 
 // MOST: row groups of a tile, at most.
 template <typename T, int EPI, int MOST>
-__global__ __launch_bounds__(kMxThreads, MOST == 8 ? 1 : 2) void mx_gemm_kernel(MxArgs a) {
+__global__ __launch_bounds__(kMxThreads, 2) void mx_gemm_kernel(MxArgs a) {
   extern __shared__ __attribute__((aligned(16))) unsigned char mx_lds[];
   // workgroups b, b + 8, .. share an XCD and its L2: an XCD takes a consecutive part of the walk
   const int tiles = EPI == MX_LINEAR ? (a.x_groups + MOST - 1) / MOST : a.tile_count[0];
@@ -304,12 +331,6 @@ __global__ __launch_bounds__(kMxThreads, MOST == 8 ? 1 : 2) void mx_gemm_kernel(
   const int q = lin - t0 * a.f_tiles, f = q / n, index = t0 + q - f * n;
   if constexpr (EPI == MX_LINEAR) t = MxTile{index * MOST, min(MOST, a.x_groups - index * MOST), 0, 0, 0};
   else t = a.tiles[index];
-  if constexpr (MOST >= 8) {
-    if (t.units == 8) return mx_tile_lds<T, EPI, 8>(a, t, f, mx_lds);
-    if (t.units == 7) return mx_tile_lds<T, EPI, 7>(a, t, f, mx_lds);
-    if (t.units == 6) return mx_tile_lds<T, EPI, 6>(a, t, f, mx_lds);
-    if (t.units == 5) return mx_tile_lds<T, EPI, 5>(a, t, f, mx_lds);
-  }
   if constexpr (MOST >= 4) {
     if (t.units == 4) return mx_tile_lds<T, EPI, 4>(a, t, f, mx_lds);
     if (t.units == 3) return mx_tile_lds<T, EPI, 3>(a, t, f, mx_lds);
@@ -320,7 +341,7 @@ __global__ __launch_bounds__(kMxThreads, MOST == 8 ? 1 : 2) void mx_gemm_kernel(
   mx_tile<T, EPI, 1>(a, t, f);
 }
 
-constexpr int mx_lds_bytes(int most) { return 2 * (most * 4096 + (most + 3) / 4 * 1024); }
+constexpr int mx_lds_bytes(int most) { return kMxSlots * (most * 4096 + 1024); }
 
 // More than 64 KB of LDS needs the kernel's limit raised, once per device (a set-up call, not stream work).
 template <typename T, int EPI, int MOST>
@@ -347,13 +368,12 @@ int launch_mx_gemm(const MxArgs& a, int most, int64_t tiles, hipStream_t st) {
   FR_REQUIRE(wgs < (int64_t(1) << 31), FR_E_SHAPE, "mxfp4 product: %lld workgroups", (long long)wgs);
   const dim3 grid(static_cast<unsigned>(wgs)), block(kMxThreads);
   switch (most) {
-    case 8: {
-      const int rc = mx_allow_lds<T, EPI, 8>();
+    case 4: {
+      const int rc = mx_allow_lds<T, EPI, 4>();
       if (rc != FR_OK) return rc;
-      hipLaunchKernelGGL((mx_gemm_kernel<T, EPI, 8>), grid, block, mx_lds_bytes(8), st, a);
+      hipLaunchKernelGGL((mx_gemm_kernel<T, EPI, 4>), grid, block, mx_lds_bytes(4), st, a);
       break;
     }
-    case 4: hipLaunchKernelGGL((mx_gemm_kernel<T, EPI, 4>), grid, block, mx_lds_bytes(4), st, a); break;
     case 2: hipLaunchKernelGGL((mx_gemm_kernel<T, EPI, 2>), grid, block, 0, st, a); break;
     default: hipLaunchKernelGGL((mx_gemm_kernel<T, EPI, 1>), grid, block, 0, st, a); break;
   }
@@ -361,34 +381,35 @@ int launch_mx_gemm(const MxArgs& a, int most, int64_t tiles, hipStream_t st) {
 }
 
 // Row groups per tile, at most, for `rows` token rows per weight matrix on average.
-int most_units(int64_t rows) { return rows > 128 ? 8 : rows > 64 ? 4 : rows > 32 ? 2 : 1; }
+int most_units(int64_t rows) { return rows > 64 ? 4 : rows > 32 ? 2 : 1; }
 
 // out[m, :] = sum over the token's pairs, in order, of their weighted rows; a pair without an expert (a token row of NaN
 // logits) has no row.
 template <typename T>
-__global__ __launch_bounds__(kMxThreads) void mx_combine_kernel(const float* __restrict__ rows, const int32_t* __restrict__ ids, int E, int topk,
-                                                                int64_t M, int H, T* __restrict__ out) {
+__global__ __launch_bounds__(kMxThreads) void mx_combine_kernel(const uint4* __restrict__ rows, const unsigned char* __restrict__ exps, int exp_pitch,
+                                                                const int32_t* __restrict__ ids, int E, int topk, int64_t M, int H,
+                                                                T* __restrict__ out) {
   typedef T vec8 __attribute__((ext_vector_type(8)));
   const int per = H / 8;
   const int64_t i = static_cast<int64_t>(blockIdx.x) * kMxThreads + threadIdx.x;
   if (i >= M * per) return;
   const int64_t m = i / per;
-  const int c = static_cast<int>(i - m * per) * 8;
+  const int c = static_cast<int>(i - m * per), b = c >> 1;
+  const int at = (b & ~3) | (b & 1) << 1 | (b >> 1 & 1);
   float s[8] = {};
   for (int j = 0; j < topk; ++j) {
     const int64_t p = m * topk + j;
     if (static_cast<unsigned>(ids[p]) >= static_cast<unsigned>(E)) continue;
-    const f32x4 lo = *reinterpret_cast<const f32x4*>(rows + p * H + c), hi = *reinterpret_cast<const f32x4*>(rows + p * H + c + 4);
+    const uint4 q = rows[p * per + c];
+    const float step = mx_row_step(exps[p * exp_pitch + at]);
+    const unsigned w[4] = {q.x, q.y, q.z, q.w};
 #pragma unroll
-    for (int r = 0; r < 4; ++r) {
-      s[r] += lo[r];
-      s[4 + r] += hi[r];
-    }
+    for (int r = 0; r < 8; ++r) s[r] += mx_row_value(static_cast<short>(w[r >> 1] >> (16 * (r & 1))), step);
   }
   vec8 o;
 #pragma unroll
   for (int r = 0; r < 8; ++r) o[r] = static_cast<T>(s[r]);
-  *reinterpret_cast<vec8*>(out + m * H + c) = o;
+  *reinterpret_cast<vec8*>(out + i * 8) = o;
 }
 
 // ---- workspaces ------------------------------------------------------------------------------------------------
@@ -412,7 +433,9 @@ struct MxLayer {
   int* tile_count;
   MxTile* tiles;
   unsigned char *x, *act;
-  float* rows;
+  uint4* rows;
+  unsigned char* row_exps;
+  int exp_pitch;
 };
 
 MxLayer mx_layer(void* ws, int64_t M, int64_t H, int64_t F, int E, int topk) {
@@ -435,7 +458,9 @@ MxLayer mx_layer(void* ws, int64_t M, int64_t H, int64_t F, int E, int topk) {
   l.tiles = b.take<MxTile>(l.tile_limit);
   l.x = b.take<unsigned char>(l.groups * mx_tiles(H) * kMxUnit);
   l.act = b.take<unsigned char>(l.groups * mx_tiles(F) * kMxUnit);
-  l.rows = b.take<float>(n * H);
+  l.rows = b.take<uint4>(n * H / 8);
+  l.exp_pitch = static_cast<int>(ceil_div(H, 2 * kMxRows)) * 4;
+  l.row_exps = b.take<unsigned char>(n * l.exp_pitch);
   l.bytes = b.at;
   return l;
 }
@@ -561,13 +586,15 @@ extern "C" int fr_fused_moe_mxfp4(const void* x, int dtype, const void* w1_tiled
   a.w_stride = static_cast<int64_t>(a.w_groups) * a.k_tiles * kMxUnit;
   a.f_tiles = static_cast<int>(ceil_div(static_cast<int64_t>(a.w_groups), int64_t(8)));
   a.rows = l.rows;
+  a.row_exps = l.row_exps;
+  a.exp_pitch = l.exp_pitch;
   a.N = static_cast<int>(H);
   rc = launch_mx_gemm<bf16_t, MX_DOWN>(a, l.most, l.tile_limit, st);
   if (rc != FR_OK) return rc;
   const dim3 grid(static_cast<unsigned>(ceil_div(M * (H / 8), int64_t(kMxThreads))));
   if (dtype == FR_BF16)
-    hipLaunchKernelGGL((mx_combine_kernel<bf16_t>), grid, dim3(kMxThreads), 0, st, l.rows, l.topk_ids, E, topk, M, (int)H, static_cast<bf16_t*>(out));
+    hipLaunchKernelGGL((mx_combine_kernel<bf16_t>), grid, dim3(kMxThreads), 0, st, l.rows, l.row_exps, l.exp_pitch, l.topk_ids, E, topk, M, (int)H, static_cast<bf16_t*>(out));
   else
-    hipLaunchKernelGGL((mx_combine_kernel<f16_t>), grid, dim3(kMxThreads), 0, st, l.rows, l.topk_ids, E, topk, M, (int)H, static_cast<f16_t*>(out));
+    hipLaunchKernelGGL((mx_combine_kernel<f16_t>), grid, dim3(kMxThreads), 0, st, l.rows, l.row_exps, l.exp_pitch, l.topk_ids, E, topk, M, (int)H, static_cast<f16_t*>(out));
   return check_launch("mx_combine_kernel");
 }
