@@ -4,7 +4,7 @@
 //
 // A workgroup of four wavefronts computes a token tile of up to kMxMaxUnits row groups (32 rows each) x 256 weight rows: a
 // wavefront holds two units of weight rows against all token rows.
-#include "mxfp4_core.h"
+#include "mxfp4_few.h"
 
 namespace fr {
 namespace {
@@ -39,8 +39,6 @@ struct MxArgs {
   int64_t M;
   int N;               // columns of rows / out
 };
-
-__device__ __forceinline__ float mx_silu_mul(float g, float u) { return g / (1.f + __expf(-g)) * u; }
 
 template <typename T, int EPI, int U>
 __device__ __forceinline__ void mx_epilogue(const MxArgs& a, const MxTile& t, int f, int wave, int lane, f32x16 (&acc)[U][2]);
@@ -413,17 +411,6 @@ __global__ __launch_bounds__(kMxThreads) void mx_combine_kernel(const uint4* __r
 }
 
 // ---- workspaces ------------------------------------------------------------------------------------------------
-struct Bump {
-  unsigned char* base;
-  int64_t at = 0;
-  template <typename T>
-  T* take(int64_t count) {
-    T* p = reinterpret_cast<T*>(base + at);
-    at = round_up(at + count * static_cast<int64_t>(sizeof(T)), 256);
-    return p;
-  }
-};
-
 struct MxLayer {
   float* topk_w;
   int32_t *topk_ids, *sorted, *expert_ids, *npost;
@@ -440,7 +427,7 @@ struct MxLayer {
 
 MxLayer mx_layer(void* ws, int64_t M, int64_t H, int64_t F, int E, int topk) {
   MxLayer l;
-  Bump b{static_cast<unsigned char*>(ws)};
+  MxBump b{static_cast<unsigned char*>(ws)};
   const int64_t n = M * topk;
   l.most = most_units(ceil_div(n, static_cast<int64_t>(E)));
   // groups of 32 slots: each holds a pair, and every expert fills up one at most
@@ -521,7 +508,8 @@ extern "C" int fr_linear_mxfp4(const void* x, int dtype, int64_t M, int64_t K, i
 extern "C" int64_t fr_moe_mxfp4_workspace_bytes(int64_t M, int64_t H, int64_t F, int E, int topk) {
   using namespace fr;
   if (check_mx_layer("fr_moe_mxfp4_workspace_bytes", M, H, F, E, topk) != FR_OK) return -1;
-  return mx_layer(nullptr, M, H, F, E, topk).bytes;
+  MxFewScratch few;
+  return mx_few_fits(M, topk) ? mx_few_workspace(nullptr, M, H, F, E, topk, &few) : mx_layer(nullptr, M, H, F, E, topk).bytes;
 }
 
 extern "C" int fr_fused_moe_mxfp4(const void* x, int dtype, const void* w1_tiled, const void* w2_tiled, const void* logits, int logits_dtype,
@@ -536,9 +524,12 @@ extern "C" int fr_fused_moe_mxfp4(const void* x, int dtype, const void* w1_tiled
   if (M == 0) return FR_OK;
   FR_REQUIRE(x && w1_tiled && w2_tiled && logits && out, FR_E_NULL, "fr_fused_moe_mxfp4: null pointer");
   FR_REQUIRE(aligned16(x) && aligned16(w1_tiled) && aligned16(w2_tiled) && aligned16(out), FR_E_ALIGN, "fr_fused_moe_mxfp4: 16-byte alignment");
-  const MxLayer l = mx_layer(workspace, M, H, F, E, topk);
-  FR_REQUIRE(workspace && workspace_bytes >= l.bytes, FR_E_WORKSPACE, "fr_fused_moe_mxfp4: workspace %lld < %lld bytes", (long long)workspace_bytes, (long long)l.bytes);
+  const int64_t need = fr_moe_mxfp4_workspace_bytes(M, H, F, E, topk);
+  FR_REQUIRE(workspace && workspace_bytes >= need, FR_E_WORKSPACE, "fr_fused_moe_mxfp4: workspace %lld < %lld bytes", (long long)workspace_bytes, (long long)need);
   FR_REQUIRE((reinterpret_cast<uintptr_t>(workspace) & 255u) == 0, FR_E_ALIGN, "fr_fused_moe_mxfp4: workspace must be 256-byte aligned");
+  if (mx_few_fits(M, topk))
+    return mx_few_layer(x, dtype, w1_tiled, w2_tiled, logits, logits_dtype, M, H, F, E, topk, renormalize, out, workspace, static_cast<hipStream_t>(stream));
+  const MxLayer l = mx_layer(workspace, M, H, F, E, topk);
   hipStream_t st = static_cast<hipStream_t>(stream);
   const int64_t n = M * topk;
   if (route_align_fits(M, E, topk, false)) {
