@@ -143,6 +143,24 @@ __device__ __forceinline__ int few_hit(const FewHits& hits, int index) {
   return 0;
 }
 
+// A lane's four fragments of K tile k of token row col and their scales.  Rows that the workgroup quantised for itself lie in LDS a tile at
+// a time, block after block, the scales behind.
+constexpr int kFewRow = 144;  // bytes of a token's K tile in LDS: 128 of codes, 8 of scales, 8 that spread the banks
+template <bool OWN>
+__device__ __forceinline__ int few_token_rows(const unsigned char* rows, int tiles, int k, int col, int half, mx_frag (&xf)[4]) {
+  if constexpr (OWN) {
+    const unsigned char* row = rows + (col * tiles + k) * kFewRow;
+#pragma unroll
+    for (int s = 0; s < 4; ++s) xf[s] = *reinterpret_cast<const mx_frag*>(row + half * 64 + s * 16);
+    return *reinterpret_cast<const int*>(row + 128 + half * 4);
+  } else {
+    const unsigned char* u = rows + static_cast<int64_t>(k) * kMxUnit;
+#pragma unroll
+    for (int s = 0; s < 4; ++s) xf[s] = *reinterpret_cast<const mx_frag*>(u + s * 1024 + (col + 32 * half) * 16);
+    return *reinterpret_cast<const int*>(u + kMxScales + (col + 32 * half) * 4);
+  }
+}
+
 constexpr int kGateupRing = 3;  // K tiles of weights on their way to a wavefront's registers
 template <typename T, bool ROUTE>
 __global__ __launch_bounds__(kFewThreads) void mx_few_gateup_kernel(MxFew a) {
@@ -204,8 +222,6 @@ __global__ __launch_bounds__(kFewThreads) void mx_few_gateup_kernel(MxFew a) {
 #pragma unroll
   for (int p = 0; p < kGateupRing; ++p)
     if (k0 + p < k1) load_w(k0 + p, p);
-  // token rows: fragment s of token m at [m][tile][half][s], the block's scales as a dword behind the four
-  constexpr int kRow = 144;  // bytes of a token's K tile in LDS: 128 of codes, 8 of scales, 8 that spread the banks
   if constexpr (ROUTE) {
     __syncthreads();
     const unsigned mine = tokens_of;
@@ -216,14 +232,13 @@ __global__ __launch_bounds__(kFewThreads) void mx_few_gateup_kernel(MxFew a) {
         const int t = c >> 5, b = (c & 31) >> 2;
         unsigned byte;
         const unsigned o = few_quant8<T>(static_cast<const T*>(a.x) + static_cast<int64_t>(m) * a.H + c * 8, c * 8 < a.H, &byte);
-        unsigned char* row = few_lds + (m * a.h_tiles + t) * kRow;
+        unsigned char* row = few_lds + (m * a.h_tiles + t) * kFewRow;
         *reinterpret_cast<unsigned*>(row + b * 16 + (c & 3) * 4) = o;
         if ((c & 3) == 0) row[128 + b] = static_cast<unsigned char>(byte);
       }
     }
     __syncthreads();
   }
-  const unsigned char* const xq = a.xq + (col + 32 * half) * 16;
   f32x16 acc[2];
 #pragma unroll
   for (int j = 0; j < 2; ++j)
@@ -235,18 +250,7 @@ __global__ __launch_bounds__(kFewThreads) void mx_few_gateup_kernel(MxFew a) {
       const int k = kk + p;
       if (k < k1) {
         mx_frag xf[4];
-        int xs;
-        if constexpr (ROUTE) {
-          const unsigned char* row = few_lds + (col * a.h_tiles + k) * kRow;
-#pragma unroll
-          for (int s = 0; s < 4; ++s) xf[s] = *reinterpret_cast<const mx_frag*>(row + half * 64 + s * 16);
-          xs = *reinterpret_cast<const int*>(row + 128 + half * 4);
-        } else {
-          const unsigned char* u = xq + k * kMxUnit;
-#pragma unroll
-          for (int s = 0; s < 4; ++s) xf[s] = *reinterpret_cast<const mx_frag*>(u + s * 1024);
-          xs = *reinterpret_cast<const int*>(a.xq + k * kMxUnit + kMxScales + (col + 32 * half) * 4);
-        }
+        const int xs = few_token_rows<ROUTE>(ROUTE ? few_lds : a.xq, a.h_tiles, k, col, half, xf);
         mx_each<0, 4>([&](auto S) {
           constexpr int s = decltype(S)::value;
           acc[0] = mx_mfma<s>(wf[p][0][s], ws[p][0], xf[s], xs, acc[0]);
@@ -410,6 +414,82 @@ __global__ __launch_bounds__(kDownThreads) void mx_few_down_kernel(MxFew a) {
 #endif
 }
 
+constexpr int kLinearRing = 4;
+// The product of a matrix with up to 32 token rows: a workgroup per 32 output features, K cut over its eight wavefronts.
+// OWN: the workgroup quantises the rows into LDS itself, else xq is the operand.
+struct MxFewLinear {
+  const void* x;
+  int64_t ldx;
+  const unsigned char *xq, *w;
+  int M, K, k_tiles;
+  int64_t N;
+  void* out;
+};
+template <typename T, bool OWN>
+__global__ __launch_bounds__(kDownThreads) void mx_few_linear_kernel(MxFewLinear a) {
+#if defined(__HIP_DEVICE_COMPILE__)
+  extern __shared__ __attribute__((aligned(16))) unsigned char few_lds[];
+  const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+  const int64_t unit = blockIdx.x;
+  const int col = min(lane & 31, a.M - 1), half = lane >> 5;
+  const int k0 = wave * a.k_tiles / kDownWaves, k1 = (wave + 1) * a.k_tiles / kDownWaves;
+  const __amdgpu_buffer_rsrc_t wr =
+      __builtin_amdgcn_make_buffer_rsrc(const_cast<unsigned char*>(a.w + unit * a.k_tiles * kMxUnit), 0, -1, 0x00020000);
+  mx_frag wf[kLinearRing][4];
+  int ws[kLinearRing];
+  auto load_w = [&](int k, int p) {
+#pragma unroll
+    for (int s = 0; s < 4; ++s) wf[p][s] = __builtin_bit_cast(mx_frag, __builtin_amdgcn_raw_buffer_load_b128(wr, lane * 16 + s * 1024, k * kMxUnit, 2));
+    ws[p] = __builtin_amdgcn_raw_buffer_load_b32(wr, lane * 4 + kMxScales, k * kMxUnit, 2);
+  };
+#pragma unroll
+  for (int p = 0; p < kLinearRing; ++p)
+    if (k0 + p < k1) load_w(k0 + p, p);
+  if constexpr (OWN) {
+    const int per = a.k_tiles * 32, chunks = a.M * per;
+    for (int c = tid; c < chunks; c += kDownThreads) {
+      const int m = c / per, i = c - m * per, b = (i & 31) >> 2;
+      unsigned byte;
+      const unsigned o = few_quant8<T>(static_cast<const T*>(a.x) + m * a.ldx + i * 8, i * 8 < a.K, &byte);
+      unsigned char* row = few_lds + (m * a.k_tiles + (i >> 5)) * kFewRow;
+      *reinterpret_cast<unsigned*>(row + b * 16 + (i & 3) * 4) = o;
+      if ((i & 3) == 0) row[128 + b] = static_cast<unsigned char>(byte);
+    }
+    __syncthreads();
+  }
+  f32x16 acc;
+#pragma unroll
+  for (int r = 0; r < 16; ++r) acc[r] = 0.f;
+  for (int kk = k0; kk < k1; kk += kLinearRing) {
+#pragma unroll
+    for (int p = 0; p < kLinearRing; ++p) {
+      const int k = kk + p;
+      if (k < k1) {
+        mx_frag xf[4];
+        const int xs = few_token_rows<OWN>(OWN ? few_lds : a.xq, a.k_tiles, k, col, half, xf);
+        mx_each<0, 4>([&](auto S) {
+          constexpr int s = decltype(S)::value;
+          acc = mx_mfma<s>(wf[p][s], ws[p], xf[s], xs, acc);
+        });
+        if (k + kLinearRing < k1) load_w(k + kLinearRing, p);
+      }
+    }
+  }
+  float* const red = reinterpret_cast<float*>(few_lds);
+  __syncthreads();  // the token rows have been read
+#pragma unroll
+  for (int r = 0; r < 16; ++r) red[(wave * 64 + lane) * kDownLane + r] = acc[r];
+  __syncthreads();
+  for (int o = tid; o < a.M * 32; o += kDownThreads) {
+    const int m = o >> 5, f = o & 31;
+    float s = 0.f;
+#pragma unroll
+    for (int w = 0; w < kDownWaves; ++w) s += red[(w * 64 + m + 32 * (f >> 4)) * kDownLane + (f & 15)];
+    if (unit * 32 + f < a.N) static_cast<T*>(a.out)[m * a.N + unit * 32 + f] = static_cast<T>(s);
+  }
+#endif
+}
+
 // Parts a unit's K tiles are cut into: enough workgroups for the card.
 int few_splits(int64_t H) {
   const int64_t units = H / kMxRows, s = 256 / units;
@@ -419,8 +499,11 @@ int few_splits(int64_t H) {
 constexpr int kRouteLds = 64 * 1024;
 // Every gateup workgroup gates all tokens (one round of its wavefronts) and quantises its expert's rows.
 bool few_routes(int64_t M, int64_t H, int E) {
-  return M <= kFewWaves * few_gate_tokens(E) && M <= 8 && M * mx_tiles(H) * 144 <= kRouteLds;
+  return M <= kFewWaves * few_gate_tokens(E) && M <= 8 && M * mx_tiles(H) * kFewRow <= kRouteLds;
 }
+
+// Every workgroup of the linear product quantises the rows.
+bool few_quantises(int64_t M, int64_t K) { return M <= 8 && M * mx_tiles(K) * kFewRow <= kRouteLds; }
 
 }  // namespace
 
@@ -471,7 +554,7 @@ int mx_few_layer(const void* x, int dtype, const void* w1, const void* w2, const
   constexpr int kRedLds = (kFewWaves - 1) * 8 * 64 * 16;
   const dim3 up(static_cast<unsigned>(a.act_tiles * 8), static_cast<unsigned>(experts)), threads(kFewThreads);
   if (route) {
-    const int rows = static_cast<int>(M) * a.h_tiles * 144, lds = rows > kRedLds ? rows : kRedLds;
+    const int rows = static_cast<int>(M) * a.h_tiles * kFewRow, lds = rows > kRedLds ? rows : kRedLds;
     if (bf) hipLaunchKernelGGL((mx_few_gateup_kernel<bf16_t, true>), up, threads, lds, st, a);
     else hipLaunchKernelGGL((mx_few_gateup_kernel<f16_t, true>), up, threads, lds, st, a);
   } else {
@@ -489,6 +572,37 @@ int mx_few_layer(const void* x, int dtype, const void* w1, const void* w2, const
   if (bf) hipLaunchKernelGGL((mx_few_down_kernel<bf16_t>), down, dim3(kDownThreads), kDownLds, st, a);
   else hipLaunchKernelGGL((mx_few_down_kernel<f16_t>), down, dim3(kDownThreads), kDownLds, st, a);
   return check_launch("mx_few_down_kernel");
+}
+
+int64_t mx_few_linear_workspace(int64_t M, int64_t K) { return few_quantises(M, K) ? 0 : mx_tiles(K) * kMxUnit; }
+
+int mx_few_linear(const void* x, int dtype, int64_t M, int64_t K, int64_t ldx, const void* w, int64_t N, void* out, void* workspace,
+                  hipStream_t st) {
+  MxFewLinear a = {};
+  a.x = x;
+  a.ldx = ldx;
+  a.xq = static_cast<const unsigned char*>(workspace);
+  a.w = static_cast<const unsigned char*>(w);
+  a.M = static_cast<int>(M);
+  a.K = static_cast<int>(K);
+  a.k_tiles = static_cast<int>(mx_tiles(K));
+  a.N = N;
+  a.out = out;
+  const bool own = few_quantises(M, K);
+  if (!own) {
+    const int rc = mx_quant_tiled(x, dtype, M, K, ldx, 1, MxGather{}, workspace, st);
+    if (rc != FR_OK) return rc;
+  }
+  const int rows = own ? a.M * a.k_tiles * kFewRow : 0, lds = rows > kDownLds ? rows : kDownLds;
+  const dim3 grid(static_cast<unsigned>(mx_groups(N))), threads(kDownThreads);
+  if (dtype == FR_BF16) {
+    if (own) hipLaunchKernelGGL((mx_few_linear_kernel<bf16_t, true>), grid, threads, lds, st, a);
+    else hipLaunchKernelGGL((mx_few_linear_kernel<bf16_t, false>), grid, threads, lds, st, a);
+  } else {
+    if (own) hipLaunchKernelGGL((mx_few_linear_kernel<f16_t, true>), grid, threads, lds, st, a);
+    else hipLaunchKernelGGL((mx_few_linear_kernel<f16_t, false>), grid, threads, lds, st, a);
+  }
+  return check_launch("mx_few_linear_kernel");
 }
 
 }  // namespace fr

@@ -43,49 +43,6 @@ struct MxArgs {
 template <typename T, int EPI, int U>
 __device__ __forceinline__ void mx_epilogue(const MxArgs& a, const MxTile& t, int f, int wave, int lane, f32x16 (&acc)[U][2]);
 
-// Fragments from memory to registers.
-template <typename T, int EPI, int U>
-__device__ __forceinline__ void mx_tile(const MxArgs& a, const MxTile& t, int f) {
-  const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-  const int wg = (f * 4 + wave) * 2;  // first of the wavefront's two weight row groups
-  f32x16 acc[U][2];
-#pragma unroll
-  for (int u = 0; u < U; ++u)
-#pragma unroll
-    for (int j = 0; j < 2; ++j)
-#pragma unroll
-      for (int r = 0; r < 16; ++r) acc[u][j][r] = 0.f;
-  if (wg < a.w_groups) {
-    const int64_t pitch = static_cast<int64_t>(a.k_tiles) * kMxUnit;
-    const unsigned char* w0 = a.w + t.expert * a.w_stride + wg * pitch;
-    const unsigned char* w1 = w0 + (wg + 1 < a.w_groups ? pitch : 0);
-    const unsigned char* x0 = a.x + t.group * pitch;
-    for (int k = 0; k < a.k_tiles; ++k) {
-      mx_frag wf[2][4];
-      int ws[2];
-#pragma unroll
-      for (int s = 0; s < 4; ++s) {
-        wf[0][s] = *reinterpret_cast<const mx_frag*>(w0 + k * kMxUnit + s * 1024 + lane * 16);
-        wf[1][s] = *reinterpret_cast<const mx_frag*>(w1 + k * kMxUnit + s * 1024 + lane * 16);
-      }
-      ws[0] = *reinterpret_cast<const int*>(w0 + k * kMxUnit + kMxScales + lane * 4);
-      ws[1] = *reinterpret_cast<const int*>(w1 + k * kMxUnit + kMxScales + lane * 4);
-#pragma unroll
-      for (int u = 0; u < U; ++u) {
-        const unsigned char* xu = x0 + u * pitch + k * kMxUnit;
-        const int xs = *reinterpret_cast<const int*>(xu + kMxScales + lane * 4);
-        mx_each<0, 4>([&](auto S) {
-          constexpr int s = decltype(S)::value;
-          const mx_frag xf = *reinterpret_cast<const mx_frag*>(xu + s * 1024 + lane * 16);
-          acc[u][0] = mx_mfma<s>(wf[0][s], ws[0], xf, xs, acc[u][0]);
-          acc[u][1] = mx_mfma<s>(wf[1][s], ws[1], xf, xs, acc[u][1]);
-        });
-      }
-    }
-  }
-  mx_epilogue<T, EPI, U>(a, t, f, wave, lane, acc);
-}
-
 // Token rows through LDS (every wavefront reads all of them), weights from memory to registers (no other wavefront reads them).  A
 // ring of kMxSlots K tiles of token rows and two of weights are under way.  All loads are spread between the MFMAs, a row
 // group's two at a time: issued in one run per K tile they held up the MFMAs behind them (8 experts, H = 4096, F = 14336, 16384 tokens: gate/up
@@ -96,7 +53,7 @@ __device__ __forceinline__ void mx_tile(const MxArgs& a, const MxTile& t, int f)
 // part lowers its clock to 1.67 GHz for it); without any load, on data that is there, this loop reaches 5.1 to 5.5.
 constexpr int kMxSlots = 4;
 template <typename T, int EPI, int U>
-__device__ __forceinline__ void mx_tile_lds(const MxArgs& a, const MxTile& t, int f, unsigned char* lds) {
+__device__ __forceinline__ void mx_tile(const MxArgs& a, const MxTile& t, int f, unsigned char* lds) {
 #if defined(__HIP_DEVICE_COMPILE__)
   typedef __attribute__((address_space(3))) void* lptr_t;
   constexpr int SLOT = U * 4096 + 1024;
@@ -185,12 +142,13 @@ __device__ __forceinline__ void mx_tile_lds(const MxArgs& a, const MxTile& t, in
               load_x1(k + 3, u);
             }
             // weights of the step before: its fragments are free
-            if constexpr (s > 0) {
-              if (u < 2) load_w1(k + 2, s - 1, p, u);
-            } else {
-              if (u < 2) {
-                load_w1(k + 1, 3, p ^ 1, u);
-                if (u == 1) load_ws(k + 1, p ^ 1);
+#pragma unroll
+            for (int j = u; j < 2; j += U) {
+              if constexpr (s > 0) {
+                load_w1(k + 2, s - 1, p, j);
+              } else {
+                load_w1(k + 1, 3, p ^ 1, j);
+                if (j == 1) load_ws(k + 1, p ^ 1);
               }
             }
             __builtin_amdgcn_sched_barrier(0);
@@ -330,13 +288,13 @@ __global__ __launch_bounds__(kMxThreads, 2) void mx_gemm_kernel(MxArgs a) {
   if constexpr (EPI == MX_LINEAR) t = MxTile{index * MOST, min(MOST, a.x_groups - index * MOST), 0, 0, 0};
   else t = a.tiles[index];
   if constexpr (MOST >= 4) {
-    if (t.units == 4) return mx_tile_lds<T, EPI, 4>(a, t, f, mx_lds);
-    if (t.units == 3) return mx_tile_lds<T, EPI, 3>(a, t, f, mx_lds);
+    if (t.units == 4) return mx_tile<T, EPI, 4>(a, t, f, mx_lds);
+    if (t.units == 3) return mx_tile<T, EPI, 3>(a, t, f, mx_lds);
   }
   if constexpr (MOST >= 2) {
-    if (t.units == 2) return mx_tile<T, EPI, 2>(a, t, f);
+    if (t.units == 2) return mx_tile<T, EPI, 2>(a, t, f, mx_lds);
   }
-  mx_tile<T, EPI, 1>(a, t, f);
+  mx_tile<T, EPI, 1>(a, t, f, mx_lds);
 }
 
 constexpr int mx_lds_bytes(int most) { return kMxSlots * (most * 4096 + 1024); }
@@ -360,22 +318,24 @@ int mx_allow_lds() {
   return FR_OK;
 }
 
+template <typename T, int EPI, int MOST>
+int mx_launch(const MxArgs& a, dim3 grid, hipStream_t st) {
+  const int rc = mx_allow_lds<T, EPI, MOST>();
+  if (rc != FR_OK) return rc;
+  hipLaunchKernelGGL((mx_gemm_kernel<T, EPI, MOST>), grid, dim3(kMxThreads), mx_lds_bytes(MOST), st, a);
+  return check_launch("mx_gemm_kernel");
+}
+
 template <typename T, int EPI>
 int launch_mx_gemm(const MxArgs& a, int most, int64_t tiles, hipStream_t st) {
   const int64_t wgs = 8 * ceil_div(tiles * a.f_tiles, int64_t(8));
   FR_REQUIRE(wgs < (int64_t(1) << 31), FR_E_SHAPE, "mxfp4 product: %lld workgroups", (long long)wgs);
-  const dim3 grid(static_cast<unsigned>(wgs)), block(kMxThreads);
+  const dim3 grid(static_cast<unsigned>(wgs));
   switch (most) {
-    case 4: {
-      const int rc = mx_allow_lds<T, EPI, 4>();
-      if (rc != FR_OK) return rc;
-      hipLaunchKernelGGL((mx_gemm_kernel<T, EPI, 4>), grid, block, mx_lds_bytes(4), st, a);
-      break;
-    }
-    case 2: hipLaunchKernelGGL((mx_gemm_kernel<T, EPI, 2>), grid, block, 0, st, a); break;
-    default: hipLaunchKernelGGL((mx_gemm_kernel<T, EPI, 1>), grid, block, 0, st, a); break;
+    case 4: return mx_launch<T, EPI, 4>(a, grid, st);
+    case 2: return mx_launch<T, EPI, 2>(a, grid, st);
+    default: return mx_launch<T, EPI, 1>(a, grid, st);
   }
-  return check_launch("mx_gemm_kernel");
 }
 
 // Row groups per tile, at most, for `rows` token rows per weight matrix on average.
@@ -468,7 +428,7 @@ int check_mx_layer(const char* who, int64_t M, int64_t H, int64_t F, int E, int 
 extern "C" int64_t fr_linear_mxfp4_workspace_bytes(int64_t M, int64_t N, int64_t K) {
   using namespace fr;
   if (M < 0 || N < 1 || K < 0 || M > (int64_t(1) << 24) || N > (int64_t(1) << 24) || K > (int64_t(1) << 20)) return -1;
-  return mx_groups(M) * mx_tiles(K) * kMxUnit;
+  return M <= kFewTokens ? mx_few_linear_workspace(M, K) : mx_groups(M) * mx_tiles(K) * kMxUnit;
 }
 
 extern "C" int fr_linear_mxfp4(const void* x, int dtype, int64_t M, int64_t K, int64_t ldx, const void* w_tiled, int64_t N, void* out,
@@ -483,9 +443,10 @@ extern "C" int fr_linear_mxfp4(const void* x, int dtype, int64_t M, int64_t K, i
   FR_REQUIRE(ldx >= K && ldx % 8 == 0 && aligned16(x) && aligned16(w_tiled) && aligned16(out), FR_E_ALIGN,
              "fr_linear_mxfp4: 16-byte alignment, ldx %% 8 == 0, ldx >= K");
   const int64_t need = fr_linear_mxfp4_workspace_bytes(M, N, K);
-  FR_REQUIRE(workspace && workspace_bytes >= need, FR_E_WORKSPACE, "fr_linear_mxfp4: workspace %lld < %lld bytes", (long long)workspace_bytes, (long long)need);
+  FR_REQUIRE(need == 0 || (workspace && workspace_bytes >= need), FR_E_WORKSPACE, "fr_linear_mxfp4: workspace %lld < %lld bytes", (long long)workspace_bytes, (long long)need);
   FR_REQUIRE((reinterpret_cast<uintptr_t>(workspace) & 255u) == 0, FR_E_ALIGN, "fr_linear_mxfp4: workspace must be 256-byte aligned");
   hipStream_t st = static_cast<hipStream_t>(stream);
+  if (M <= kFewTokens) return mx_few_linear(x, dtype, M, K, ldx, w_tiled, N, out, workspace, st);
   const int64_t groups = mx_groups(M);
   int rc = mx_quant_tiled(x, dtype, M, K, ldx, groups, MxGather{}, workspace, st);
   if (rc != FR_OK) return rc;

@@ -126,13 +126,14 @@ def linear_mxfp4(x: torch.Tensor, weight: MXFP4Weight, workspace_buf: torch.Tens
     ws = _workspace(workspace_buf, need, x.device)
     with _on(x.device):
         N.check(N.lib().fr_linear_mxfp4(x.data_ptr(), N.dtype_code(x.dtype), M, K, _row_stride(x), weight.data.data_ptr(), weight.N,
-                                        out.data_ptr(), ws.data_ptr(), ws.numel(), N.stream_ptr(x.device)))
+                                        out.data_ptr(), 0 if ws is None else ws.data_ptr(), 0 if ws is None else ws.numel(),
+                                        N.stream_ptr(x.device)))
     return out
 
 
-def _workspace(buf: torch.Tensor | None, nbytes: int, device) -> torch.Tensor:
+def _workspace(buf: torch.Tensor | None, nbytes: int, device) -> torch.Tensor | None:
     if buf is None:
-        return torch.empty((max(nbytes, 256),), dtype=torch.uint8, device=device)
+        return torch.empty((nbytes,), dtype=torch.uint8, device=device) if nbytes else None
     assert buf.dtype == torch.uint8 and buf.is_contiguous() and buf.device == device, \
         "workspace_buf must be a contiguous uint8 tensor on the operands' device"
     return buf

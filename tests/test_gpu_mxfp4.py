@@ -325,7 +325,7 @@ def test_refusals(native):
         lambda: fr.dequantize_rows_mxfp4(codes, scales, dtype=torch.float64), lambda: fr.dequantize_rows_mxfp4(codes[:, ::2], scales),
         lambda: fr.prepare_linear_mxfp4(codes[:0], scales[:0]), lambda: fr.prepare_linear_mxfp4(w1, s1),
         lambda: fr.linear_mxfp4(x[:, :32], weight), lambda: fr.linear_mxfp4(x.float(), weight),
-        lambda: fr.linear_mxfp4(x, weight, workspace_buf=torch.empty(16, dtype=torch.uint8, device="cuda")),
+        lambda: fr.linear_mxfp4(x.repeat(5, 1), weight, workspace_buf=torch.empty(16, dtype=torch.uint8, device="cuda")),
         lambda: fr.linear_mxfp4(x, weight, workspace_buf=torch.empty(1 << 20, dtype=torch.uint8)),
         lambda: fr.prepare_weights_mxfp4(w1, s1, w2[:, :32], s2[:, :32]), lambda: fr.prepare_weights_mxfp4(w1[:, :96], s1[:, :96], w2, s2),
         lambda: fr.fused_moe_mxfp4(x, experts, logits, 2), lambda: fr.fused_moe_mxfp4(x, experts, logits, 0),

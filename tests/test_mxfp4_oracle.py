@@ -102,8 +102,8 @@ def test_c_entry_points_refuse(native):
     _refused(native, -3, m, P, N.FR_F32, 4, 64, 64, P, 8, P, P, big, None)
     _refused(native, -1, m, P, N.FR_BF16, 4, 64, 64, None, 8, P, P, big, None)
     _refused(native, -4, m, P, N.FR_BF16, 4, 64, 32, P, 8, P, P, big, None)
-    _refused(native, -5, m, P, N.FR_BF16, 4, 64, 64, P, 8, P, P, 128, None)
-    _refused(native, -5, m, P, N.FR_BF16, 4, 64, 64, P, 8, P, None, big, None)
+    _refused(native, -5, m, P, N.FR_BF16, 40, 64, 64, P, 8, P, P, 128, None)
+    _refused(native, -5, m, P, N.FR_BF16, 20, 64, 64, P, 8, P, None, big, None)
     assert native.fr_linear_mxfp4(None, N.FR_BF16, 0, 64, 64, None, 8, None, None, 0, None) == 0
     assert native.fr_linear_mxfp4_workspace_bytes(4, 0, 64) == -1
     f = "fr_fused_moe_mxfp4"
