@@ -32,7 +32,8 @@ int64_t mx_few_workspace(void* ws, int64_t M, int64_t H, int64_t F, int E, int t
 int mx_few_layer(const void* x, int dtype, const void* w1, const void* w2, const void* logits, int logits_dtype, int64_t M, int64_t H,
                  int64_t F, int E, int topk, int renorm, void* out, void* workspace, hipStream_t st);
 
-// linear_mxfp4 for M <= kFewTokens
+// linear_mxfp4 for few rows: whether it takes them, its workspace, the product
+bool mx_few_linear_fits(int64_t M, int64_t N);
 int64_t mx_few_linear_workspace(int64_t M, int64_t K);
 int mx_few_linear(const void* x, int dtype, int64_t M, int64_t K, int64_t ldx, const void* w, int64_t N, void* out, void* workspace,
                   hipStream_t st);

@@ -415,8 +415,8 @@ __global__ __launch_bounds__(kDownThreads) void mx_few_down_kernel(MxFew a) {
 }
 
 constexpr int kLinearRing = 4;
-// The product of a matrix with up to 32 token rows: a workgroup per 32 output features, K cut over its eight wavefronts.
-// OWN: the workgroup quantises the rows into LDS itself, else xq is the operand.
+// The product of a matrix with up to 32 U token rows: a workgroup per 32 output features, K cut over its eight wavefronts.
+// OWN (U = 1): the workgroup quantises the rows into LDS itself, else xq is the operand.
 struct MxFewLinear {
   const void* x;
   int64_t ldx;
@@ -425,13 +425,13 @@ struct MxFewLinear {
   int64_t N;
   void* out;
 };
-template <typename T, bool OWN>
+template <typename T, int U, bool OWN>
 __global__ __launch_bounds__(kDownThreads) void mx_few_linear_kernel(MxFewLinear a) {
 #if defined(__HIP_DEVICE_COMPILE__)
   extern __shared__ __attribute__((aligned(16))) unsigned char few_lds[];
   const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
   const int64_t unit = blockIdx.x;
-  const int col = min(lane & 31, a.M - 1), half = lane >> 5;
+  const int half = lane >> 5;
   const int k0 = wave * a.k_tiles / kDownWaves, k1 = (wave + 1) * a.k_tiles / kDownWaves;
   const __amdgpu_buffer_rsrc_t wr =
       __builtin_amdgcn_make_buffer_rsrc(const_cast<unsigned char*>(a.w + unit * a.k_tiles * kMxUnit), 0, -1, 0x00020000);
@@ -457,35 +457,44 @@ __global__ __launch_bounds__(kDownThreads) void mx_few_linear_kernel(MxFewLinear
     }
     __syncthreads();
   }
-  f32x16 acc;
+  f32x16 acc[U];
 #pragma unroll
-  for (int r = 0; r < 16; ++r) acc[r] = 0.f;
+  for (int u = 0; u < U; ++u)
+#pragma unroll
+    for (int r = 0; r < 16; ++r) acc[u][r] = 0.f;
   for (int kk = k0; kk < k1; kk += kLinearRing) {
 #pragma unroll
     for (int p = 0; p < kLinearRing; ++p) {
       const int k = kk + p;
       if (k < k1) {
-        mx_frag xf[4];
-        const int xs = few_token_rows<OWN>(OWN ? few_lds : a.xq, a.k_tiles, k, col, half, xf);
-        mx_each<0, 4>([&](auto S) {
-          constexpr int s = decltype(S)::value;
-          acc = mx_mfma<s>(wf[p][s], ws[p], xf[s], xs, acc);
-        });
+#pragma unroll
+        for (int u = 0; u < U; ++u) {
+          mx_frag xf[4];
+          const int col = min(lane & 31, a.M - 1 - u * 32);  // lanes behind the last row repeat it (a row group has one at least)
+          const int xs = few_token_rows<OWN>(OWN ? few_lds : a.xq + static_cast<int64_t>(u) * a.k_tiles * kMxUnit, a.k_tiles, k, col, half, xf);
+          mx_each<0, 4>([&](auto S) {
+            constexpr int s = decltype(S)::value;
+            acc[u] = mx_mfma<s>(wf[p][s], ws[p], xf[s], xs, acc[u]);
+          });
+        }
         if (k + kLinearRing < k1) load_w(k + kLinearRing, p);
       }
     }
   }
   float* const red = reinterpret_cast<float*>(few_lds);
-  __syncthreads();  // the token rows have been read
 #pragma unroll
-  for (int r = 0; r < 16; ++r) red[(wave * 64 + lane) * kDownLane + r] = acc[r];
-  __syncthreads();
-  for (int o = tid; o < a.M * 32; o += kDownThreads) {
-    const int m = o >> 5, f = o & 31;
-    float s = 0.f;
+  for (int u = 0; u < U; ++u) {
+    __syncthreads();  // the token rows, or the last row group's sums, have been read
 #pragma unroll
-    for (int w = 0; w < kDownWaves; ++w) s += red[(w * 64 + m + 32 * (f >> 4)) * kDownLane + (f & 15)];
-    if (unit * 32 + f < a.N) static_cast<T*>(a.out)[m * a.N + unit * 32 + f] = static_cast<T>(s);
+    for (int r = 0; r < 16; ++r) red[(wave * 64 + lane) * kDownLane + r] = acc[u][r];
+    __syncthreads();
+    for (int o = tid; o < min(a.M - u * 32, 32) * 32; o += kDownThreads) {
+      const int m = o >> 5, f = o & 31;
+      float s = 0.f;
+#pragma unroll
+      for (int w = 0; w < kDownWaves; ++w) s += red[(w * 64 + m + 32 * (f >> 4)) * kDownLane + (f & 15)];
+      if (unit * 32 + f < a.N) static_cast<T*>(a.out)[(m + u * 32) * a.N + unit * 32 + f] = static_cast<T>(s);
+    }
   }
 #endif
 }
@@ -503,7 +512,7 @@ bool few_routes(int64_t M, int64_t H, int E) {
 }
 
 // Every workgroup of the linear product quantises the rows.
-bool few_quantises(int64_t M, int64_t K) { return M <= 8 && M * mx_tiles(K) * kFewRow <= kRouteLds; }
+bool few_quantises(int64_t M, int64_t K) { return M <= 4 && M * mx_tiles(K) * kFewRow <= kRouteLds; }
 
 }  // namespace
 
@@ -574,7 +583,22 @@ int mx_few_layer(const void* x, int dtype, const void* w1, const void* w2, const
   return check_launch("mx_few_down_kernel");
 }
 
-int64_t mx_few_linear_workspace(int64_t M, int64_t K) { return few_quantises(M, K) ? 0 : mx_tiles(K) * kMxUnit; }
+bool mx_few_linear_fits(int64_t M, int64_t N) { return M <= kFewTokens || (M <= 4 * kFewTokens && mx_groups(N) <= 512); }
+
+int64_t mx_few_linear_workspace(int64_t M, int64_t K) { return few_quantises(M, K) ? 0 : mx_groups(M) * mx_tiles(K) * kMxUnit; }
+
+namespace {
+template <typename T>
+void launch_few_linear(const MxFewLinear& a, bool own, hipStream_t st) {
+  const int rows = own ? a.M * a.k_tiles * kFewRow : 0, lds = rows > kDownLds ? rows : kDownLds;
+  const dim3 grid(static_cast<unsigned>(mx_groups(a.N))), threads(kDownThreads);
+  if (own) hipLaunchKernelGGL((mx_few_linear_kernel<T, 1, true>), grid, threads, lds, st, a);
+  else if (a.M <= 32) hipLaunchKernelGGL((mx_few_linear_kernel<T, 1, false>), grid, threads, lds, st, a);
+  else if (a.M <= 64) hipLaunchKernelGGL((mx_few_linear_kernel<T, 2, false>), grid, threads, lds, st, a);
+  else if (a.M <= 96) hipLaunchKernelGGL((mx_few_linear_kernel<T, 3, false>), grid, threads, lds, st, a);
+  else hipLaunchKernelGGL((mx_few_linear_kernel<T, 4, false>), grid, threads, lds, st, a);
+}
+}  // namespace
 
 int mx_few_linear(const void* x, int dtype, int64_t M, int64_t K, int64_t ldx, const void* w, int64_t N, void* out, void* workspace,
                   hipStream_t st) {
@@ -590,18 +614,11 @@ int mx_few_linear(const void* x, int dtype, int64_t M, int64_t K, int64_t ldx, c
   a.out = out;
   const bool own = few_quantises(M, K);
   if (!own) {
-    const int rc = mx_quant_tiled(x, dtype, M, K, ldx, 1, MxGather{}, workspace, st);
+    const int rc = mx_quant_tiled(x, dtype, M, K, ldx, mx_groups(M), MxGather{}, workspace, st);
     if (rc != FR_OK) return rc;
   }
-  const int rows = own ? a.M * a.k_tiles * kFewRow : 0, lds = rows > kDownLds ? rows : kDownLds;
-  const dim3 grid(static_cast<unsigned>(mx_groups(N))), threads(kDownThreads);
-  if (dtype == FR_BF16) {
-    if (own) hipLaunchKernelGGL((mx_few_linear_kernel<bf16_t, true>), grid, threads, lds, st, a);
-    else hipLaunchKernelGGL((mx_few_linear_kernel<bf16_t, false>), grid, threads, lds, st, a);
-  } else {
-    if (own) hipLaunchKernelGGL((mx_few_linear_kernel<f16_t, true>), grid, threads, lds, st, a);
-    else hipLaunchKernelGGL((mx_few_linear_kernel<f16_t, false>), grid, threads, lds, st, a);
-  }
+  if (dtype == FR_BF16) launch_few_linear<bf16_t>(a, own, st);
+  else launch_few_linear<f16_t>(a, own, st);
   return check_launch("mx_few_linear_kernel");
 }
 

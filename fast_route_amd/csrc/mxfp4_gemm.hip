@@ -10,7 +10,7 @@ namespace fr {
 namespace {
 
 constexpr int kMxThreads = 256;
-enum { MX_LINEAR = 0, MX_SILU = 1, MX_DOWN = 2 };
+enum { MX_LINEAR = 0, MX_SILU = 1, MX_DOWN = 2, MX_PART = 3 };  // MX_PART: the down product, K cut over workgroups
 
 struct MxArgs {
   const unsigned char* x;  // operand of the token rows
@@ -33,6 +33,7 @@ struct MxArgs {
   uint4* rows;             // [n_pairs, N] integers, eight to an element
   unsigned char* row_exps; // [n_pairs, exp_pitch]: blocks 4 i + (0, 1, 2, 3) at 4 i + (0, 2, 1, 3)
   int exp_pitch;
+  float* part_rows;        // MX_PART: [slices][n_pairs, N]
   // MX_LINEAR
   void* out;
   int64_t ldo;
@@ -52,18 +53,21 @@ __device__ __forceinline__ void mx_epilogue(const MxArgs& a, const MxTile& t, in
 // of four wavefronts moves a third less through L1 but stalls more: 2098 / 1039 us.  A stream of these MFMAs alone reaches 6.4 PFLOP/s (the
 // part lowers its clock to 1.67 GHz for it); without any load, on data that is there, this loop reaches 5.1 to 5.5.
 constexpr int kMxSlots = 4;
-template <typename T, int EPI, int U>
+template <typename T, int EPI, int U, bool ALONE>
 __device__ __forceinline__ void mx_tile(const MxArgs& a, const MxTile& t, int f, unsigned char* lds) {
 #if defined(__HIP_DEVICE_COMPILE__)
   typedef __attribute__((address_space(3))) void* lptr_t;
-  constexpr int SLOT = U * 4096 + 1024;
+  constexpr int SLOT = U * 4096 + 1024, RING = ALONE && U <= 2 ? 4 : 2, AUX = ALONE ? 2 : 0;
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int wg = min((f * 4 + wave) * 2, a.w_groups - 1), wg1 = min(wg + 1, a.w_groups - 1);
-  const int pitch = a.k_tiles * kMxUnit, last = a.k_tiles - 1;
-  const unsigned char* const w0 = a.w + t.expert * a.w_stride + static_cast<int64_t>(wg) * pitch;
-  const unsigned char* const w1 = a.w + t.expert * a.w_stride + static_cast<int64_t>(wg1) * pitch;
-  const __amdgpu_buffer_rsrc_t xr =
-      __builtin_amdgcn_make_buffer_rsrc(const_cast<unsigned char*>(a.x + static_cast<int64_t>(t.group) * pitch), 0, -1, 0x00020000);
+  const int pitch = a.k_tiles * kMxUnit;
+  // the workgroup's K tiles: all of them, or slice blockIdx.y of gridDim.y
+  const int k_first = EPI == MX_PART ? static_cast<int>(blockIdx.y) * a.k_tiles / static_cast<int>(gridDim.y) : 0;
+  const int k_end = EPI == MX_PART ? (static_cast<int>(blockIdx.y) + 1) * a.k_tiles / static_cast<int>(gridDim.y) : a.k_tiles;
+  const int last = k_end - k_first - 1;
+  const unsigned char* const w0 = a.w + t.expert * a.w_stride + static_cast<int64_t>(wg) * pitch + k_first * kMxUnit;
+  const unsigned char* const x0 = a.x + static_cast<int64_t>(t.group) * pitch + k_first * kMxUnit;
+  const __amdgpu_buffer_rsrc_t xr = __builtin_amdgcn_make_buffer_rsrc(const_cast<unsigned char*>(x0), 0, -1, 0x00020000);
   // a K tile of token rows: wavefront w takes fragment w of every row group and a copy of all their scales
   const int code_off = lane * 16, scale_off = min(lane >> 4, U - 1) * pitch + kMxScales + (lane & 15) * 16;
   f32x16 acc[U][2];
@@ -73,8 +77,8 @@ __device__ __forceinline__ void mx_tile(const MxArgs& a, const MxTile& t, int f,
     for (int j = 0; j < 2; ++j)
 #pragma unroll
       for (int r = 0; r < 16; ++r) acc[u][j][r] = 0.f;
-  mx_frag wf[2][2][4], xf[U];  // weights of K tile k in half k & 1
-  int ws[2][2], xs[2][U];
+  mx_frag wf[RING][2][4], xf[U];  // weights of K tile k in part k % RING
+  int ws[RING][2], xs[2][U];
   auto load_x1 = [&](int k, int u) {  // u == U: the scales
     const int kc = min(k, last);
     unsigned char* slot = lds + (k & (kMxSlots - 1)) * SLOT;
@@ -90,13 +94,13 @@ __device__ __forceinline__ void mx_tile(const MxArgs& a, const MxTile& t, int f,
   const int d01 = (wg1 - wg) * pitch;
   auto load_w1 = [&](int k, int s, int p, int j) {
     const int kc = min(k, last);
-    wf[p][j][s] = __builtin_bit_cast(mx_frag, __builtin_amdgcn_raw_buffer_load_b128(r0, lane * 16 + s * 1024, (j ? d01 : 0) + kc * kMxUnit, 0));
+    wf[p][j][s] = __builtin_bit_cast(mx_frag, __builtin_amdgcn_raw_buffer_load_b128(r0, lane * 16 + s * 1024, (j ? d01 : 0) + kc * kMxUnit, AUX));
   };
   auto load_w = [&](int k, int s, int p) { load_w1(k, s, p, 0); load_w1(k, s, p, 1); };
   auto load_ws = [&](int k, int p) {
     const int kc = min(k, last);
-    ws[p][0] = __builtin_amdgcn_raw_buffer_load_b32(r0, lane * 4 + kMxScales, kc * kMxUnit, 0);
-    ws[p][1] = __builtin_amdgcn_raw_buffer_load_b32(r0, lane * 4 + kMxScales, d01 + kc * kMxUnit, 0);
+    ws[p][0] = __builtin_amdgcn_raw_buffer_load_b32(r0, lane * 4 + kMxScales, kc * kMxUnit, AUX);
+    ws[p][1] = __builtin_amdgcn_raw_buffer_load_b32(r0, lane * 4 + kMxScales, d01 + kc * kMxUnit, AUX);
   };
   auto read_x = [&](int k, int s, int u) {
     return *reinterpret_cast<const mx_frag*>(lds + (k & (kMxSlots - 1)) * SLOT + u * 4096 + s * 1024 + lane * 16);
@@ -105,21 +109,24 @@ __device__ __forceinline__ void mx_tile(const MxArgs& a, const MxTile& t, int f,
   load_x(0);
   load_x(1);
   load_x(2);
-  load_ws(0, 0);
 #pragma unroll
-  for (int s = 0; s < 7; ++s) load_w(s >> 2, s & 3, s >> 2);
+  for (int p = 0; p < RING; ++p) {
+    if (p < RING - 1) load_ws(p, p);
+#pragma unroll
+    for (int s = 0; s < (p < RING - 1 ? 4 : 3); ++s) load_w(p, s, p);
+  }
   __builtin_amdgcn_sched_barrier(0);
-  // K tile 0 of the token rows has landed: 2 (U + 1) + 16 loads are newer
-  asm volatile("s_waitcnt vmcnt(%0)" ::"n"(2 * (U + 1) + 14) : "memory");
+  // K tile 0 of the token rows has landed: 2 (U + 1) + 10 RING - 4 loads are newer
+  asm volatile("s_waitcnt vmcnt(%0)" ::"n"(2 * (U + 1) + 10 * RING - 6) : "memory");
   __builtin_amdgcn_s_barrier();
 #pragma unroll
   for (int u = 0; u < U; ++u) {
     xf[u] = read_x(0, 0, u);
     xs[0][u] = read_xs(0, u);
   }
-  for (int k0 = 0; k0 <= last; k0 += 2) {
+  for (int k0 = 0; k0 <= last; k0 += RING) {
 #pragma unroll
-    for (int p = 0; p < 2; ++p) {
+    for (int p = 0; p < RING; ++p) {
       const int k = k0 + p;
       if (p == 0 || k <= last) {
         mx_each<0, 4>([&](auto S) {
@@ -133,22 +140,22 @@ __device__ __forceinline__ void mx_tile(const MxArgs& a, const MxTile& t, int f,
 #pragma unroll
           for (int u = 0; u < U; ++u) {
 #pragma unroll
-            for (int j = 0; j < 2; ++j) acc[u][j] = mx_mfma<s>(wf[p][j][s], ws[p][j], xf[u], xs[p][u], acc[u][j]);
+            for (int j = 0; j < 2; ++j) acc[u][j] = mx_mfma<s>(wf[p][j][s], ws[p][j], xf[u], xs[p & 1][u], acc[u][j]);
             __builtin_amdgcn_sched_barrier(0);
             if constexpr (s < 3) xf[u] = read_x(k, s + 1, u);
             else {
               xf[u] = read_x(k + 1, 0, u);
-              xs[p ^ 1][u] = read_xs(k + 1, u);
+              xs[(p + 1) & 1][u] = read_xs(k + 1, u);
               load_x1(k + 3, u);
             }
             // weights of the step before: its fragments are free
 #pragma unroll
             for (int j = u; j < 2; j += U) {
               if constexpr (s > 0) {
-                load_w1(k + 2, s - 1, p, j);
+                load_w1(k + RING, s - 1, p, j);
               } else {
-                load_w1(k + 1, 3, p ^ 1, j);
-                if (j == 1) load_ws(k + 1, p ^ 1);
+                load_w1(k + RING - 1, 3, (p + RING - 1) % RING, j);
+                if (j == 1) load_ws(k + RING - 1, (p + RING - 1) % RING);
               }
             }
             __builtin_amdgcn_sched_barrier(0);
@@ -239,6 +246,20 @@ __device__ __forceinline__ void mx_epilogue(const MxArgs& a, const MxTile& t, in
           *reinterpret_cast<unsigned short*>(a.row_exps + static_cast<int64_t>(pair) * a.exp_pitch + wg * 2 + half * 2) =
               static_cast<unsigned short>(bytes[0] | bytes[1] << 8);
         }
+      } else if constexpr (EPI == MX_PART) {
+        const int pair = a.sorted[slot];
+        if (pair < a.n_pairs) {
+          const float s = a.topk_w[pair];
+#pragma unroll
+          for (int j = 0; j < 2; ++j) {
+            if (wg + j < a.w_groups) {
+              float* row = a.part_rows + (static_cast<int64_t>(blockIdx.y) * a.n_pairs + pair) * a.N + (wg + j) * 32 + half * 16;
+#pragma unroll
+              for (int r = 0; r < 16; r += 4)
+                *reinterpret_cast<f32x4*>(row + r) = f32x4{acc[u][j][r] * s, acc[u][j][r + 1] * s, acc[u][j][r + 2] * s, acc[u][j][r + 3] * s};
+            }
+          }
+        }
       } else {
         typedef T vec8 __attribute__((ext_vector_type(8)));
 #pragma unroll
@@ -265,6 +286,18 @@ __device__ __forceinline__ void mx_epilogue(const MxArgs& a, const MxTile& t, in
   }
 }
 
+template <typename T, int EPI, int MOST, bool ALONE>
+__device__ __forceinline__ void mx_tile_of(const MxArgs& a, const MxTile& t, int f, unsigned char* lds) {
+  if constexpr (MOST >= 4) {
+    if (t.units == 4) return mx_tile<T, EPI, 4, ALONE>(a, t, f, lds);
+    if (t.units == 3) return mx_tile<T, EPI, 3, ALONE>(a, t, f, lds);
+  }
+  if constexpr (MOST >= 2) {
+    if (t.units == 2) return mx_tile<T, EPI, 2, ALONE>(a, t, f, lds);
+  }
+  mx_tile<T, EPI, 1, ALONE>(a, t, f, lds);
+}
+
 // MOST: row groups of a tile, at most.
 template <typename T, int EPI, int MOST>
 __global__ __launch_bounds__(kMxThreads, 2) void mx_gemm_kernel(MxArgs a) {
@@ -287,14 +320,8 @@ __global__ __launch_bounds__(kMxThreads, 2) void mx_gemm_kernel(MxArgs a) {
   const int q = lin - t0 * a.f_tiles, f = q / n, index = t0 + q - f * n;
   if constexpr (EPI == MX_LINEAR) t = MxTile{index * MOST, min(MOST, a.x_groups - index * MOST), 0, 0, 0};
   else t = a.tiles[index];
-  if constexpr (MOST >= 4) {
-    if (t.units == 4) return mx_tile<T, EPI, 4>(a, t, f, mx_lds);
-    if (t.units == 3) return mx_tile<T, EPI, 3>(a, t, f, mx_lds);
-  }
-  if constexpr (MOST >= 2) {
-    if (t.units == 2) return mx_tile<T, EPI, 2>(a, t, f, mx_lds);
-  }
-  mx_tile<T, EPI, 1>(a, t, f, mx_lds);
+  if (n == 1) mx_tile_of<T, EPI, MOST, true>(a, t, f, mx_lds);
+  else mx_tile_of<T, EPI, MOST, false>(a, t, f, mx_lds);
 }
 
 constexpr int mx_lds_bytes(int most) { return kMxSlots * (most * 4096 + 1024); }
@@ -318,6 +345,32 @@ int mx_allow_lds() {
   return FR_OK;
 }
 
+// The same from fp32 rows of K slices, added in order.
+template <typename T>
+__global__ __launch_bounds__(kMxThreads) void mx_combine_parts_kernel(const float* __restrict__ rows, int slices, int64_t n, const int32_t* __restrict__ ids,
+                                                                      int E, int topk, int64_t M, int H, T* __restrict__ out) {
+  typedef T vec4 __attribute__((ext_vector_type(4)));
+  const int per = H / 4;
+  const int64_t i = static_cast<int64_t>(blockIdx.x) * kMxThreads + threadIdx.x;
+  if (i >= M * per) return;
+  const int64_t m = i / per;
+  const int c = static_cast<int>(i - m * per) * 4;
+  f32x4 s = {0.f, 0.f, 0.f, 0.f};
+  for (int j = 0; j < topk; ++j) {
+    const int64_t p = m * topk + j;
+    if (static_cast<unsigned>(ids[p]) >= static_cast<unsigned>(E)) continue;
+    for (int v = 0; v < slices; ++v) {
+      const f32x4 t = *reinterpret_cast<const f32x4*>(rows + (v * n + p) * H + c);
+#pragma unroll
+      for (int r = 0; r < 4; ++r) s[r] += t[r];
+    }
+  }
+  vec4 o;
+#pragma unroll
+  for (int r = 0; r < 4; ++r) o[r] = static_cast<T>(s[r]);
+  *reinterpret_cast<vec4*>(out + i * 4) = o;
+}
+
 template <typename T, int EPI, int MOST>
 int mx_launch(const MxArgs& a, dim3 grid, hipStream_t st) {
   const int rc = mx_allow_lds<T, EPI, MOST>();
@@ -327,10 +380,10 @@ int mx_launch(const MxArgs& a, dim3 grid, hipStream_t st) {
 }
 
 template <typename T, int EPI>
-int launch_mx_gemm(const MxArgs& a, int most, int64_t tiles, hipStream_t st) {
+int launch_mx_gemm(const MxArgs& a, int most, int64_t tiles, hipStream_t st, int slices = 1) {
   const int64_t wgs = 8 * ceil_div(tiles * a.f_tiles, int64_t(8));
   FR_REQUIRE(wgs < (int64_t(1) << 31), FR_E_SHAPE, "mxfp4 product: %lld workgroups", (long long)wgs);
-  const dim3 grid(static_cast<unsigned>(wgs));
+  const dim3 grid(static_cast<unsigned>(wgs), static_cast<unsigned>(slices));
   switch (most) {
     case 4: return mx_launch<T, EPI, 4>(a, grid, st);
     case 2: return mx_launch<T, EPI, 2>(a, grid, st);
@@ -383,7 +436,19 @@ struct MxLayer {
   uint4* rows;
   unsigned char* row_exps;
   int exp_pitch;
+  int slices;  // of the down product's K
+  float* part_rows;
 };
+
+// K slices of the down product: where the token tiles are few and low, enough for two workgroups per CU, of four K tiles each at least.
+int mx_slices(int64_t n, int64_t H, int64_t F, int E, int most) {
+  if (n == 0) return 1;
+  const int64_t per = ceil_div(n, static_cast<int64_t>(E)), experts = n < E ? n : E;
+  const int64_t wgs = experts * ceil_div(per, int64_t(most) * kMxRows) * ceil_div(H, 8 * kMxRows);
+  int64_t s = most <= 2 ? 512 / wgs : 1;
+  if (s > mx_tiles(F) / 4) s = mx_tiles(F) / 4;
+  return static_cast<int>(s < 1 ? 1 : s > 8 ? 8 : s);
+}
 
 MxLayer mx_layer(void* ws, int64_t M, int64_t H, int64_t F, int E, int topk) {
   MxLayer l;
@@ -405,9 +470,11 @@ MxLayer mx_layer(void* ws, int64_t M, int64_t H, int64_t F, int E, int topk) {
   l.tiles = b.take<MxTile>(l.tile_limit);
   l.x = b.take<unsigned char>(l.groups * mx_tiles(H) * kMxUnit);
   l.act = b.take<unsigned char>(l.groups * mx_tiles(F) * kMxUnit);
-  l.rows = b.take<uint4>(n * H / 8);
+  l.slices = mx_slices(n, H, F, E, l.most);
+  l.part_rows = b.take<float>(l.slices > 1 ? l.slices * n * H : 0);
+  l.rows = b.take<uint4>(l.slices > 1 ? 0 : n * H / 8);
   l.exp_pitch = static_cast<int>(ceil_div(H, 2 * kMxRows)) * 4;
-  l.row_exps = b.take<unsigned char>(n * l.exp_pitch);
+  l.row_exps = b.take<unsigned char>(l.slices > 1 ? 0 : n * l.exp_pitch);
   l.bytes = b.at;
   return l;
 }
@@ -428,7 +495,7 @@ int check_mx_layer(const char* who, int64_t M, int64_t H, int64_t F, int E, int 
 extern "C" int64_t fr_linear_mxfp4_workspace_bytes(int64_t M, int64_t N, int64_t K) {
   using namespace fr;
   if (M < 0 || N < 1 || K < 0 || M > (int64_t(1) << 24) || N > (int64_t(1) << 24) || K > (int64_t(1) << 20)) return -1;
-  return M <= kFewTokens ? mx_few_linear_workspace(M, K) : mx_groups(M) * mx_tiles(K) * kMxUnit;
+  return mx_few_linear_fits(M, N) ? mx_few_linear_workspace(M, K) : mx_groups(M) * mx_tiles(K) * kMxUnit;
 }
 
 extern "C" int fr_linear_mxfp4(const void* x, int dtype, int64_t M, int64_t K, int64_t ldx, const void* w_tiled, int64_t N, void* out,
@@ -446,7 +513,7 @@ extern "C" int fr_linear_mxfp4(const void* x, int dtype, int64_t M, int64_t K, i
   FR_REQUIRE(need == 0 || (workspace && workspace_bytes >= need), FR_E_WORKSPACE, "fr_linear_mxfp4: workspace %lld < %lld bytes", (long long)workspace_bytes, (long long)need);
   FR_REQUIRE((reinterpret_cast<uintptr_t>(workspace) & 255u) == 0, FR_E_ALIGN, "fr_linear_mxfp4: workspace must be 256-byte aligned");
   hipStream_t st = static_cast<hipStream_t>(stream);
-  if (M <= kFewTokens) return mx_few_linear(x, dtype, M, K, ldx, w_tiled, N, out, workspace, st);
+  if (mx_few_linear_fits(M, N)) return mx_few_linear(x, dtype, M, K, ldx, w_tiled, N, out, workspace, st);
   const int64_t groups = mx_groups(M);
   int rc = mx_quant_tiled(x, dtype, M, K, ldx, groups, MxGather{}, workspace, st);
   if (rc != FR_OK) return rc;
@@ -541,6 +608,19 @@ extern "C" int fr_fused_moe_mxfp4(const void* x, int dtype, const void* w1_tiled
   a.row_exps = l.row_exps;
   a.exp_pitch = l.exp_pitch;
   a.N = static_cast<int>(H);
+  if (l.slices > 1) {
+    a.part_rows = l.part_rows;
+    rc = launch_mx_gemm<bf16_t, MX_PART>(a, l.most, l.tile_limit, st, l.slices);
+    if (rc != FR_OK) return rc;
+    const dim3 grid(static_cast<unsigned>(ceil_div(M * (H / 4), int64_t(kMxThreads))));
+    if (dtype == FR_BF16)
+      hipLaunchKernelGGL((mx_combine_parts_kernel<bf16_t>), grid, dim3(kMxThreads), 0, st, l.part_rows, l.slices, n, l.topk_ids, E, topk, M, (int)H,
+                         static_cast<bf16_t*>(out));
+    else
+      hipLaunchKernelGGL((mx_combine_parts_kernel<f16_t>), grid, dim3(kMxThreads), 0, st, l.part_rows, l.slices, n, l.topk_ids, E, topk, M, (int)H,
+                         static_cast<f16_t*>(out));
+    return check_launch("mx_combine_parts_kernel");
+  }
   rc = launch_mx_gemm<bf16_t, MX_DOWN>(a, l.most, l.tile_limit, st);
   if (rc != FR_OK) return rc;
   const dim3 grid(static_cast<unsigned>(ceil_div(M * (H / 8), int64_t(kMxThreads))));

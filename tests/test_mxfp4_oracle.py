@@ -126,7 +126,9 @@ def test_c_entry_points_refuse(native):
     layer(-5, size=1024)
     layer(-4, ws=ctypes.c_void_p((1 << 20) + 128))
     assert native.fr_moe_mxfp4_workspace_bytes(4, 64, 64, 8, 9) == -1
-    assert native.fr_moe_mxfp4_workspace_bytes(0, 64, 64, 8, 2) >= 0
+    for M in (0, 1, 32, 33, 300, 1 << 20):
+        for H, F, E, k in ((64, 64, 8, 2), (32, 32, 1, 1), (4096, 14336, 8, 2), (2048, 1408, 64, 6), (1056, 1120, 256, 9)):
+            assert native.fr_moe_mxfp4_workspace_bytes(M, H, F, E, k) >= 0
 
 
 def test_python_entry_points_refuse_cpu_tensors():
