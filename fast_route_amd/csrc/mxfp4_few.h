@@ -27,7 +27,7 @@ struct MxFewScratch {
   int* arrived;
   unsigned char *xq, *act;
 };
-bool mx_few_fits(int64_t M, int topk);
+bool mx_few_fits(int64_t M, int64_t F, int E, int topk);
 int64_t mx_few_workspace(void* ws, int64_t M, int64_t H, int64_t F, int E, int topk, MxFewScratch* s);
 int mx_few_layer(const void* x, int dtype, const void* w1, const void* w2, const void* logits, int logits_dtype, int64_t M, int64_t H,
                  int64_t F, int E, int topk, int renorm, void* out, void* workspace, hipStream_t st);

@@ -5,7 +5,8 @@
 // multiplies them; its operand for the token rows is read at 16 bytes per token and fragment, lanes behind the last token repeat it.
 //
 //   front   gating (a wavefront per token or several tokens to one), hidden states to MXFP4
-//   gateup  a workgroup per 32 activated features and hit expert, K cut over its four wavefronts; SiLU * up, quantised from fp32
+//   gateup  a workgroup per 32 activated features and hit expert, K cut over its four wavefronts (where K is short and the workgroups are many: a
+//           wavefront each); SiLU * up, quantised from fp32
 //   down    a workgroup per 32 output features and part of the experts' K tiles, cut over its eight wavefronts; the routed weight and the sum
 //           over experts in registers, the parts added in order by the workgroup that comes last
 //
@@ -29,7 +30,7 @@ struct MxFew {
   int64_t w1_stride, w2_stride;           // bytes of an expert's
   float* topk_w;                          // [M, topk]
   int32_t* ids;
-  unsigned char *xq, *act;                // operands: hidden states (one row group), activated rows (one row group per hit expert)
+  unsigned char *xq, *act;                // operands: hidden states, activated rows of each hit expert; a row group each
   float* parts;                           // [H / 32][splits][M][32]
   int* arrived;                           // [H / 32], zero before `down`
   int splits;
@@ -98,11 +99,11 @@ __global__ __launch_bounds__(kFewThreads) void mx_few_front_kernel(MxFew a, int 
     return;
   }
   const int t = blockIdx.x - gate_blocks, chunk = threadIdx.x & 31, b = chunk >> 2;
-  unsigned char* u = a.xq + static_cast<int64_t>(t) * kMxUnit;
   const int k = t * kMxTileK + chunk * 8;
   for (int m = threadIdx.x >> 5; m < a.M; m += kFewThreads / 32) {
     unsigned byte;
     const unsigned o = few_quant8<T>(static_cast<const T*>(a.x) + static_cast<int64_t>(m) * a.H + k, k < a.H, &byte);
+    unsigned char* u = a.xq + static_cast<int64_t>(t) * kMxUnit;
     *reinterpret_cast<unsigned*>(u + mx_code_at(m, b) + (chunk & 3) * 4) = o;
     if ((chunk & 3) == 0) u[mx_scale_at(m, b)] = static_cast<unsigned char>(byte);
   }
@@ -161,18 +162,20 @@ __device__ __forceinline__ int few_token_rows(const unsigned char* rows, int til
   }
 }
 
+// SHARED: the workgroup's four wavefronts cut K of one block of 32 activated features, else each has a block to
+// itself.
 constexpr int kGateupRing = 3;  // K tiles of weights on their way to a wavefront's registers
-template <typename T, bool ROUTE>
+template <typename T, bool SHARED, bool ROUTE, bool NT>
 __global__ __launch_bounds__(kFewThreads) void mx_few_gateup_kernel(MxFew a) {
 #if defined(__HIP_DEVICE_COMPILE__)
   __shared__ int32_t ids[kFewPairs];
-  __shared__ float weights[kFewPairs];
+  __shared__ float weights[ROUTE ? kFewPairs : 1];
   __shared__ unsigned char present[256];
   __shared__ FewHits hits;
   __shared__ unsigned tokens_of;  // bit m: token m goes to this workgroup's expert
   extern __shared__ __attribute__((aligned(16))) unsigned char few_lds[];
   const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
-  const int n = a.M * a.topk, blk = blockIdx.x, index = blockIdx.y;
+  const int n = a.M * a.topk, index = blockIdx.y, blk = SHARED ? blockIdx.x : blockIdx.x * kFewWaves + wave;
   if (tid == 0) tokens_of = 0;
   if constexpr (ROUTE) {
     few_gate(a, 0, a.M, kFewWaves, weights, ids);
@@ -182,7 +185,7 @@ __global__ __launch_bounds__(kFewThreads) void mx_few_gateup_kernel(MxFew a) {
   __syncthreads();
   few_present(ids, n, a.E, present, hits, kFewThreads);
   if constexpr (ROUTE) {
-    if (blk == 0 && index == 0) {
+    if (blockIdx.x == 0 && index == 0) {
       for (int p = tid; p < n; p += kFewThreads) {
         a.topk_w[p] = weights[p];
         a.ids[p] = ids[p];
@@ -192,22 +195,12 @@ __global__ __launch_bounds__(kFewThreads) void mx_few_gateup_kernel(MxFew a) {
   }
   if (index >= few_hit_count(hits)) return;
   const int expert = few_hit(hits, index);
-  for (int p = tid; p < n; p += kFewThreads)
-    if (ids[p] == expert) atomicOr(&tokens_of, 1u << (p / a.topk));
-  const int col = min(lane & 31, a.M - 1), half = lane >> 5;
-  unsigned char* const act = a.act + (static_cast<int64_t>(index) * a.act_tiles + (blk >> 3)) * kMxUnit;
-  if (blk >= a.act_blocks) {  // behind the last activated feature: zeros up to a whole K tile
-    __syncthreads();
-    if (wave == 0 && (lane & 31) < a.M && (tokens_of >> col & 1)) {
-      *reinterpret_cast<uint2*>(act + mx_code_at(col, blk & 7) + half * 8) = uint2{0, 0};
-      if (half == 0) act[mx_scale_at(col, blk & 7)] = 127;
-    }
-    return;
-  }
+  const int half = lane >> 5;
+  const bool stream = blk < a.act_blocks;  // behind the last activated feature: zeros up to a whole K tile
   const int pitch = a.h_tiles * kMxUnit;
-  const unsigned char* const w0 = a.w1 + expert * a.w1_stride + static_cast<int64_t>(blk) * 2 * pitch;
+  const unsigned char* const w0 = a.w1 + expert * a.w1_stride + static_cast<int64_t>(stream ? blk : 0) * 2 * pitch;
   const __amdgpu_buffer_rsrc_t wr = __builtin_amdgcn_make_buffer_rsrc(const_cast<unsigned char*>(w0), 0, -1, 0x00020000);
-  const int k0 = wave * a.h_tiles / kFewWaves, k1 = (wave + 1) * a.h_tiles / kFewWaves;
+  const int k0 = SHARED ? wave * a.h_tiles / kFewWaves : 0, k1 = !stream ? k0 : SHARED ? (wave + 1) * a.h_tiles / kFewWaves : a.h_tiles;
   mx_frag wf[kGateupRing][2][4];
   int ws[kGateupRing][2];
   auto load_w = [&](int k, int p) {
@@ -215,15 +208,17 @@ __global__ __launch_bounds__(kFewThreads) void mx_few_gateup_kernel(MxFew a) {
     for (int j = 0; j < 2; ++j) {
 #pragma unroll
       for (int s = 0; s < 4; ++s)
-        wf[p][j][s] = __builtin_bit_cast(mx_frag, __builtin_amdgcn_raw_buffer_load_b128(wr, lane * 16 + s * 1024, j * pitch + k * kMxUnit, 2));
-      ws[p][j] = __builtin_amdgcn_raw_buffer_load_b32(wr, lane * 4 + kMxScales, j * pitch + k * kMxUnit, 2);
+        wf[p][j][s] = __builtin_bit_cast(mx_frag, __builtin_amdgcn_raw_buffer_load_b128(wr, lane * 16 + s * 1024, j * pitch + k * kMxUnit, NT ? 2 : 0));
+      ws[p][j] = __builtin_amdgcn_raw_buffer_load_b32(wr, lane * 4 + kMxScales, j * pitch + k * kMxUnit, NT ? 2 : 0);
     }
   };
 #pragma unroll
   for (int p = 0; p < kGateupRing; ++p)
     if (k0 + p < k1) load_w(k0 + p, p);
+  for (int p = tid; p < n; p += kFewThreads)
+    if (ids[p] == expert) atomicOr(&tokens_of, 1u << (p / a.topk));
+  __syncthreads();
   if constexpr (ROUTE) {
-    __syncthreads();
     const unsigned mine = tokens_of;
     const int chunks = a.h_tiles * 32;
     for (int m = 0; m < a.M; ++m) {
@@ -239,6 +234,9 @@ __global__ __launch_bounds__(kFewThreads) void mx_few_gateup_kernel(MxFew a) {
     }
     __syncthreads();
   }
+  // the lane's token; one that goes elsewhere reads a row that is read anyway (a hit expert has a token)
+  const bool mine = tokens_of >> (lane & 31) & 1;
+  const int col = mine ? lane & 31 : __ffs(tokens_of) - 1;
   f32x16 acc[2];
 #pragma unroll
   for (int j = 0; j < 2; ++j)
@@ -260,28 +258,29 @@ __global__ __launch_bounds__(kFewThreads) void mx_few_gateup_kernel(MxFew a) {
       }
     }
   }
-  // the wavefronts' sums meet in the first one
-  f32x4* const red = reinterpret_cast<f32x4*>(few_lds);
-  __syncthreads();  // the token rows have been read
-  if (wave > 0) {
+  if constexpr (SHARED) {  // the wavefronts' sums meet in the first one
+    f32x4* const red = reinterpret_cast<f32x4*>(few_lds);
+    __syncthreads();  // the token rows have been read
+    if (wave > 0) {
 #pragma unroll
-    for (int j = 0; j < 2; ++j)
+      for (int j = 0; j < 2; ++j)
 #pragma unroll
-      for (int q = 0; q < 4; ++q)
-        red[((wave - 1) * 8 + j * 4 + q) * 64 + lane] = f32x4{acc[j][q * 4], acc[j][q * 4 + 1], acc[j][q * 4 + 2], acc[j][q * 4 + 3]};
+        for (int q = 0; q < 4; ++q)
+          red[((wave - 1) * 8 + j * 4 + q) * 64 + lane] = f32x4{acc[j][q * 4], acc[j][q * 4 + 1], acc[j][q * 4 + 2], acc[j][q * 4 + 3]};
+    }
+    __syncthreads();
+    if (wave > 0) return;
+#pragma unroll
+    for (int v = 0; v < kFewWaves - 1; ++v)
+#pragma unroll
+      for (int j = 0; j < 2; ++j)
+#pragma unroll
+        for (int q = 0; q < 4; ++q) {
+          const f32x4 t = red[(v * 8 + j * 4 + q) * 64 + lane];
+#pragma unroll
+          for (int r = 0; r < 4; ++r) acc[j][q * 4 + r] += t[r];
+        }
   }
-  __syncthreads();
-  if (wave > 0) return;
-#pragma unroll
-  for (int v = 0; v < kFewWaves - 1; ++v)
-#pragma unroll
-    for (int j = 0; j < 2; ++j)
-#pragma unroll
-      for (int q = 0; q < 4; ++q) {
-        const f32x4 t = red[(v * 8 + j * 4 + q) * 64 + lane];
-#pragma unroll
-        for (int r = 0; r < 4; ++r) acc[j][q * 4 + r] += t[r];
-      }
   float v[16];
   unsigned amax = 0;
 #pragma unroll
@@ -291,9 +290,10 @@ __global__ __launch_bounds__(kFewThreads) void mx_few_gateup_kernel(MxFew a) {
     amax = amax > m ? amax : m;
   }
   const unsigned byte = mx_scale_byte(mx_pair_max(amax));
-  if ((lane & 31) < a.M && (tokens_of >> col & 1)) {
-    *reinterpret_cast<uint2*>(act + mx_code_at(col, blk & 7) + half * 8) = uint2{mx_pack8(v, byte), mx_pack8(v + 8, byte)};
-    if (half == 0) act[mx_scale_at(col, blk & 7)] = static_cast<unsigned char>(byte);
+  unsigned char* const act = a.act + (static_cast<int64_t>(index) * a.act_tiles + (blk >> 3)) * kMxUnit;
+  if (mine) {
+    *reinterpret_cast<uint2*>(act + mx_code_at(lane & 31, blk & 7) + half * 8) = uint2{mx_pack8(v, byte), mx_pack8(v + 8, byte)};
+    if (half == 0) act[mx_scale_at(lane & 31, blk & 7)] = static_cast<unsigned char>(byte);
   }
 #endif
 }
@@ -301,7 +301,7 @@ __global__ __launch_bounds__(kFewThreads) void mx_few_gateup_kernel(MxFew a) {
 constexpr int kDownRing = 4;
 constexpr int kDownLane = 17;  // floats of a lane's sums in LDS: 16 and one that spreads the banks
 constexpr int kDownLds = kDownWaves * 64 * kDownLane * 4;
-template <typename T>
+template <typename T, bool NT>
 __global__ __launch_bounds__(kDownThreads) void mx_few_down_kernel(MxFew a) {
 #if defined(__HIP_DEVICE_COMPILE__)
   __shared__ int32_t ids[kFewPairs];
@@ -321,23 +321,26 @@ __global__ __launch_bounds__(kDownThreads) void mx_few_down_kernel(MxFew a) {
   // K tiles of all hit experts in a row; this wavefront's part of them
   const int total = few_hit_count(hits) * tiles, parts = a.splits * kDownWaves, part = split * kDownWaves + wave;
   const int i0 = static_cast<int>(static_cast<int64_t>(part) * total / parts), i1 = static_cast<int>(static_cast<int64_t>(part + 1) * total / parts);
-  const int col = min(lane & 31, a.M - 1), half = lane >> 5, pitch = tiles * kMxUnit;
+  const int half = lane >> 5, pitch = tiles * kMxUnit;
+  const int col = min(lane & 31, a.M - 1);
   f32x16 sum, acc;
 #pragma unroll
   for (int r = 0; r < 16; ++r) sum[r] = acc[r] = 0.f;
   mx_frag wf[kDownRing][4], xf[kDownRing][4];
   int ws[kDownRing], xs[kDownRing];
-  int li = i0 / tiles, lk = i0 - li * tiles, le = i0 < i1 ? few_hit(hits, li) : 0;  // next tile to load: its expert's index, K tile, expert
+  // next tile to load: its expert's index, K tile, expert
+  int li = i0 / tiles, lk = i0 - li * tiles, le = i0 < i1 ? few_hit(hits, li) : 0;
+  const __amdgpu_buffer_rsrc_t xr = __builtin_amdgcn_make_buffer_rsrc(a.act, 0, -1, 0x00020000);
   auto load = [&](int p) {
-    const unsigned char* w = a.w2 + le * a.w2_stride + static_cast<int64_t>(unit) * pitch + lk * kMxUnit;
-    const unsigned char* x = a.act + static_cast<int64_t>(li) * pitch + lk * kMxUnit;
+    const unsigned char* w = a.w2 + le * a.w2_stride + static_cast<int64_t>(unit) * pitch;
+    const __amdgpu_buffer_rsrc_t wr = __builtin_amdgcn_make_buffer_rsrc(const_cast<unsigned char*>(w), 0, -1, 0x00020000);
 #pragma unroll
-    for (int s = 0; s < 4; ++s) {
-      wf[p][s] = __builtin_nontemporal_load(reinterpret_cast<const mx_frag*>(w + s * 1024 + lane * 16));
-      xf[p][s] = *reinterpret_cast<const mx_frag*>(x + s * 1024 + (col + 32 * half) * 16);
-    }
-    ws[p] = __builtin_nontemporal_load(reinterpret_cast<const int*>(w + kMxScales + lane * 4));
-    xs[p] = *reinterpret_cast<const int*>(x + kMxScales + (col + 32 * half) * 4);
+    for (int s = 0; s < 4; ++s) wf[p][s] = __builtin_bit_cast(mx_frag, __builtin_amdgcn_raw_buffer_load_b128(wr, lane * 16 + s * 1024, lk * kMxUnit, NT ? 2 : 0));
+    ws[p] = __builtin_amdgcn_raw_buffer_load_b32(wr, lane * 4 + kMxScales, lk * kMxUnit, NT ? 2 : 0);
+    const int at = li * pitch + lk * kMxUnit;  // below 2^31, see mx_few_fits
+#pragma unroll
+    for (int s = 0; s < 4; ++s) xf[p][s] = __builtin_bit_cast(mx_frag, __builtin_amdgcn_raw_buffer_load_b128(xr, (col + 32 * half) * 16 + s * 1024, at, 0));
+    xs[p] = __builtin_amdgcn_raw_buffer_load_b32(xr, (col + 32 * half) * 4 + kMxScales, at, 0);
     if (++lk == tiles) {
       lk = 0;
       ++li;
@@ -382,11 +385,11 @@ __global__ __launch_bounds__(kDownThreads) void mx_few_down_kernel(MxFew a) {
     }
   }
   float* const red = reinterpret_cast<float*>(few_lds);
+  const int outs = a.M * 32;
+  float* const mine = a.parts + (static_cast<int64_t>(unit) * a.splits + split) * outs;
 #pragma unroll
   for (int r = 0; r < 16; ++r) red[(wave * 64 + lane) * kDownLane + r] = sum[r];
   __syncthreads();
-  const int outs = a.M * 32;
-  float* const mine = a.parts + (static_cast<int64_t>(unit) * a.splits + split) * outs;
   for (int o = tid; o < outs; o += kDownThreads) {
     const int m = o >> 5, f = o & 31;
     float s = 0.f;
@@ -425,7 +428,7 @@ struct MxFewLinear {
   int64_t N;
   void* out;
 };
-template <typename T, int U, bool OWN>
+template <typename T, int U, bool OWN, bool NT>
 __global__ __launch_bounds__(kDownThreads) void mx_few_linear_kernel(MxFewLinear a) {
 #if defined(__HIP_DEVICE_COMPILE__)
   extern __shared__ __attribute__((aligned(16))) unsigned char few_lds[];
@@ -439,8 +442,8 @@ __global__ __launch_bounds__(kDownThreads) void mx_few_linear_kernel(MxFewLinear
   int ws[kLinearRing];
   auto load_w = [&](int k, int p) {
 #pragma unroll
-    for (int s = 0; s < 4; ++s) wf[p][s] = __builtin_bit_cast(mx_frag, __builtin_amdgcn_raw_buffer_load_b128(wr, lane * 16 + s * 1024, k * kMxUnit, 2));
-    ws[p] = __builtin_amdgcn_raw_buffer_load_b32(wr, lane * 4 + kMxScales, k * kMxUnit, 2);
+    for (int s = 0; s < 4; ++s) wf[p][s] = __builtin_bit_cast(mx_frag, __builtin_amdgcn_raw_buffer_load_b128(wr, lane * 16 + s * 1024, k * kMxUnit, NT ? 2 : 0));
+    ws[p] = __builtin_amdgcn_raw_buffer_load_b32(wr, lane * 4 + kMxScales, k * kMxUnit, NT ? 2 : 0);
   };
 #pragma unroll
   for (int p = 0; p < kLinearRing; ++p)
@@ -505,7 +508,8 @@ int few_splits(int64_t H) {
   return static_cast<int>(s < 1 ? 1 : s > 8 ? 8 : s);
 }
 
-constexpr int kRouteLds = 64 * 1024;
+constexpr int kGateupLds = (kFewWaves - 1) * 8 * 64 * 16;
+constexpr int kRouteLds = 56 * 1024;  // with the kernels' static arrays below the limit that needs no set-up
 // Every gateup workgroup gates all tokens (one round of its wavefronts) and quantises its expert's rows.
 bool few_routes(int64_t M, int64_t H, int E) {
   return M <= kFewWaves * few_gate_tokens(E) && M <= 8 && M * mx_tiles(H) * kFewRow <= kRouteLds;
@@ -516,7 +520,10 @@ bool few_quantises(int64_t M, int64_t K) { return M <= 4 && M * mx_tiles(K) * kF
 
 }  // namespace
 
-bool mx_few_fits(int64_t M, int topk) { return M >= 1 && M <= kFewTokens && M * topk <= kFewPairs; }
+bool mx_few_fits(int64_t M, int64_t F, int E, int topk) {
+  const int64_t n = M * topk, experts = n < E ? n : E;
+  return M >= 1 && M <= kFewTokens && n <= kFewPairs && experts * mx_tiles(F) * kMxUnit < (int64_t(1) << 31);
+}
 
 int64_t mx_few_workspace(void* ws, int64_t M, int64_t H, int64_t F, int E, int topk, MxFewScratch* s) {
   MxBump b{static_cast<unsigned char*>(ws)};
@@ -529,6 +536,32 @@ int64_t mx_few_workspace(void* ws, int64_t M, int64_t H, int64_t F, int E, int t
   s->act = b.take<unsigned char>(experts * mx_tiles(F) * kMxUnit);
   return b.at;
 }
+
+namespace {
+template <typename T, bool NT>
+int launch_few(const MxFew& a, hipStream_t st) {
+  const int n = a.M * a.topk, experts = n < a.E ? n : a.E;
+  const dim3 threads(kFewThreads), shared(static_cast<unsigned>(a.act_tiles * 8), static_cast<unsigned>(experts));
+  if (few_routes(a.M, a.H, a.E)) {
+    const int rows = a.M * a.h_tiles * kFewRow, lds = rows > kGateupLds ? rows : kGateupLds;
+    hipLaunchKernelGGL((mx_few_gateup_kernel<T, true, true, NT>), shared, threads, lds, st, a);
+  } else {
+    const int gate_blocks = static_cast<int>(ceil_div(static_cast<int64_t>(a.M), int64_t(few_gate_tokens(a.E)) * kFewWaves));
+    hipLaunchKernelGGL((mx_few_front_kernel<T>), dim3(static_cast<unsigned>(gate_blocks + a.h_tiles)), threads, 0, st, a, gate_blocks);
+    const int rc = check_launch("mx_few_front_kernel");
+    if (rc != FR_OK) return rc;
+    const dim3 apart(static_cast<unsigned>(a.act_tiles * 8 / kFewWaves), static_cast<unsigned>(experts));
+    const bool alone = a.h_tiles <= 8 && static_cast<int64_t>(a.act_blocks) * experts >= 1024;
+    if (alone) hipLaunchKernelGGL((mx_few_gateup_kernel<T, false, false, NT>), apart, threads, 0, st, a);
+    else hipLaunchKernelGGL((mx_few_gateup_kernel<T, true, false, NT>), shared, threads, kGateupLds, st, a);
+  }
+  const int rc = check_launch("mx_few_gateup_kernel");
+  if (rc != FR_OK) return rc;
+  const dim3 down(static_cast<unsigned>(a.H / kMxRows), static_cast<unsigned>(a.splits));
+  hipLaunchKernelGGL((mx_few_down_kernel<T, NT>), down, dim3(kDownThreads), kDownLds, st, a);
+  return check_launch("mx_few_down_kernel");
+}
+}  // namespace
 
 int mx_few_layer(const void* x, int dtype, const void* w1, const void* w2, const void* logits, int logits_dtype, int64_t M, int64_t H,
                  int64_t F, int E, int topk, int renorm, void* out, void* workspace, hipStream_t st) {
@@ -558,45 +591,25 @@ int mx_few_layer(const void* x, int dtype, const void* w1, const void* w2, const
   a.arrived = s.arrived;
   a.splits = few_splits(H);
   a.out = out;
-  const bool bf = dtype == FR_BF16, route = few_routes(M, H, E);
   const int64_t n = M * topk, experts = n < E ? n : E;
-  constexpr int kRedLds = (kFewWaves - 1) * 8 * 64 * 16;
-  const dim3 up(static_cast<unsigned>(a.act_tiles * 8), static_cast<unsigned>(experts)), threads(kFewThreads);
-  if (route) {
-    const int rows = static_cast<int>(M) * a.h_tiles * kFewRow, lds = rows > kRedLds ? rows : kRedLds;
-    if (bf) hipLaunchKernelGGL((mx_few_gateup_kernel<bf16_t, true>), up, threads, lds, st, a);
-    else hipLaunchKernelGGL((mx_few_gateup_kernel<f16_t, true>), up, threads, lds, st, a);
-  } else {
-    const int gate_blocks = static_cast<int>(ceil_div(M, int64_t(few_gate_tokens(E)) * kFewWaves));
-    const dim3 front(static_cast<unsigned>(gate_blocks + a.h_tiles));
-    if (bf) hipLaunchKernelGGL((mx_few_front_kernel<bf16_t>), front, threads, 0, st, a, gate_blocks);
-    else hipLaunchKernelGGL((mx_few_front_kernel<f16_t>), front, threads, 0, st, a, gate_blocks);
-    const int rc = check_launch("mx_few_front_kernel");
-    if (rc != FR_OK) return rc;
-    hipLaunchKernelGGL((mx_few_gateup_kernel<bf16_t, false>), up, threads, kRedLds, st, a);
-  }
-  int rc = check_launch("mx_few_gateup_kernel");
-  if (rc != FR_OK) return rc;
-  const dim3 down(static_cast<unsigned>(H / kMxRows), static_cast<unsigned>(a.splits));
-  if (bf) hipLaunchKernelGGL((mx_few_down_kernel<bf16_t>), down, dim3(kDownThreads), kDownLds, st, a);
-  else hipLaunchKernelGGL((mx_few_down_kernel<f16_t>), down, dim3(kDownThreads), kDownLds, st, a);
-  return check_launch("mx_few_down_kernel");
+  if (mx_streams(experts * (a.w1_stride + a.w2_stride))) return dtype == FR_BF16 ? launch_few<bf16_t, true>(a, st) : launch_few<f16_t, true>(a, st);
+  return dtype == FR_BF16 ? launch_few<bf16_t, false>(a, st) : launch_few<f16_t, false>(a, st);
 }
 
-bool mx_few_linear_fits(int64_t M, int64_t N) { return M <= kFewTokens || (M <= 4 * kFewTokens && mx_groups(N) <= 512); }
+bool mx_few_linear_fits(int64_t M, int64_t N) { return M <= 32 || (M <= 128 && mx_groups(N) <= 512); }
 
 int64_t mx_few_linear_workspace(int64_t M, int64_t K) { return few_quantises(M, K) ? 0 : mx_groups(M) * mx_tiles(K) * kMxUnit; }
 
 namespace {
-template <typename T>
+template <typename T, bool NT>
 void launch_few_linear(const MxFewLinear& a, bool own, hipStream_t st) {
   const int rows = own ? a.M * a.k_tiles * kFewRow : 0, lds = rows > kDownLds ? rows : kDownLds;
   const dim3 grid(static_cast<unsigned>(mx_groups(a.N))), threads(kDownThreads);
-  if (own) hipLaunchKernelGGL((mx_few_linear_kernel<T, 1, true>), grid, threads, lds, st, a);
-  else if (a.M <= 32) hipLaunchKernelGGL((mx_few_linear_kernel<T, 1, false>), grid, threads, lds, st, a);
-  else if (a.M <= 64) hipLaunchKernelGGL((mx_few_linear_kernel<T, 2, false>), grid, threads, lds, st, a);
-  else if (a.M <= 96) hipLaunchKernelGGL((mx_few_linear_kernel<T, 3, false>), grid, threads, lds, st, a);
-  else hipLaunchKernelGGL((mx_few_linear_kernel<T, 4, false>), grid, threads, lds, st, a);
+  if (own) hipLaunchKernelGGL((mx_few_linear_kernel<T, 1, true, NT>), grid, threads, lds, st, a);
+  else if (a.M <= 32) hipLaunchKernelGGL((mx_few_linear_kernel<T, 1, false, NT>), grid, threads, lds, st, a);
+  else if (a.M <= 64) hipLaunchKernelGGL((mx_few_linear_kernel<T, 2, false, NT>), grid, threads, lds, st, a);
+  else if (a.M <= 96) hipLaunchKernelGGL((mx_few_linear_kernel<T, 3, false, NT>), grid, threads, lds, st, a);
+  else hipLaunchKernelGGL((mx_few_linear_kernel<T, 4, false, NT>), grid, threads, lds, st, a);
 }
 }  // namespace
 
@@ -617,8 +630,8 @@ int mx_few_linear(const void* x, int dtype, int64_t M, int64_t K, int64_t ldx, c
     const int rc = mx_quant_tiled(x, dtype, M, K, ldx, mx_groups(M), MxGather{}, workspace, st);
     if (rc != FR_OK) return rc;
   }
-  if (dtype == FR_BF16) launch_few_linear<bf16_t>(a, own, st);
-  else launch_few_linear<f16_t>(a, own, st);
+  if (mx_streams(mx_groups(N) * a.k_tiles * kMxUnit)) dtype == FR_BF16 ? launch_few_linear<bf16_t, true>(a, own, st) : launch_few_linear<f16_t, true>(a, own, st);
+  else dtype == FR_BF16 ? launch_few_linear<bf16_t, false>(a, own, st) : launch_few_linear<f16_t, false>(a, own, st);
   return check_launch("mx_few_linear_kernel");
 }
 

@@ -12,6 +12,11 @@ namespace {
 constexpr int kMxThreads = 256;
 enum { MX_LINEAR = 0, MX_SILU = 1, MX_DOWN = 2, MX_PART = 3 };  // MX_PART: the down product, K cut over workgroups
 
+// What a workgroup multiplies: row groups group .. group + units - 1 of an expert's.
+struct MxSpan {
+  int group, units, expert;
+};
+
 struct MxArgs {
   const unsigned char* x;  // operand of the token rows
   const unsigned char* w;  // operand(s) of the weights
@@ -19,7 +24,7 @@ struct MxArgs {
   int k_tiles;
   int w_groups;            // row groups of an expert's weights
   int f_tiles;             // tiles of eight weight row groups
-  // grouped: the tile list; else tiles of most_units row groups out of x_groups
+  // grouped: the tile list; else tiles of kMxMaxUnits row groups out of x_groups
   const int* tile_count;
   const MxTile* tiles;
   int x_groups;
@@ -42,7 +47,7 @@ struct MxArgs {
 };
 
 template <typename T, int EPI, int U>
-__device__ __forceinline__ void mx_epilogue(const MxArgs& a, const MxTile& t, int f, int wave, int lane, f32x16 (&acc)[U][2]);
+__device__ __forceinline__ void mx_epilogue(const MxArgs& a, const MxSpan& t, int f, int wave, int lane, f32x16 (&acc)[U][2]);
 
 // Token rows through LDS (every wavefront reads all of them), weights from memory to registers (no other wavefront reads them).  A
 // ring of kMxSlots K tiles of token rows and two of weights are under way.  All loads are spread between the MFMAs, a row
@@ -53,11 +58,11 @@ __device__ __forceinline__ void mx_epilogue(const MxArgs& a, const MxTile& t, in
 // of four wavefronts moves a third less through L1 but stalls more: 2098 / 1039 us.  A stream of these MFMAs alone reaches 6.4 PFLOP/s (the
 // part lowers its clock to 1.67 GHz for it); without any load, on data that is there, this loop reaches 5.1 to 5.5.
 constexpr int kMxSlots = 4;
-template <typename T, int EPI, int U, bool ALONE>
-__device__ __forceinline__ void mx_tile(const MxArgs& a, const MxTile& t, int f, unsigned char* lds) {
+template <typename T, int EPI, int U, bool NT>
+__device__ __forceinline__ void mx_tile(const MxArgs& a, const MxSpan& t, int f, unsigned char* lds) {
 #if defined(__HIP_DEVICE_COMPILE__)
   typedef __attribute__((address_space(3))) void* lptr_t;
-  constexpr int SLOT = U * 4096 + 1024, RING = ALONE && U <= 2 ? 4 : 2, AUX = ALONE ? 2 : 0;
+  constexpr int SLOT = U * 4096 + 1024, RING = 2, AUX = NT ? 2 : 0;
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int wg = min((f * 4 + wave) * 2, a.w_groups - 1), wg1 = min(wg + 1, a.w_groups - 1);
   const int pitch = a.k_tiles * kMxUnit;
@@ -173,7 +178,7 @@ __device__ __forceinline__ void mx_tile(const MxArgs& a, const MxTile& t, int f,
 
 // acc[u][j]: the lane's 16 consecutive features of token row `lane % 32` of row group u.
 template <typename T, int EPI, int U>
-__device__ __forceinline__ void mx_epilogue(const MxArgs& a, const MxTile& t, int f, int wave, int lane, f32x16 (&acc)[U][2]) {
+__device__ __forceinline__ void mx_epilogue(const MxArgs& a, const MxSpan& t, int f, int wave, int lane, f32x16 (&acc)[U][2]) {
   const int wg = (f * 4 + wave) * 2, col = lane & 31, half = lane >> 5;
   if constexpr (EPI == MX_SILU) {
     const int blk = f * 4 + wave;  // of 32 activated features; the operand's last K tile is filled up with zeros
@@ -286,113 +291,78 @@ __device__ __forceinline__ void mx_epilogue(const MxArgs& a, const MxTile& t, in
   }
 }
 
-template <typename T, int EPI, int MOST, bool ALONE>
-__device__ __forceinline__ void mx_tile_of(const MxArgs& a, const MxTile& t, int f, unsigned char* lds) {
-  if constexpr (MOST >= 4) {
-    if (t.units == 4) return mx_tile<T, EPI, 4, ALONE>(a, t, f, lds);
-    if (t.units == 3) return mx_tile<T, EPI, 3, ALONE>(a, t, f, lds);
-  }
-  if constexpr (MOST >= 2) {
-    if (t.units == 2) return mx_tile<T, EPI, 2, ALONE>(a, t, f, lds);
-  }
-  mx_tile<T, EPI, 1, ALONE>(a, t, f, lds);
+template <typename T, int EPI, bool NT>
+__device__ __forceinline__ void mx_tile_of(const MxArgs& a, const MxSpan& t, int f, unsigned char* lds) {
+  if (t.units == 4) mx_tile<T, EPI, 4, NT>(a, t, f, lds);
+  else if (t.units == 3) mx_tile<T, EPI, 3, NT>(a, t, f, lds);
+  else if (t.units == 2) mx_tile<T, EPI, 2, NT>(a, t, f, lds);
+  else mx_tile<T, EPI, 1, NT>(a, t, f, lds);
 }
 
-// MOST: row groups of a tile, at most.
-template <typename T, int EPI, int MOST>
+template <typename T, int EPI, bool NT>
 __global__ __launch_bounds__(kMxThreads, 2) void mx_gemm_kernel(MxArgs a) {
   extern __shared__ __attribute__((aligned(16))) unsigned char mx_lds[];
   // workgroups b, b + 8, .. share an XCD and its L2: an XCD takes a consecutive part of the walk
-  const int tiles = EPI == MX_LINEAR ? (a.x_groups + MOST - 1) / MOST : a.tile_count[0];
+  const int tiles = EPI == MX_LINEAR ? (a.x_groups + kMxMaxUnits - 1) / kMxMaxUnits : a.tile_count[0];
   const int total = tiles * a.f_tiles, per = (total + 7) / 8;
   const int i = blockIdx.x >> 3, lin = (blockIdx.x & 7) * per + i;
   if (i >= per || lin >= total) return;
-  MxTile t;
-  int n, t0;
   const int guess = lin / a.f_tiles;  // a tile of the chunk that lin belongs to
+  MxTile e;
   if constexpr (EPI == MX_LINEAR) {
-    t0 = guess / kMxChunk * kMxChunk;
-    n = min(kMxChunk, tiles - t0);
+    e.first = e.expert = e.index0 = 0;
+    e.count = a.x_groups;
+    e.n = tiles;
+    e.chunk0 = guess / kMxChunk * kMxChunk;
+    e.chunk_n = min(kMxChunk, tiles - e.chunk0);
   } else {
-    t0 = a.tiles[guess].chunk0;
-    n = a.tiles[guess].chunk_n;
+    e = a.tiles[guess];
   }
-  const int q = lin - t0 * a.f_tiles, f = q / n, index = t0 + q - f * n;
-  if constexpr (EPI == MX_LINEAR) t = MxTile{index * MOST, min(MOST, a.x_groups - index * MOST), 0, 0, 0};
-  else t = a.tiles[index];
-  if (n == 1) mx_tile_of<T, EPI, MOST, true>(a, t, f, mx_lds);
-  else mx_tile_of<T, EPI, MOST, false>(a, t, f, mx_lds);
+  const int q = lin - e.chunk0 * a.f_tiles, f = q / e.chunk_n, i0 = e.chunk0 - e.index0 + q - f * e.chunk_n;
+  const int base = e.count / e.n, rem = e.count - base * e.n;  // the first rem tiles are a row group taller
+  const MxSpan t = {e.first + i0 * base + min(i0, rem), base + (i0 < rem ? 1 : 0), e.expert};
+  // a tile alone on its weights reads them past the caches if the call streams them; those that share a weight tile meet in L2
+  if (NT && e.chunk_n == 1) mx_tile_of<T, EPI, true>(a, t, f, mx_lds);
+  else mx_tile_of<T, EPI, false>(a, t, f, mx_lds);
 }
 
-constexpr int mx_lds_bytes(int most) { return kMxSlots * (most * 4096 + 1024); }
+constexpr int kMxLds = kMxSlots * (kMxMaxUnits * 4096 + 1024);
 
 // More than 64 KB of LDS needs the kernel's limit raised, once per device (a set-up call, not stream work).
-template <typename T, int EPI, int MOST>
+template <typename T, int EPI, bool NT>
 int mx_allow_lds() {
-  if (mx_lds_bytes(MOST) <= 65536) return FR_OK;
   constexpr int kMaxDevices = 64;
   static bool set[kMaxDevices] = {};  // a race between threads sets the same limit twice
   int dev = 0;
   hipError_t e = hipGetDevice(&dev);
   if (e != hipSuccess || dev < 0 || dev >= kMaxDevices) return fail(FR_E_LAUNCH, "mxfp4 product: device %d (%s)", dev, hipGetErrorString(e));
   if (set[dev]) return FR_OK;
-  e = hipFuncSetAttribute(reinterpret_cast<const void*>(&mx_gemm_kernel<T, EPI, MOST>), hipFuncAttributeMaxDynamicSharedMemorySize, mx_lds_bytes(MOST));
+  e = hipFuncSetAttribute(reinterpret_cast<const void*>(&mx_gemm_kernel<T, EPI, NT>), hipFuncAttributeMaxDynamicSharedMemorySize, kMxLds);
   if (e != hipSuccess) {
     (void)hipGetLastError();
-    return fail(FR_E_LAUNCH, "mxfp4 product: %d bytes of LDS: %s", mx_lds_bytes(MOST), hipGetErrorString(e));
+    return fail(FR_E_LAUNCH, "mxfp4 product: %d bytes of LDS: %s", kMxLds, hipGetErrorString(e));
   }
   set[dev] = true;
   return FR_OK;
 }
 
-// The same from fp32 rows of K slices, added in order.
-template <typename T>
-__global__ __launch_bounds__(kMxThreads) void mx_combine_parts_kernel(const float* __restrict__ rows, int slices, int64_t n, const int32_t* __restrict__ ids,
-                                                                      int E, int topk, int64_t M, int H, T* __restrict__ out) {
-  typedef T vec4 __attribute__((ext_vector_type(4)));
-  const int per = H / 4;
-  const int64_t i = static_cast<int64_t>(blockIdx.x) * kMxThreads + threadIdx.x;
-  if (i >= M * per) return;
-  const int64_t m = i / per;
-  const int c = static_cast<int>(i - m * per) * 4;
-  f32x4 s = {0.f, 0.f, 0.f, 0.f};
-  for (int j = 0; j < topk; ++j) {
-    const int64_t p = m * topk + j;
-    if (static_cast<unsigned>(ids[p]) >= static_cast<unsigned>(E)) continue;
-    for (int v = 0; v < slices; ++v) {
-      const f32x4 t = *reinterpret_cast<const f32x4*>(rows + (v * n + p) * H + c);
-#pragma unroll
-      for (int r = 0; r < 4; ++r) s[r] += t[r];
-    }
-  }
-  vec4 o;
-#pragma unroll
-  for (int r = 0; r < 4; ++r) o[r] = static_cast<T>(s[r]);
-  *reinterpret_cast<vec4*>(out + i * 4) = o;
-}
-
-template <typename T, int EPI, int MOST>
-int mx_launch(const MxArgs& a, dim3 grid, hipStream_t st) {
-  const int rc = mx_allow_lds<T, EPI, MOST>();
+template <typename T, int EPI, bool NT>
+int launch_mx_gemm_as(const MxArgs& a, dim3 grid, hipStream_t st) {
+  const int rc = mx_allow_lds<T, EPI, NT>();
   if (rc != FR_OK) return rc;
-  hipLaunchKernelGGL((mx_gemm_kernel<T, EPI, MOST>), grid, dim3(kMxThreads), mx_lds_bytes(MOST), st, a);
+  hipLaunchKernelGGL((mx_gemm_kernel<T, EPI, NT>), grid, dim3(kMxThreads), kMxLds, st, a);
   return check_launch("mx_gemm_kernel");
 }
 
+// tiles: token tiles, at most; matrices: weight matrices that the call reads, at most
 template <typename T, int EPI>
-int launch_mx_gemm(const MxArgs& a, int most, int64_t tiles, hipStream_t st, int slices = 1) {
+int launch_mx_gemm(const MxArgs& a, int64_t tiles, int64_t matrices, hipStream_t st, int slices = 1) {
   const int64_t wgs = 8 * ceil_div(tiles * a.f_tiles, int64_t(8));
   FR_REQUIRE(wgs < (int64_t(1) << 31), FR_E_SHAPE, "mxfp4 product: %lld workgroups", (long long)wgs);
   const dim3 grid(static_cast<unsigned>(wgs), static_cast<unsigned>(slices));
-  switch (most) {
-    case 4: return mx_launch<T, EPI, 4>(a, grid, st);
-    case 2: return mx_launch<T, EPI, 2>(a, grid, st);
-    default: return mx_launch<T, EPI, 1>(a, grid, st);
-  }
+  if (mx_streams(matrices * a.w_groups * a.k_tiles * kMxUnit)) return launch_mx_gemm_as<T, EPI, true>(a, grid, st);
+  return launch_mx_gemm_as<T, EPI, false>(a, grid, st);
 }
-
-// Row groups per tile, at most, for `rows` token rows per weight matrix on average.
-int most_units(int64_t rows) { return rows > 64 ? 4 : rows > 32 ? 2 : 1; }
 
 // out[m, :] = sum over the token's pairs, in order, of their weighted rows; a pair without an expert (a token row of NaN
 // logits) has no row.
@@ -423,13 +393,38 @@ __global__ __launch_bounds__(kMxThreads) void mx_combine_kernel(const uint4* __r
   *reinterpret_cast<vec8*>(out + i * 8) = o;
 }
 
+// The same from fp32 rows of K slices, added in order.
+template <typename T>
+__global__ __launch_bounds__(kMxThreads) void mx_combine_parts_kernel(const float* __restrict__ rows, int slices, int64_t n, const int32_t* __restrict__ ids,
+                                                                      int E, int topk, int64_t M, int H, T* __restrict__ out) {
+  typedef T vec4 __attribute__((ext_vector_type(4)));
+  const int per = H / 4;
+  const int64_t i = static_cast<int64_t>(blockIdx.x) * kMxThreads + threadIdx.x;
+  if (i >= M * per) return;
+  const int64_t m = i / per;
+  const int c = static_cast<int>(i - m * per) * 4;
+  f32x4 s = {0.f, 0.f, 0.f, 0.f};
+  for (int j = 0; j < topk; ++j) {
+    const int64_t p = m * topk + j;
+    if (static_cast<unsigned>(ids[p]) >= static_cast<unsigned>(E)) continue;
+    for (int v = 0; v < slices; ++v) {
+      const f32x4 t = *reinterpret_cast<const f32x4*>(rows + (v * n + p) * H + c);
+#pragma unroll
+      for (int r = 0; r < 4; ++r) s[r] += t[r];
+    }
+  }
+  vec4 o;
+#pragma unroll
+  for (int r = 0; r < 4; ++r) o[r] = static_cast<T>(s[r]);
+  *reinterpret_cast<vec4*>(out + i * 4) = o;
+}
+
 // ---- workspaces ------------------------------------------------------------------------------------------------
 struct MxLayer {
   float* topk_w;
   int32_t *topk_ids, *sorted, *expert_ids, *npost;
   void* align_ws;
   int64_t align_bytes, groups, tile_limit, bytes;
-  int most;
   int* tile_count;
   MxTile* tiles;
   unsigned char *x, *act;
@@ -440,13 +435,17 @@ struct MxLayer {
   float* part_rows;
 };
 
-// K slices of the down product: where the token tiles are few and low, enough for two workgroups per CU, of four K tiles each at least.
-int mx_slices(int64_t n, int64_t H, int64_t F, int E, int most) {
+// K slices of the down product: where its workgroups are few (a narrow layer, few rows) more of them, of four K tiles at least, as long
+// as their fp32 rows, written and read, stay below a tenth of the weights' bytes or 16 MB.  H = 1024, F = 3584, 8 experts, 100 tokens: down
+// 11.4 -> 7.3 us; H = 4096, F = 14336, 40 tokens 57.7 -> 47.0.
+int mx_slices(int64_t n, int64_t H, int64_t F, int E) {
   if (n == 0) return 1;
-  const int64_t per = ceil_div(n, static_cast<int64_t>(E)), experts = n < E ? n : E;
-  const int64_t wgs = experts * ceil_div(per, int64_t(most) * kMxRows) * ceil_div(H, 8 * kMxRows);
-  int64_t s = most <= 2 ? 512 / wgs : 1;
+  const int64_t experts = n < E ? n : E, tiles = experts * ceil_div(ceil_div(n, experts), int64_t(kMxMaxUnits) * kMxRows);
+  const int64_t wgs = tiles * ceil_div(H, 8 * kMxRows);
+  int64_t s = 512 / wgs;
   if (s > mx_tiles(F) / 4) s = mx_tiles(F) / 4;
+  const int64_t weights = experts * H * F * 17 / 32, most = weights / 10 > (16 << 20) ? weights / 10 : 16 << 20;
+  if (s > most / (n * H * 8)) s = most / (n * H * 8);
   return static_cast<int>(s < 1 ? 1 : s > 8 ? 8 : s);
 }
 
@@ -454,11 +453,10 @@ MxLayer mx_layer(void* ws, int64_t M, int64_t H, int64_t F, int E, int topk) {
   MxLayer l;
   MxBump b{static_cast<unsigned char*>(ws)};
   const int64_t n = M * topk;
-  l.most = most_units(ceil_div(n, static_cast<int64_t>(E)));
   // groups of 32 slots: each holds a pair, and every expert fills up one at most
   l.groups = n < (n + int64_t(E) * (kMxRows - 1)) / kMxRows ? n : (n + int64_t(E) * (kMxRows - 1)) / kMxRows;
   const int64_t experts = n < E ? n : E;
-  l.tile_limit = l.groups / l.most + experts;  // an expert has a lower tile than the limit at most once
+  l.tile_limit = l.groups / kMxMaxUnits + experts;  // an expert has a lower tile than the limit at most once
   l.topk_w = b.take<float>(n);
   l.topk_ids = b.take<int32_t>(n);
   l.sorted = b.take<int32_t>(n + int64_t(E) * (kMxRows - 1));
@@ -470,7 +468,7 @@ MxLayer mx_layer(void* ws, int64_t M, int64_t H, int64_t F, int E, int topk) {
   l.tiles = b.take<MxTile>(l.tile_limit);
   l.x = b.take<unsigned char>(l.groups * mx_tiles(H) * kMxUnit);
   l.act = b.take<unsigned char>(l.groups * mx_tiles(F) * kMxUnit);
-  l.slices = mx_slices(n, H, F, E, l.most);
+  l.slices = mx_slices(n, H, F, E);
   l.part_rows = b.take<float>(l.slices > 1 ? l.slices * n * H : 0);
   l.rows = b.take<uint4>(l.slices > 1 ? 0 : n * H / 8);
   l.exp_pitch = static_cast<int>(ceil_div(H, 2 * kMxRows)) * 4;
@@ -528,16 +526,15 @@ extern "C" int fr_linear_mxfp4(const void* x, int dtype, int64_t M, int64_t K, i
   a.ldo = N;
   a.M = M;
   a.N = static_cast<int>(N);
-  const int most = most_units(M);
-  return dtype == FR_BF16 ? launch_mx_gemm<bf16_t, MX_LINEAR>(a, most, ceil_div(groups, int64_t(most)), st)
-                          : launch_mx_gemm<f16_t, MX_LINEAR>(a, most, ceil_div(groups, int64_t(most)), st);
+  return dtype == FR_BF16 ? launch_mx_gemm<bf16_t, MX_LINEAR>(a, ceil_div(groups, int64_t(kMxMaxUnits)), 1, st)
+                          : launch_mx_gemm<f16_t, MX_LINEAR>(a, ceil_div(groups, int64_t(kMxMaxUnits)), 1, st);
 }
 
 extern "C" int64_t fr_moe_mxfp4_workspace_bytes(int64_t M, int64_t H, int64_t F, int E, int topk) {
   using namespace fr;
   if (check_mx_layer("fr_moe_mxfp4_workspace_bytes", M, H, F, E, topk) != FR_OK) return -1;
   MxFewScratch few;
-  return mx_few_fits(M, topk) ? mx_few_workspace(nullptr, M, H, F, E, topk, &few) : mx_layer(nullptr, M, H, F, E, topk).bytes;
+  return mx_few_fits(M, F, E, topk) ? mx_few_workspace(nullptr, M, H, F, E, topk, &few) : mx_layer(nullptr, M, H, F, E, topk).bytes;
 }
 
 extern "C" int fr_fused_moe_mxfp4(const void* x, int dtype, const void* w1_tiled, const void* w2_tiled, const void* logits, int logits_dtype,
@@ -555,11 +552,11 @@ extern "C" int fr_fused_moe_mxfp4(const void* x, int dtype, const void* w1_tiled
   const int64_t need = fr_moe_mxfp4_workspace_bytes(M, H, F, E, topk);
   FR_REQUIRE(workspace && workspace_bytes >= need, FR_E_WORKSPACE, "fr_fused_moe_mxfp4: workspace %lld < %lld bytes", (long long)workspace_bytes, (long long)need);
   FR_REQUIRE((reinterpret_cast<uintptr_t>(workspace) & 255u) == 0, FR_E_ALIGN, "fr_fused_moe_mxfp4: workspace must be 256-byte aligned");
-  if (mx_few_fits(M, topk))
+  if (mx_few_fits(M, F, E, topk))
     return mx_few_layer(x, dtype, w1_tiled, w2_tiled, logits, logits_dtype, M, H, F, E, topk, renormalize, out, workspace, static_cast<hipStream_t>(stream));
   const MxLayer l = mx_layer(workspace, M, H, F, E, topk);
   hipStream_t st = static_cast<hipStream_t>(stream);
-  const int64_t n = M * topk;
+  const int64_t n = M * topk, experts = n < E ? n : E;
   if (route_align_fits(M, E, topk, false)) {
     rc = route_align_small(logits, logits_dtype, M, E, topk, renormalize, kMxRows, l.topk_w, l.topk_ids, l.sorted, l.expert_ids, l.npost, nullptr, 0,
                            nullptr, nullptr, st);
@@ -573,8 +570,6 @@ extern "C" int fr_fused_moe_mxfp4(const void* x, int dtype, const void* w1_tiled
   g.expert_ids = l.expert_ids;
   g.npost = l.npost;
   g.topk = topk;
-  g.E = E;
-  g.most_units = l.most;
   g.tile_count = l.tile_count;
   g.tiles = l.tiles;
   rc = mx_quant_tiled(x, dtype, n, H, H, l.groups, g, l.x, st);
@@ -595,7 +590,7 @@ extern "C" int fr_fused_moe_mxfp4(const void* x, int dtype, const void* w1_tiled
   a.w_groups = static_cast<int>(2 * F / kMxRows);
   a.w_stride = static_cast<int64_t>(a.w_groups) * a.k_tiles * kMxUnit;
   a.f_tiles = 2 * a.act_tiles;  // whole units of activated features: the last ones are filled up with zeros
-  rc = launch_mx_gemm<bf16_t, MX_SILU>(a, l.most, l.tile_limit, st);
+  rc = launch_mx_gemm<bf16_t, MX_SILU>(a, l.tile_limit, experts, st);
   if (rc != FR_OK) return rc;
   // down
   a.x = l.act;
@@ -610,7 +605,7 @@ extern "C" int fr_fused_moe_mxfp4(const void* x, int dtype, const void* w1_tiled
   a.N = static_cast<int>(H);
   if (l.slices > 1) {
     a.part_rows = l.part_rows;
-    rc = launch_mx_gemm<bf16_t, MX_PART>(a, l.most, l.tile_limit, st, l.slices);
+    rc = launch_mx_gemm<bf16_t, MX_PART>(a, l.tile_limit, experts, st, l.slices);
     if (rc != FR_OK) return rc;
     const dim3 grid(static_cast<unsigned>(ceil_div(M * (H / 4), int64_t(kMxThreads))));
     if (dtype == FR_BF16)
@@ -621,7 +616,7 @@ extern "C" int fr_fused_moe_mxfp4(const void* x, int dtype, const void* w1_tiled
                          static_cast<f16_t*>(out));
     return check_launch("mx_combine_parts_kernel");
   }
-  rc = launch_mx_gemm<bf16_t, MX_DOWN>(a, l.most, l.tile_limit, st);
+  rc = launch_mx_gemm<bf16_t, MX_DOWN>(a, l.tile_limit, experts, st);
   if (rc != FR_OK) return rc;
   const dim3 grid(static_cast<unsigned>(ceil_div(M * (H / 8), int64_t(kMxThreads))));
   if (dtype == FR_BF16)

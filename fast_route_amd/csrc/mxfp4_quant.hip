@@ -114,7 +114,7 @@ __global__ __launch_bounds__(kMxThreads) void mx_tile_weights_kernel(const unsig
 }
 
 // The tile list of the experts' runs (one workgroup; E <= kMxThreads): an expert's groups of 32 slots, which are consecutive, are cut into as
-// few tiles of at most `most_units` as hold them, of heights that differ by one at most.
+// few tiles of at most kMxMaxUnits as hold them, of heights that differ by one at most.
 __device__ void mx_tile_list(const MxGather& g) {
   __shared__ int first[kMxThreads], count[kMxThreads], sum[kMxThreads];
   const int e = threadIdx.x, nb = g.npost[0] / kMxRows;
@@ -127,7 +127,7 @@ __device__ void mx_tile_list(const MxGather& g) {
     atomicAdd(&count[id], 1);
   }
   __syncthreads();
-  const int n = (count[e] + g.most_units - 1) / g.most_units;
+  const int n = (count[e] + kMxMaxUnits - 1) / kMxMaxUnits;
   sum[e] = n;
   __syncthreads();
   for (int d = 1; d < kMxThreads; d <<= 1) {
@@ -141,10 +141,9 @@ __device__ void mx_tile_list(const MxGather& g) {
   if (n == 0) return;
   const int chunks = (n + kMxChunk - 1) / kMxChunk;
   for (int i = 0; i < n; ++i) {
-    const int lo = static_cast<int>(static_cast<int64_t>(i) * count[e] / n), hi = static_cast<int>(static_cast<int64_t>(i + 1) * count[e] / n);
     const int c = static_cast<int>((static_cast<int64_t>(i + 1) * chunks - 1) / n);  // chunk c: tiles [c n / chunks, (c + 1) n / chunks)
     const int c0 = static_cast<int>(static_cast<int64_t>(c) * n / chunks), c1 = static_cast<int>(static_cast<int64_t>(c + 1) * n / chunks);
-    g.tiles[at + i] = MxTile{first[e] + lo, hi - lo, e, at + c0, c1 - c0};
+    g.tiles[at + i] = MxTile{first[e], count[e], e, at, n, at + c0, c1 - c0};
   }
 }
 
