@@ -219,18 +219,18 @@ __global__ __launch_bounds__(kFewThreads) void mx_few_gateup_kernel(MxFew a) {
     if (ids[p] == expert) atomicOr(&tokens_of, 1u << (p / a.topk));
   __syncthreads();
   if constexpr (ROUTE) {
-    const unsigned mine = tokens_of;
-    const int chunks = a.h_tiles * 32;
-    for (int m = 0; m < a.M; ++m) {
-      if (!(mine >> m & 1)) continue;
-      for (int c = tid; c < chunks; c += kFewThreads) {
-        const int t = c >> 5, b = (c & 31) >> 2;
-        unsigned byte;
-        const unsigned o = few_quant8<T>(static_cast<const T*>(a.x) + static_cast<int64_t>(m) * a.H + c * 8, c * 8 < a.H, &byte);
-        unsigned char* row = few_lds + (m * a.h_tiles + t) * kFewRow;
-        *reinterpret_cast<unsigned*>(row + b * 16 + (c & 3) * 4) = o;
-        if ((c & 3) == 0) row[128 + b] = static_cast<unsigned char>(byte);
-      }
+    // the expert's tokens, all their chunks of 8 elements over the threads
+    const int chunks = a.h_tiles * 32, all = __popc(tokens_of) * chunks;
+    for (int i = tid; i < all; i += kFewThreads) {
+      const int r = i / chunks, c = i - r * chunks, t = c >> 5, b = (c & 31) >> 2;
+      unsigned left = tokens_of;
+      for (int q = 0; q < r; ++q) left &= left - 1;
+      const int m = __ffs(left) - 1;
+      unsigned byte;
+      const unsigned o = few_quant8<T>(static_cast<const T*>(a.x) + static_cast<int64_t>(m) * a.H + c * 8, c * 8 < a.H, &byte);
+      unsigned char* row = few_lds + (m * a.h_tiles + t) * kFewRow;
+      *reinterpret_cast<unsigned*>(row + b * 16 + (c & 3) * 4) = o;
+      if ((c & 3) == 0) row[128 + b] = static_cast<unsigned char>(byte);
     }
     __syncthreads();
   }
@@ -502,18 +502,21 @@ __global__ __launch_bounds__(kDownThreads) void mx_few_linear_kernel(MxFewLinear
 #endif
 }
 
-// Parts a unit's K tiles are cut into: enough workgroups for the card.
-int few_splits(int64_t H) {
-  const int64_t units = H / kMxRows, s = 256 / units;
+// Parts a unit's K tiles are cut into: enough workgroups for the card, as long as a wavefront has four tiles - the parts meet in memory, which
+// takes longer than a few tiles more.
+int few_splits(int64_t M, int64_t H, int64_t F, int E, int topk) {
+  const int64_t n = M * topk, experts = n < E ? n : E;
+  const int64_t card = 256 / (H / kMxRows), work = experts * mx_tiles(F) / (4 * kDownWaves);
+  const int64_t s = card < work ? card : work;
   return static_cast<int>(s < 1 ? 1 : s > 8 ? 8 : s);
 }
 
 constexpr int kGateupLds = (kFewWaves - 1) * 8 * 64 * 16;
 constexpr int kRouteLds = 56 * 1024;  // with the kernels' static arrays below the limit that needs no set-up
-// Every gateup workgroup gates all tokens (one round of its wavefronts) and quantises its expert's rows.
-bool few_routes(int64_t M, int64_t H, int E) {
-  return M <= kFewWaves * few_gate_tokens(E) && M <= 8 && M * mx_tiles(H) * kFewRow <= kRouteLds;
-}
+// Every gateup workgroup gates all tokens and quantises its expert's rows: a launch of 4 us less for up to 6 us more in each workgroup.  Two launches /
+// three, us: H = 1024, F = 3584, 8 experts, top-2, 1 token 15.5 / 18.6, 2 15.0 / 17.9, 5 25.1 / 25.9; H = 4096, F = 14336 4 96 / 97, 8 133 / 125;
+// H = 2048, F = 1408, 64 experts, top-6 1 19.0 / 20.3, 4 26.3 / 23.2.
+bool few_routes(int64_t M, int64_t H, int E) { return M <= (E <= 32 ? 4 : 2) && M * mx_tiles(H) * kFewRow <= kRouteLds; }
 
 // Every workgroup of the linear product quantises the rows.
 bool few_quantises(int64_t M, int64_t K) { return M <= 4 && M * mx_tiles(K) * kFewRow <= kRouteLds; }
@@ -531,7 +534,7 @@ int64_t mx_few_workspace(void* ws, int64_t M, int64_t H, int64_t F, int E, int t
   s->topk_w = b.take<float>(n);
   s->ids = b.take<int32_t>(n);
   s->arrived = b.take<int>(H / kMxRows);
-  s->parts = b.take<float>(static_cast<int64_t>(few_splits(H)) * M * H);
+  s->parts = b.take<float>(static_cast<int64_t>(few_splits(M, H, F, E, topk)) * M * H);
   s->xq = b.take<unsigned char>(mx_tiles(H) * kMxUnit);
   s->act = b.take<unsigned char>(experts * mx_tiles(F) * kMxUnit);
   return b.at;
@@ -589,7 +592,7 @@ int mx_few_layer(const void* x, int dtype, const void* w1, const void* w2, const
   a.act = s.act;
   a.parts = s.parts;
   a.arrived = s.arrived;
-  a.splits = few_splits(H);
+  a.splits = few_splits(M, H, F, E, topk);
   a.out = out;
   const int64_t n = M * topk, experts = n < E ? n : E;
   if (mx_streams(experts * (a.w1_stride + a.w2_stride))) return dtype == FR_BF16 ? launch_few<bf16_t, true>(a, st) : launch_few<f16_t, true>(a, st);
