@@ -34,22 +34,26 @@ class MXFP4Experts(NamedTuple):
     F: int
 
 
+_HERE = contextlib.nullcontext()
+
+
 def _on(device: torch.device):
     """The device of a call's tensors as the current one, where it is another."""
-    return contextlib.nullcontext() if device.index == torch.cuda.current_device() else torch.cuda.device(device)
+    return _HERE if device.index == torch.cuda.current_device() else torch.cuda.device(device)
 
 
-def _check_rows(x: torch.Tensor, what: str) -> None:
+def _check_rows(x: torch.Tensor, what: str):
+    """Rows, row length and row stride of a 2-D tensor that the kernels read row by row."""
     N.require_cuda(x)
     assert x.dim() == 2 and x.dtype in _FLOATS, "%s must be a 2-D float16 or bfloat16 tensor" % what
-    assert x.shape[1] > 0 and x.shape[1] % BLOCK == 0, "%s: row length must be a positive multiple of 32" % what
-    assert x.shape[0] <= 1 or (x.stride(0) >= x.shape[1] and x.stride(0) % 8 == 0), \
-        "%s: rows must not overlap and lie a multiple of 8 elements apart" % what
-    assert x.stride(1) == 1, "%s must be contiguous along its rows" % what
-
-
-def _row_stride(x: torch.Tensor) -> int:
-    return x.stride(0) if x.shape[0] > 1 else x.shape[1]
+    rows, K = x.shape
+    ld, step = x.stride()
+    assert K > 0 and K % BLOCK == 0, "%s: row length must be a positive multiple of 32" % what
+    assert step == 1, "%s must be contiguous along its rows" % what
+    if rows <= 1:
+        return rows, K, K
+    assert ld >= K and ld % 8 == 0, "%s: rows must not overlap and lie a multiple of 8 elements apart" % what
+    return rows, K, ld
 
 
 def _check_codes(codes: torch.Tensor, scales: torch.Tensor, what: str) -> None:
@@ -57,8 +61,8 @@ def _check_codes(codes: torch.Tensor, scales: torch.Tensor, what: str) -> None:
     assert codes.device == scales.device, "%s: codes and scales on different devices" % what
     assert codes.dtype == torch.uint8 and scales.dtype == torch.uint8, "%s: codes and scales must be uint8" % what
     assert codes.is_contiguous() and scales.is_contiguous(), "%s: codes and scales must be contiguous" % what
-    assert codes.dim() >= 2 and codes.shape[-1] > 0 and codes.shape[-1] % (BLOCK // 2) == 0 \
-        and scales.shape == codes.shape[:-1] + (codes.shape[-1] // (BLOCK // 2),), \
+    *lead, half = codes.shape
+    assert lead and half > 0 and half % (BLOCK // 2) == 0 and scales.shape == (*lead, half // (BLOCK // 2)), \
         "%s: codes must be [.., K / 2] and scales [.., K / 32]" % what
 
 
@@ -69,13 +73,13 @@ def quantize_rows_mxfp4(x: torch.Tensor):
     elements are rounded to the nearest of 0, 1/2, 1, 3/2, 2, 3, 4, 6 units, ties to the even code, and what exceeds 6
     becomes 6.  The even element of a pair is in the low half of its byte.  A block that holds an infinity or a NaN has b = 255
     and zero codes: all of it reads back as NaN."""
-    _check_rows(x, "x")
-    rows, K = x.shape
-    codes = torch.empty((rows, K // 2), dtype=torch.uint8, device=x.device)
-    scales = torch.empty((rows, K // BLOCK), dtype=torch.uint8, device=x.device)
-    with _on(x.device):
-        N.check(N.lib().fr_quant_mxfp4_rows(x.data_ptr(), N.dtype_code(x.dtype), rows, K, _row_stride(x), codes.data_ptr(),
-                                            scales.data_ptr(), N.stream_ptr(x.device)))
+    rows, K, ld = _check_rows(x, "x")
+    dev = x.device
+    codes = torch.empty((rows, K // 2), dtype=torch.uint8, device=dev)
+    scales = codes.new_empty((rows, K // BLOCK))
+    with _on(dev):
+        N.check(N.lib().fr_quant_mxfp4_rows(x.data_ptr(), N.dtype_code(x.dtype), rows, K, ld, codes.data_ptr(), scales.data_ptr(),
+                                            N.stream_ptr(dev)))
     return codes, scales
 
 
@@ -114,20 +118,19 @@ def prepare_linear_mxfp4(codes: torch.Tensor, scales: torch.Tensor) -> MXFP4Weig
 def linear_mxfp4(x: torch.Tensor, weight: MXFP4Weight, workspace_buf: torch.Tensor | None = None) -> torch.Tensor:
     """x [M, K] (f16/bf16, rows a multiple of 8 elements apart) times the transpose of a prepared weight matrix [N, K]: x is
     quantised to MXFP4 row by row, the product accumulates in fp32, the result [M, N] has x's type."""
-    _check_rows(x, "x")
-    assert x.shape[1] == weight.K, "Incompatible dimensions"
-    assert x.device == weight.data.device, "x and weight on different devices"
-    M, K = x.shape
-    out = torch.empty((M, weight.N), dtype=x.dtype, device=x.device)
+    M, K, ld = _check_rows(x, "x")
+    dev = x.device
+    assert K == weight.K, "Incompatible dimensions"
+    assert dev == weight.data.device, "x and weight on different devices"
+    out = torch.empty((M, weight.N), dtype=x.dtype, device=dev)
     if M == 0:
         return out
     need = N.lib().fr_linear_mxfp4_workspace_bytes(M, weight.N, K)
     assert need >= 0, "linear_mxfp4: %d rows of %d elements are too large" % (M, K)
-    ws = _workspace(workspace_buf, need, x.device)
-    with _on(x.device):
-        N.check(N.lib().fr_linear_mxfp4(x.data_ptr(), N.dtype_code(x.dtype), M, K, _row_stride(x), weight.data.data_ptr(), weight.N,
-                                        out.data_ptr(), 0 if ws is None else ws.data_ptr(), 0 if ws is None else ws.numel(),
-                                        N.stream_ptr(x.device)))
+    ws = _workspace(workspace_buf, need, dev)
+    with _on(dev):
+        N.check(N.lib().fr_linear_mxfp4(x.data_ptr(), N.dtype_code(x.dtype), M, K, ld, weight.data.data_ptr(), weight.N, out.data_ptr(),
+                                        0 if ws is None else ws.data_ptr(), 0 if ws is None else ws.numel(), N.stream_ptr(dev)))
     return out
 
 

@@ -7,11 +7,13 @@ reference's own Attention module is for this bench.  The MoE is the gate-matrix 
 point of layers/stable_route.py.  Usage:
 
     python -m fast_route_amd.transformer_layer_bench [-n FFN] [-k HIDDEN] [-e EXPERTS] [--topk K]
-        [-b BATCH] [--n_head H] [--head_dim D] [--seqs 32,64,...]
+        [-b BATCH] [--n_head H] [--head_dim D] [--seqs 32,64,...] [--mxfp4]
 
 prints one JSON line per sequence length: median / p20 / p80 milliseconds of the whole
 layer and of the MoE alone, the MoE share, and the reference's TFLOPS figure
 (2*b*seq*n*k + 2*b*seq*seq*n_head*head_dim per layer time).
+
+--mxfp4: the same layer with its projections' and experts' weights in MXFP4 (linear_mxfp4, fused_moe_mxfp4).
 """
 from __future__ import annotations
 
@@ -20,6 +22,7 @@ import json
 
 import torch
 
+from .layers.mxfp4 import fused_moe_mxfp4, linear_mxfp4, prepare_linear_mxfp4, prepare_weights_mxfp4, quantize_rows_mxfp4
 from .layers.stable_route import fused_moe
 
 
@@ -35,6 +38,37 @@ class Attention(torch.nn.Module):
         q, k, v = self.qkv(x).view(b, s, 3, self.n_head, self.head_dim).permute(2, 0, 3, 1, 4)
         o = torch.nn.functional.scaled_dot_product_attention(q, k, v, is_causal=True)
         return self.proj(o.transpose(1, 2).reshape(b, s, self.n_head * self.head_dim))
+
+
+class AttentionMXFP4:
+    """Attention whose projections' weights are held in MXFP4, from those of an Attention."""
+
+    def __init__(self, attn: Attention):
+        self.n_head, self.head_dim = attn.n_head, attn.head_dim
+        self.qkv = prepare_linear_mxfp4(*quantize_rows_mxfp4(attn.qkv.weight.detach()))
+        self.proj = prepare_linear_mxfp4(*quantize_rows_mxfp4(attn.proj.weight.detach()))
+
+    def __call__(self, x: torch.Tensor) -> torch.Tensor:
+        b, s, hidden = x.shape
+        qkv = linear_mxfp4(x.reshape(b * s, hidden), self.qkv)
+        q, k, v = qkv.view(b, s, 3, self.n_head, self.head_dim).permute(2, 0, 3, 1, 4)
+        o = torch.nn.functional.scaled_dot_product_attention(q, k, v, is_causal=True)
+        return linear_mxfp4(o.transpose(1, 2).reshape(b * s, self.n_head * self.head_dim), self.proj).view(b, s, -1)
+
+
+def quantize_experts_mxfp4(w1: torch.Tensor, w2: torch.Tensor):
+    """Expert weights w1 [E, 2F, H] and w2 [E, H, F] quantised and laid out for fused_moe_mxfp4."""
+    held = []
+    for w in (w1, w2):
+        codes, scales = quantize_rows_mxfp4(w.reshape(-1, w.shape[2]))
+        held += [codes.view(*w.shape[:2], -1), scales.view(*w.shape[:2], -1)]
+    return prepare_weights_mxfp4(*held)
+
+
+def transformer_layer_mxfp4(attn, x, gate, experts, topk):
+    """transformer_layer with MXFP4 weights; the router's logits from the unquantised hidden states."""
+    h = (attn(x) + x).view(-1, x.shape[-1])
+    return fused_moe_mxfp4(h, experts, h @ gate, topk, renormalize=True)
 
 
 def transformer_layer(attn, x, gate, w1, w2, topk):
@@ -57,7 +91,7 @@ def _quantiles_ms(fn, reps: int, warmup: int):
 
 
 def run(seq: int, n: int, k: int, e: int, topk: int, b: int, n_head: int, head_dim: int, seed: int = 1337,
-        reps: int = 20, warmup: int = 3, dtype=torch.float16, weights=None):
+        reps: int = 20, warmup: int = 3, dtype=torch.float16, weights=None, mxfp4: bool = False):
     g = torch.Generator(device="cuda").manual_seed(seed)
     x = torch.randn((b, seq, k), device="cuda", dtype=dtype, generator=g) / 10
     if weights is None:
@@ -69,9 +103,23 @@ def run(seq: int, n: int, k: int, e: int, topk: int, b: int, n_head: int, head_d
     gate, w1, w2, attn = weights
     with torch.no_grad():
         h = (attn(x) + x).view(-1, k)
-        layer = _quantiles_ms(lambda: transformer_layer(attn, x, gate, w1, w2, topk), reps, warmup)
-        moe = _quantiles_ms(lambda: fused_moe(h, gate, w1, w2, topk, True, False), reps, warmup)
-        out = transformer_layer(attn, x, gate, w1, w2, topk)
+        if mxfp4:
+            attn4, experts = AttentionMXFP4(attn), quantize_experts_mxfp4(w1, w2)
+
+            def whole():
+                return transformer_layer_mxfp4(attn4, x, gate, experts, topk)
+
+            def experts_only():
+                return fused_moe_mxfp4(h, experts, h @ gate, topk)
+        else:
+            def whole():
+                return transformer_layer(attn, x, gate, w1, w2, topk)
+
+            def experts_only():
+                return fused_moe(h, gate, w1, w2, topk, True, False)
+        layer = _quantiles_ms(whole, reps, warmup)
+        moe = _quantiles_ms(experts_only, reps, warmup)
+        out = whole()
     flops = 2.0 * b * seq * n * k + 2.0 * b * seq * seq * n_head * head_dim  # the reference's figure
     rec = {"seq": seq, "batch": b, "layer_ms": round(layer[0], 4), "layer_ms_p20": round(layer[1], 4),
            "layer_ms_p80": round(layer[2], 4), "moe_ms": round(moe[0], 4), "moe_share": round(moe[0] / layer[0], 4),
@@ -89,13 +137,14 @@ def main():
     ap.add_argument("-b", type=int, default=1)
     ap.add_argument("--n_head", type=int, default=32)
     ap.add_argument("--head_dim", type=int, default=128)
+    ap.add_argument("--mxfp4", action="store_true", help="weights in MXFP4")
     ap.add_argument("--seqs", default=",".join(str(2 ** i) for i in range(5, 15)))
     args = ap.parse_args()
     assert torch.cuda.is_available(), "needs an MI355X"
     weights = None
     for seq in [int(s) for s in args.seqs.split(",")]:
         rec, _, weights = run(seq, args.n, args.k, args.e, args.topk, args.b, args.n_head, args.head_dim, args.seed,
-                              weights=weights)
+                              weights=weights, mxfp4=args.mxfp4)
         print(json.dumps(rec), flush=True)
 
 

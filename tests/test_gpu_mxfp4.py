@@ -338,3 +338,72 @@ def test_refusals(native):
             call()
             print("case", i, "was not refused", flush=True)
     torch.cuda.synchronize()
+
+
+def test_transformer_layer_runs_on_mxfp4_weights(native):
+    """Projections, attention and experts together, as the bench's --mxfp4 calls them, against the same layer step by step in
+    64 bits from the operators' own inputs: the projections' result is what the attention gets, its sum what the experts get."""
+    from fast_route_amd import transformer_layer_bench as tb
+    hidden, n_head, head_dim, F, E, topk = 256, 4, 64, 320, 8, 2
+    torch.manual_seed(5)
+    attn = tb.Attention(hidden, n_head, head_dim, torch.float16).to("cuda")
+    attn4 = tb.AttentionMXFP4(attn)
+    g = torch.Generator(device="cuda").manual_seed(6)
+    gate, w1, w2 = (torch.randn(s, device="cuda", dtype=torch.float16, generator=g) / d
+                    for s, d in (((hidden, E), 16), ((E, 2 * F, hidden), 12), ((E, hidden, F), 18)))
+    experts = tb.quantize_experts_mxfp4(w1, w2)
+    q1 = [t.reshape(E, 2 * F, -1) for t in oracle.mxfp4_quant_rows(w1.cpu().view(-1, hidden))]
+    q2 = [t.reshape(E, hidden, -1) for t in oracle.mxfp4_quant_rows(w2.cpu().view(-1, F))]
+    for b, s in ((1, 1), (2, 33), (1, 300)):
+        x = torch.randn((b, s, hidden), device="cuda", dtype=torch.float16, generator=g)
+        with torch.no_grad():
+            h = (attn4(x) + x).view(-1, hidden)
+            logits = h @ gate
+            out = tb.transformer_layer_mxfp4(attn4, x, gate, experts, topk)
+            qkv = attn4.qkv
+            got = tb.linear_mxfp4(x.view(-1, hidden), qkv)
+        wq = oracle.mxfp4_held(attn.qkv.weight.detach().cpu())
+        xv = oracle.mxfp4_held(x.cpu().view(-1, hidden))
+        ref, terms = xv @ wq.T, np.abs(xv) @ np.abs(wq).T
+        bound = 2.0 ** -11 * np.abs(ref) + _sum_error(terms, hidden) * 1.001 + 2.0 ** -22
+        assert (np.abs(got.double().cpu().numpy() - ref) <= bound).all()
+        _check_layer(out, h.cpu(), logits.cpu(), (*q1, *q2), topk, True, torch.float16)
+
+
+def test_first_calls_of_a_process_under_capture(native):
+    """Nothing has run before: the captured calls are the kernels' first, replays equal the eager calls that follow."""
+    import subprocess
+    import sys
+    import os
+    root = os.path.dirname(os.path.dirname(os.path.abspath(__file__)))
+    code = """
+import torch, fast_route_amd as fr
+g = torch.Generator(device="cuda").manual_seed(1)
+E, H, F, k = 8, 512, 384, 2
+held = []
+for shape in ((E, 2 * F, H), (E, H, F)):
+    c, s = fr.quantize_rows_mxfp4(torch.randn(shape, device="cuda", generator=g).bfloat16().view(-1, shape[2]) / 16)
+    held += [c.view(shape[0], shape[1], -1), s.view(shape[0], shape[1], -1)]
+weights = fr.prepare_weights_mxfp4(*held)
+lin = fr.prepare_linear_mxfp4(*fr.quantize_rows_mxfp4(torch.randn((640, H), device="cuda", generator=g).bfloat16()))
+calls = []
+for M in (1, 20, 300):
+    x = torch.randn((M, H), device="cuda", generator=g).bfloat16()
+    l = torch.randn((M, E), device="cuda", generator=g)
+    calls.append((x, l))
+torch.cuda.synchronize()
+graph = torch.cuda.CUDAGraph()
+with torch.cuda.graph(graph):
+    outs = [(fr.fused_moe_mxfp4(x, weights, l, k), fr.linear_mxfp4(x, lin)) for x, l in calls]
+for i in range(3):
+    for x, l in calls:
+        x.normal_(generator=g)
+        l.normal_(generator=g)
+    graph.replay()
+    torch.cuda.synchronize()
+    for (x, l), (a, b) in zip(calls, outs):
+        assert torch.equal(a, fr.fused_moe_mxfp4(x, weights, l, k)) and torch.equal(b, fr.linear_mxfp4(x, lin)), i
+print("captured first calls ok")
+"""
+    run = subprocess.run([sys.executable, "-c", code], cwd=root, capture_output=True, text=True, timeout=110)
+    assert run.returncode == 0 and "captured first calls ok" in run.stdout, run.stderr[-2000:]
