@@ -23,7 +23,7 @@ struct MxArgs {
   int64_t w_stride;        // bytes of an expert's weights
   int k_tiles;
   int w_groups;            // row groups of an expert's weights
-  int f_tiles;             // tiles of eight weight row groups
+  int f_tiles;             // tiles of 4 J weight row groups
   // grouped: the tile list; else tiles of kMxMaxUnits row groups out of x_groups
   const int* tile_count;
   const MxTile* tiles;
@@ -46,8 +46,8 @@ struct MxArgs {
   int N;               // columns of rows / out
 };
 
-template <typename T, int EPI, int U>
-__device__ __forceinline__ void mx_epilogue(const MxArgs& a, const MxSpan& t, int f, int wave, int lane, f32x16 (&acc)[U][2]);
+template <typename T, int EPI, int U, int J>
+__device__ __forceinline__ void mx_epilogue(const MxArgs& a, const MxSpan& t, int f, int wave, int lane, f32x16 (&acc)[U][J]);
 
 // Token rows through LDS (every wavefront reads all of them), weights from memory to registers (no other wavefront reads them).  A
 // ring of kMxSlots K tiles of token rows and two of weights are under way.  All loads are spread between the MFMAs, a row
@@ -58,13 +58,13 @@ __device__ __forceinline__ void mx_epilogue(const MxArgs& a, const MxSpan& t, in
 // of four wavefronts moves a third less through L1 but stalls more: 2098 / 1039 us.  A stream of these MFMAs alone reaches 6.4 PFLOP/s (the
 // part lowers its clock to 1.67 GHz for it); without any load, on data that is there, this loop reaches 5.1 to 5.5.
 constexpr int kMxSlots = 4;
-template <typename T, int EPI, int U, bool NT>
+template <typename T, int EPI, int U, int J, bool NT>
 __device__ __forceinline__ void mx_tile(const MxArgs& a, const MxSpan& t, int f, unsigned char* lds) {
 #if defined(__HIP_DEVICE_COMPILE__)
   typedef __attribute__((address_space(3))) void* lptr_t;
   constexpr int SLOT = U * 4096 + 1024, RING = 2, AUX = NT ? 2 : 0;
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-  const int wg = min((f * 4 + wave) * 2, a.w_groups - 1), wg1 = min(wg + 1, a.w_groups - 1);
+  const int wg = min((f * 4 + wave) * J, a.w_groups - 1), wg1 = min(wg + 1, a.w_groups - 1);
   const int pitch = a.k_tiles * kMxUnit;
   // the workgroup's K tiles: all of them, or slice blockIdx.y of gridDim.y
   const int k_first = EPI == MX_PART ? static_cast<int>(blockIdx.y) * a.k_tiles / static_cast<int>(gridDim.y) : 0;
@@ -75,15 +75,15 @@ __device__ __forceinline__ void mx_tile(const MxArgs& a, const MxSpan& t, int f,
   const __amdgpu_buffer_rsrc_t xr = __builtin_amdgcn_make_buffer_rsrc(const_cast<unsigned char*>(x0), 0, -1, 0x00020000);
   // a K tile of token rows: wavefront w takes fragment w of every row group and a copy of all their scales
   const int code_off = lane * 16, scale_off = min(lane >> 4, U - 1) * pitch + kMxScales + (lane & 15) * 16;
-  f32x16 acc[U][2];
+  f32x16 acc[U][J];
 #pragma unroll
   for (int u = 0; u < U; ++u)
 #pragma unroll
-    for (int j = 0; j < 2; ++j)
+    for (int j = 0; j < J; ++j)
 #pragma unroll
       for (int r = 0; r < 16; ++r) acc[u][j][r] = 0.f;
-  mx_frag wf[RING][2][4], xf[U];  // weights of K tile k in part k % RING
-  int ws[RING][2], xs[2][U];
+  mx_frag wf[RING][J][4], xf[U];  // weights of K tile k in part k % RING
+  int ws[RING][J], xs[2][U];
   auto load_x1 = [&](int k, int u) {  // u == U: the scales
     const int kc = min(k, last);
     unsigned char* slot = lds + (k & (kMxSlots - 1)) * SLOT;
@@ -101,11 +101,14 @@ __device__ __forceinline__ void mx_tile(const MxArgs& a, const MxSpan& t, int f,
     const int kc = min(k, last);
     wf[p][j][s] = __builtin_bit_cast(mx_frag, __builtin_amdgcn_raw_buffer_load_b128(r0, lane * 16 + s * 1024, (j ? d01 : 0) + kc * kMxUnit, AUX));
   };
-  auto load_w = [&](int k, int s, int p) { load_w1(k, s, p, 0); load_w1(k, s, p, 1); };
+  auto load_w = [&](int k, int s, int p) {
+#pragma unroll
+    for (int j = 0; j < J; ++j) load_w1(k, s, p, j);
+  };
   auto load_ws = [&](int k, int p) {
     const int kc = min(k, last);
-    ws[p][0] = __builtin_amdgcn_raw_buffer_load_b32(r0, lane * 4 + kMxScales, kc * kMxUnit, AUX);
-    ws[p][1] = __builtin_amdgcn_raw_buffer_load_b32(r0, lane * 4 + kMxScales, d01 + kc * kMxUnit, AUX);
+#pragma unroll
+    for (int j = 0; j < J; ++j) ws[p][j] = __builtin_amdgcn_raw_buffer_load_b32(r0, lane * 4 + kMxScales, (j ? d01 : 0) + kc * kMxUnit, AUX);
   };
   auto read_x = [&](int k, int s, int u) {
     return *reinterpret_cast<const mx_frag*>(lds + (k & (kMxSlots - 1)) * SLOT + u * 4096 + s * 1024 + lane * 16);
@@ -121,8 +124,8 @@ __device__ __forceinline__ void mx_tile(const MxArgs& a, const MxSpan& t, int f,
     for (int s = 0; s < (p < RING - 1 ? 4 : 3); ++s) load_w(p, s, p);
   }
   __builtin_amdgcn_sched_barrier(0);
-  // K tile 0 of the token rows has landed: 2 (U + 1) + 10 RING - 4 loads are newer
-  asm volatile("s_waitcnt vmcnt(%0)" ::"n"(2 * (U + 1) + 10 * RING - 6) : "memory");
+  // K tile 0 of the token rows has landed: 2 (U + 1) + 5 J RING - 2 J loads are newer
+  asm volatile("s_waitcnt vmcnt(%0)" ::"n"(2 * (U + 1) + 5 * J * RING - 3 * J) : "memory");
   __builtin_amdgcn_s_barrier();
 #pragma unroll
   for (int u = 0; u < U; ++u) {
@@ -138,14 +141,14 @@ __device__ __forceinline__ void mx_tile(const MxArgs& a, const MxSpan& t, int f,
           constexpr int s = decltype(S)::value;
           if constexpr (s == 3) {
             // K tile k + 1 of the token rows has landed, everybody's loads of it behind the barrier (this wavefront has issued U + 1 of
-            // k + 2 and 18 of weights since); and slot (k + 3) & 3, that of k - 1, has been read by everybody.
-            asm volatile("s_waitcnt vmcnt(%0)" ::"n"(U + 1 + 14) : "memory");
+            // k + 2 and 9 J of weights since); and slot (k + 3) & 3, that of k - 1, has been read by everybody.
+            asm volatile("s_waitcnt vmcnt(%0)" ::"n"(U + 1 + 7 * J) : "memory");
             __builtin_amdgcn_s_barrier();
           }
 #pragma unroll
           for (int u = 0; u < U; ++u) {
 #pragma unroll
-            for (int j = 0; j < 2; ++j) acc[u][j] = mx_mfma<s>(wf[p][j][s], ws[p][j], xf[u], xs[p & 1][u], acc[u][j]);
+            for (int j = 0; j < J; ++j) acc[u][j] = mx_mfma<s>(wf[p][j][s], ws[p][j], xf[u], xs[p & 1][u], acc[u][j]);
             __builtin_amdgcn_sched_barrier(0);
             if constexpr (s < 3) xf[u] = read_x(k, s + 1, u);
             else {
@@ -155,12 +158,12 @@ __device__ __forceinline__ void mx_tile(const MxArgs& a, const MxSpan& t, int f,
             }
             // weights of the step before: its fragments are free
 #pragma unroll
-            for (int j = u; j < 2; j += U) {
+            for (int j = u; j < J; j += U) {
               if constexpr (s > 0) {
                 load_w1(k + RING, s - 1, p, j);
               } else {
                 load_w1(k + RING - 1, 3, (p + RING - 1) % RING, j);
-                if (j == 1) load_ws(k + RING - 1, (p + RING - 1) % RING);
+                if (j == J - 1) load_ws(k + RING - 1, (p + RING - 1) % RING);
               }
             }
             __builtin_amdgcn_sched_barrier(0);
@@ -172,14 +175,14 @@ __device__ __forceinline__ void mx_tile(const MxArgs& a, const MxSpan& t, int f,
     }
   }
   asm volatile("s_waitcnt vmcnt(0)" ::: "memory");  // no load of this workgroup's is under way to LDS
-  mx_epilogue<T, EPI, U>(a, t, f, wave, lane, acc);
+  mx_epilogue<T, EPI, U, J>(a, t, f, wave, lane, acc);
 #endif
 }
 
 // acc[u][j]: the lane's 16 consecutive features of token row `lane % 32` of row group u.
-template <typename T, int EPI, int U>
-__device__ __forceinline__ void mx_epilogue(const MxArgs& a, const MxSpan& t, int f, int wave, int lane, f32x16 (&acc)[U][2]) {
-  const int wg = (f * 4 + wave) * 2, col = lane & 31, half = lane >> 5;
+template <typename T, int EPI, int U, int J>
+__device__ __forceinline__ void mx_epilogue(const MxArgs& a, const MxSpan& t, int f, int wave, int lane, f32x16 (&acc)[U][J]) {
+  const int wg = (f * 4 + wave) * J, col = lane & 31, half = lane >> 5;
   if constexpr (EPI == MX_SILU) {
     const int blk = f * 4 + wave;  // of 32 activated features; the operand's last K tile is filled up with zeros
     const bool pad = blk >= a.act_blocks;
@@ -210,9 +213,9 @@ __device__ __forceinline__ void mx_epilogue(const MxArgs& a, const MxSpan& t, in
         const bool live = pair < a.n_pairs;
         const float s = live ? a.topk_w[pair] : 0.f;
         if (live && wg < a.w_groups) {
-          unsigned bytes[2];
+          unsigned bytes[2] = {};
 #pragma unroll
-          for (int j = 0; j < 2; ++j) {
+          for (int j = 0; j < J; ++j) {
             float v[16];
             unsigned amax = 0;
 #pragma unroll
@@ -248,15 +251,16 @@ __device__ __forceinline__ void mx_epilogue(const MxArgs& a, const MxSpan& t, in
                                    __builtin_amdgcn_perm(q[r + 5], q[r + 4], 0x05040100u), __builtin_amdgcn_perm(q[r + 7], q[r + 6], 0x05040100u)};
             }
           }
-          *reinterpret_cast<unsigned short*>(a.row_exps + static_cast<int64_t>(pair) * a.exp_pitch + wg * 2 + half * 2) =
-              static_cast<unsigned short>(bytes[0] | bytes[1] << 8);
+          unsigned char* exps = a.row_exps + static_cast<int64_t>(pair) * a.exp_pitch + (wg >> 1) * 4 + half * 2;
+          if constexpr (J == 2) *reinterpret_cast<unsigned short*>(exps) = static_cast<unsigned short>(bytes[0] | bytes[1] << 8);
+          else exps[wg & 1] = static_cast<unsigned char>(bytes[0]);
         }
       } else if constexpr (EPI == MX_PART) {
         const int pair = a.sorted[slot];
         if (pair < a.n_pairs) {
           const float s = a.topk_w[pair];
 #pragma unroll
-          for (int j = 0; j < 2; ++j) {
+          for (int j = 0; j < J; ++j) {
             if (wg + j < a.w_groups) {
               float* row = a.part_rows + (static_cast<int64_t>(blockIdx.y) * a.n_pairs + pair) * a.N + (wg + j) * 32 + half * 16;
 #pragma unroll
@@ -268,7 +272,7 @@ __device__ __forceinline__ void mx_epilogue(const MxArgs& a, const MxSpan& t, in
       } else {
         typedef T vec8 __attribute__((ext_vector_type(8)));
 #pragma unroll
-        for (int j = 0; j < 2; ++j) {
+        for (int j = 0; j < J; ++j) {
           const f32x16 v = acc[u][j];
           const int c = (wg + j) * 32 + half * 16;
           vec8 o[2];
@@ -291,15 +295,15 @@ __device__ __forceinline__ void mx_epilogue(const MxArgs& a, const MxSpan& t, in
   }
 }
 
-template <typename T, int EPI, bool NT>
+template <typename T, int EPI, int J, bool NT>
 __device__ __forceinline__ void mx_tile_of(const MxArgs& a, const MxSpan& t, int f, unsigned char* lds) {
-  if (t.units == 4) mx_tile<T, EPI, 4, NT>(a, t, f, lds);
-  else if (t.units == 3) mx_tile<T, EPI, 3, NT>(a, t, f, lds);
-  else if (t.units == 2) mx_tile<T, EPI, 2, NT>(a, t, f, lds);
-  else mx_tile<T, EPI, 1, NT>(a, t, f, lds);
+  if (t.units == 4) mx_tile<T, EPI, 4, J, NT>(a, t, f, lds);
+  else if (t.units == 3) mx_tile<T, EPI, 3, J, NT>(a, t, f, lds);
+  else if (t.units == 2) mx_tile<T, EPI, 2, J, NT>(a, t, f, lds);
+  else mx_tile<T, EPI, 1, J, NT>(a, t, f, lds);
 }
 
-template <typename T, int EPI, bool NT>
+template <typename T, int EPI, int J, bool NT>
 __global__ __launch_bounds__(kMxThreads, 2) void mx_gemm_kernel(MxArgs a) {
   extern __shared__ __attribute__((aligned(16))) unsigned char mx_lds[];
   // workgroups b, b + 8, .. share an XCD and its L2: an XCD takes a consecutive part of the walk
@@ -322,14 +326,15 @@ __global__ __launch_bounds__(kMxThreads, 2) void mx_gemm_kernel(MxArgs a) {
   const int base = e.count / e.n, rem = e.count - base * e.n;  // the first rem tiles are a row group taller
   const MxSpan t = {e.first + i0 * base + min(i0, rem), base + (i0 < rem ? 1 : 0), e.expert};
   // a tile alone on its weights reads them past the caches if the call streams them; those that share a weight tile meet in L2
-  if (NT && e.chunk_n == 1) mx_tile_of<T, EPI, true>(a, t, f, mx_lds);
-  else mx_tile_of<T, EPI, false>(a, t, f, mx_lds);
+  if (NT && e.chunk_n == 1) mx_tile_of<T, EPI, J, true>(a, t, f, mx_lds);
+  else mx_tile_of<T, EPI, J, false>(a, t, f, mx_lds);
 }
 
+constexpr int64_t kMxNarrowBelow = 128;  // workgroups, see launch_mx_gemm
 constexpr int kMxLds = kMxSlots * (kMxMaxUnits * 4096 + 1024);
 
 // More than 64 KB of LDS needs the kernel's limit raised, once per device (a set-up call, not stream work).
-template <typename T, int EPI, bool NT>
+template <typename T, int EPI, int J, bool NT>
 int mx_allow_lds() {
   constexpr int kMaxDevices = 64;
   static bool set[kMaxDevices] = {};  // a race between threads sets the same limit twice
@@ -337,7 +342,7 @@ int mx_allow_lds() {
   hipError_t e = hipGetDevice(&dev);
   if (e != hipSuccess || dev < 0 || dev >= kMaxDevices) return fail(FR_E_LAUNCH, "mxfp4 product: device %d (%s)", dev, hipGetErrorString(e));
   if (set[dev]) return FR_OK;
-  e = hipFuncSetAttribute(reinterpret_cast<const void*>(&mx_gemm_kernel<T, EPI, NT>), hipFuncAttributeMaxDynamicSharedMemorySize, kMxLds);
+  e = hipFuncSetAttribute(reinterpret_cast<const void*>(&mx_gemm_kernel<T, EPI, J, NT>), hipFuncAttributeMaxDynamicSharedMemorySize, kMxLds);
   if (e != hipSuccess) {
     (void)hipGetLastError();
     return fail(FR_E_LAUNCH, "mxfp4 product: %d bytes of LDS: %s", kMxLds, hipGetErrorString(e));
@@ -346,22 +351,32 @@ int mx_allow_lds() {
   return FR_OK;
 }
 
-template <typename T, int EPI, bool NT>
+template <typename T, int EPI, int J, bool NT>
 int launch_mx_gemm_as(const MxArgs& a, dim3 grid, hipStream_t st) {
-  const int rc = mx_allow_lds<T, EPI, NT>();
+  const int rc = mx_allow_lds<T, EPI, J, NT>();
   if (rc != FR_OK) return rc;
-  hipLaunchKernelGGL((mx_gemm_kernel<T, EPI, NT>), grid, dim3(kMxThreads), kMxLds, st, a);
+  hipLaunchKernelGGL((mx_gemm_kernel<T, EPI, J, NT>), grid, dim3(kMxThreads), kMxLds, st, a);
   return check_launch("mx_gemm_kernel");
 }
-
-// tiles: token tiles, at most; matrices: weight matrices that the call reads, at most
-template <typename T, int EPI>
-int launch_mx_gemm(const MxArgs& a, int64_t tiles, int64_t matrices, hipStream_t st, int slices = 1) {
+template <typename T, int EPI, int J>
+int launch_mx_gemm_wide(MxArgs a, int64_t tiles, int64_t matrices, hipStream_t st, int slices) {
+  if (EPI != MX_SILU) a.f_tiles = static_cast<int>(ceil_div(static_cast<int64_t>(a.w_groups), int64_t(4 * J)));
   const int64_t wgs = 8 * ceil_div(tiles * a.f_tiles, int64_t(8));
   FR_REQUIRE(wgs < (int64_t(1) << 31), FR_E_SHAPE, "mxfp4 product: %lld workgroups", (long long)wgs);
   const dim3 grid(static_cast<unsigned>(wgs), static_cast<unsigned>(slices));
-  if (mx_streams(matrices * a.w_groups * a.k_tiles * kMxUnit)) return launch_mx_gemm_as<T, EPI, true>(a, grid, st);
-  return launch_mx_gemm_as<T, EPI, false>(a, grid, st);
+  if (mx_streams(matrices * a.w_groups * a.k_tiles * kMxUnit)) return launch_mx_gemm_as<T, EPI, J, true>(a, grid, st);
+  return launch_mx_gemm_as<T, EPI, J, false>(a, grid, st);
+}
+
+// tiles: token tiles, at most; likely: token tiles with even loads; matrices: weight matrices that the call reads, at most.  Where tiles of 256 weight rows
+// would leave half of the CUs without a workgroup, tiles of 128: twice the workgroups, and twice the LDS reads per MFMA.  H = 4096, F = 14336, 8 experts,
+// 256 tokens (128 workgroups) down 72 -> 55 us; 200 x 12288 x 4096 (96) 16.0 -> 12.6; but 509 (192) 19.7 -> 21.0, 600 tokens (256) 77 -> 81.
+template <typename T, int EPI>
+int launch_mx_gemm(const MxArgs& a, int64_t tiles, int64_t likely, int64_t matrices, hipStream_t st, int slices = 1) {
+  if constexpr (EPI == MX_LINEAR || EPI == MX_DOWN) {
+    if (likely * ceil_div(static_cast<int64_t>(a.w_groups), int64_t(8)) <= kMxNarrowBelow) return launch_mx_gemm_wide<T, EPI, 1>(a, tiles, matrices, st, slices);
+  }
+  return launch_mx_gemm_wide<T, EPI, 2>(a, tiles, matrices, st, slices);
 }
 
 // out[m, :] = sum over the token's pairs, in order, of their weighted rows; a pair without an expert (a token row of NaN
@@ -520,14 +535,14 @@ extern "C" int fr_linear_mxfp4(const void* x, int dtype, int64_t M, int64_t K, i
   a.w = static_cast<const unsigned char*>(w_tiled);
   a.k_tiles = static_cast<int>(mx_tiles(K));
   a.w_groups = static_cast<int>(mx_groups(N));
-  a.f_tiles = static_cast<int>(ceil_div(static_cast<int64_t>(a.w_groups), int64_t(8)));
   a.x_groups = static_cast<int>(groups);
   a.out = out;
   a.ldo = N;
   a.M = M;
   a.N = static_cast<int>(N);
-  return dtype == FR_BF16 ? launch_mx_gemm<bf16_t, MX_LINEAR>(a, ceil_div(groups, int64_t(kMxMaxUnits)), 1, st)
-                          : launch_mx_gemm<f16_t, MX_LINEAR>(a, ceil_div(groups, int64_t(kMxMaxUnits)), 1, st);
+  const int64_t token_tiles = ceil_div(groups, int64_t(kMxMaxUnits));
+  return dtype == FR_BF16 ? launch_mx_gemm<bf16_t, MX_LINEAR>(a, token_tiles, token_tiles, 1, st)
+                          : launch_mx_gemm<f16_t, MX_LINEAR>(a, token_tiles, token_tiles, 1, st);
 }
 
 extern "C" int64_t fr_moe_mxfp4_workspace_bytes(int64_t M, int64_t H, int64_t F, int E, int topk) {
@@ -556,7 +571,7 @@ extern "C" int fr_fused_moe_mxfp4(const void* x, int dtype, const void* w1_tiled
     return mx_few_layer(x, dtype, w1_tiled, w2_tiled, logits, logits_dtype, M, H, F, E, topk, renormalize, out, workspace, static_cast<hipStream_t>(stream));
   const MxLayer l = mx_layer(workspace, M, H, F, E, topk);
   hipStream_t st = static_cast<hipStream_t>(stream);
-  const int64_t n = M * topk, experts = n < E ? n : E;
+  const int64_t n = M * topk, experts = n < E ? n : E, likely = experts * ceil_div(ceil_div(n, experts), int64_t(kMxMaxUnits) * kMxRows);
   if (route_align_fits(M, E, topk, false)) {
     rc = route_align_small(logits, logits_dtype, M, E, topk, renormalize, kMxRows, l.topk_w, l.topk_ids, l.sorted, l.expert_ids, l.npost, nullptr, 0,
                            nullptr, nullptr, st);
@@ -590,7 +605,7 @@ extern "C" int fr_fused_moe_mxfp4(const void* x, int dtype, const void* w1_tiled
   a.w_groups = static_cast<int>(2 * F / kMxRows);
   a.w_stride = static_cast<int64_t>(a.w_groups) * a.k_tiles * kMxUnit;
   a.f_tiles = 2 * a.act_tiles;  // whole units of activated features: the last ones are filled up with zeros
-  rc = launch_mx_gemm<bf16_t, MX_SILU>(a, l.tile_limit, experts, st);
+  rc = launch_mx_gemm<bf16_t, MX_SILU>(a, l.tile_limit, likely, experts, st);
   if (rc != FR_OK) return rc;
   // down
   a.x = l.act;
@@ -598,14 +613,13 @@ extern "C" int fr_fused_moe_mxfp4(const void* x, int dtype, const void* w1_tiled
   a.k_tiles = a.act_tiles;
   a.w_groups = static_cast<int>(H / kMxRows);
   a.w_stride = static_cast<int64_t>(a.w_groups) * a.k_tiles * kMxUnit;
-  a.f_tiles = static_cast<int>(ceil_div(static_cast<int64_t>(a.w_groups), int64_t(8)));
   a.rows = l.rows;
   a.row_exps = l.row_exps;
   a.exp_pitch = l.exp_pitch;
   a.N = static_cast<int>(H);
   if (l.slices > 1) {
     a.part_rows = l.part_rows;
-    rc = launch_mx_gemm<bf16_t, MX_PART>(a, l.tile_limit, experts, st, l.slices);
+    rc = launch_mx_gemm<bf16_t, MX_PART>(a, l.tile_limit, likely, experts, st, l.slices);
     if (rc != FR_OK) return rc;
     const dim3 grid(static_cast<unsigned>(ceil_div(M * (H / 4), int64_t(kMxThreads))));
     if (dtype == FR_BF16)
@@ -616,7 +630,7 @@ extern "C" int fr_fused_moe_mxfp4(const void* x, int dtype, const void* w1_tiled
                          static_cast<f16_t*>(out));
     return check_launch("mx_combine_parts_kernel");
   }
-  rc = launch_mx_gemm<bf16_t, MX_DOWN>(a, l.tile_limit, experts, st);
+  rc = launch_mx_gemm<bf16_t, MX_DOWN>(a, l.tile_limit, likely, experts, st);
   if (rc != FR_OK) return rc;
   const dim3 grid(static_cast<unsigned>(ceil_div(M * (H / 8), int64_t(kMxThreads))));
   if (dtype == FR_BF16)
