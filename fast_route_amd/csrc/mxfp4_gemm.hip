@@ -2,8 +2,8 @@
 //
 //   C[m, f] = sum_k X[m, k] W[f, k],   both operands e2m1 codes with a power-of-two scale per 32 elements of k, fp32 sums.
 //
-// A workgroup of four wavefronts computes a token tile of up to kMxMaxUnits row groups (32 rows each) x 256 weight rows: a
-// wavefront holds two units of weight rows against all token rows.
+// A workgroup of four wavefronts computes a token tile of up to kMxMaxUnits row groups (32 rows each) x 256 weight rows, or 128 where
+// workgroups are few: a wavefront holds J = 2 units of weight rows, or one, against all token rows.
 #include "mxfp4_few.h"
 
 namespace fr {

@@ -186,7 +186,10 @@ LAYERS = [  # M, H, F, E, topk, zipf
     (7, 1024, 512, 8, 2, False), (15, 320, 288, 16, 4, True), (16, 256, 768, 4, 1, False), (17, 512, 256, 8, 2, False),
     (24, 512, 1024, 8, 2, False), (60, 256, 512, 2, 2, False), (100, 288, 352, 5, 2, True), (130, 512, 256, 8, 2, False),
     (333, 256, 512, 8, 2, False), (700, 512, 256, 8, 2, True), (1500, 256, 320, 4, 2, False), (513, 128, 1408, 64, 6, True),
-    (2100, 64, 96, 200, 8, False), (300, 96, 64, 1, 1, False), (1025, 320, 288, 3, 2, True)]
+    (2100, 64, 96, 200, 8, False), (300, 96, 64, 1, 1, False), (1025, 320, 288, 3, 2, True),
+    # the last and first sizes on either side of the forms for few tokens, and of 256 and 128 weight rows per workgroup
+    (31, 256, 288, 16, 8, False), (32, 256, 288, 16, 8, True), (33, 256, 288, 16, 8, False), (32, 96, 160, 40, 9, False), (1, 64, 64, 256, 256, False),
+    (4, 1024, 256, 8, 2, False), (5, 1024, 256, 8, 2, False), (1200, 800, 128, 64, 6, True), (2000, 2080, 64, 64, 2, False)]
 
 
 @pytest.mark.parametrize("dtype", TYPES)
@@ -407,3 +410,100 @@ print("captured first calls ok")
 """
     run = subprocess.run([sys.executable, "-c", code], cwd=root, capture_output=True, text=True, timeout=110)
     assert run.returncode == 0 and "captured first calls ok" in run.stdout, run.stderr[-2000:]
+
+
+def _values64(codes, scales):
+    """What codes and scales on the GPU stand for, in 64 bits."""
+    from fast_route_amd import dequantize_rows_mxfp4
+    return dequantize_rows_mxfp4(codes, scales, dtype=torch.float32).double()
+
+
+def _held64(x):
+    """Rows [rows, K] on the GPU as the format holds them, in 64 bits."""
+    blocks = x.double().view(x.shape[0], -1, 32)
+    top = blocks.abs().amax(dim=2, keepdim=True)
+    unit = torch.ldexp(torch.ones_like(top), torch.frexp(top).exponent - 3)
+    v = blocks / torch.where(top > 0, unit, torch.ones_like(unit))
+    step = torch.where(v.abs() < 2, 0.5, torch.where(v.abs() < 4, 1.0, 2.0))
+    return ((torch.round(v / step) * step).clamp(-6, 6) * unit).reshape(x.shape)
+
+
+def _random_weights(shape, seed):
+    from fast_route_amd import quantize_rows_mxfp4
+    g = torch.Generator(device="cuda").manual_seed(seed)
+    w = torch.empty(shape, dtype=torch.bfloat16, device="cuda").normal_(0, 0.02, generator=g)
+    codes, scales = quantize_rows_mxfp4(w.view(-1, shape[-1]))
+    return codes.view(*shape[:-1], -1), scales.view(*shape[:-1], -1)
+
+
+@pytest.mark.parametrize("M", [2, 20, 100, 140, 600])
+def test_linear_on_weights_larger_than_the_caches_keep(native, M):
+    from fast_route_amd import linear_mxfp4, prepare_linear_mxfp4
+    N_, K = 70000, 4096
+    codes, scales = _random_weights((N_, K), 3)
+    x = _rows(M, K, torch.bfloat16, M).cuda()
+    got = linear_mxfp4(x, prepare_linear_mxfp4(codes, scales)).double()
+    xv = _held64(x)
+    for at in range(0, N_, 14000):
+        w = _values64(codes[at:at + 14000], scales[at:at + 14000])
+        ref, terms = xv @ w.t(), xv.abs() @ w.abs().t()
+        assert ((got[:, at:at + 14000] - ref).abs() <= 2.0 ** -8 * ref.abs() + _sum_error(terms, K) * 1.01).all()
+
+
+@pytest.mark.parametrize("M", [1, 6, 30, 45, 200, 700])
+def test_layer_on_weights_larger_than_the_caches_keep(native, M):
+    """Norm of the difference: half a step of bf16 in every value, 2^-8, and as much again for activated rows that rounded the other way
+    (test_layer bounds those one by one)."""
+    from fast_route_amd import fused_moe_mxfp4, prepare_weights_mxfp4
+    E, H, F, topk = 8, 4096, 8192, 2
+    w1, s1 = _random_weights((E, 2 * F, H), 5)
+    w2, s2 = _random_weights((E, H, F), 6)
+    g = torch.Generator(device="cuda").manual_seed(M)
+    x = torch.randn((M, H), device="cuda", generator=g).bfloat16()
+    logits = torch.randn((M, E), device="cuda", generator=g)
+    got = fused_moe_mxfp4(x, prepare_weights_mxfp4(w1, s1, w2, s2), logits, topk).double()
+    top, ids = torch.topk(logits.double(), topk, dim=1)
+    share, xv, ref = torch.softmax(top, dim=1), _held64(x), torch.zeros((M, H), dtype=torch.float64, device="cuda")
+    for e in range(E):
+        token, slot = (ids == e).nonzero(as_tuple=True)
+        if token.numel() == 0:
+            continue
+        both = xv[token] @ _values64(w1[e], s1[e]).t()
+        act = _held64(both[:, :F] * torch.sigmoid(both[:, :F]) * both[:, F:])
+        ref[token] += (act @ _values64(w2[e], s2[e]).t()) * share[token, slot][:, None]
+    assert (got - ref).norm() <= 2.0 ** -7 * ref.norm()
+    assert (got - ref).norm(dim=1).max() <= 2.0 ** -6 * ref.norm(dim=1).max()
+
+
+@pytest.mark.parametrize("M", [3, 100])
+def test_bad_weights_stay_in_their_expert(native, M):
+    """A NaN scale in w2 makes one output feature NaN, and only for tokens of that expert; one in w1 their whole rows."""
+    from fast_route_amd import fused_moe_mxfp4
+    E, H, F, k = 4, 256, 288, 2
+    x, logits, q = _layer_inputs(M, H, F, E, torch.bfloat16, 71)
+    good = fused_moe_mxfp4(x.cuda(), _prepared(q), logits.cuda(), k)
+    hit = (torch.topk(logits, k, dim=1).indices == 2).any(dim=1).cuda()
+    bad = [t.copy() for t in q]
+    bad[3][2, 33, 4] = 255
+    got = fused_moe_mxfp4(x.cuda(), _prepared(bad), logits.cuda(), k)
+    want = torch.zeros(M, H, dtype=torch.bool, device="cuda")
+    want[:, 33] = hit
+    assert torch.equal(got.isnan(), want) and torch.equal(got[~want], good[~want])
+    bad = [t.copy() for t in q]
+    bad[1][2, 100, 0] = 255
+    got = fused_moe_mxfp4(x.cuda(), _prepared(bad), logits.cuda(), k)
+    assert torch.equal(got.isnan(), hit[:, None].expand(M, H)) and torch.equal(got[~hit], good[~hit])
+
+
+def test_launches_of_a_few_tokens(native, kernels_of):
+    """Up to four tokens the whole layer is two launches, up to 32 three; a product of up to four rows is one."""
+    from fast_route_amd import fused_moe_mxfp4, linear_mxfp4, prepare_linear_mxfp4
+    x, logits, q = _layer_inputs(32, 256, 288, 8, torch.bfloat16, 5)
+    weights, x, logits = _prepared(q), x.cuda(), logits.cuda()
+    lin = prepare_linear_mxfp4(*(torch.from_numpy(t).cuda() for t in _weight(96, 256, 3)))
+    for M, layer, product in ((1, 2, 1), (4, 2, 1), (5, 3, 2), (32, 3, 2)):
+        for call, want in ((lambda: fused_moe_mxfp4(x[:M], weights, logits[:M], 2), layer), (lambda: linear_mxfp4(x[:M], lin), product)):
+            call()
+            torch.cuda.synchronize()
+            names = [n for n in kernels_of(call)[1] if "mx_" in n]
+            assert len(names) == want, names
