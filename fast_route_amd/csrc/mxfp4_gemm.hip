@@ -303,6 +303,16 @@ __device__ __forceinline__ void mx_tile_of(const MxArgs& a, const MxSpan& t, int
   else mx_tile<T, EPI, 1, J, NT>(a, t, f, lds);
 }
 
+// Blocks behind the last activated feature, up to a whole K tile: zero codes, scales of 1.
+__device__ __forceinline__ void mx_fill(const MxArgs& a, const MxSpan& t, int f) {
+  const int lane = threadIdx.x & 63, blk = f * 4 + (threadIdx.x >> 6), col = lane & 31;
+  for (int u = 0; u < t.units; ++u) {
+    unsigned char* unit = a.act + (static_cast<int64_t>(t.group + u) * a.act_tiles + (blk >> 3)) * kMxUnit;
+    *reinterpret_cast<uint2*>(unit + mx_code_at(col, blk & 7) + (lane >> 5) * 8) = uint2{0, 0};
+    if (lane < 32) unit[mx_scale_at(col, blk & 7)] = 127;
+  }
+}
+
 template <typename T, int EPI, int J, bool NT>
 __global__ __launch_bounds__(kMxThreads, 2) void mx_gemm_kernel(MxArgs a) {
   extern __shared__ __attribute__((aligned(16))) unsigned char mx_lds[];
@@ -325,6 +335,9 @@ __global__ __launch_bounds__(kMxThreads, 2) void mx_gemm_kernel(MxArgs a) {
   const int q = lin - e.chunk0 * a.f_tiles, f = q / e.chunk_n, i0 = e.chunk0 - e.index0 + q - f * e.chunk_n;
   const int base = e.count / e.n, rem = e.count - base * e.n;  // the first rem tiles are a row group taller
   const MxSpan t = {e.first + i0 * base + min(i0, rem), base + (i0 < rem ? 1 : 0), e.expert};
+  if constexpr (EPI == MX_SILU) {
+    if (f * 4 >= a.act_blocks) return mx_fill(a, t, f);
+  }
   // a tile alone on its weights reads them past the caches if the call streams them; those that share a weight tile meet in L2
   if (NT && e.chunk_n == 1) mx_tile_of<T, EPI, J, true>(a, t, f, mx_lds);
   else mx_tile_of<T, EPI, J, false>(a, t, f, mx_lds);
