@@ -406,14 +406,26 @@ __global__ __launch_bounds__(kMxThreads) void mx_combine_kernel(const uint4* __r
   const int c = static_cast<int>(i - m * per), b = c >> 1;
   const int at = (b & ~3) | (b & 1) << 1 | (b >> 1 & 1);
   float s[8] = {};
-  for (int j = 0; j < topk; ++j) {
-    const int64_t p = m * topk + j;
-    if (static_cast<unsigned>(ids[p]) >= static_cast<unsigned>(E)) continue;
-    const uint4 q = rows[p * per + c];
-    const float step = mx_row_step(exps[p * exp_pitch + at]);
-    const unsigned w[4] = {q.x, q.y, q.z, q.w};
+  // two pairs' loads under way together: 64 experts, H = 2048, top-6, 8192 tokens one / two / four 49 / 39 / 43 us, H = 4096, top-2, 16384 83 / 69 / 72
+  for (int j0 = 0; j0 < topk; j0 += 2) {
+    uint4 q[2];
+    unsigned e[2];
+    bool has[2];
 #pragma unroll
-    for (int r = 0; r < 8; ++r) s[r] += mx_row_value(static_cast<short>(w[r >> 1] >> (16 * (r & 1))), step);
+    for (int u = 0; u < 2; ++u) {
+      const int64_t p = m * topk + min(j0 + u, topk - 1);  // a pair without an expert has memory, but no row in it
+      has[u] = j0 + u < topk && static_cast<unsigned>(ids[p]) < static_cast<unsigned>(E);
+      q[u] = rows[p * per + c];
+      e[u] = exps[p * exp_pitch + at];
+    }
+#pragma unroll
+    for (int u = 0; u < 2; ++u) {
+      if (!has[u]) continue;
+      const float step = mx_row_step(e[u]);
+      const unsigned w[4] = {q[u].x, q[u].y, q[u].z, q[u].w};
+#pragma unroll
+      for (int r = 0; r < 8; ++r) s[r] += mx_row_value(static_cast<short>(w[r >> 1] >> (16 * (r & 1))), step);
+    }
   }
   vec8 o;
 #pragma unroll
