@@ -133,7 +133,8 @@ struct MxGather {
   int* tile_count = nullptr;
   MxTile* tiles = nullptr;
 };
-int mx_quant_tiled(const void* x, int dtype, int64_t rows, int64_t K, int64_t ldx, int64_t groups, const MxGather& g, void* out,
+// nt: x is read past the caches.
+int mx_quant_tiled(const void* x, int dtype, int64_t rows, int64_t K, int64_t ldx, int64_t groups, const MxGather& g, bool nt, void* out,
                    hipStream_t st);
 
 }  // namespace fr

@@ -632,7 +632,7 @@ int mx_few_linear(const void* x, int dtype, int64_t M, int64_t K, int64_t ldx, c
   a.out = out;
   const bool own = few_quantises(M, K);
   if (!own) {
-    const int rc = mx_quant_tiled(x, dtype, M, K, ldx, mx_groups(M), MxGather{}, workspace, st);
+    const int rc = mx_quant_tiled(x, dtype, M, K, ldx, mx_groups(M), MxGather{}, false, workspace, st);
     if (rc != FR_OK) return rc;
   }
   if (mx_streams(mx_groups(N) * a.k_tiles * kMxUnit)) dtype == FR_BF16 ? launch_few_linear<bf16_t, true>(a, own, st) : launch_few_linear<f16_t, true>(a, own, st);

@@ -553,7 +553,8 @@ extern "C" int fr_linear_mxfp4(const void* x, int dtype, int64_t M, int64_t K, i
   hipStream_t st = static_cast<hipStream_t>(stream);
   if (mx_few_linear_fits(M, N)) return mx_few_linear(x, dtype, M, K, ldx, w_tiled, N, out, workspace, st);
   const int64_t groups = mx_groups(M);
-  int rc = mx_quant_tiled(x, dtype, M, K, ldx, groups, MxGather{}, workspace, st);
+  // x is read past the caches where it and the result would not both stay: 8192 x 4096 in, 12288 features out 24 -> 17.5 us
+  int rc = mx_quant_tiled(x, dtype, M, K, ldx, groups, MxGather{}, mx_streams(2 * M * (K + N)), workspace, st);
   if (rc != FR_OK) return rc;
   MxArgs a = {};
   a.x = static_cast<const unsigned char*>(workspace);
@@ -612,7 +613,7 @@ extern "C" int fr_fused_moe_mxfp4(const void* x, int dtype, const void* w1_tiled
   g.topk = topk;
   g.tile_count = l.tile_count;
   g.tiles = l.tiles;
-  rc = mx_quant_tiled(x, dtype, n, H, H, l.groups, g, l.x, st);
+  rc = mx_quant_tiled(x, dtype, n, H, H, l.groups, g, false, l.x, st);
   if (rc != FR_OK) return rc;
   MxArgs a = {};
   a.tile_count = l.tile_count;

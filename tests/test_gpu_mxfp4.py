@@ -450,6 +450,43 @@ def test_linear_on_weights_larger_than_the_caches_keep(native, M):
         assert ((got[:, at:at + 14000] - ref).abs() <= 2.0 ** -8 * ref.abs() + _sum_error(terms, K) * 1.01).all()
 
 
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("apart", [0, 8])
+def test_rows_larger_than_the_caches_keep(native, dtype, apart):
+    """Codes, scales and values are those of the same rows in calls of 1000."""
+    from fast_route_amd import dequantize_rows_mxfp4, quantize_rows_mxfp4
+    rows, K = 17001, 4096
+    x = torch.randn((rows, K + apart), device="cuda", generator=torch.Generator(device="cuda").manual_seed(8)).to(dtype)[:, :K]
+    x[16000, 33] = float("nan")
+    codes, scales = quantize_rows_mxfp4(x)
+    values = [dequantize_rows_mxfp4(codes, scales, dtype=t) for t in (torch.float16, torch.bfloat16, torch.float32)]
+    for at in range(0, rows, 1000):
+        c, s = quantize_rows_mxfp4(x[at:at + 1000].contiguous())
+        assert torch.equal(codes[at:at + 1000], c) and torch.equal(scales[at:at + 1000], s)
+        for v in values:
+            assert torch.equal(v[at:at + 1000].nan_to_num(7e4), dequantize_rows_mxfp4(c, s, dtype=v.dtype).nan_to_num(7e4))
+    _same_codes(codes[-1001:], scales[-1001:], x[-1001:].cpu())
+
+
+@pytest.mark.parametrize("apart", [0, 8])
+def test_linear_of_rows_larger_than_the_caches_keep(native, apart):
+    from fast_route_amd import linear_mxfp4, prepare_linear_mxfp4
+    M, K, N_ = 8205, 2080, 6176
+    codes, scales = _random_weights((N_, K), 9)
+    x = torch.randn((M, K + apart), device="cuda", generator=torch.Generator(device="cuda").manual_seed(10)).bfloat16()[:, :K]
+    x[8200, 2079] = float("inf")
+    got = linear_mxfp4(x, prepare_linear_mxfp4(codes, scales)).double()
+    assert got[8200].isnan().all()
+    got[8200] = 0
+    w = _values64(codes, scales)
+    for at in range(0, M, 1641):
+        xv = _held64(x[at:at + 1641].contiguous()).nan_to_num(0.0)
+        if at <= 8200 < at + 1641:
+            xv[8200 - at] = 0
+        ref, terms = xv @ w.t(), xv.abs() @ w.abs().t()
+        assert ((got[at:at + 1641] - ref).abs() <= 2.0 ** -8 * ref.abs() + _sum_error(terms, K) * 1.01).all()
+
+
 @pytest.mark.parametrize("M", [1, 6, 30, 45, 200, 700])
 def test_layer_on_weights_larger_than_the_caches_keep(native, M):
     """Norm of the difference: half a step of bf16 in every value, 2^-8, and as much again for activated rows that rounded the other way
