@@ -42,12 +42,23 @@ struct MxArgs {
   // MX_LINEAR
   void* out;
   int64_t ldo;
+  bool out_past;       // whole lines of out are written past the caches
   int64_t M;
   int N;               // columns of rows / out
 };
 
+typedef unsigned u32x4 __attribute__((ext_vector_type(4)));
+
+// A lane holds 32 bytes of a row and feature unit, so its stores fill a line in four instructions of 64 scattered 16-byte pieces.  Where a wavefront has 64
+// features they are turned in LDS (32 rows of 128 bytes, a row group at a time) and leave as whole lines: 8192 x 12288 x 4096 213 -> 206 us, down product
+// of 64 experts, H = 2048, F = 1408, 8192 tokens 151 -> 144.  A result larger than the caches keep goes past them, to 189 us (286 in pieces); pairs'
+// rows do not, the sum over pairs finds them there (39 us against 45, the product itself 144 against 142).
+template <int EPI, int J>
+constexpr bool kMxTurned = J == 2 && (EPI == MX_LINEAR || EPI == MX_DOWN);
+constexpr int kMxTurnPitch = 128 + 16;
+
 template <typename T, int EPI, int U, int J>
-__device__ __forceinline__ void mx_epilogue(const MxArgs& a, const MxSpan& t, int f, int wave, int lane, f32x16 (&acc)[U][J]);
+__device__ __forceinline__ void mx_epilogue(const MxArgs& a, const MxSpan& t, int f, int wave, int lane, unsigned char* lds, f32x16 (&acc)[U][J]);
 
 // Token rows through LDS (every wavefront reads all of them), weights from memory to registers (no other wavefront reads them).  A
 // ring of kMxSlots K tiles of token rows and two of weights are under way.  All loads are spread between the MFMAs, a row
@@ -175,13 +186,14 @@ __device__ __forceinline__ void mx_tile(const MxArgs& a, const MxSpan& t, int f,
     }
   }
   asm volatile("s_waitcnt vmcnt(0)" ::: "memory");  // no load of this workgroup's is under way to LDS
-  mx_epilogue<T, EPI, U, J>(a, t, f, wave, lane, acc);
+  if constexpr (kMxTurned<EPI, J>) __syncthreads();  // nor does any wavefront still read there: it is the epilogue's
+  mx_epilogue<T, EPI, U, J>(a, t, f, wave, lane, lds + wave * (32 * kMxTurnPitch), acc);
 #endif
 }
 
 // acc[u][j]: the lane's 16 consecutive features of token row `lane % 32` of row group u.
 template <typename T, int EPI, int U, int J>
-__device__ __forceinline__ void mx_epilogue(const MxArgs& a, const MxSpan& t, int f, int wave, int lane, f32x16 (&acc)[U][J]) {
+__device__ __forceinline__ void mx_epilogue(const MxArgs& a, const MxSpan& t, int f, int wave, int lane, unsigned char* lds, f32x16 (&acc)[U][J]) {
   const int wg = (f * 4 + wave) * J, col = lane & 31, half = lane >> 5;
   if constexpr (EPI == MX_SILU) {
     const int blk = f * 4 + wave;  // of 32 activated features; the operand's last K tile is filled up with zeros
@@ -208,7 +220,26 @@ __device__ __forceinline__ void mx_epilogue(const MxArgs& a, const MxSpan& t, in
 #pragma unroll
     for (int u = 0; u < U; ++u) {
       const int64_t slot = static_cast<int64_t>(t.group + u) * kMxRows + col;
+      uint4* const turn = reinterpret_cast<uint4*>(lds + col * kMxTurnPitch + half * 32);
+      // rows of the group from LDS to `to(row)`, the address of their 64 features or null
+      auto turned = [&](auto to) {
+        __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+        __builtin_amdgcn_wave_barrier();
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+          const int r = i * 8 + (lane >> 3);
+          const uint4 v = *reinterpret_cast<const uint4*>(lds + r * kMxTurnPitch + (lane & 7) * 16);
+          uint4* const row = to(r);
+          if (row) {
+            if (EPI == MX_LINEAR && a.out_past) __builtin_nontemporal_store(__builtin_bit_cast(u32x4, v), reinterpret_cast<u32x4*>(row) + (lane & 7));
+            else row[lane & 7] = v;
+          }
+        }
+        __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+        __builtin_amdgcn_wave_barrier();
+      };
       if constexpr (EPI == MX_DOWN) {
+        const bool whole = kMxTurned<EPI, J> && wg + 1 < a.w_groups;
         const int pair = a.sorted[slot];
         const bool live = pair < a.n_pairs;
         const float s = live ? a.topk_w[pair] : 0.f;
@@ -244,7 +275,7 @@ __device__ __forceinline__ void mx_epilogue(const MxArgs& a, const MxSpan& t, in
                 if (magnitude(v[r]) >= 0x7F800000u) q[r] = v[r] != v[r] ? 0x8000u : v[r] > 0.f ? 0x7FFFu : 0x8001u;
             }
             if (wg + j < a.w_groups) {
-              uint4* row = a.rows + (static_cast<int64_t>(pair) * a.N + (wg + j) * 32 + half * 16) / 8;
+              uint4* row = whole ? turn + j * 4 : a.rows + (static_cast<int64_t>(pair) * a.N + (wg + j) * 32 + half * 16) / 8;
 #pragma unroll
               for (int r = 0; r < 16; r += 8)
                 row[r / 8] = uint4{__builtin_amdgcn_perm(q[r + 1], q[r], 0x05040100u), __builtin_amdgcn_perm(q[r + 3], q[r + 2], 0x05040100u),
@@ -255,6 +286,11 @@ __device__ __forceinline__ void mx_epilogue(const MxArgs& a, const MxSpan& t, in
           if constexpr (J == 2) *reinterpret_cast<unsigned short*>(exps) = static_cast<unsigned short>(bytes[0] | bytes[1] << 8);
           else exps[wg & 1] = static_cast<unsigned char>(bytes[0]);
         }
+        if (whole)
+          turned([&](int r) {
+            const int p = __shfl(pair, r);
+            return p < a.n_pairs ? a.rows + (static_cast<int64_t>(p) * a.N + wg * 32) / 8 : nullptr;
+          });
       } else if constexpr (EPI == MX_PART) {
         const int pair = a.sorted[slot];
         if (pair < a.n_pairs) {
@@ -271,6 +307,7 @@ __device__ __forceinline__ void mx_epilogue(const MxArgs& a, const MxSpan& t, in
         }
       } else {
         typedef T vec8 __attribute__((ext_vector_type(8)));
+        const bool whole = kMxTurned<EPI, J> && (wg + 2) * 32 <= a.N && (a.ldo & 7) == 0;
 #pragma unroll
         for (int j = 0; j < J; ++j) {
           const f32x16 v = acc[u][j];
@@ -278,7 +315,10 @@ __device__ __forceinline__ void mx_epilogue(const MxArgs& a, const MxSpan& t, in
           vec8 o[2];
 #pragma unroll
           for (int r = 0; r < 16; ++r) o[r >> 3][r & 7] = static_cast<T>(v[r]);
-          if (slot < a.M) {
+          if (whole) {
+            turn[j * 4] = __builtin_bit_cast(uint4, o[0]);
+            turn[j * 4 + 1] = __builtin_bit_cast(uint4, o[1]);
+          } else if (slot < a.M) {
             T* row = static_cast<T*>(a.out) + slot * a.ldo + c;
             if (c + 16 <= a.N && (a.ldo & 7) == 0) {
               *reinterpret_cast<vec8*>(row) = o[0];
@@ -290,6 +330,11 @@ __device__ __forceinline__ void mx_epilogue(const MxArgs& a, const MxSpan& t, in
             }
           }
         }
+        if (whole)
+          turned([&](int r) {
+            const int64_t m = static_cast<int64_t>(t.group + u) * kMxRows + r;
+            return m < a.M ? reinterpret_cast<uint4*>(static_cast<T*>(a.out) + m * a.ldo + wg * 32) : nullptr;
+          });
       }
     }
   }
@@ -345,6 +390,7 @@ __global__ __launch_bounds__(kMxThreads, 2) void mx_gemm_kernel(MxArgs a) {
 
 constexpr int64_t kMxNarrowBelow = 128;  // workgroups, see launch_mx_gemm
 constexpr int kMxLds = kMxSlots * (kMxMaxUnits * 4096 + 1024);
+static_assert(kMxThreads / 64 * 32 * kMxTurnPitch <= kMxLds, "the epilogue's rows lie in the ring");
 
 // More than 64 KB of LDS needs the kernel's limit raised, once per device (a set-up call, not stream work).
 template <typename T, int EPI, int J, bool NT>
@@ -564,6 +610,7 @@ extern "C" int fr_linear_mxfp4(const void* x, int dtype, int64_t M, int64_t K, i
   a.x_groups = static_cast<int>(groups);
   a.out = out;
   a.ldo = N;
+  a.out_past = mx_streams(2 * M * N);
   a.M = M;
   a.N = static_cast<int>(N);
   const int64_t token_tiles = ceil_div(groups, int64_t(kMxMaxUnits));

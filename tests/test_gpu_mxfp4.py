@@ -468,13 +468,13 @@ def test_rows_larger_than_the_caches_keep(native, dtype, apart):
     _same_codes(codes[-1001:], scales[-1001:], x[-1001:].cpu())
 
 
-@pytest.mark.parametrize("apart", [0, 8])
-def test_linear_of_rows_larger_than_the_caches_keep(native, apart):
+@pytest.mark.parametrize("apart,K,N_", [(0, 2080, 6176), (8, 2080, 6176), (0, 2080, 8264), (0, 2080, 8260)])
+def test_linear_of_rows_larger_than_the_caches_keep(native, apart, K, N_):
     from fast_route_amd import linear_mxfp4, prepare_linear_mxfp4
-    M, K, N_ = 8205, 2080, 6176
+    M = 8205
     codes, scales = _random_weights((N_, K), 9)
     x = torch.randn((M, K + apart), device="cuda", generator=torch.Generator(device="cuda").manual_seed(10)).bfloat16()[:, :K]
-    x[8200, 2079] = float("inf")
+    x[8200, K - 1] = float("inf")
     got = linear_mxfp4(x, prepare_linear_mxfp4(codes, scales)).double()
     assert got[8200].isnan().all()
     got[8200] = 0
