@@ -337,7 +337,7 @@ int fr_mxfp4_tile_weights(const void* codes, const void* scales, int64_t matrice
 
 /* out[M, N] = q(x)[M, K] @ w[N, K]^T: x (f16 / bf16, row stride ldx, a multiple of 8) quantised to MXFP4 on the way, w laid out by
  * fr_mxfp4_tile_weights(.., 1, N, K, 0, ..), fp32 accumulation, out dense in x's type.  M and N any size;
- * `workspace`: 256-byte aligned, fr_linear_mxfp4_workspace_bytes(M, N, K) bytes. */
+ * `workspace`: 256-byte aligned, fr_linear_mxfp4_workspace_bytes(M, N, K) bytes (0: none is needed, may be NULL). */
 int64_t fr_linear_mxfp4_workspace_bytes(int64_t M, int64_t N, int64_t K);
 int fr_linear_mxfp4(const void* x, int dtype, int64_t M, int64_t K, int64_t ldx, const void* w_tiled, int64_t N, void* out,
                     void* workspace, int64_t workspace_bytes, void* stream);
