@@ -91,20 +91,6 @@ __device__ __forceinline__ unsigned mx_pair_max(unsigned v) {
   return v > o ? v : o;
 }
 
-// A pair's weighted row between the down product and the sum over a token's pairs: 16 consecutive values as 16-bit integers times a shared
-// step, |q| <= 32766.  A value is off by at most half a step, 2^-15 of the largest of its 16 (1e-5 of a row's values on average, a
-// twentieth of the last rounding to fp16), in little more than half the bytes of fp32.  An infinity is +-32767, a NaN -32768.
-constexpr int kMxRowBlock = 16;
-constexpr float kMxRowMagic = 12582912.f;  // 3 2^22: the low bits of a sum with it are the integer nearest to the other summand
-// exponent byte k + 127 of a block whose largest finite magnitude, in [2^k, 2^(k + 1)), has these bits; below 2^-112 the step no longer shrinks
-__device__ __forceinline__ unsigned mx_row_byte(unsigned amax) { return max(amax >> 23, 15u); }
-__device__ __forceinline__ float mx_row_factor(unsigned byte) { return __uint_as_float((127 + 14 + 127 - byte) << 23) * (1.f - 0x1p-14f); }
-__device__ __forceinline__ float mx_row_step(unsigned byte) { return __uint_as_float((byte - 14) << 23) * (1.f / (1.f - 0x1p-14f)); }
-__device__ __forceinline__ float mx_row_value(int q, float step) {
-  const float v = static_cast<float>(q) * step;
-  return q == 32767 ? __builtin_inff() : q > -32767 ? v : q == -32768 ? __builtin_nanf("") : -__builtin_inff();
-}
-
 // Weights that a call reads once and that are more than the memory-side cache (256 MB) may keep from one call to the next are read past the
 // caches: 8 experts, H = 4096, F = 14336, 40 tokens gate/up 91.7 -> 85.4 us, down 47.0 -> 43.9; but H = 1024, F = 3584 (17 MB), 50 tokens
 // 7.9 -> 9.0, 10.6 -> 15.1.

@@ -11,6 +11,8 @@ namespace {
 
 constexpr int kMxThreads = 256;
 enum { MX_LINEAR = 0, MX_SILU = 1, MX_DOWN = 2, MX_PART = 3 };  // MX_PART: the down product, K cut over workgroups
+template <int EPI>
+constexpr bool kMxPairs = EPI == MX_DOWN || EPI == MX_PART;  // results are weighted rows of pairs
 
 // What a workgroup multiplies: row groups group .. group + units - 1 of an expert's.
 struct MxSpan {
@@ -31,14 +33,11 @@ struct MxArgs {
   // MX_SILU: operand of the activated rows, its tiles along K, blocks of 32 activated features
   unsigned char* act;
   int act_tiles, act_blocks;
-  // MX_DOWN: rows of the pairs
+  // MX_DOWN, MX_PART: rows of the pairs
   const int32_t* sorted;
   const float* topk_w;
   int n_pairs;
-  uint4* rows;             // [n_pairs, N] integers, eight to an element
-  unsigned char* row_exps; // [n_pairs, exp_pitch]: blocks 4 i + (0, 1, 2, 3) at 4 i + (0, 2, 1, 3)
-  int exp_pitch;
-  float* part_rows;        // MX_PART: [slices][n_pairs, N]
+  float* rows;             // [slices][n_pairs, N]; MX_DOWN: one slice
   // MX_LINEAR
   void* out;
   int64_t ldo;
@@ -49,13 +48,16 @@ struct MxArgs {
 
 typedef unsigned u32x4 __attribute__((ext_vector_type(4)));
 
-// A lane holds 32 bytes of a row and feature unit, so its stores fill a line in four instructions of 64 scattered 16-byte pieces.  Where a wavefront has 64
-// features they are turned in LDS (32 rows of 128 bytes, a row group at a time) and leave as whole lines: 8192 x 12288 x 4096 213 -> 206 us, down product
-// of 64 experts, H = 2048, F = 1408, 8192 tokens 151 -> 144.  A result larger than the caches keep goes past them, to 189 us (286 in pieces); pairs'
-// rows do not, the sum over pairs finds them there (39 us against 45, the product itself 144 against 142).
+// A lane holds 16 consecutive features of a row and feature unit, so its stores fill lines in instructions of 64 scattered 16-byte pieces.  Where a
+// wavefront has 64 features they are turned in LDS (32 rows of 64 features, a row group at a time) and leave as whole lines: 8192 x 12288 x 4096 213 -> 206 us,
+// down product of 64 experts, H = 2048, F = 1408, 8192 tokens 208 -> 175, of 8, H = 4096, F = 14336, 16384 1112 -> 1067; K slices would lose, 50 tokens on 8
+// experts, H = 1024, F = 3584 6.7 -> 7.3.  A product larger than the caches keep goes past them, @@ (286 in pieces).
 template <int EPI, int J>
 constexpr bool kMxTurned = J == 2 && (EPI == MX_LINEAR || EPI == MX_DOWN);
-constexpr int kMxTurnPitch = 128 + 16;
+template <int EPI>
+constexpr int kMxTurnPieces = kMxPairs<EPI> ? 16 : 8;  // 16-byte pieces of a row: fp32, or a 2-byte type
+template <int EPI>
+constexpr int kMxTurnPitch = kMxTurnPieces<EPI> * 16 + 16;
 
 template <typename T, int EPI, int U, int J>
 __device__ __forceinline__ void mx_epilogue(const MxArgs& a, const MxSpan& t, int f, int wave, int lane, unsigned char* lds, f32x16 (&acc)[U][J]);
@@ -187,7 +189,7 @@ __device__ __forceinline__ void mx_tile(const MxArgs& a, const MxSpan& t, int f,
   }
   asm volatile("s_waitcnt vmcnt(0)" ::: "memory");  // no load of this workgroup's is under way to LDS
   if constexpr (kMxTurned<EPI, J>) __syncthreads();  // nor does any wavefront still read there: it is the epilogue's
-  mx_epilogue<T, EPI, U, J>(a, t, f, wave, lane, lds + wave * (32 * kMxTurnPitch), acc);
+  mx_epilogue<T, EPI, U, J>(a, t, f, wave, lane, lds + wave * (32 * kMxTurnPitch<EPI>), acc);
 #endif
 }
 
@@ -219,92 +221,49 @@ __device__ __forceinline__ void mx_epilogue(const MxArgs& a, const MxSpan& t, in
   } else {
 #pragma unroll
     for (int u = 0; u < U; ++u) {
+      constexpr int PIECES = kMxTurnPieces<EPI>, PITCH = kMxTurnPitch<EPI>;
       const int64_t slot = static_cast<int64_t>(t.group + u) * kMxRows + col;
-      uint4* const turn = reinterpret_cast<uint4*>(lds + col * kMxTurnPitch + half * 32);
+      u32x4* const turn = reinterpret_cast<u32x4*>(lds + col * PITCH + half * (PIECES * 4));  // + j * PIECES / 2: the lane's pieces of unit j
       // rows of the group from LDS to `to(row)`, the address of their 64 features or null
       auto turned = [&](auto to) {
         __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
         __builtin_amdgcn_wave_barrier();
 #pragma unroll
-        for (int i = 0; i < 4; ++i) {
-          const int r = i * 8 + (lane >> 3);
-          const uint4 v = *reinterpret_cast<const uint4*>(lds + r * kMxTurnPitch + (lane & 7) * 16);
-          uint4* const row = to(r);
+        for (int i = 0; i < PIECES / 2; ++i) {
+          const int r = i * (64 / PIECES) + lane / PIECES;
+          const u32x4 v = *reinterpret_cast<const u32x4*>(lds + r * PITCH + lane % PIECES * 16);
+          u32x4* const row = to(r);
           if (row) {
-            if (EPI == MX_LINEAR && a.out_past) __builtin_nontemporal_store(__builtin_bit_cast(u32x4, v), reinterpret_cast<u32x4*>(row) + (lane & 7));
-            else row[lane & 7] = v;
+            if (EPI == MX_LINEAR && a.out_past) __builtin_nontemporal_store(v, row + lane % PIECES);
+            else row[lane % PIECES] = v;
           }
         }
         __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
         __builtin_amdgcn_wave_barrier();
       };
-      if constexpr (EPI == MX_DOWN) {
+      if constexpr (kMxPairs<EPI>) {
+        // Weighted rows stay in fp32 until the pairs are summed.
         const bool whole = kMxTurned<EPI, J> && wg + 1 < a.w_groups;
         const int pair = a.sorted[slot];
         const bool live = pair < a.n_pairs;
         const float s = live ? a.topk_w[pair] : 0.f;
-        if (live && wg < a.w_groups) {
-          unsigned bytes[2] = {};
+        float* const rows = a.rows + (EPI == MX_PART ? static_cast<int64_t>(blockIdx.y) * a.n_pairs * a.N : 0) + wg * 32;
+        if (live) {
 #pragma unroll
           for (int j = 0; j < J; ++j) {
-            float v[16];
-            unsigned amax = 0;
-#pragma unroll
-            for (int r = 0; r < 16; ++r) {
-              v[r] = acc[u][j][r] * s;
-              const unsigned m = magnitude(v[r]);
-              amax = amax > m ? amax : m;
-            }
-            const bool odd = amax >= 0x7F800000u;
-            if (odd) {
-              amax = 0;
-#pragma unroll
-              for (int r = 0; r < 16; ++r) {
-                const unsigned m = magnitude(v[r]);
-                amax = m < 0x7F800000u && m > amax ? m : amax;
-              }
-            }
-            bytes[j] = mx_row_byte(amax);
-            const float factor = mx_row_factor(bytes[j]);
-            unsigned q[16];
-#pragma unroll
-            for (int r = 0; r < 16; ++r) q[r] = __float_as_uint(__builtin_fmaf(v[r], factor, kMxRowMagic));
-            if (odd) {
-#pragma unroll
-              for (int r = 0; r < 16; ++r)
-                if (magnitude(v[r]) >= 0x7F800000u) q[r] = v[r] != v[r] ? 0x8000u : v[r] > 0.f ? 0x7FFFu : 0x8001u;
-            }
             if (wg + j < a.w_groups) {
-              uint4* row = whole ? turn + j * 4 : a.rows + (static_cast<int64_t>(pair) * a.N + (wg + j) * 32 + half * 16) / 8;
+              u32x4* const row = whole ? turn + j * (PIECES / 2) : reinterpret_cast<u32x4*>(rows + static_cast<int64_t>(pair) * a.N + j * 32 + half * 16);
 #pragma unroll
-              for (int r = 0; r < 16; r += 8)
-                row[r / 8] = uint4{__builtin_amdgcn_perm(q[r + 1], q[r], 0x05040100u), __builtin_amdgcn_perm(q[r + 3], q[r + 2], 0x05040100u),
-                                   __builtin_amdgcn_perm(q[r + 5], q[r + 4], 0x05040100u), __builtin_amdgcn_perm(q[r + 7], q[r + 6], 0x05040100u)};
+              for (int r = 0; r < 16; r += 4)
+                row[r / 4] = __builtin_bit_cast(u32x4, f32x4{acc[u][j][r] * s, acc[u][j][r + 1] * s, acc[u][j][r + 2] * s, acc[u][j][r + 3] * s});
             }
           }
-          unsigned char* exps = a.row_exps + static_cast<int64_t>(pair) * a.exp_pitch + (wg >> 1) * 4 + half * 2;
-          if constexpr (J == 2) *reinterpret_cast<unsigned short*>(exps) = static_cast<unsigned short>(bytes[0] | bytes[1] << 8);
-          else exps[wg & 1] = static_cast<unsigned char>(bytes[0]);
         }
         if (whole)
           turned([&](int r) {
             const int p = __shfl(pair, r);
-            return p < a.n_pairs ? a.rows + (static_cast<int64_t>(p) * a.N + wg * 32) / 8 : nullptr;
+            return p < a.n_pairs ? reinterpret_cast<u32x4*>(rows + static_cast<int64_t>(p) * a.N) : nullptr;
           });
-      } else if constexpr (EPI == MX_PART) {
-        const int pair = a.sorted[slot];
-        if (pair < a.n_pairs) {
-          const float s = a.topk_w[pair];
-#pragma unroll
-          for (int j = 0; j < J; ++j) {
-            if (wg + j < a.w_groups) {
-              float* row = a.part_rows + (static_cast<int64_t>(blockIdx.y) * a.n_pairs + pair) * a.N + (wg + j) * 32 + half * 16;
-#pragma unroll
-              for (int r = 0; r < 16; r += 4)
-                *reinterpret_cast<f32x4*>(row + r) = f32x4{acc[u][j][r] * s, acc[u][j][r + 1] * s, acc[u][j][r + 2] * s, acc[u][j][r + 3] * s};
-            }
-          }
-        }
       } else {
         typedef T vec8 __attribute__((ext_vector_type(8)));
         const bool whole = kMxTurned<EPI, J> && (wg + 2) * 32 <= a.N && (a.ldo & 7) == 0;
@@ -316,8 +275,8 @@ __device__ __forceinline__ void mx_epilogue(const MxArgs& a, const MxSpan& t, in
 #pragma unroll
           for (int r = 0; r < 16; ++r) o[r >> 3][r & 7] = static_cast<T>(v[r]);
           if (whole) {
-            turn[j * 4] = __builtin_bit_cast(uint4, o[0]);
-            turn[j * 4 + 1] = __builtin_bit_cast(uint4, o[1]);
+            turn[j * (PIECES / 2)] = __builtin_bit_cast(u32x4, o[0]);
+            turn[j * (PIECES / 2) + 1] = __builtin_bit_cast(u32x4, o[1]);
           } else if (slot < a.M) {
             T* row = static_cast<T*>(a.out) + slot * a.ldo + c;
             if (c + 16 <= a.N && (a.ldo & 7) == 0) {
@@ -333,7 +292,7 @@ __device__ __forceinline__ void mx_epilogue(const MxArgs& a, const MxSpan& t, in
         if (whole)
           turned([&](int r) {
             const int64_t m = static_cast<int64_t>(t.group + u) * kMxRows + r;
-            return m < a.M ? reinterpret_cast<uint4*>(static_cast<T*>(a.out) + m * a.ldo + wg * 32) : nullptr;
+            return m < a.M ? reinterpret_cast<u32x4*>(static_cast<T*>(a.out) + m * a.ldo + wg * 32) : nullptr;
           });
       }
     }
@@ -390,7 +349,7 @@ __global__ __launch_bounds__(kMxThreads, 2) void mx_gemm_kernel(MxArgs a) {
 
 constexpr int64_t kMxNarrowBelow = 128;  // workgroups, see launch_mx_gemm
 constexpr int kMxLds = kMxSlots * (kMxMaxUnits * 4096 + 1024);
-static_assert(kMxThreads / 64 * 32 * kMxTurnPitch <= kMxLds, "the epilogue's rows lie in the ring");
+static_assert(kMxThreads / 64 * 32 * kMxTurnPitch<MX_DOWN> <= kMxLds, "the epilogue's rows lie in the ring");
 
 // More than 64 KB of LDS needs the kernel's limit raised, once per device (a set-up call, not stream work).
 template <typename T, int EPI, int J, bool NT>
@@ -438,51 +397,12 @@ int launch_mx_gemm(const MxArgs& a, int64_t tiles, int64_t likely, int64_t matri
   return launch_mx_gemm_wide<T, EPI, 2>(a, tiles, matrices, st, slices);
 }
 
-// out[m, :] = sum over the token's pairs, in order, of their weighted rows; a pair without an expert (a token row of NaN
-// logits) has no row.
+// out[m, :] = sum over the token's pairs and their slices, in order, of weighted rows [slices][n, H]; a pair without an expert (a
+// token row of NaN logits) has no row.  Bound by memory: each row is read once, past the caches, two of a token's under way together.  64 experts, H = 2048,
+// top-6, 8192 tokens one / two / four at a time 99 / 96 / 96 us, two past the caches 73 (435 MB, 6.0 TB/s); H = 4096, top-2, 16384 129 / 113 / 128, 111.
 template <typename T>
-__global__ __launch_bounds__(kMxThreads) void mx_combine_kernel(const uint4* __restrict__ rows, const unsigned char* __restrict__ exps, int exp_pitch,
-                                                                const int32_t* __restrict__ ids, int E, int topk, int64_t M, int H,
-                                                                T* __restrict__ out) {
-  typedef T vec8 __attribute__((ext_vector_type(8)));
-  const int per = H / 8;
-  const int64_t i = static_cast<int64_t>(blockIdx.x) * kMxThreads + threadIdx.x;
-  if (i >= M * per) return;
-  const int64_t m = i / per;
-  const int c = static_cast<int>(i - m * per), b = c >> 1;
-  const int at = (b & ~3) | (b & 1) << 1 | (b >> 1 & 1);
-  float s[8] = {};
-  // two pairs' loads under way together: 64 experts, H = 2048, top-6, 8192 tokens one / two / four 49 / 39 / 43 us, H = 4096, top-2, 16384 83 / 69 / 72
-  for (int j0 = 0; j0 < topk; j0 += 2) {
-    uint4 q[2];
-    unsigned e[2];
-    bool has[2];
-#pragma unroll
-    for (int u = 0; u < 2; ++u) {
-      const int64_t p = m * topk + min(j0 + u, topk - 1);  // a pair without an expert has memory, but no row in it
-      has[u] = j0 + u < topk && static_cast<unsigned>(ids[p]) < static_cast<unsigned>(E);
-      q[u] = rows[p * per + c];
-      e[u] = exps[p * exp_pitch + at];
-    }
-#pragma unroll
-    for (int u = 0; u < 2; ++u) {
-      if (!has[u]) continue;
-      const float step = mx_row_step(e[u]);
-      const unsigned w[4] = {q[u].x, q[u].y, q[u].z, q[u].w};
-#pragma unroll
-      for (int r = 0; r < 8; ++r) s[r] += mx_row_value(static_cast<short>(w[r >> 1] >> (16 * (r & 1))), step);
-    }
-  }
-  vec8 o;
-#pragma unroll
-  for (int r = 0; r < 8; ++r) o[r] = static_cast<T>(s[r]);
-  *reinterpret_cast<vec8*>(out + i * 8) = o;
-}
-
-// The same from fp32 rows of K slices, added in order.
-template <typename T>
-__global__ __launch_bounds__(kMxThreads) void mx_combine_parts_kernel(const float* __restrict__ rows, int slices, int64_t n, const int32_t* __restrict__ ids,
-                                                                      int E, int topk, int64_t M, int H, T* __restrict__ out) {
+__global__ __launch_bounds__(kMxThreads) void mx_combine_kernel(const float* __restrict__ rows, int slices, int64_t n, const int32_t* __restrict__ ids,
+                                                                int E, int topk, int64_t M, int H, T* __restrict__ out) {
   typedef T vec4 __attribute__((ext_vector_type(4)));
   const int per = H / 4;
   const int64_t i = static_cast<int64_t>(blockIdx.x) * kMxThreads + threadIdx.x;
@@ -490,13 +410,25 @@ __global__ __launch_bounds__(kMxThreads) void mx_combine_parts_kernel(const floa
   const int64_t m = i / per;
   const int c = static_cast<int>(i - m * per) * 4;
   f32x4 s = {0.f, 0.f, 0.f, 0.f};
-  for (int j = 0; j < topk; ++j) {
-    const int64_t p = m * topk + j;
-    if (static_cast<unsigned>(ids[p]) >= static_cast<unsigned>(E)) continue;
-    for (int v = 0; v < slices; ++v) {
-      const f32x4 t = *reinterpret_cast<const f32x4*>(rows + (v * n + p) * H + c);
+  int j = 0, v = 0;  // next pair of the token and slice
+  while (j < topk) {
+    f32x4 q[2];
+    bool has[2];
 #pragma unroll
-      for (int r = 0; r < 4; ++r) s[r] += t[r];
+    for (int u = 0; u < 2; ++u) {
+      const int64_t p = m * topk + min(j, topk - 1);  // a pair without an expert has memory, but no row in it
+      has[u] = j < topk && static_cast<unsigned>(ids[p]) < static_cast<unsigned>(E);
+      q[u] = __builtin_nontemporal_load(reinterpret_cast<const f32x4*>(rows + (v * n + p) * H + c));
+      if (++v == slices) {
+        v = 0;
+        ++j;
+      }
+    }
+#pragma unroll
+    for (int u = 0; u < 2; ++u) {
+      if (!has[u]) continue;
+#pragma unroll
+      for (int r = 0; r < 4; ++r) s[r] += q[u][r];
     }
   }
   vec4 o;
@@ -514,11 +446,8 @@ struct MxLayer {
   int* tile_count;
   MxTile* tiles;
   unsigned char *x, *act;
-  uint4* rows;
-  unsigned char* row_exps;
-  int exp_pitch;
-  int slices;  // of the down product's K
-  float* part_rows;
+  int slices;   // of the down product's K
+  float* rows;  // [slices][n, H]
 };
 
 // K slices of the down product: where its workgroups are few (a narrow layer, few rows) more of them, of four K tiles at least, as long
@@ -555,10 +484,7 @@ MxLayer mx_layer(void* ws, int64_t M, int64_t H, int64_t F, int E, int topk) {
   l.x = b.take<unsigned char>(l.groups * mx_tiles(H) * kMxUnit);
   l.act = b.take<unsigned char>(l.groups * mx_tiles(F) * kMxUnit);
   l.slices = mx_slices(n, H, F, E);
-  l.part_rows = b.take<float>(l.slices > 1 ? l.slices * n * H : 0);
-  l.rows = b.take<uint4>(l.slices > 1 ? 0 : n * H / 8);
-  l.exp_pitch = static_cast<int>(ceil_div(H, 2 * kMxRows)) * 4;
-  l.row_exps = b.take<unsigned char>(l.slices > 1 ? 0 : n * l.exp_pitch);
+  l.rows = b.take<float>(l.slices * n * H);
   l.bytes = b.at;
   return l;
 }
@@ -687,28 +613,14 @@ extern "C" int fr_fused_moe_mxfp4(const void* x, int dtype, const void* w1_tiled
   a.w_groups = static_cast<int>(H / kMxRows);
   a.w_stride = static_cast<int64_t>(a.w_groups) * a.k_tiles * kMxUnit;
   a.rows = l.rows;
-  a.row_exps = l.row_exps;
-  a.exp_pitch = l.exp_pitch;
   a.N = static_cast<int>(H);
-  if (l.slices > 1) {
-    a.part_rows = l.part_rows;
-    rc = launch_mx_gemm<bf16_t, MX_PART>(a, l.tile_limit, likely, experts, st, l.slices);
-    if (rc != FR_OK) return rc;
-    const dim3 grid(static_cast<unsigned>(ceil_div(M * (H / 4), int64_t(kMxThreads))));
-    if (dtype == FR_BF16)
-      hipLaunchKernelGGL((mx_combine_parts_kernel<bf16_t>), grid, dim3(kMxThreads), 0, st, l.part_rows, l.slices, n, l.topk_ids, E, topk, M, (int)H,
-                         static_cast<bf16_t*>(out));
-    else
-      hipLaunchKernelGGL((mx_combine_parts_kernel<f16_t>), grid, dim3(kMxThreads), 0, st, l.part_rows, l.slices, n, l.topk_ids, E, topk, M, (int)H,
-                         static_cast<f16_t*>(out));
-    return check_launch("mx_combine_parts_kernel");
-  }
-  rc = launch_mx_gemm<bf16_t, MX_DOWN>(a, l.tile_limit, likely, experts, st);
+  rc = l.slices > 1 ? launch_mx_gemm<bf16_t, MX_PART>(a, l.tile_limit, likely, experts, st, l.slices)
+                    : launch_mx_gemm<bf16_t, MX_DOWN>(a, l.tile_limit, likely, experts, st);
   if (rc != FR_OK) return rc;
-  const dim3 grid(static_cast<unsigned>(ceil_div(M * (H / 8), int64_t(kMxThreads))));
+  const dim3 grid(static_cast<unsigned>(ceil_div(M * (H / 4), int64_t(kMxThreads))));
   if (dtype == FR_BF16)
-    hipLaunchKernelGGL((mx_combine_kernel<bf16_t>), grid, dim3(kMxThreads), 0, st, l.rows, l.row_exps, l.exp_pitch, l.topk_ids, E, topk, M, (int)H, static_cast<bf16_t*>(out));
+    hipLaunchKernelGGL((mx_combine_kernel<bf16_t>), grid, dim3(kMxThreads), 0, st, l.rows, l.slices, n, l.topk_ids, E, topk, M, (int)H, static_cast<bf16_t*>(out));
   else
-    hipLaunchKernelGGL((mx_combine_kernel<f16_t>), grid, dim3(kMxThreads), 0, st, l.rows, l.row_exps, l.exp_pitch, l.topk_ids, E, topk, M, (int)H, static_cast<f16_t*>(out));
+    hipLaunchKernelGGL((mx_combine_kernel<f16_t>), grid, dim3(kMxThreads), 0, st, l.rows, l.slices, n, l.topk_ids, E, topk, M, (int)H, static_cast<f16_t*>(out));
   return check_launch("mx_combine_kernel");
 }

@@ -83,9 +83,8 @@ def fused_moe_mxfp4(hidden_states, w1, w1_scale, w2, w2_scale, logits, topk: int
     """The layer in 64 bits: (out [M, H], doubt [M, H]).  doubt bounds what 32-bit sums may change by way of the activated
     rows' quantisation: a gate or up sum of K products is taken to be off by at most (K / 64 + 4) 2^-24 of the sum of the
     products' magnitudes (a rounding per 64 products, four more where these are summed), the activated value by that through silu'(g) <= 1.1
-    and |silu(g)| <= |g|, plus 2^-20 of itself for the exponential and the quotient.  A pair's weighted row may be kept in 16-bit
-    integers with a step of 2^-14 of the power of two at or below the largest of 16 values, or more bits, before the pairs are
-    summed: half a step, 2^-15 of the largest."""
+    and |silu(g)| <= |g|, plus 2^-20 of itself for the exponential and the quotient.  Everything else is
+    summed in 32 bits, which doubt leaves to the caller."""
     x = mxfp4_held(hidden_states)
     weights, ids = gating_topk(logits, topk, renormalize)
     weights, ids = _rows64(weights), ids.numpy() if isinstance(ids, torch.Tensor) else np.asarray(ids)
@@ -103,7 +102,5 @@ def fused_moe_mxfp4(hidden_states, w1, w1_scale, w2, w2_scale, logits, topk: int
         share = weights[token, slot][:, None]
         rows = (mxfp4_held(act) @ m2.T) * share
         np.add.at(out, token, rows)
-        largest = np.abs(rows).reshape(rows.shape[0], -1, 16).max(axis=2)
-        np.add.at(doubt, token, np.repeat(largest, 16, axis=1) * (1 + 2.0 ** -10) * 2.0 ** -15)
         np.add.at(doubt, token, (mxfp4_doubt(act, err) @ np.abs(m2).T) * share)
     return out, doubt
