@@ -107,6 +107,14 @@ def _tiled(codes: torch.Tensor, scales: torch.Tensor, gate_up: bool) -> torch.Te
     return out
 
 
+def _check_tiled(data: torch.Tensor, matrices: int, rows: int, K: int, device: torch.device, what: str) -> None:
+    """A prepared weight's data are what its sizes say: the kernels read all of it by these sizes."""
+    assert data.device == device, "%s on another device than the rows" % what
+    units = matrices * ((rows + 31) // 32) * ((K + 255) // 256)  # of 32 rows x 256 elements
+    assert data.dtype == torch.uint8 and data.is_contiguous() and data.numel() == units * 4352, \
+        "%s: not the data of a prepared weight of these sizes" % what
+
+
 def prepare_linear_mxfp4(codes: torch.Tensor, scales: torch.Tensor) -> MXFP4Weight:
     """One-off layout of a weight matrix [N, K] in MXFP4 (codes uint8 [N, K / 2], scales uint8 [N, K / 32], as
     quantize_rows_mxfp4 returns them) for linear_mxfp4.  The originals may be freed afterwards."""
@@ -121,7 +129,7 @@ def linear_mxfp4(x: torch.Tensor, weight: MXFP4Weight, workspace_buf: torch.Tens
     M, K, ld = _check_rows(x, "x")
     dev = x.device
     assert K == weight.K, "Incompatible dimensions"
-    assert dev == weight.data.device, "x and weight on different devices"
+    _check_tiled(weight.data, 1, weight.N, K, dev, "weight")
     out = torch.empty((M, weight.N), dtype=x.dtype, device=dev)
     if M == 0:
         return out
@@ -168,7 +176,9 @@ def fused_moe_mxfp4(hidden_states: torch.Tensor, weights: MXFP4Experts, gating_o
     assert gating_output.shape == (M, weights.E), "Number of tokens mismatch"
     assert gating_output.is_contiguous(), "gating_output must be contiguous"
     dev = hidden_states.device
-    assert gating_output.device == dev and weights.w1.device == dev, "operands on different devices"
+    assert gating_output.device == dev, "operands on different devices"
+    _check_tiled(weights.w1, weights.E, 2 * weights.F, H, dev, "w1")
+    _check_tiled(weights.w2, weights.E, H, weights.F, dev, "w2")
     topk = int(topk)
     need = N.lib().fr_moe_mxfp4_workspace_bytes(M, H, weights.F, weights.E, topk)
     assert need >= 0, N.lib().fr_last_error_string().decode()

@@ -56,3 +56,27 @@ def test_a_feature_does_not_depend_on_its_neighbours(native, M, H, F, E, topk, d
     was, now = plain[:, large].double(), got[:, large].double()
     normal = was.abs() >= torch.finfo(dtype).smallest_normal
     assert normal.double().mean() > 0.99 and torch.equal(now[normal], was[normal] * 2.0 ** shift)
+
+
+def test_handles_whose_data_are_others_are_refused(native):
+    """Nothing is launched on a prepared weight whose data do not match its sizes or lie elsewhere."""
+    import fast_route_amd as fr
+    w1, s1, w2, s2 = _weights(4, 64, 96, 1)
+    experts = fr.prepare_weights_mxfp4(w1, s1, w2, s2)
+    lin = fr.prepare_linear_mxfp4(w1[0], s1[0])
+    x, logits = _tokens(40, 64, 4, torch.bfloat16, 2)
+    assert fr.linear_mxfp4(x, lin).shape == (40, 192) and fr.fused_moe_mxfp4(x, experts, logits, 2).shape == x.shape
+    wide = torch.cat([logits, logits], dim=1)
+    bad = [
+        lambda: fr.linear_mxfp4(x, lin._replace(N=4096)), lambda: fr.linear_mxfp4(x, lin._replace(data=lin.data[:4352])),
+        lambda: fr.linear_mxfp4(x, lin._replace(data=lin.data.cpu())), lambda: fr.linear_mxfp4(x, lin._replace(data=lin.data.to(torch.int32))),
+        lambda: fr.fused_moe_mxfp4(x, experts._replace(w2=experts.w2.cpu()), logits, 2),
+        lambda: fr.fused_moe_mxfp4(x, experts._replace(w1=experts.w1.cpu()), logits, 2),
+        lambda: fr.fused_moe_mxfp4(x, experts._replace(F=128), logits, 2), lambda: fr.fused_moe_mxfp4(x, experts._replace(w2=experts.w2[4352:]), logits, 2),
+        lambda: fr.fused_moe_mxfp4(x, experts._replace(E=8), wide, 2),
+    ]
+    for i, call in enumerate(bad):
+        with pytest.raises(AssertionError):
+            call()
+            print("case", i, "was not refused", flush=True)
+    torch.cuda.synchronize()

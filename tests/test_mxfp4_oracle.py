@@ -141,3 +141,19 @@ def test_python_entry_points_refuse_cpu_tensors():
                  lambda: fr.fused_moe_mxfp4(x, fr.MXFP4Experts(codes, codes, 1, 64, 64), torch.zeros(4, 1), 1)):
         with pytest.raises(AssertionError):
             call()
+
+
+def test_prepared_weights_of_other_sizes_are_refused(native):
+    """A handle whose data are not what its sizes say would be read beyond its end: the check that every product makes first, on
+    the CPU; the sizes are those that the layout's own entry point states."""
+    from fast_route_amd.layers.mxfp4 import _check_tiled
+    cpu = torch.device("cpu")
+    for matrices, rows, K in ((1, 1, 32), (1, 33, 256), (3, 64, 288), (8, 1120, 1056)):
+        nbytes = native.fr_mxfp4_tiled_bytes(matrices, rows, K)
+        data = torch.empty(nbytes, dtype=torch.uint8)
+        _check_tiled(data, matrices, rows, K, cpu, "w")
+        bad = [(data[:-1], rows, K, cpu), (data, rows + 32, K, cpu), (data, rows, K + 256, cpu), (data[::2], rows, K, cpu),
+               (torch.empty(nbytes, dtype=torch.int8), rows, K, cpu), (data, rows, K, torch.device("meta"))]
+        for d, r, k, dev in bad:
+            with pytest.raises(AssertionError):
+                _check_tiled(d, matrices, r, k, dev, "w")
