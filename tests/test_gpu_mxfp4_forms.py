@@ -1,10 +1,11 @@
 """The forms of the MXFP4 layer and product that sizes choose between: values that no form may lose, and each form's own
 tails, repeats, captures and streams."""
-import numpy as np
+import json
+import os
+import tempfile
+
 import pytest
 import torch
-
-import oracle
 
 pytestmark = pytest.mark.gpu
 
@@ -80,3 +81,122 @@ def test_handles_whose_data_are_others_are_refused(native):
             call()
             print("case", i, "was not refused", flush=True)
     torch.cuda.synchronize()
+
+
+# ---- inputs on which every sum is exact --------------------------------------------------------------------------
+# Elements are levels of the format times powers of two that cancel between the operands, gate sums are 32 exactly (silu(32) is 32 in
+# 32 bits: 1 + exp(-32) rounds to 1), up sums a level, so activated rows are 32 times a level and are held exactly, and the down
+# sums are whole numbers of 1/4 times powers of two, below 2^24 of them; routed weights are 1, 1/2 or 1/4.  The result is the exact one rounded
+# once: there is no tolerance, and one wrong element fails.
+
+LEVELS = (0.0, 0.5, 1.0, 1.5, 2.0, 3.0, 4.0, 6.0)
+ONE, FOUR = 2, 6  # codes
+
+
+def _levels():
+    half = torch.tensor(LEVELS, dtype=torch.float64, device="cuda")
+    return torch.cat([half, -half])
+
+
+def _packed(codes):
+    return (codes[..., 0::2] | codes[..., 1::2] << 4).to(torch.uint8)
+
+
+def _values(packed, scales):
+    """Packed codes [rows, K / 2] and scale bytes [rows, K / 32] in 64 bits."""
+    codes = torch.stack([packed & 15, packed >> 4], dim=2).reshape(packed.shape[0], -1).int()
+    return _levels()[codes] * torch.exp2(scales.double() - 127).repeat_interleave(32, dim=1)
+
+
+class ExactLayer:
+    def __init__(self, H, F, E, seed=0):
+        from fast_route_amd import prepare_weights_mxfp4
+        g = torch.Generator(device="cuda").manual_seed(seed)
+        self.H, self.F, self.E, self.gen = H, F, E, g
+        self.shift = torch.randint(-3, 4, (H // 32,), device="cuda", generator=g)  # of a block of x; the weights' is the opposite
+        some = min(8, 1 << ((H // 16).bit_length() - 1))  # columns 0, 16, .. of x are 4: so many of them make a gate sum of 32
+        w1 = torch.zeros((E, 2 * F, H), dtype=torch.uint8, device="cuda")
+
+        def fixed(count):
+            return 16 * torch.rand((E, F, H // 16), device="cuda", generator=g).topk(count, dim=2).indices
+        w1[:, :F].scatter_(2, fixed(some), {8: ONE, 4: 4, 2: FOUR}[some])  # 8 x 1, 4 x 2, 2 x 4
+        pair = fixed(2)  # 4 and -4 cancel in an up sum
+        w1[:, F:].scatter_(2, pair[..., :1], ONE).scatter_(2, pair[..., 1:], 8 | ONE)
+        column = 16 * torch.randint(0, H // 16, (E, F, 1), device="cuda", generator=g) + torch.randint(1, 16, (E, F, 1), device="cuda", generator=g)
+        w1[:, F:].scatter_(2, column, (ONE + 8 * torch.randint(0, 2, (E, F, 1), device="cuda", generator=g)).to(torch.uint8))
+        self.w1, self.s1 = _packed(w1), (127 - self.shift).to(torch.uint8).expand(E, 2 * F, H // 32).contiguous()
+        self.w2 = _packed(torch.randint(0, 16, (E, H, F), dtype=torch.uint8, device="cuda", generator=g))
+        self.s2 = torch.randint(117, 119, (E, H, F // 32), device="cuda", generator=g).to(torch.uint8)
+        self.experts = prepare_weights_mxfp4(self.w1, self.s1, self.w2, self.s2)
+
+    def tokens(self, M, topk, dtype):
+        """Hidden states, logits and the layer's result."""
+        assert topk in (1, 2, 4) and self.F * 36 * 2 * 4 * topk < 1 << 24
+        codes = torch.randint(0, 16, (M, self.H), device="cuda", generator=self.gen)
+        codes[:, ::16] = FOUR
+        x = (_levels()[codes] * torch.exp2(self.shift.double()).repeat_interleave(32)).to(dtype)
+        ids = torch.rand((M, self.E), device="cuda", generator=self.gen).topk(topk, dim=1).indices
+        logits = torch.full((M, self.E), -100.0, device="cuda").scatter_(1, ids, 0.0)
+        out = torch.zeros((M, self.H), dtype=torch.float64, device="cuda")
+        for e in range(self.E):
+            token = (ids == e).any(dim=1).nonzero()[:, 0]
+            if token.numel():
+                both = x[token].double() @ _values(self.w1[e], self.s1[e]).t()
+                assert (both[:, :self.F] == 32).all() and both.abs().max() <= 32
+                out[token] += 32 * both[:, self.F:] @ _values(self.w2[e], self.s2[e]).t() / topk
+        return x, logits, out.float().to(dtype)
+
+
+def _grids(call):
+    """What a call returns and its kernels of this path in order: (name, grid)."""
+    with torch.profiler.profile(activities=[torch.profiler.ProfilerActivity.CUDA]) as prof:
+        out = call()
+        torch.cuda.synchronize()
+    with tempfile.TemporaryDirectory() as d:
+        path = os.path.join(d, "trace.json")
+        prof.export_chrome_trace(path)
+        with open(path) as f:
+            events = [e for e in json.load(f)["traceEvents"] if e.get("cat") == "kernel" and "mx_" in e["name"]]
+    return out, [(e["name"], tuple(e["args"]["grid"])) for e in sorted(events, key=lambda e: e["ts"])]
+
+
+def _form(M, H, F, E, topk, kernels):
+    """The form that a layer's launches show: few tokens ("route": two launches, "alone": a feature block per wavefront of the gate/up product, "shared":
+    per workgroup; parts of the down product), or the products by tiles (K slices of the down product, weight row groups of a wavefront)."""
+    n = M * topk
+    experts, act_tiles = min(n, E), -(-F // 256)
+    by_name = {k: [g for name, g in kernels if k in name] for k in ("few_front", "few_gateup", "few_down", "gemm")}
+    if by_name["few_down"]:
+        (gateup,), (down,) = by_name["few_gateup"], by_name["few_down"]
+        assert gateup[1] == experts and down[0] == H // 32
+        kind = "route" if not by_name["few_front"] else {act_tiles * 2: "alone", act_tiles * 8: "shared"}[gateup[0]]
+        return kind, down[1]
+    down = by_name["gemm"][1]
+    tiles = min(n, (n + 31 * E) // 32) // 4 + experts
+    wide = {8 * -(-tiles * -(-(H // 32) // (4 * j)) // 8): j for j in (1, 2)}
+    return "tiles", down[1], wide[down[0]]
+
+
+# M, H, F, E, topk, form
+EXACT = [(1, 1024, 3584, 8, 2, ("route", 1)), (4, 1024, 3584, 8, 2, ("route", 3)), (5, 1024, 3584, 8, 2, ("alone", 3)),
+         (32, 2048, 1408, 64, 4, ("alone", 4)), (6, 256, 2048, 8, 2, ("alone", 2)), (6, 256, 2016, 8, 2, ("shared", 2)),
+         (6, 2048, 2048, 8, 1, ("shared", 1)), (9, 2048, 2048, 8, 1, ("alone", 2)), (9, 2080, 2048, 8, 1, ("shared", 2)),
+         (24, 4096, 8192, 8, 2, ("shared", 2)), (32, 512, 1408, 64, 4, ("alone", 8)), (2, 4096, 8192, 8, 2, ("route", 2)),
+         (50, 1024, 3584, 8, 2, ("tiles", 3, 2)), (40, 1056, 2336, 12, 4, ("tiles", 2, 2)), (45, 4096, 8192, 8, 2, ("tiles", 4, 2)),
+         (200, 4096, 8192, 8, 2, ("tiles", 1, 1)), (700, 4096, 8192, 8, 2, ("tiles", 1, 2)), (1200, 800, 128, 64, 4, ("tiles", 1, 2)),
+         (2000, 2080, 64, 64, 2, ("tiles", 1, 2)), (300, 320, 1120, 12, 4, ("tiles", 1, 1)), (8192, 1056, 96, 3, 1, ("tiles", 1, 2))]
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("M,H,F,E,topk,form", EXACT)
+def test_exact_layer(native, M, H, F, E, topk, form, dtype):
+    """The exact result, by the form that the sizes were chosen for."""
+    from fast_route_amd import fused_moe_mxfp4
+    _say(f"exact layer M={M} H={H} F={F} E={E} topk={topk} {form} {dtype}")
+    layer = ExactLayer(H, F, E, seed=M)
+    x, logits, want = layer.tokens(M, topk, dtype)
+    assert want.isfinite().all()
+    got = fused_moe_mxfp4(x, layer.experts, logits, topk)
+    assert torch.equal(got, want)
+    got, kernels = _grids(lambda: fused_moe_mxfp4(x, layer.experts, logits, topk))
+    assert torch.equal(got, want) and _form(M, H, F, E, topk, kernels) == form
