@@ -200,3 +200,72 @@ def test_exact_layer(native, M, H, F, E, topk, form, dtype):
     assert torch.equal(got, want)
     got, kernels = _grids(lambda: fused_moe_mxfp4(x, layer.experts, logits, topk))
     assert torch.equal(got, want) and _form(M, H, F, E, topk, kernels) == form
+
+
+# forms whose workgroups meet through memory: parts of the few-token down product, K slices of the other
+JOINED = [(4, 1024, 3584, 8, 2), (5, 1024, 3584, 8, 2), (32, 2048, 1408, 64, 4), (24, 4096, 2048, 8, 2), (50, 1024, 3584, 8, 2), (40, 1056, 2336, 12, 4)]
+
+
+@pytest.mark.parametrize("M,H,F,E,topk", JOINED)
+def test_joined_parts_in_one_workspace(native, M, H, F, E, topk):
+    """Call after call in one workspace, other inputs each time, whatever it held before: no part and no count of an earlier call is
+    taken for the present one's."""
+    from fast_route_amd import fused_moe_mxfp4
+    _say(f"joined M={M} H={H} F={F} E={E} topk={topk}")
+    layer = ExactLayer(H, F, E, seed=1)
+    calls = [layer.tokens(M, topk, torch.bfloat16) for _ in range(3)]
+    ws = torch.empty(native.fr_moe_mxfp4_workspace_bytes(M, H, F, E, topk), dtype=torch.uint8, device="cuda")
+    for fill in (0x00, 0xFF, 0x5A, None):
+        if fill is not None:
+            ws.fill_(fill)
+        outs = [fused_moe_mxfp4(x, layer.experts, logits, topk, workspace_buf=ws) for x, logits, _ in calls * 4]
+        for i, got in enumerate(outs):
+            assert torch.equal(got, calls[i % 3][2]), f"fill {fill}, call {i}"
+    x, logits, want = calls[0]
+    given = x.clone()
+    assert fused_moe_mxfp4(given, layer.experts, logits, topk, inplace=True, workspace_buf=ws) is given and torch.equal(given, want)
+
+
+@pytest.mark.parametrize("M,H,F,E,topk", JOINED)
+def test_joined_parts_captured_and_replayed(native, M, H, F, E, topk):
+    """A graph of two calls in one workspace, replayed on other inputs with eager calls and synchronizations between the replays."""
+    from fast_route_amd import fused_moe_mxfp4
+    _say(f"joined captured M={M} H={H} F={F} E={E} topk={topk}")
+    layer = ExactLayer(H, F, E, seed=2)
+    calls = [layer.tokens(M, topk, torch.bfloat16) for _ in range(4)]
+    sx, sl = [calls[0][0].clone() for _ in range(2)], [calls[0][1].clone() for _ in range(2)]
+    ws = torch.full((native.fr_moe_mxfp4_workspace_bytes(M, H, F, E, topk),), 0xFF, dtype=torch.uint8, device="cuda")
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        outs = [fused_moe_mxfp4(sx[i], layer.experts, sl[i], topk, workspace_buf=ws) for i in range(2)]
+    for replay in range(5):
+        use = [calls[replay % 4], calls[(replay + 1) % 4]]
+        for i in range(2):
+            sx[i].copy_(use[i][0])
+            sl[i].copy_(use[i][1])
+        graph.replay()
+        torch.cuda.synchronize()
+        for i in range(2):
+            assert torch.equal(outs[i], use[i][2]), f"replay {replay}, call {i}"
+        x, logits, want = calls[(replay + 2) % 4]
+        assert torch.equal(fused_moe_mxfp4(x, layer.experts, logits, topk, workspace_buf=ws), want)
+
+
+def test_joined_parts_on_two_streams(native):
+    """Both joined forms at once on streams of their own, workspaces from the allocator, other inputs in turn."""
+    from fast_route_amd import fused_moe_mxfp4
+    H, F, E, topk = 1024, 3584, 8, 2
+    layer = ExactLayer(H, F, E, seed=3)
+    calls = [[layer.tokens(M, topk, torch.bfloat16) for _ in range(2)] for M in (5, 50)]
+    torch.cuda.synchronize()
+    streams, got = [torch.cuda.Stream(), torch.cuda.Stream()], [[], []]
+    for r in range(12):
+        for i, s in enumerate(streams):
+            with torch.cuda.stream(s):
+                x, logits, _ = calls[i][r % 2]
+                got[i].append(fused_moe_mxfp4(x, layer.experts, logits, topk))
+    torch.cuda.synchronize()
+    for i in range(2):
+        for r, g in enumerate(got[i]):
+            assert torch.equal(g, calls[i][r % 2][2]), f"stream {i}, call {r}"
