@@ -269,3 +269,47 @@ def test_joined_parts_on_two_streams(native):
     for i in range(2):
         for r, g in enumerate(got[i]):
             assert torch.equal(g, calls[i][r % 2][2]), f"stream {i}, call {r}"
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("M,H,F,E,topk", JOINED + [(9, 2048, 2048, 8, 1), (300, 320, 1120, 12, 4), (1200, 800, 128, 64, 4)])
+def test_bad_values_stay_where_they_are(native, M, H, F, E, topk, dtype):
+    """An infinity in a token row makes that row NaN; a token of NaN logits changes nobody else's row; a NaN scale in w2 makes one
+    feature of its expert's tokens NaN, one in w1 their rows."""
+    from fast_route_amd import fused_moe_mxfp4, prepare_weights_mxfp4
+    _say(f"bad values M={M} H={H} F={F} E={E} topk={topk} {dtype}")
+    layer = ExactLayer(H, F, E, seed=4)
+    x, logits, want = layer.tokens(M, topk, dtype)
+    row = torch.arange(M, device="cuda")
+    bad = x.clone()
+    bad[M - 1, H - 1] = float("inf")
+    got = fused_moe_mxfp4(bad, layer.experts, logits, topk)
+    assert got[M - 1].isnan().all() and torch.equal(got[row != M - 1], want[row != M - 1])
+    for value in (float("nan"), float("-inf")):
+        odd = logits.clone()
+        odd[1] = value
+        assert torch.equal(fused_moe_mxfp4(x, layer.experts, odd, topk)[row != 1], want[row != 1])
+    expert = int(logits[0].argmax())
+    hit = logits[:, expert] == 0
+    s2 = layer.s2.clone()
+    s2[expert, H - 3, F // 32 - 1] = 255
+    got = fused_moe_mxfp4(x, prepare_weights_mxfp4(layer.w1, layer.s1, layer.w2, s2), logits, topk)
+    nan = torch.zeros((M, H), dtype=torch.bool, device="cuda")
+    nan[:, H - 3] = hit
+    assert torch.equal(got.isnan(), nan) and torch.equal(got[~nan], want[~nan])
+    s1 = layer.s1.clone()
+    s1[expert, 2 * F - 1, H // 32 - 1] = 255
+    got = fused_moe_mxfp4(x, prepare_weights_mxfp4(layer.w1, s1, layer.w2, layer.s2), logits, topk)
+    assert got[hit].isnan().all() and torch.equal(got[~hit], want[~hit])
+
+
+def test_logits_anywhere_in_memory(native):
+    """Rows of logits need no alignment: a dense slice that begins at any element."""
+    from fast_route_amd import fused_moe_mxfp4
+    for M, E, topk in ((3, 3, 2), (20, 7, 2), (60, 5, 2), (900, 33, 4)):
+        layer = ExactLayer(64, 64, E, seed=5)
+        x, logits, want = layer.tokens(M, topk, torch.bfloat16)
+        for dtype in (torch.float32, torch.bfloat16):
+            held = torch.zeros(M * E + 1, device="cuda", dtype=dtype)
+            held[1:] = logits.view(-1)
+            assert torch.equal(fused_moe_mxfp4(x, layer.experts, held[1:].view(M, E), topk), want), (M, E, dtype)
