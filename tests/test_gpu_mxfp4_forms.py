@@ -313,3 +313,27 @@ def test_logits_anywhere_in_memory(native):
             held = torch.zeros(M * E + 1, device="cuda", dtype=dtype)
             held[1:] = logits.view(-1)
             assert torch.equal(fused_moe_mxfp4(x, layer.experts, held[1:].view(M, E), topk), want), (M, E, dtype)
+
+
+LINEAR = [(M, 4096, K) for M in (1, 4, 5, 32, 33, 60, 100, 129, 512) for K in (4096, 14336)] + [
+    (4, 96, 99 * 256), (4, 96, 100 * 256), (300, 1031, 4096), (600, 12287, 1024), (130, 72, 12288), (2000, 520, 288)]
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("M,N_,K", LINEAR)
+def test_exact_linear(native, M, N_, K, dtype):
+    """Levels times powers of two that cancel: sums are whole numbers of 1/4 below 2^24 of them, the result the exact one rounded once."""
+    from fast_route_amd import linear_mxfp4, prepare_linear_mxfp4
+    _say(f"exact linear {M}x{N_}x{K} {dtype}")
+    assert K * 36 * 2 * 4 < 1 << 24
+    g = torch.Generator(device="cuda").manual_seed(M + N_ + K)
+    shift = torch.randint(-3, 4, (K // 32,), device="cuda", generator=g)
+    codes = torch.randint(0, 16, (M, K), device="cuda", generator=g)
+    codes[:, ::32] = FOUR
+    x = (_levels()[codes] * torch.exp2(shift.double()).repeat_interleave(32)).to(dtype)
+    w = _packed(torch.randint(0, 16, (N_, K), dtype=torch.uint8, device="cuda", generator=g))
+    scales = (torch.randint(120, 122, (N_, K // 32), device="cuda", generator=g) - shift).to(torch.uint8)
+    got, kernels = _grids(lambda: linear_mxfp4(x, prepare_linear_mxfp4(w, scales)))
+    assert torch.equal(got, (x.double() @ _values(w, scales).t()).float().to(dtype))
+    names = [name for name, _ in kernels if "tile_weights" not in name]
+    assert len(names) == (1 if M <= 4 and K < 25600 else 2)  # up to four rows that fit in LDS are quantised inside the product
