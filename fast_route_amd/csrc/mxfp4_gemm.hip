@@ -10,7 +10,11 @@ namespace fr {
 namespace {
 
 constexpr int kMxThreads = 256;
-enum { MX_LINEAR = 0, MX_SILU = 1, MX_DOWN = 2, MX_PART = 3 };  // MX_PART: the down product, K cut over workgroups
+// MX_PART: the down product, K cut over workgroups; MX_PAST: a linear product whose whole lines are written past the caches.  (A flag of the
+// call would not do: the compiler makes one plain store of both kinds.)
+enum { MX_LINEAR = 0, MX_SILU = 1, MX_DOWN = 2, MX_PART = 3, MX_PAST = 4 };
+template <int EPI>
+constexpr bool kMxLinear = EPI == MX_LINEAR || EPI == MX_PAST;
 template <int EPI>
 constexpr bool kMxPairs = EPI == MX_DOWN || EPI == MX_PART;  // results are weighted rows of pairs
 
@@ -38,10 +42,9 @@ struct MxArgs {
   const float* topk_w;
   int n_pairs;
   float* rows;             // [slices][n_pairs, N]; MX_DOWN: one slice
-  // MX_LINEAR
+  // MX_LINEAR, MX_PAST
   void* out;
   int64_t ldo;
-  bool out_past;       // whole lines of out are written past the caches
   int64_t M;
   int N;               // columns of rows / out
 };
@@ -53,7 +56,7 @@ typedef unsigned u32x4 __attribute__((ext_vector_type(4)));
 // down product of 64 experts, H = 2048, F = 1408, 8192 tokens 208 -> 175, of 8, H = 4096, F = 14336, 16384 1112 -> 1067; K slices would lose, 50 tokens on 8
 // experts, H = 1024, F = 3584 6.7 -> 7.3.  A product larger than the caches keep goes past them, @@ (286 in pieces).
 template <int EPI, int J>
-constexpr bool kMxTurned = J == 2 && (EPI == MX_LINEAR || EPI == MX_DOWN);
+constexpr bool kMxTurned = J == 2 && (kMxLinear<EPI> || EPI == MX_DOWN);
 template <int EPI>
 constexpr int kMxTurnPieces = kMxPairs<EPI> ? 16 : 8;  // 16-byte pieces of a row: fp32, or a 2-byte type
 template <int EPI>
@@ -234,7 +237,7 @@ __device__ __forceinline__ void mx_epilogue(const MxArgs& a, const MxSpan& t, in
           const u32x4 v = *reinterpret_cast<const u32x4*>(lds + r * PITCH + lane % PIECES * 16);
           u32x4* const row = to(r);
           if (row) {
-            if (EPI == MX_LINEAR && a.out_past) __builtin_nontemporal_store(v, row + lane % PIECES);
+            if constexpr (EPI == MX_PAST) __builtin_nontemporal_store(v, row + lane % PIECES);
             else row[lane % PIECES] = v;
           }
         }
@@ -321,13 +324,13 @@ template <typename T, int EPI, int J, bool NT>
 __global__ __launch_bounds__(kMxThreads, 2) void mx_gemm_kernel(MxArgs a) {
   extern __shared__ __attribute__((aligned(16))) unsigned char mx_lds[];
   // workgroups b, b + 8, .. share an XCD and its L2: an XCD takes a consecutive part of the walk
-  const int tiles = EPI == MX_LINEAR ? (a.x_groups + kMxMaxUnits - 1) / kMxMaxUnits : a.tile_count[0];
+  const int tiles = kMxLinear<EPI> ? (a.x_groups + kMxMaxUnits - 1) / kMxMaxUnits : a.tile_count[0];
   const int total = tiles * a.f_tiles, per = (total + 7) / 8;
   const int i = blockIdx.x >> 3, lin = (blockIdx.x & 7) * per + i;
   if (i >= per || lin >= total) return;
   const int guess = lin / a.f_tiles;  // a tile of the chunk that lin belongs to
   MxTile e;
-  if constexpr (EPI == MX_LINEAR) {
+  if constexpr (kMxLinear<EPI>) {
     e.first = e.expert = e.index0 = 0;
     e.count = a.x_groups;
     e.n = tiles;
@@ -536,10 +539,11 @@ extern "C" int fr_linear_mxfp4(const void* x, int dtype, int64_t M, int64_t K, i
   a.x_groups = static_cast<int>(groups);
   a.out = out;
   a.ldo = N;
-  a.out_past = mx_streams(2 * M * N);
   a.M = M;
   a.N = static_cast<int>(N);
   const int64_t token_tiles = ceil_div(groups, int64_t(kMxMaxUnits));
+  if (mx_streams(2 * M * N))  // tiles enough for 256 weight rows
+    return dtype == FR_BF16 ? launch_mx_gemm_wide<bf16_t, MX_PAST, 2>(a, token_tiles, 1, st, 1) : launch_mx_gemm_wide<f16_t, MX_PAST, 2>(a, token_tiles, 1, st, 1);
   return dtype == FR_BF16 ? launch_mx_gemm<bf16_t, MX_LINEAR>(a, token_tiles, token_tiles, 1, st)
                           : launch_mx_gemm<f16_t, MX_LINEAR>(a, token_tiles, token_tiles, 1, st);
 }
