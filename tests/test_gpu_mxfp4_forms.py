@@ -337,3 +337,28 @@ def test_exact_linear(native, M, N_, K, dtype):
     assert torch.equal(got, (x.double() @ _values(w, scales).t()).float().to(dtype))
     names = [name for name, _ in kernels if "tile_weights" not in name]
     assert len(names) == (1 if M <= 4 and K < 25600 else 2)  # up to four rows that fit in LDS are quantised inside the product
+
+
+def test_offsets_beyond_32_bits(native):
+    """More than 2^31 elements of rows: the same 4096 rows again and again, every block the first one's result."""
+    from fast_route_amd import dequantize_rows_mxfp4, fused_moe_mxfp4, linear_mxfp4, prepare_linear_mxfp4, quantize_rows_mxfp4
+    H, block, times = 4096, 4096, 129
+    layer = ExactLayer(H, 64, 3, seed=6)
+    x, logits, want = layer.tokens(block, 1, torch.bfloat16)
+    many, many_logits = x.repeat(times, 1), logits.repeat(times, 1)
+    assert many.numel() > 1 << 31
+    _say("beyond 32 bits: layer")
+    got = fused_moe_mxfp4(many, layer.experts, many_logits, 1).view(times, block, H)
+    assert all(torch.equal(got[i], want) for i in range(times))
+    del got
+    _say("beyond 32 bits: linear")
+    narrow = x[:, :64].contiguous()
+    weight = prepare_linear_mxfp4(*quantize_rows_mxfp4(x[:, :64]))  # [4096, 64]: as many output features as rows
+    first = linear_mxfp4(narrow, weight)
+    got = linear_mxfp4(many[:, :64], weight).view(times, block, H)  # rows 8 KB apart
+    assert all(torch.equal(got[i], first) for i in range(times))
+    del got
+    _say("beyond 32 bits: quantisation")
+    codes, scales = quantize_rows_mxfp4(many)
+    back = dequantize_rows_mxfp4(codes, scales).view(times, block, H)
+    assert all(torch.equal(back[i], x) for i in range(times))
