@@ -53,8 +53,9 @@ typedef unsigned u32x4 __attribute__((ext_vector_type(4)));
 
 // A lane holds 16 consecutive features of a row and feature unit, so its stores fill lines in instructions of 64 scattered 16-byte pieces.  Where a
 // wavefront has 64 features they are turned in LDS (32 rows of 64 features, a row group at a time) and leave as whole lines: 8192 x 12288 x 4096 213 -> 206 us,
-// down product of 64 experts, H = 2048, F = 1408, 8192 tokens 208 -> 175, of 8, H = 4096, F = 14336, 16384 1112 -> 1067; K slices would lose, 50 tokens on 8
-// experts, H = 1024, F = 3584 6.7 -> 7.3.  A product larger than the caches keep goes past them, @@ (286 in pieces).
+// down product of 64 experts, H = 2048, F = 1408, 8192 tokens 207 -> 174, of 8, H = 4096, F = 14336, 16384 1112 -> 1067; K slices would lose, 50 tokens on 8
+// experts, H = 1024, F = 3584 6.7 -> 7.3.  A product larger than the caches keep goes past them, 206 -> 191 (286 in pieces).
+// A product whose N is no multiple of 8 is stored value by value: 4096 x 12287 x 4096 254 us, 12288 99.
 template <int EPI, int J>
 constexpr bool kMxTurned = J == 2 && (kMxLinear<EPI> || EPI == MX_DOWN);
 template <int EPI>
@@ -140,7 +141,7 @@ __device__ __forceinline__ void mx_tile(const MxArgs& a, const MxSpan& t, int f,
     for (int s = 0; s < (p < RING - 1 ? 4 : 3); ++s) load_w(p, s, p);
   }
   __builtin_amdgcn_sched_barrier(0);
-  // K tile 0 of the token rows has landed: 2 (U + 1) + 5 J RING - 2 J loads are newer
+  // K tile 0 of the token rows has landed: 2 (U + 1) + 8 J loads are newer, of which J, of K tile 1, are waited for too
   asm volatile("s_waitcnt vmcnt(%0)" ::"n"(2 * (U + 1) + 5 * J * RING - 3 * J) : "memory");
   __builtin_amdgcn_s_barrier();
 #pragma unroll
@@ -157,7 +158,8 @@ __device__ __forceinline__ void mx_tile(const MxArgs& a, const MxSpan& t, int f,
           constexpr int s = decltype(S)::value;
           if constexpr (s == 3) {
             // K tile k + 1 of the token rows has landed, everybody's loads of it behind the barrier (this wavefront has issued U + 1 of
-            // k + 2 and 9 J of weights since); and slot (k + 3) & 3, that of k - 1, has been read by everybody.
+            // k + 2 and 9 J of weights since, the oldest 2 J of them fragment 3 and scales of K tile k, which the MFMAs below need); and slot
+            // (k + 3) & 3, that of k - 1, has been read by everybody.
             asm volatile("s_waitcnt vmcnt(%0)" ::"n"(U + 1 + 7 * J) : "memory");
             __builtin_amdgcn_s_barrier();
           }

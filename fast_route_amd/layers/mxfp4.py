@@ -125,7 +125,8 @@ def prepare_linear_mxfp4(codes: torch.Tensor, scales: torch.Tensor) -> MXFP4Weig
 
 def linear_mxfp4(x: torch.Tensor, weight: MXFP4Weight, workspace_buf: torch.Tensor | None = None) -> torch.Tensor:
     """x [M, K] (f16/bf16, rows a multiple of 8 elements apart) times the transpose of a prepared weight matrix [N, K]: x is
-    quantised to MXFP4 row by row, the product accumulates in fp32, the result [M, N] has x's type."""
+    quantised to MXFP4 row by row, the product accumulates in fp32, the result [M, N] has x's type.  Any N; for more than 128 rows a
+    multiple of 8 is the fast case."""
     M, K, ld = _check_rows(x, "x")
     dev = x.device
     assert K == weight.K, "Incompatible dimensions"
