@@ -1,9 +1,10 @@
 """ctypes binding of libfast_route_hip.so (the C ABI in include/fast_route_hip.h)."""
 from __future__ import annotations
 
+import contextlib
 import ctypes
 import os
-from ctypes import c_char_p, c_int, c_int32, c_int64, c_void_p
+from ctypes import c_char_p, c_float, c_int, c_int32, c_int64, c_void_p
 
 import torch
 
@@ -34,6 +35,8 @@ SIGNATURES = {
     "fr_last_error_string": (c_char_p, []),
     "fr_gating_topk": (c_int, [c_void_p, c_int, c_int64, c_int64, c_int64, c_int, c_int, c_void_p, c_void_p, c_void_p]),
     "fr_route_gate": (c_int, [c_void_p, c_void_p, c_int, c_int64, c_int64, c_int64, c_int, c_int, c_void_p, c_void_p, c_void_p]),
+    "fr_gating_grouped": (c_int, [c_void_p, c_int, c_int64, c_int64, c_int64, c_void_p, c_int, c_int, c_int, c_int, c_int, c_float, c_void_p,
+                                  c_void_p, c_void_p]),
     "fr_moe_align_workspace_bytes": (c_int64, [c_int64, c_int]),
     "fr_moe_align": (c_int, [c_void_p, c_int, c_int64, c_int, c_int, c_void_p, c_void_p, c_void_p, c_void_p, c_int64, c_void_p]),
     "fr_moe_grouped_gemm": (c_int, [c_void_p, c_int64, c_void_p, c_void_p, c_void_p, c_void_p, c_void_p, c_void_p,
@@ -67,6 +70,10 @@ SIGNATURES = {
     "fr_moe_mxfp4_workspace_bytes": (c_int64, [c_int64, c_int64, c_int64, c_int, c_int]),
     "fr_fused_moe_mxfp4": (c_int, [c_void_p, c_int, c_void_p, c_void_p, c_void_p, c_int, c_int64, c_int64, c_int64, c_int, c_int,
                                    c_int, c_void_p, c_void_p, c_int64, c_void_p]),
+    "fr_rotary": (c_int, [c_char_p, c_void_p]),
+    "fr_attention": (c_int, [c_char_p, c_void_p]),
+    "fr_paged_attention_workspace_bytes": (c_int64, [c_int64, c_int64, c_int64, c_int64, c_int64]),
+    "fr_paged_attention": (c_int, [c_char_p, c_void_p]),
     "fr_fused_moe_noalloc": (c_int, [c_void_p, c_void_p, c_void_p, c_void_p, c_int, c_int64, c_int64, c_int64, c_int, c_int,
                                      c_int, c_int, c_void_p, c_void_p]),
     "fr_probe_mfma_stream": (c_int, [c_int, c_int, c_int, c_void_p, c_void_p, c_void_p, c_void_p]),
@@ -123,3 +130,11 @@ def stream_ptr(device) -> int:
 def require_cuda(*tensors) -> None:
     for t in tensors:
         assert t.is_cuda, "fast_route_amd operators need tensors on an MI355X device (no CPU path)"
+
+
+_HERE = contextlib.nullcontext()
+
+
+def on(device: torch.device):
+    """The device of a call's tensors as the current one, where it is another."""
+    return _HERE if device.index == torch.cuda.current_device() else torch.cuda.device(device)

@@ -1,0 +1,63 @@
+// What the attention kernels share: matrix instructions by type, exchanges between lane rows, transposed reads of LDS.
+#pragma once
+#include "fr_common.h"
+
+namespace fr {
+namespace {
+
+template <typename T> struct Attn;
+template <> struct Attn<bf16_t> {
+  typedef bf16x4 vec4;
+  typedef bf16x8 vec8;
+  static __device__ __forceinline__ f32x4 mma16(vec8 a, vec8 b, f32x4 c) { return __builtin_amdgcn_mfma_f32_16x16x32_bf16(a, b, c, 0, 0, 0); }
+  static __device__ __forceinline__ f32x16 mma32(vec8 a, vec8 b, f32x16 c) { return __builtin_amdgcn_mfma_f32_32x32x16_bf16(a, b, c, 0, 0, 0); }
+};
+template <> struct Attn<f16_t> {
+  typedef f16x4 vec4;
+  typedef f16x8 vec8;
+  static __device__ __forceinline__ f32x4 mma16(vec8 a, vec8 b, f32x4 c) { return __builtin_amdgcn_mfma_f32_16x16x32_f16(a, b, c, 0, 0, 0); }
+  static __device__ __forceinline__ f32x16 mma32(vec8 a, vec8 b, f32x16 c) { return __builtin_amdgcn_mfma_f32_32x32x16_f16(a, b, c, 0, 0, 0); }
+};
+
+typedef short i16x4 __attribute__((ext_vector_type(4)));
+
+// A group of 16 lanes reads a 4 x 16 matrix of 16-bit elements, lane l the four from column 4 (l % 4) of row (l / 4) % 4 at `at`; lane l gets
+// column l % 16, rows 0 .. 3.
+template <typename T>
+__device__ __forceinline__ typename Attn<T>::vec4 read_transposed(const T* at) {
+  const i16x4 v = __builtin_amdgcn_ds_read_tr16_b64_v4i16((__attribute__((address_space(3))) i16x4*)at);
+  return __builtin_bit_cast(typename Attn<T>::vec4, v);
+}
+
+template <typename V4>
+__device__ __forceinline__ auto join8(V4 a, V4 b) { return __builtin_shufflevector(a, b, 0, 1, 2, 3, 4, 5, 6, 7); }
+
+// Over the lanes that differ in bit 4 (5) of their number: of the two values, in both lanes.
+__device__ __forceinline__ float max_over_16(float v) {
+  const auto x = __builtin_amdgcn_permlane16_swap(__float_as_uint(v), __float_as_uint(v), false, false);
+  return fmaxf(__uint_as_float(x[0]), __uint_as_float(x[1]));
+}
+__device__ __forceinline__ float max_over_32(float v) {
+  const auto x = __builtin_amdgcn_permlane32_swap(__float_as_uint(v), __float_as_uint(v), false, false);
+  return fmaxf(__uint_as_float(x[0]), __uint_as_float(x[1]));
+}
+__device__ __forceinline__ float sum_over_16(float v) {
+  const auto x = __builtin_amdgcn_permlane16_swap(__float_as_uint(v), __float_as_uint(v), false, false);
+  return __uint_as_float(x[0]) + __uint_as_float(x[1]);
+}
+__device__ __forceinline__ float sum_over_32(float v) {
+  const auto x = __builtin_amdgcn_permlane32_swap(__float_as_uint(v), __float_as_uint(v), false, false);
+  return __uint_as_float(x[0]) + __uint_as_float(x[1]);
+}
+
+__device__ __forceinline__ float exp2_of(float v) { return __builtin_amdgcn_exp2f(v); }
+
+constexpr float kLog2e = 1.4426950408889634f;
+
+// Scores are kept in units of a factor 2.  A running maximum that lags behind the scores by up to kLag of them leaves the results as they
+// are - every term and the sum carry the same 2^lag - and the output rows need not be rescaled for each new maximum.  Terms reach 2^kLag, far
+// inside fp16, and keep their relative precision; the sums are fp32.
+constexpr float kLag = 8.f;
+
+}  // namespace
+}  // namespace fr

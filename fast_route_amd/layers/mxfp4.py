@@ -7,7 +7,6 @@ accumulate in fp32 and results are rounded once, to the activations' type.
 """
 from __future__ import annotations
 
-import contextlib
 from typing import NamedTuple
 
 import torch
@@ -32,14 +31,6 @@ class MXFP4Experts(NamedTuple):
     E: int
     H: int
     F: int
-
-
-_HERE = contextlib.nullcontext()
-
-
-def _on(device: torch.device):
-    """The device of a call's tensors as the current one, where it is another."""
-    return _HERE if device.index == torch.cuda.current_device() else torch.cuda.device(device)
 
 
 def _check_rows(x: torch.Tensor, what: str):
@@ -77,7 +68,7 @@ def quantize_rows_mxfp4(x: torch.Tensor):
     dev = x.device
     codes = torch.empty((rows, K // 2), dtype=torch.uint8, device=dev)
     scales = codes.new_empty((rows, K // BLOCK))
-    with _on(dev):
+    with N.on(dev):
         N.check(N.lib().fr_quant_mxfp4_rows(x.data_ptr(), N.dtype_code(x.dtype), rows, K, ld, codes.data_ptr(), scales.data_ptr(),
                                             N.stream_ptr(dev)))
     return codes, scales
@@ -90,7 +81,7 @@ def dequantize_rows_mxfp4(codes: torch.Tensor, scales: torch.Tensor, dtype: torc
     assert dtype in _FLOATS or dtype == torch.float32, "dtype must be float16, bfloat16 or float32"
     K = codes.shape[-1] * 2
     out = torch.empty(codes.shape[:-1] + (K,), dtype=dtype, device=codes.device)
-    with _on(codes.device):
+    with N.on(codes.device):
         N.check(N.lib().fr_dequant_mxfp4_rows(codes.data_ptr(), scales.data_ptr(), out.numel() // K, K, N.dtype_code(dtype),
                                               out.data_ptr(), N.stream_ptr(codes.device)))
     return out
@@ -101,7 +92,7 @@ def _tiled(codes: torch.Tensor, scales: torch.Tensor, gate_up: bool) -> torch.Te
     nbytes = N.lib().fr_mxfp4_tiled_bytes(matrices, rows, K)
     assert nbytes >= 0, "weights of %d x %d x %d are too large" % (matrices, rows, K)
     out = torch.empty((nbytes,), dtype=torch.uint8, device=codes.device)
-    with _on(codes.device):
+    with N.on(codes.device):
         N.check(N.lib().fr_mxfp4_tile_weights(codes.data_ptr(), scales.data_ptr(), matrices, rows, K, int(gate_up), out.data_ptr(),
                                               N.stream_ptr(codes.device)))
     return out
@@ -137,7 +128,7 @@ def linear_mxfp4(x: torch.Tensor, weight: MXFP4Weight, workspace_buf: torch.Tens
     need = N.lib().fr_linear_mxfp4_workspace_bytes(M, weight.N, K)
     assert need >= 0, "linear_mxfp4: %d rows of %d elements are too large" % (M, K)
     ws = _workspace(workspace_buf, need, dev)
-    with _on(dev):
+    with N.on(dev):
         N.check(N.lib().fr_linear_mxfp4(x.data_ptr(), N.dtype_code(x.dtype), M, K, ld, weight.data.data_ptr(), weight.N, out.data_ptr(),
                                         0 if ws is None else ws.data_ptr(), 0 if ws is None else ws.numel(), N.stream_ptr(dev)))
     return out
@@ -187,7 +178,7 @@ def fused_moe_mxfp4(hidden_states: torch.Tensor, weights: MXFP4Experts, gating_o
     if M == 0:
         return out
     ws = _workspace(workspace_buf, need, dev)
-    with _on(dev):
+    with N.on(dev):
         N.check(N.lib().fr_fused_moe_mxfp4(hidden_states.data_ptr(), N.dtype_code(hidden_states.dtype), weights.w1.data_ptr(),
                                            weights.w2.data_ptr(), gating_output.data_ptr(), N.dtype_code(gating_output.dtype), M, H,
                                            weights.F, weights.E, topk, int(bool(renormalize)), out.data_ptr(), ws.data_ptr(),

@@ -70,6 +70,20 @@ int fr_gating_topk(const void* logits, int logits_dtype, int64_t M, int64_t E, i
 int fr_route_gate(const void* hidden, const void* gate, int dtype, int64_t M, int64_t H, int64_t E,
                   int topk, int renormalize, float* weights_out, int32_t* ids_out, void* stream);
 
+/* Routing by scores with a bias and groups.  No counterpart in the reference.
+ *   score s = softmax(logits) over the E experts (FR_SCORE_SOFTMAX) or sigmoid(logits) (FR_SCORE_SIGMOID);
+ *   choice c = s + bias with a bias (fp32 [E]), the logit itself without one (bias NULL);
+ *   `groups` runs of E / groups experts each; a group's worth is its largest c, with a bias the sum of its two largest;
+ *   ids_out: the topk experts of largest c in the `kept` groups of largest worth, in that order; ties: the lower index;
+ *   weights_out: their s, divided by their sum if renormalize (zeros if that is zero), times `scale`.
+ * With a bias, s and c are 64-bit floats, so that the order does not hang on how a score was rounded.  A NaN counts as -infinity
+ * (as a logit, as a choice); infinite logits share a softmax row equally, and so do all experts of a row of nothing but -infinity.
+ * Limits: 1 <= E <= 1024, groups <= 64 and divides E, topk <= 64 and <= kept * E / groups; logits_dtype in {FR_F16, FR_BF16, FR_F32}. */
+#define FR_SCORE_SOFTMAX 0
+#define FR_SCORE_SIGMOID 1
+int fr_gating_grouped(const void* logits, int logits_dtype, int64_t M, int64_t E, int64_t ld, const float* bias, int groups, int kept,
+                      int topk, int scoring, int renormalize, float scale, float* weights_out, int32_t* ids_out, void* stream);
+
 /* ---- routing arrays ------------------------------------------------------
  * Block-aligned stable counting sort of the n = M*topk flat expert ids.
  *   sorted_token_ids : int32[n + E*(block-1)], fully written; padding = n
@@ -352,6 +366,63 @@ int64_t fr_moe_mxfp4_workspace_bytes(int64_t M, int64_t H, int64_t F, int E, int
 int fr_fused_moe_mxfp4(const void* x, int dtype, const void* w1_tiled, const void* w2_tiled, const void* logits, int logits_dtype,
                        int64_t M, int64_t H, int64_t F, int E, int topk, int renormalize, void* out, void* workspace,
                        int64_t workspace_bytes, void* stream);
+
+/* ---- attention ---------------------------------------------------------------
+ * No counterpart in the reference, whose layer bench runs its attention in torch.  f16 / bf16, fp32 accumulation.  Strides count
+ * elements; the elements of a head lie next to each other.  `heads` query heads share `kv_heads` key and value heads, consecutive ones the same.
+ *
+ * Rotary positions.  Pair i of a head's first `turned` dimensions is turned by position * freq[i] radians and scaled by
+ * `factor`: pairs (i, i + turned / 2) or, interleaved, (2 i, 2 i + 1); the other dimensions stay.  turns[i] = freq[i] / (2 pi) * 2^64,
+ * rounded, modulo 2^64 (uint64, device).  q [T, heads, dim] and k [T, kv_heads, dim] to q_out and k_out, which may be q and k themselves.
+ * With slots (not NULL), k_out's row and v's of token t also go to slot slots[t] of the cache: page slots[t] / page_size, place
+ * slots[t] % page_size; a slot outside [0, pages * page_size) keeps nothing.  A slot that two tokens name holds pieces of either.
+ * positions, slots: int64 where *_i64 is 1, else int32; any position.  turned even, <= 512; dim <= 1024.  Rows of 16-byte aligned
+ * addresses and strides, turned % 16 == 0 and dim % 8 == 0 are the fast case. */
+typedef struct fr_rotary_args {
+  const void *q, *k, *v;
+  void *q_out, *k_out, *k_cache, *v_cache;
+  const void *positions, *slots, *turns;
+  int64_t T, heads, kv_heads, dim, turned, pages, page_size;
+  int64_t q_token, q_head, k_token, k_head, v_token, v_head, q_out_token, q_out_head, k_out_token, k_out_head;
+  int64_t k_cache_page, k_cache_slot, k_cache_head, v_cache_page, v_cache_slot, v_cache_head;
+  int64_t dtype, interleaved, positions_i64, slots_i64;
+  double factor;
+} fr_rotary_args;
+int fr_rotary(const fr_rotary_args* args, void* stream);
+
+/* Packed prompts: sequence b's rows are cu_q[b] .. cu_q[b + 1] - 1 of q [rows, heads, dim], its keys cu_k[b] .. cu_k[b + 1] - 1 of k and v
+ * [keys, kv_heads, dim] (cu_* int32 [B + 1], device, not falling; taken inside [0, rows] and [0, keys]); out[r, h] = sum_j p_j v_j, p = softmax of
+ * scale * q[r, h] . k_j over the sequence's keys or, causal, those up to its row's place counted from the end: row i of n sees keys 0 .. m - n + i of m.
+ * A row that sees no key is zeros.  Keys that a row does not see do not reach it, whatever they hold.  Rows behind the last sequence (and in front of
+ * the first) are left as they were; with `fill` those behind it are set to zero.  heads a multiple of kv_heads; dim a multiple of 8 up to
+ * 256; q, k, v, out 16-byte aligned with strides of multiples of 8 elements; rows and keys below 2^30; scale in [1e-20, 1e20].  `out` may be q itself. */
+typedef struct fr_attention_args {
+  const void *q, *k, *v, *cu_q, *cu_k;
+  void* out;
+  int64_t B, rows, keys, heads, kv_heads, dim;
+  int64_t q_row, q_head, k_row, k_head, v_row, v_head, out_row, out_head;
+  int64_t dtype, causal, fill;
+  double scale;
+} fr_attention_args;
+int fr_attention(const fr_attention_args* args, void* stream);
+
+/* One query row per sequence over a paged cache: out[b, h] = sum_j p_j v_j, p = softmax over j < lengths[b] of scale * q[b, h] . k_j, key j of
+ * sequence b in place j % page_size of page table[b, j / page_size].  lengths int32 [B], table int32 [B, table_pages] (row stride table_row).
+ * A length is taken as 0 below it and as the table's end behind it; keys in a page outside [0, pages) take no part; a row without keys is
+ * zeros.  Pages behind a length are not looked at.  heads a multiple of kv_heads; dim a multiple of 8 up to 256; q, out, k_cache, v_cache 16-byte
+ * aligned with strides of multiples of 8 elements; any page_size, multiples of 16 are the fast case; table_pages * page_size <= 2^30; scale in [1e-20, 1e20].
+ * `workspace`: 16-byte aligned, fr_paged_attention_workspace_bytes(.., most = table_pages * page_size) bytes (0: none is needed; -1: sizes outside the
+ * limits); two calls that may overlap in time need one each.  `slots` and `page_shift` are the call's own. */
+typedef struct fr_paged_args {
+  const void *q, *k_cache, *v_cache, *table, *lengths;
+  void *out, *workspace;
+  int64_t workspace_bytes, B, heads, kv_heads, dim, pages, page_size, table_pages, table_row;
+  int64_t q_row, q_head, out_row, out_head, k_cache_page, k_cache_slot, k_cache_head, v_cache_page, v_cache_slot, v_cache_head;
+  int64_t dtype, slots, page_shift;
+  double scale;
+} fr_paged_args;
+int64_t fr_paged_attention_workspace_bytes(int64_t B, int64_t heads, int64_t kv_heads, int64_t dim, int64_t most);
+int fr_paged_attention(const fr_paged_args* args, void* stream);
 
 /* ---- measurement aid -------------------------------------------------------
  * A pure stream of bf16 MFMAs (no loads, no LDS) on every CU: `iters` rounds over 256 accumulator

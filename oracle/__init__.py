@@ -31,3 +31,8 @@ from .mxfp4_oracle import (  # noqa: F401
     mxfp4_round,
     mxfp4_values,
 )
+from .serving_oracle import (  # noqa: F401
+    attention,
+    grouped_topk,
+    rotary,
+)
