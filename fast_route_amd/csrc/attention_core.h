@@ -32,6 +32,16 @@ __device__ __forceinline__ typename Attn<T>::vec4 read_transposed(const T* at) {
 template <typename V4>
 __device__ __forceinline__ auto join8(V4 a, V4 b) { return __builtin_shufflevector(a, b, 0, 1, 2, 3, 4, 5, 6, 7); }
 
+#if defined(__HIP_DEVICE_COMPILE__)  // buffer resources exist in the device pass only
+// `bytes` from a pointer that all lanes share: loads behind them are dropped.
+__device__ __forceinline__ __amdgpu_buffer_rsrc_t uniform_buffer(const void* p, int bytes) {
+  const uint64_t at = reinterpret_cast<uint64_t>(p);
+  const uint64_t there = static_cast<uint64_t>(__builtin_amdgcn_readfirstlane(static_cast<int>(at >> 32))) << 32 |
+                         static_cast<unsigned>(__builtin_amdgcn_readfirstlane(static_cast<int>(at)));
+  return __builtin_amdgcn_make_buffer_rsrc(reinterpret_cast<void*>(there), 0, __builtin_amdgcn_readfirstlane(bytes), 0x00020000);
+}
+#endif
+
 // Over the lanes that differ in bit 4 (5) of their number: of the two values, in both lanes.
 __device__ __forceinline__ float max_over_16(float v) {
   const auto x = __builtin_amdgcn_permlane16_swap(__float_as_uint(v), __float_as_uint(v), false, false);
