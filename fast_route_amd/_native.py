@@ -71,6 +71,7 @@ SIGNATURES = {
     "fr_fused_moe_mxfp4": (c_int, [c_void_p, c_int, c_void_p, c_void_p, c_void_p, c_int, c_int64, c_int64, c_int64, c_int, c_int,
                                    c_int, c_void_p, c_void_p, c_int64, c_void_p]),
     "fr_rotary": (c_int, [c_char_p, c_void_p]),
+    "fr_attention_workspace_bytes": (c_int64, [c_int64, c_int64, c_int64, c_int64, c_int64, c_int64]),
     "fr_attention": (c_int, [c_char_p, c_void_p]),
     "fr_paged_attention_workspace_bytes": (c_int64, [c_int64, c_int64, c_int64, c_int64, c_int64]),
     "fr_paged_attention": (c_int, [c_char_p, c_void_p]),

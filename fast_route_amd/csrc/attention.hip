@@ -24,52 +24,82 @@ __device__ __forceinline__ void att_range(const int32_t* cu, int64_t b, int64_t 
   *end = b == B ? all : att_clamp(cu[b + 1], *begin, all);
 }
 
-// Tile `nth` of the tiles in descending order of their place: its sequence (-1: none) and place.
-__device__ __forceinline__ void att_place(const fr_attention_args& a, int64_t nth, int64_t* seq, int* place) {
+__device__ __forceinline__ int att_total(int v) {  // over the wavefront, in every lane
+  v += partner_i32<1>(v);
+  v += partner_i32<2>(v);
+  v += partner_i32<4>(v);
+  v += partner_i32<8>(v);
+  return (__builtin_amdgcn_readlane(v, 0) + __builtin_amdgcn_readlane(v, 16)) + (__builtin_amdgcn_readlane(v, 32) + __builtin_amdgcn_readlane(v, 48));
+}
+
+struct AttPlace {
+  int tile;                  // of the sequence, -1: none
+  int q_begin, n, k_begin, m;  // its rows and keys
+};
+
+// Tile `nth` of the tiles in descending order of their place.  The first 64 sequences' (most often all) lengths stay in the lanes.
+__device__ __forceinline__ AttPlace att_place(const fr_attention_args& a, int nth) {
   const int lane = threadIdx.x & 63;
   const int64_t share = a.heads / a.kv_heads, count = a.B + (a.fill ? 1 : 0);
-  const int32_t* cu = reinterpret_cast<const int32_t*>(a.cu_q);
-  auto tiles_of = [&](int64_t b) -> int {
-    if (b >= count) return 0;
+  const int32_t* const cu_q = reinterpret_cast<const int32_t*>(a.cu_q);
+  const int32_t* const cu_k = reinterpret_cast<const int32_t*>(a.cu_k);
+  struct Rows { int begin, n; };
+  auto range = [](const int32_t* cu, int64_t b, int64_t B, int64_t all) -> Rows {
     int64_t begin, end;
-    att_range(cu, b, a.B, a.rows, &begin, &end);
-    return static_cast<int>(((end - begin) * share + kAttTile - 1) / kAttTile);
+    att_range(cu, b, B, all, &begin, &end);
+    return Rows{static_cast<int>(begin), static_cast<int>(end - begin)};
   };
-  const int mine = tiles_of(lane);  // of the first 64 sequences, most often all
+  auto tiles_in = [&](Rows r) { return static_cast<int>((r.n * share + kAttTile - 1) / kAttTile); };
+  auto tiles_of = [&](int64_t b) { return b < count ? tiles_in(range(cu_q, b, a.B, a.rows)) : 0; };
+  Rows mine_q = {0, 0}, mine_k = {0, 0};
+  if (lane < count) mine_q = range(cu_q, lane, a.B, a.rows);
+  if (lane < a.B) mine_k = range(cu_k, lane, a.B, a.keys);
+  const int mine = tiles_in(mine_q);
   auto total = [&](auto f) {
     int v = f(mine);
     for (int64_t b = lane + kWave; b < count; b += kWave) v += f(tiles_of(b));
-#pragma unroll
-    for (int s = 1; s < kWave; s <<= 1) v += __shfl_xor(v, s, kWave);
-    return v;
+    return att_total(v);
   };
-  *seq = -1;
-  int lo = 0, hi = static_cast<int>((a.rows * share + kAttTile - 1) / kAttTile);  // tiles at places >= lo: more than nth; >= hi: not
-  if (total([&](int t) { return t; }) <= nth) return;
+  AttPlace p = {-1, 0, 0, 0, 0};
+  const int all = total([](int t) { return t; });
+  if (all <= nth) return p;
+  int64_t seq = -1;
+  int lo = 0;
   if (count == 1) {
-    *seq = 0;
-    *place = tiles_of(0) - 1 - static_cast<int>(nth);
-    return;
-  }
-  while (hi - lo > 1) {
-    const int mid = (lo + hi) >> 1;
-    if (total([&](int t) { return t > mid ? t - mid : 0; }) > nth) lo = mid;
-    else hi = mid;
-  }
-  int left = static_cast<int>(nth) - total([&](int t) { return t > lo + 1 ? t - lo - 1 : 0; });  // which of the sequences with a tile there
-  for (int64_t b0 = 0; b0 < count; b0 += kWave) {
-    const uint64_t has = __ballot((b0 ? tiles_of(b0 + lane) : mine) > lo);
-    const int n = __popcll(has);
-    if (left < n) {
-      const int before = __popcll(has & ((1ull << lane) - 1));
-      const uint64_t hit = __ballot(((has >> lane) & 1) && before == left);
-      if (!hit) return;
-      *seq = b0 + __ffsll(static_cast<unsigned long long>(hit)) - 1;
-      *place = lo;
-      return;
+    seq = 0;
+    lo = all - 1 - nth;
+  } else {
+    int hi = static_cast<int>((a.rows * share + kAttTile - 1) / kAttTile);  // tiles at places >= lo: more than nth; >= hi: not
+    while (hi - lo > 1) {
+      const int mid = (lo + hi) >> 1;
+      if (total([&](int t) { return t > mid ? t - mid : 0; }) > nth) lo = mid;
+      else hi = mid;
     }
-    left -= n;
+    int left = nth - total([&](int t) { return t > lo + 1 ? t - lo - 1 : 0; });  // which of the sequences with a tile there
+    for (int64_t b0 = 0; b0 < count; b0 += kWave) {
+      const uint64_t has = __ballot((b0 ? tiles_of(b0 + lane) : mine) > lo);
+      const int there = __popcll(has);
+      if (left < there) {
+        const uint64_t hit = __ballot(((has >> lane) & 1) && __popcll(has & ((1ull << lane) - 1)) == left);
+        if (!hit) return p;
+        seq = b0 + __ffsll(static_cast<unsigned long long>(hit)) - 1;
+        break;
+      }
+      left -= there;
+    }
+    if (seq < 0) return p;
   }
+  p.tile = __builtin_amdgcn_readfirstlane(lo);
+  const int l = __builtin_amdgcn_readfirstlane(static_cast<int>(seq & 63));
+  if (seq >= kWave) {
+    mine_q = range(cu_q, seq, a.B, a.rows);
+    mine_k = seq < a.B ? range(cu_k, seq, a.B, a.keys) : Rows{0, 0};
+  }
+  p.q_begin = __builtin_amdgcn_readlane(mine_q.begin, l);
+  p.n = __builtin_amdgcn_readlane(mine_q.n, l);
+  p.k_begin = __builtin_amdgcn_readlane(mine_k.begin, l);
+  p.m = __builtin_amdgcn_readlane(mine_k.n, l);
+  return p;
 }
 
 template <int DP>
@@ -95,16 +125,30 @@ __device__ __forceinline__ bool not_finite(unsigned w) {
   return (w & e) == e || (w & (e << 16)) == (e << 16);
 }
 
-// The wavefront's rows one by one, keys to lanes and then dimensions to lanes, fp32: no product of a masked key is formed.
+// Results of a part of the keys: [part][row][head] rows of DP sums, then as many maxima (in units of a factor 2) and sums of the softmax.
+template <int DP>
+struct AttPart {
+  float *rows, *tops, *sums;
+  __device__ __forceinline__ AttPart(const fr_attention_args& a, int part, int64_t row, int head) {
+    const int64_t all = a.rows * a.heads, at = part * all + row * a.heads + head;
+    float* const to = reinterpret_cast<float*>(a.workspace);
+    rows = to + at * DP;
+    tops = to + a.parts * all * DP + at;
+    sums = to + a.parts * all * (DP + 1) + at;
+  }
+};
+
+// The wavefront's rows one by one over keys k_first .. k_last - 1, keys to lanes and then dimensions to lanes, fp32: no product of a masked key is formed.
 template <typename T, int DP>
-__device__ void attention_rows(const fr_attention_args& a, const T* kc, const T* vc, int64_t row0, int64_t rows, int64_t q_begin, int n, int m, int kv, int share) {
+__device__ void attention_rows(const fr_attention_args& a, const T* kc, const T* vc, int64_t row0, int64_t rows, AttPlace at, int kv, int share, int part, int k_first,
+                               int k_last) {
   typedef typename Attn<T>::vec8 vec8;
   const int lane = threadIdx.x & 63, dim = static_cast<int>(a.dim);
   const float scale = static_cast<float>(a.scale) * kLog2e;
   for (int i = 0; i < kAttRows && row0 + i < rows; ++i) {
     const int token = static_cast<int>((row0 + i) / share), head = kv * share + static_cast<int>(row0 + i - static_cast<int64_t>(token) * share);
-    const int count = a.causal ? (m - n + token + 1 < 0 ? 0 : m - n + token + 1) : m;
-    const T* q = reinterpret_cast<const T*>(a.q) + (q_begin + token) * a.q_row + head * a.q_head;
+    const int seen = a.causal ? at.m - at.n + token + 1 : at.m, count = seen < k_last ? seen : k_last;
+    const T* q = reinterpret_cast<const T*>(a.q) + (at.q_begin + token) * a.q_row + head * a.q_head;
     auto score = [&](int key) {
       float s = 0.f;
       for (int d = 0; d < dim; d += 8) {
@@ -115,13 +159,13 @@ __device__ void attention_rows(const fr_attention_args& a, const T* kc, const T*
       return s * scale;
     };
     float top = -INFINITY, sum = 0.f, acc[DP / kWave];
-    for (int key = lane; key < count; key += kWave) top = fmaxf(top, score(key));
+    for (int key = k_first + lane; key < count; key += kWave) top = fmaxf(top, score(key));
 #pragma unroll
     for (int s = 1; s < kWave; s <<= 1) top = fmaxf(top, __shfl_xor(top, s, kWave));
     const float from = top == -INFINITY ? 0.f : top;
 #pragma unroll
     for (int d = 0; d < DP / kWave; ++d) acc[d] = 0.f;
-    for (int k0 = 0; k0 < count; k0 += kWave) {
+    for (int k0 = k_first; k0 < count; k0 += kWave) {
       const float p = k0 + lane < count ? exp2_of(score(k0 + lane) - from) : 0.f;
       sum += p;
       for (int j = 0; j < kWave && k0 + j < count; ++j) {
@@ -133,7 +177,14 @@ __device__ void attention_rows(const fr_attention_args& a, const T* kc, const T*
     }
 #pragma unroll
     for (int s = 1; s < kWave; s <<= 1) sum += __shfl_xor(sum, s, kWave);
-    T* to = reinterpret_cast<T*>(a.out) + (q_begin + token) * a.out_row + head * a.out_head;
+    if (a.parts > 1) {
+      const AttPart<DP> to(a, part, at.q_begin + token, head);
+#pragma unroll
+      for (int d = 0; d < DP / kWave; ++d) to.rows[d * kWave + lane] = d * kWave + lane < dim ? acc[d] : 0.f;
+      if (lane == 0) to.tops[0] = top, to.sums[0] = sum;
+      continue;
+    }
+    T* to = reinterpret_cast<T*>(a.out) + (at.q_begin + token) * a.out_row + head * a.out_head;
 #pragma unroll
     for (int d = 0; d < DP / kWave; ++d)
       if (d * kWave + lane < dim) to[d * kWave + lane] = static_cast<T>(sum == 0.f ? 0.f : acc[d] / sum);
@@ -151,27 +202,20 @@ __global__ __launch_bounds__(kAttThreads, 2) void attention_kernel(fr_attention_
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), half = lane >> 5, low = lane & 31;
   const int kv_heads = static_cast<int>(a.kv_heads), share = static_cast<int>(a.heads / a.kv_heads), dim = static_cast<int>(a.dim);
   // Workgroups go to the eight XCDs in turn: those of a key head to one of them, whose L2 then holds its keys once.
-  int kv;
-  int64_t nth;
+  int kv, item;
   if (kv_heads % 8 == 0) {
-    const int64_t i = blockIdx.x / 8;
-    kv = static_cast<int>(blockIdx.x % 8) * (kv_heads / 8) + static_cast<int>(i % (kv_heads / 8));
-    nth = i / (kv_heads / 8);
+    const int i = blockIdx.x / 8;
+    kv = blockIdx.x % 8 * (kv_heads / 8) + i % (kv_heads / 8);
+    item = i / (kv_heads / 8);
   } else {
     kv = blockIdx.x % kv_heads;
-    nth = blockIdx.x / kv_heads;
+    item = blockIdx.x / kv_heads;
   }
-  int64_t seq;
-  int place = 0;
-  att_place(a, nth, &seq, &place);
-  if (seq < 0) return;
-  seq = __builtin_amdgcn_readfirstlane(static_cast<int>(seq));
-  place = __builtin_amdgcn_readfirstlane(place);
-  int64_t q_begin, q_end, k_begin = 0, k_end = 0;
-  att_range(reinterpret_cast<const int32_t*>(a.cu_q), seq, a.B, a.rows, &q_begin, &q_end);
-  if (seq < a.B) att_range(reinterpret_cast<const int32_t*>(a.cu_k), seq, a.B, a.keys, &k_begin, &k_end);
-  const int n = static_cast<int>(q_end - q_begin), m = static_cast<int>(k_end - k_begin);
-  const int64_t rows = static_cast<int64_t>(n) * share, row0 = static_cast<int64_t>(place) * kAttTile, wave_row0 = row0 + wave * kAttRows;
+  const int parts = static_cast<int>(a.parts), part = item % parts;
+  const AttPlace at = att_place(a, item / parts);
+  if (at.tile < 0) return;
+  const int n = at.n, m = at.m, q_begin = at.q_begin;
+  const int64_t rows = static_cast<int64_t>(n) * share, row0 = static_cast<int64_t>(at.tile) * kAttTile, wave_row0 = row0 + wave * kAttRows;
   if (row0 >= rows) return;
   // the lane's row: token and query head; keys up to `limit` are seen
   const bool live = wave_row0 + low < rows;
@@ -183,7 +227,8 @@ __global__ __launch_bounds__(kAttThreads, 2) void attention_kernel(fr_attention_
   const int wave_first = __builtin_amdgcn_readfirstlane(limit), wave_last = wave_row0 >= rows ? -1 : __builtin_amdgcn_readlane(limit, 31);
   const int group_first = a.causal ? m - n + static_cast<int>(row0 / share) : m - 1;
   const int group_last = a.causal ? m - n + static_cast<int>(last_row / share) : m - 1;
-  const int blocks = group_last < 0 ? 0 : group_last / S::kKeys + 1;
+  const int all_blocks = group_last < 0 ? 0 : group_last / S::kKeys + 1;
+  const int first = static_cast<int>(static_cast<int64_t>(all_blocks) * part / parts), blocks = static_cast<int>(static_cast<int64_t>(all_blocks) * (part + 1) / parts);
 
   vec8 q[S::kSteps];
   {
@@ -195,8 +240,8 @@ __global__ __launch_bounds__(kAttThreads, 2) void attention_kernel(fr_attention_
     }
   }
   const float scale = static_cast<float>(a.scale) * kLog2e, lag = kLag / scale;
-  const T* const kc = reinterpret_cast<const T*>(a.k) + k_begin * a.k_row + kv * a.k_head;
-  const T* const vc = reinterpret_cast<const T*>(a.v) + k_begin * a.v_row + kv * a.v_head;
+  const T* const kc = reinterpret_cast<const T*>(a.k) + at.k_begin * a.k_row + kv * a.k_head;
+  const T* const vc = reinterpret_cast<const T*>(a.v) + at.k_begin * a.v_row + kv * a.v_head;
   if (threadIdx.x == 0) odd = 0;
   if (dim < DP) {  // the dimensions that there are not stay zero: no load goes there
     for (int i = threadIdx.x; i < 4 * S::kBlock / 16; i += kAttThreads) reinterpret_cast<i32x4*>(shared)[i] = i32x4{0, 0, 0, 0};
@@ -239,8 +284,8 @@ __global__ __launch_bounds__(kAttThreads, 2) void attention_kernel(fr_attention_
   float top = -INFINITY, sum = 0.f;  // unscaled, in both halves, lagging; the sum of the lane's own keys
 
   __syncthreads();
-  if (blocks > 0) load(0);
-  for (int block = 0; block < blocks; ++block) {
+  if (first < blocks) load(first);
+  for (int block = first; block < blocks; ++block) {
     const int k0 = block * S::kKeys;
     const char* const buffer = shared + (block & 1) * S::kBlock;
     asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
@@ -315,10 +360,22 @@ __global__ __launch_bounds__(kAttThreads, 2) void attention_kernel(fr_attention_
 
   __syncthreads();
   if (odd) {
-    attention_rows<T, DP>(a, kc, vc, wave_row0, rows, q_begin, n, m, kv, share);
+    attention_rows<T, DP>(a, kc, vc, wave_row0, rows, at, kv, share, part, first * S::kKeys, blocks * S::kKeys < m ? blocks * S::kKeys : m);
     return;
   }
   sum = sum_over_32(sum);
+  if (parts > 1) {
+    if (live) {
+      const AttPart<DP> to(a, part, q_begin + token, head);
+#pragma unroll
+      for (int t = 0; t < S::kTiles; ++t)
+#pragma unroll
+        for (int r = 0; r < 4; ++r)
+          *reinterpret_cast<f32x4*>(to.rows + t * 32 + r * 8 + half * 4) = f32x4{o[t][r * 4], o[t][r * 4 + 1], o[t][r * 4 + 2], o[t][r * 4 + 3]};
+      if (half == 0) to.tops[0] = top * scale, to.sums[0] = sum;
+    }
+    return;
+  }
   const float by = sum == 0.f ? 0.f : 1.f / sum;  // a row that sees no key: zeros
   if (live) {
     T* const to = reinterpret_cast<T*>(a.out) + (q_begin + token) * a.out_row + head * a.out_head + half * 4;
@@ -336,36 +393,95 @@ __global__ __launch_bounds__(kAttThreads, 2) void attention_kernel(fr_attention_
 #endif
 }
 
+// Joins the parts of the keys: four dimensions of a row's head to a thread.
+template <typename T, int DP>
+__global__ __launch_bounds__(kAttThreads) void attention_join_kernel(fr_attention_args a) {
+  constexpr int kLanes = DP / 4;
+  const int64_t i = static_cast<int64_t>(blockIdx.x) * kAttThreads + threadIdx.x, at = i / kLanes, row = at / a.heads;
+  const int d = static_cast<int>(i % kLanes) * 4, head = static_cast<int>(at - row * a.heads), parts = static_cast<int>(a.parts);
+  const int32_t* const cu = reinterpret_cast<const int32_t*>(a.cu_q);
+  if (row >= (a.fill ? a.rows : att_clamp(cu[a.B], 0, a.rows)) || row < cu[0] || d >= a.dim) return;  // of no sequence
+  const int64_t all = a.rows * a.heads;
+  const AttPart<DP> from(a, 0, row, head);
+  float top = -INFINITY, sum = 0.f;
+  for (int p = 0; p < parts; ++p) top = fmaxf(top, from.tops[p * all]);
+  f32x4 x = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll 4
+  for (int p = 0; p < parts; ++p) {
+    const float mine = from.tops[p * all], by = mine == -INFINITY ? 0.f : exp2_of(mine - top);
+    sum += by * from.sums[p * all];
+    x += *reinterpret_cast<const f32x4*>(from.rows + p * all * DP + d) * by;
+  }
+  typename Attn<T>::vec4 y;
+#pragma unroll
+  for (int e = 0; e < 4; ++e) y[e] = static_cast<T>(sum == 0.f ? 0.f : x[e] / sum);
+  *reinterpret_cast<typename Attn<T>::vec4*>(reinterpret_cast<T*>(a.out) + row * a.out_row + head * a.out_head + d) = y;
+}
+
+int att_dim(int64_t dim) { return dim <= 64 ? 64 : dim <= 128 ? 128 : dim <= 192 ? 192 : 256; }
+
+// Workgroups of a part: every sequence's last tile may be a part of one; the rows behind the last sequence are one more.
+int64_t att_tiles(int64_t B, int64_t rows, int64_t share, bool fill) { return ceil_div(rows * share, kAttTile) + B + (fill ? 1 : 0) - 1; }
+
+// Parts that the keys are split into: as many as fill the chip's 512 places for workgroups where the tiles do not, none of less than kAttPartKeys keys
+// of a sequence of average length (the lengths themselves are on the device).
+constexpr int64_t kAttPlaces = 512, kAttPartKeys = 256, kAttMostParts = 32;
+int64_t att_parts(int64_t B, int64_t rows, int64_t keys, int64_t heads, int64_t kv_heads) {
+  if (B < 1 || rows < 1) return 1;
+  const int64_t groups = (ceil_div(rows * (heads / kv_heads), kAttTile) + B - 1) * kv_heads;
+  int64_t parts = kAttPlaces / groups;
+  const int64_t useful = keys / B / kAttPartKeys;
+  parts = parts < useful ? parts : useful;
+  return parts < 1 ? 1 : (parts > kAttMostParts ? kAttMostParts : parts);
+}
+
 template <typename T, int DP>
 int launch_attention(const fr_attention_args& a, hipStream_t st) {
-  // every sequence's last tile may be a part of one; the rows behind the last sequence are one more
-  const int64_t tiles = ceil_div(a.rows * (a.heads / a.kv_heads), kAttTile) + a.B + (a.fill ? 1 : 0) - 1;
-  hipLaunchKernelGGL((attention_kernel<T, DP>), dim3(static_cast<unsigned>(tiles * a.kv_heads)), dim3(kAttThreads), 0, st, a);
-  return check_launch("attention_kernel");
+  const int64_t tiles = att_tiles(a.B, a.rows, a.heads / a.kv_heads, a.fill != 0);
+  hipLaunchKernelGGL((attention_kernel<T, DP>), dim3(static_cast<unsigned>(tiles * a.parts * a.kv_heads)), dim3(kAttThreads), 0, st, a);
+  const int rc = check_launch("attention_kernel");
+  if (rc != FR_OK || a.parts == 1) return rc;
+  hipLaunchKernelGGL((attention_join_kernel<T, DP>), dim3(static_cast<unsigned>(ceil_div(a.rows * a.heads * (DP / 4), kAttThreads))), dim3(kAttThreads), 0, st, a);
+  return check_launch("attention_join_kernel");
 }
 
 template <typename T>
 int dispatch_attention(const fr_attention_args& a, hipStream_t st) {
-  if (a.dim <= 64) return launch_attention<T, 64>(a, st);
-  if (a.dim <= 128) return launch_attention<T, 128>(a, st);
-  if (a.dim <= 192) return launch_attention<T, 192>(a, st);
-  return launch_attention<T, 256>(a, st);
+  switch (att_dim(a.dim)) {
+    case 64: return launch_attention<T, 64>(a, st);
+    case 128: return launch_attention<T, 128>(a, st);
+    case 192: return launch_attention<T, 192>(a, st);
+    default: return launch_attention<T, 256>(a, st);
+  }
+}
+
+int check_attention_sizes(int64_t B, int64_t rows, int64_t keys, int64_t heads, int64_t kv_heads, int64_t dim) {
+  FR_REQUIRE(heads >= 1 && kv_heads >= 1 && heads % kv_heads == 0 && heads <= 65536, FR_E_SHAPE, "fr_attention: %lld heads over %lld key heads", (long long)heads,
+             (long long)kv_heads);
+  FR_REQUIRE(dim >= 8 && dim <= 256 && dim % 8 == 0, FR_E_SHAPE, "fr_attention: head size %lld: a multiple of 8 up to 256", (long long)dim);
+  FR_REQUIRE(rows >= 0 && rows < (int64_t(1) << 30) && keys >= 0 && keys < (int64_t(1) << 30), FR_E_SHAPE, "fr_attention: %lld rows, %lld keys: below 2^30",
+             (long long)rows, (long long)keys);
+  FR_REQUIRE(B >= 0 && B <= (1 << 20) && (rows + B * kAttTile) * heads < (int64_t(1) << 37), FR_E_SHAPE, "fr_attention: %lld sequences, %lld rows of %lld heads",
+             (long long)B, (long long)rows, (long long)heads);
+  return FR_OK;
 }
 
 }  // namespace
 }  // namespace fr
 
+extern "C" int64_t fr_attention_workspace_bytes(int64_t B, int64_t rows, int64_t keys, int64_t heads, int64_t kv_heads, int64_t dim) {
+  using namespace fr;
+  if (check_attention_sizes(B, rows, keys, heads, kv_heads, dim) != FR_OK) return -1;
+  const int64_t parts = att_parts(B, rows, keys, heads, kv_heads);
+  return parts == 1 ? 0 : parts * rows * heads * (att_dim(dim) + 2) * 4;
+}
+
 extern "C" int fr_attention(const fr_attention_args* args, void* stream) {
   using namespace fr;
   FR_REQUIRE(args, FR_E_NULL, "fr_attention: null pointer");
-  const fr_attention_args& a = *args;
-  FR_REQUIRE(a.heads >= 1 && a.kv_heads >= 1 && a.heads % a.kv_heads == 0 && a.heads <= 65536, FR_E_SHAPE, "fr_attention: %lld heads over %lld key heads",
-             (long long)a.heads, (long long)a.kv_heads);
-  FR_REQUIRE(a.dim >= 8 && a.dim <= 256 && a.dim % 8 == 0, FR_E_SHAPE, "fr_attention: head size %lld: a multiple of 8 up to 256", (long long)a.dim);
-  FR_REQUIRE(a.rows >= 0 && a.rows < (int64_t(1) << 30) && a.keys >= 0 && a.keys < (int64_t(1) << 30), FR_E_SHAPE, "fr_attention: %lld rows, %lld keys: below 2^30",
-             (long long)a.rows, (long long)a.keys);
-  FR_REQUIRE(a.B >= 0 && a.B <= (1 << 20) && (a.rows + a.B * kAttTile) * a.heads < (int64_t(1) << 37), FR_E_SHAPE, "fr_attention: %lld sequences, %lld rows of %lld heads",
-             (long long)a.B, (long long)a.rows, (long long)a.heads);
+  fr_attention_args a = *args;
+  const int rc = check_attention_sizes(a.B, a.rows, a.keys, a.heads, a.kv_heads, a.dim);
+  if (rc != FR_OK) return rc;
   FR_REQUIRE(a.dtype == FR_F16 || a.dtype == FR_BF16, FR_E_DTYPE, "fr_attention: dtype %lld not in {f16, bf16}", (long long)a.dtype);
   FR_REQUIRE(a.scale >= 1e-20 && a.scale <= 1e20, FR_E_SHAPE, "fr_attention: scale %g outside [1e-20, 1e20]", a.scale);
   if (a.rows == 0 || (a.B == 0 && !a.fill)) return FR_OK;
@@ -375,6 +491,10 @@ extern "C" int fr_attention(const fr_attention_args* args, void* stream) {
              "fr_attention: q, k, v and out: 16-byte aligned, strides multiples of 8 elements");
   FR_REQUIRE(a.k_row >= 0 && a.k_row < (1 << 23) && a.v_row >= 0 && a.v_row < (1 << 23), FR_E_SHAPE, "fr_attention: keys %lld and values %lld elements apart: below 2^23",
              (long long)a.k_row, (long long)a.v_row);
+  const int64_t need = fr_attention_workspace_bytes(a.B, a.rows, a.keys, a.heads, a.kv_heads, a.dim);
+  FR_REQUIRE(need == 0 || (a.workspace && aligned16(a.workspace) && a.workspace_bytes >= need), FR_E_WORKSPACE,
+             "fr_attention: workspace of %lld bytes, %lld needed", (long long)a.workspace_bytes, (long long)need);
+  a.parts = att_parts(a.B, a.rows, a.keys, a.heads, a.kv_heads);
   hipStream_t st = static_cast<hipStream_t>(stream);
   return a.dtype == FR_BF16 ? dispatch_attention<bf16_t>(a, st) : dispatch_attention<f16_t>(a, st);
 }

@@ -12,7 +12,7 @@ import torch
 from .. import _native as N
 
 _FLOATS = (torch.float16, torch.bfloat16)
-_PACKED = struct.Struct("@23qd")  # fr_attention_args
+_PACKED = struct.Struct("@26qd")  # fr_attention_args
 _PAGED = struct.Struct("@29qd")  # fr_paged_args
 
 
@@ -38,7 +38,8 @@ def _output(out: torch.Tensor | None, q: torch.Tensor) -> torch.Tensor:
 
 
 def attention_varlen(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, cu_seqlens_q: torch.Tensor, cu_seqlens_k: torch.Tensor | None = None,
-                     causal: bool = True, scale: float | None = None, out: torch.Tensor | None = None) -> torch.Tensor:
+                     causal: bool = True, scale: float | None = None, out: torch.Tensor | None = None,
+                     workspace_buf: torch.Tensor | None = None) -> torch.Tensor:
     """Attention of packed sequences: q [tokens, heads, head size], k and v [keys, kv heads, head size] in f16/bf16 (parts of a joint
     projection's result, for instance), sequence b's rows from cu_seqlens_q[b] to cu_seqlens_q[b + 1] and its keys from cu_seqlens_k[b] on
     (int32 [sequences + 1]; without cu_seqlens_k the same).  heads a multiple of kv heads, consecutive ones share a key head; `scale`
@@ -62,12 +63,16 @@ def attention_varlen(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, cu_seqle
     assert k.device == dev and v.device == dev and cu_seqlens_q.device == dev and cu_k.device == dev, "operands on different devices"
     fill = out is None
     out = _output(out, q)
+    B, (keys, kv_heads, _), lib = cu_seqlens_q.shape[0] - 1, k.shape, N.lib()
+    need = lib.fr_attention_workspace_bytes(B, rows, keys, heads, kv_heads, dim)
+    assert need >= 0, lib.fr_last_error_string().decode()
+    ws = _workspace(workspace_buf, need, dev)
     args = _PACKED.pack(q.data_ptr(), k.data_ptr(), v.data_ptr(), cu_seqlens_q.data_ptr(), cu_k.data_ptr(), out.data_ptr(),
-                        cu_seqlens_q.shape[0] - 1, rows, k.shape[0], heads, k.shape[1], dim, q_row, q_head, k_row, k_head, v_row, v_head,
-                        out.stride(0), out.stride(1), N.dtype_code(dtype), int(bool(causal)), int(fill),
+                        0 if ws is None else ws.data_ptr(), 0 if ws is None else ws.numel(), B, rows, keys, heads, kv_heads, dim,
+                        q_row, q_head, k_row, k_head, v_row, v_head, out.stride(0), out.stride(1), N.dtype_code(dtype), int(bool(causal)), int(fill), 0,
                         float(dim ** -0.5 if scale is None else scale))
     with N.on(dev):
-        N.check(N.lib().fr_attention(args, N.stream_ptr(dev)))
+        N.check(lib.fr_attention(args, N.stream_ptr(dev)))
     return out
 
 
