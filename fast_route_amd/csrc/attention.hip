@@ -37,10 +37,12 @@ struct AttPlace {
   int q_begin, n, k_begin, m;  // its rows and keys
 };
 
-// Tile `nth` of the tiles in descending order of their place.  The first 64 sequences' (most often all) lengths stay in the lanes.
+// Tile `nth` of the tiles in descending order of their place.  The first 256 sequences' tiles stay in the lanes: a search step is a
+// handful of instructions there and a round trip to L2 beyond (96 sequences of 128 rows: 6.7 us of a workgroup's 16 when only 64 did).
+constexpr int kAttHeld = 4;
 __device__ __forceinline__ AttPlace att_place(const fr_attention_args& a, int nth) {
   const int lane = threadIdx.x & 63;
-  const int64_t share = a.heads / a.kv_heads, count = a.B + (a.fill ? 1 : 0);
+  const int share = static_cast<int>(a.heads / a.kv_heads), count = static_cast<int>(a.B + (a.fill ? 1 : 0));
   const int32_t* const cu_q = reinterpret_cast<const int32_t*>(a.cu_q);
   const int32_t* const cu_k = reinterpret_cast<const int32_t*>(a.cu_k);
   struct Rows { int begin, n; };
@@ -49,48 +51,59 @@ __device__ __forceinline__ AttPlace att_place(const fr_attention_args& a, int nt
     att_range(cu, b, B, all, &begin, &end);
     return Rows{static_cast<int>(begin), static_cast<int>(end - begin)};
   };
-  auto tiles_in = [&](Rows r) { return static_cast<int>((r.n * share + kAttTile - 1) / kAttTile); };
-  auto tiles_of = [&](int64_t b) { return b < count ? tiles_in(range(cu_q, b, a.B, a.rows)) : 0; };
-  Rows mine_q = {0, 0}, mine_k = {0, 0};
+  auto tiles_in = [&](int n) { return (n * share + kAttTile - 1) / kAttTile; };
+  auto tiles_of = [&](int b) { return b < count ? tiles_in(range(cu_q, b, a.B, a.rows).n) : 0; };
+  Rows mine_q = {0, 0}, mine_k = {0, 0};  // of sequence `lane`
   if (lane < count) mine_q = range(cu_q, lane, a.B, a.rows);
   if (lane < a.B) mine_k = range(cu_k, lane, a.B, a.keys);
-  const int mine = tiles_in(mine_q);
+  int mine[kAttHeld];  // tiles of sequences lane + 64 j
+#pragma unroll
+  for (int j = 0; j < kAttHeld; ++j) mine[j] = j == 0 ? tiles_in(mine_q.n) : (j * kWave < count ? tiles_of(lane + j * kWave) : 0);
   auto total = [&](auto f) {
-    int v = f(mine);
-    for (int64_t b = lane + kWave; b < count; b += kWave) v += f(tiles_of(b));
+    int v = f(mine[0]);
+    if (count > kWave) {
+#pragma unroll
+      for (int j = 1; j < kAttHeld; ++j) v += f(mine[j]);
+      for (int b = lane + kAttHeld * kWave; b < count; b += kWave) v += f(tiles_of(b));
+    }
     return att_total(v);
   };
   AttPlace p = {-1, 0, 0, 0, 0};
-  const int all = total([](int t) { return t; });
-  if (all <= nth) return p;
-  int64_t seq = -1;
-  int lo = 0;
+  int seq = 0, lo = 0;
   if (count == 1) {
-    seq = 0;
-    lo = all - 1 - nth;
+    lo = __builtin_amdgcn_readfirstlane(mine[0]) - 1 - nth;
+    if (lo < 0) return p;
   } else {
-    int hi = static_cast<int>((a.rows * share + kAttTile - 1) / kAttTile);  // tiles at places >= lo: more than nth; >= hi: not
+    if (total([](int t) { return t; }) <= nth) return p;
+    int hi = tiles_in(static_cast<int>(a.rows));  // tiles at places >= lo: more than nth; >= hi: not
+    for (int step = 1; lo + step < hi; step <<= 1) {  // most sequences are short beside all of them
+      if (total([&](int t) { return t > lo + step ? t - lo - step : 0; }) <= nth) {
+        hi = lo + step;
+        break;
+      }
+      lo += step;
+    }
     while (hi - lo > 1) {
       const int mid = (lo + hi) >> 1;
       if (total([&](int t) { return t > mid ? t - mid : 0; }) > nth) lo = mid;
       else hi = mid;
     }
     int left = nth - total([&](int t) { return t > lo + 1 ? t - lo - 1 : 0; });  // which of the sequences with a tile there
-    for (int64_t b0 = 0; b0 < count; b0 += kWave) {
-      const uint64_t has = __ballot((b0 ? tiles_of(b0 + lane) : mine) > lo);
+    seq = -1;
+    for (int b0 = 0; b0 < count && seq < 0; b0 += kWave) {
+      const uint64_t has = __ballot((b0 ? tiles_of(b0 + lane) : mine[0]) > lo);
       const int there = __popcll(has);
       if (left < there) {
         const uint64_t hit = __ballot(((has >> lane) & 1) && __popcll(has & ((1ull << lane) - 1)) == left);
         if (!hit) return p;
         seq = b0 + __ffsll(static_cast<unsigned long long>(hit)) - 1;
-        break;
       }
       left -= there;
     }
     if (seq < 0) return p;
   }
   p.tile = __builtin_amdgcn_readfirstlane(lo);
-  const int l = __builtin_amdgcn_readfirstlane(static_cast<int>(seq & 63));
+  const int l = __builtin_amdgcn_readfirstlane(seq & 63);
   if (seq >= kWave) {
     mine_q = range(cu_q, seq, a.B, a.rows);
     mine_k = seq < a.B ? range(cu_k, seq, a.B, a.keys) : Rows{0, 0};
@@ -109,13 +122,16 @@ struct AttShape {
   static constexpr int kChunks = DP / 8;                            // 16-byte pieces of a row
   static constexpr int kRow = DP * 2, kBlock = kKeys * kRow;        // bytes
   static constexpr int kLoads = kKeys * kChunks / kAttThreads;      // pieces of a block that a thread loads
-  static constexpr int kSteps = DP / 16, kTiles = DP / 32;
-  // Rows lie in LDS with their pieces exchanged: K so that 8 rows' pieces of one place meet in no bank, V so that the four rows of a
-  // transposed read, 32 elements each, do not.
+  static constexpr int kSteps = DP / 32, kTiles = DP / 16;
+  // Rows lie in LDS with their pieces exchanged, so that 16 rows' pieces of one place (K) and eight rows' 32 bytes of one place (V: lanes 0 .. 31 of a
+  // transposed read, or 0 .. 15 and 32 .. 47) meet in no bank of the 64; rows of an odd multiple of 128 bytes alternate between their
+  // halves by themselves.  (256 dimensions: 8 rows of K, registers being short, and lanes 0 .. 31 of V, a load's rows being eight.)
   static constexpr bool kWide = DP % 128 == 0;
-  static constexpr int kValueBases = kWide ? 4 : 2;
-  static __device__ __forceinline__ int k_piece(int row, int chunk) { return chunk ^ (row & 7); }
-  static __device__ __forceinline__ int v_piece(int row, int chunk) { return chunk ^ (kWide ? (row & 3) << 2 : ((row >> 1) & 1) << 2); }
+  static constexpr int kKeyBases = DP == 128 ? 4 : 2, kValueBases = kWide ? 8 : 4;
+  static __device__ __forceinline__ int k_piece(int row, int chunk) { return chunk ^ (DP == 128 ? row & 15 : kWide ? row & 7 : (row >> 1) & 7); }
+  static __device__ __forceinline__ int v_piece(int row, int chunk) {
+    return chunk ^ (DP == 256 ? (row & 7) << 1 : kWide ? (row & 3) << 1 | ((row >> 2 ^ row >> 3) & 1) << 3 : ((row >> 1) & 1) << 1 | ((row >> 2 ^ row >> 3) & 1) << 2);
+  }
 };
 
 // A 16-bit float that is infinite or not a number, in either half of a word.
@@ -140,13 +156,13 @@ struct AttPart {
 
 // The wavefront's rows one by one over keys k_first .. k_last - 1, keys to lanes and then dimensions to lanes, fp32: no product of a masked key is formed.
 template <typename T, int DP>
-__device__ void attention_rows(const fr_attention_args& a, const T* kc, const T* vc, int64_t row0, int64_t rows, AttPlace at, int kv, int share, int part, int k_first,
+__device__ void attention_rows(const fr_attention_args& a, const T* kc, const T* vc, int row0, int rows, AttPlace at, int kv, int share, int part, int k_first,
                                int k_last) {
   typedef typename Attn<T>::vec8 vec8;
   const int lane = threadIdx.x & 63, dim = static_cast<int>(a.dim);
   const float scale = static_cast<float>(a.scale) * kLog2e;
   for (int i = 0; i < kAttRows && row0 + i < rows; ++i) {
-    const int token = static_cast<int>((row0 + i) / share), head = kv * share + static_cast<int>(row0 + i - static_cast<int64_t>(token) * share);
+    const int token = (row0 + i) / share, head = kv * share + (row0 + i - token * share);
     const int seen = a.causal ? at.m - at.n + token + 1 : at.m, count = seen < k_last ? seen : k_last;
     const T* q = reinterpret_cast<const T*>(a.q) + (at.q_begin + token) * a.q_row + head * a.q_head;
     auto score = [&](int key) {
@@ -199,7 +215,7 @@ __global__ __launch_bounds__(kAttThreads, 2) void attention_kernel(fr_attention_
   typedef AttShape<DP> S;
   __shared__ __attribute__((aligned(16))) char shared[4 * S::kBlock];  // K in two buffers, V in two
   __shared__ int odd;  // a block with masked keys has values that are not finite
-  const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), half = lane >> 5, low = lane & 31;
+  const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), quarter = lane >> 4, low = lane & 15;
   const int kv_heads = static_cast<int>(a.kv_heads), share = static_cast<int>(a.heads / a.kv_heads), dim = static_cast<int>(a.dim);
   // Workgroups go to the eight XCDs in turn: those of a key head to one of them, whose L2 then holds its keys once.
   int kv, item;
@@ -215,146 +231,181 @@ __global__ __launch_bounds__(kAttThreads, 2) void attention_kernel(fr_attention_
   const AttPlace at = att_place(a, item / parts);
   if (at.tile < 0) return;
   const int n = at.n, m = at.m, q_begin = at.q_begin;
-  const int64_t rows = static_cast<int64_t>(n) * share, row0 = static_cast<int64_t>(at.tile) * kAttTile, wave_row0 = row0 + wave * kAttRows;
+  const int rows = n * share, row0 = at.tile * kAttTile, wave_row0 = row0 + wave * kAttRows;
   if (row0 >= rows) return;
-  // the lane's row: token and query head; keys up to `limit` are seen
-  const bool live = wave_row0 + low < rows;
-  const int64_t row = live ? wave_row0 + low : rows - 1;
-  const int token = static_cast<int>(row / share), head = kv * share + static_cast<int>(row - static_cast<int64_t>(token) * share);
-  const int limit = a.causal ? m - n + token : m - 1;
-  // of the wavefront's first and last row and of the workgroup's
-  const int64_t last_row = row0 + kAttTile < rows ? row0 + kAttTile - 1 : rows - 1;
-  const int wave_first = __builtin_amdgcn_readfirstlane(limit), wave_last = wave_row0 >= rows ? -1 : __builtin_amdgcn_readlane(limit, 31);
-  const int group_first = a.causal ? m - n + static_cast<int>(row0 / share) : m - 1;
-  const int group_last = a.causal ? m - n + static_cast<int>(last_row / share) : m - 1;
-  const int all_blocks = group_last < 0 ? 0 : group_last / S::kKeys + 1;
-  const int first = static_cast<int>(static_cast<int64_t>(all_blocks) * part / parts), blocks = static_cast<int>(static_cast<int64_t>(all_blocks) * (part + 1) / parts);
-
-  vec8 q[S::kSteps];
-  {
-    const T* from = reinterpret_cast<const T*>(a.q) + (q_begin + token) * a.q_row + head * a.q_head;
+  // the lane's two rows, 16 apart: token and query head; keys up to `limit` are seen
+  int token[2], head[2], limit[2];
+  bool live[2];
 #pragma unroll
-    for (int s = 0; s < S::kSteps; ++s) {
-      const int d = s * 16 + half * 8;
-      q[s] = d < dim ? *reinterpret_cast<const vec8*>(from + d) : vec8{0, 0, 0, 0, 0, 0, 0, 0};
-    }
+  for (int i = 0; i < 2; ++i) {
+    const int r = wave_row0 + 16 * i + low;
+    live[i] = r < rows;
+    token[i] = (live[i] ? r : rows - 1) / share;
+    head[i] = kv * share + (live[i] ? r : rows - 1) - token[i] * share;
+    limit[i] = a.causal ? m - n + token[i] : m - 1;
   }
+  // of the wavefront's first and last row and of the workgroup's
+  const int last_row = row0 + kAttTile < rows ? row0 + kAttTile - 1 : rows - 1;
+  const int wave_first = __builtin_amdgcn_readfirstlane(limit[0]), wave_last = wave_row0 >= rows ? -1 : __builtin_amdgcn_readlane(limit[1], 15);
+  const int group_first = a.causal ? m - n + row0 / share : m - 1;
+  const int group_last = a.causal ? m - n + last_row / share : m - 1;
+  const int all_blocks = group_last < 0 ? 0 : group_last / S::kKeys + 1;
+  // 2^30 / 32 blocks times 32 parts: 32 bits
+  const int first = static_cast<int>(static_cast<unsigned>(all_blocks) * part / parts), blocks = static_cast<int>(static_cast<unsigned>(all_blocks) * (part + 1) / parts);
+
   const float scale = static_cast<float>(a.scale) * kLog2e, lag = kLag / scale;
   const T* const kc = reinterpret_cast<const T*>(a.k) + at.k_begin * a.k_row + kv * a.k_head;
   const T* const vc = reinterpret_cast<const T*>(a.v) + at.k_begin * a.v_row + kv * a.v_head;
   if (threadIdx.x == 0) odd = 0;
   if (dim < DP) {  // the dimensions that there are not stay zero: no load goes there
     for (int i = threadIdx.x; i < 4 * S::kBlock / 16; i += kAttThreads) reinterpret_cast<i32x4*>(shared)[i] = i32x4{0, 0, 0, 0};
+    __syncthreads();
   }
-  // Where this thread's pieces of a block come from: bytes from the block's first row.
-  int k_from[S::kLoads], v_from[S::kLoads];
+  // Where this thread's pieces of a block come from: bytes from the block's first row; where the pieces of a load are whole rows, from the
+  // load's, one register for all loads (their pieces are exchanged alike).  Rows behind the last key and dimensions that there are
+  // not lie behind the resource's end: dropped.
+  constexpr bool kRows = kAttThreads % S::kChunks == 0;
+  constexpr int kOffsets = kRows ? 1 : S::kLoads, kStep = kRows ? kAttThreads / S::kChunks : 0;
+  int k_from[kOffsets], v_from[kOffsets];
 #pragma unroll
-  for (int i = 0; i < S::kLoads; ++i) {
+  for (int i = 0; i < kOffsets; ++i) {
     const int at = i * kAttThreads + threadIdx.x, r = at / S::kChunks, kd = S::k_piece(r, at % S::kChunks) * 8, vd = S::v_piece(r, at % S::kChunks) * 8;
-    k_from[i] = kd < dim ? (r * static_cast<int>(a.k_row) + kd) * 2 : -1;  // -1: behind every resource's end
+    k_from[i] = kd < dim ? (r * static_cast<int>(a.k_row) + kd) * 2 : -1;
     v_from[i] = vd < dim ? (r * static_cast<int>(a.v_row) + vd) * 2 : -1;
   }
   typedef __attribute__((address_space(3))) void* lds_ptr;
-  auto load = [&](int block) {
+  auto load = [&](const T* from, int row, const int (&offset)[kOffsets], char* to, int block) {
     const int k0 = block * S::kKeys, there = m - k0 < S::kKeys ? m - k0 : S::kKeys;
-    const __amdgpu_buffer_rsrc_t kr = uniform_buffer(kc + k0 * a.k_row, ((there - 1) * static_cast<int>(a.k_row) + dim) * 2);
-    const __amdgpu_buffer_rsrc_t vr = uniform_buffer(vc + k0 * a.v_row, ((there - 1) * static_cast<int>(a.v_row) + dim) * 2);
-    char* const kt = shared + (block & 1) * S::kBlock;
 #pragma unroll
     for (int i = 0; i < S::kLoads; ++i) {
-      __builtin_amdgcn_raw_ptr_buffer_load_lds(kr, (lds_ptr)(kt + (i * kAttThreads + wave * kWave) * 16), 16, k_from[i], 0, 0, 0);
-      __builtin_amdgcn_raw_ptr_buffer_load_lds(vr, (lds_ptr)(kt + 2 * S::kBlock + (i * kAttThreads + wave * kWave) * 16), 16, v_from[i], 0, 0, 0);
+      const int left = there - i * kStep;
+      const __amdgpu_buffer_rsrc_t r = uniform_buffer(from + static_cast<int64_t>(k0 + i * kStep) * row, left > 0 ? ((left - 1) * row + dim) * 2 : 0);
+      __builtin_amdgcn_raw_ptr_buffer_load_lds(r, (lds_ptr)(to + (block & 1) * S::kBlock + (i * kAttThreads + wave * kWave) * 16), 16, offset[kRows ? 0 : i], 0, 0, 0);
     }
   };
-  // What this lane reads of a block's rows: see k_piece and v_piece.
-  int k_at[4], v_at[S::kValueBases];
+  auto load_k = [&](int block) { load(kc, static_cast<int>(a.k_row), k_from, shared, block); };
+  auto load_v = [&](int block) { load(vc, static_cast<int>(a.v_row), v_from, shared + 2 * S::kBlock, block); };
+  if (first < blocks) {
+    load_k(first);
+    load_v(first);
+  }
+  vec8 q[2][S::kSteps];
 #pragma unroll
-  for (int j = 0; j < 4; ++j) k_at[j] = low * S::kRow + S::k_piece(low, 2 * j + half) * 16;
+  for (int i = 0; i < 2; ++i) {
+    const T* from = reinterpret_cast<const T*>(a.q) + (q_begin + token[i]) * a.q_row + head[i] * a.q_head;
+#pragma unroll
+    for (int s = 0; s < S::kSteps; ++s) {
+      const int d = s * 32 + quarter * 8;
+      q[i][s] = d < dim ? *reinterpret_cast<const vec8*>(from + d) : vec8{0, 0, 0, 0, 0, 0, 0, 0};
+    }
+  }
+  // What this lane reads of a block's rows: see k_piece and v_piece.
+  int k_at[S::kKeyBases], v_at[S::kValueBases];
+#pragma unroll
+  for (int j = 0; j < S::kKeyBases; ++j) k_at[j] = low * S::kRow + S::k_piece(low, 4 * j + quarter) * 16;
 #pragma unroll
   for (int j = 0; j < S::kValueBases; ++j) {
-    const int r = half * 4 + ((lane & 15) >> 2);
-    v_at[j] = 2 * S::kBlock + r * S::kRow + S::v_piece(r, j * 4 + ((lane >> 4) & 1) * 2 + ((lane & 3) >> 1)) * 16 + (lane & 1) * 8;
+    const int r = quarter * 4 + (low >> 2);
+    v_at[j] = 2 * S::kBlock + r * S::kRow + S::v_piece(r, j * 2 + ((low & 3) >> 1)) * 16 + (low & 1) * 8;
   }
 
-  f32x16 o[S::kTiles];
+  f32x4 o[2][S::kTiles];
 #pragma unroll
-  for (int t = 0; t < S::kTiles; ++t)
+  for (int i = 0; i < 2; ++i)
 #pragma unroll
-    for (int r = 0; r < 16; ++r) o[t][r] = 0.f;
-  float top = -INFINITY, sum = 0.f;  // unscaled, in both halves, lagging; the sum of the lane's own keys
+    for (int t = 0; t < S::kTiles; ++t) o[i][t] = f32x4{0.f, 0.f, 0.f, 0.f};
+  float top[2] = {-INFINITY, -INFINITY}, sum[2] = {0.f, 0.f};  // unscaled, in all four lanes of a row, lagging; the sum of the lane's own keys
 
-  __syncthreads();
-  if (first < blocks) load(first);
   for (int block = first; block < blocks; ++block) {
     const int k0 = block * S::kKeys;
     const char* const buffer = shared + (block & 1) * S::kBlock;
     asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
     __syncthreads();  // the block is there, and the one before it has been read
-    if (block + 1 < blocks) load(block + 1);
-    if (k0 + S::kKeys > m) {  // behind the last key: zeros, whatever lies there
-      for (int i = threadIdx.x; i < (S::kKeys - (m - k0)) * S::kChunks; i += kAttThreads)
-        *reinterpret_cast<i32x4*>(const_cast<char*>(buffer) + 2 * S::kBlock + ((m - k0) * S::kChunks + i) * 16) = i32x4{0, 0, 0, 0};
-      __syncthreads();
+    if (block + 1 < blocks) {
+      load_k(block + 1);
+      load_v(block + 1);
     }
-    if (a.causal && k0 + S::kKeys - 1 > group_first) {
-      bool bad = false;
-      for (int i = threadIdx.x; i < S::kBlock / 16; i += kAttThreads) {
-        const i32x4 w = *reinterpret_cast<const i32x4*>(buffer + 2 * S::kBlock + i * 16);
-        bad = bad || not_finite<T>(w[0]) || not_finite<T>(w[1]) || not_finite<T>(w[2]) || not_finite<T>(w[3]);
+    if (a.causal || k0 + S::kKeys > m) {
+      char* const values = shared + 2 * S::kBlock + (block & 1) * S::kBlock;
+      if (k0 + S::kKeys > m) {  // behind the last key: zeros, whatever lies there
+        for (int i = threadIdx.x; i < (S::kKeys - (m - k0)) * S::kChunks; i += kAttThreads)
+          *reinterpret_cast<i32x4*>(values + ((m - k0) * S::kChunks + i) * 16) = i32x4{0, 0, 0, 0};
+        __syncthreads();
       }
-      if (bad) odd = 1;
+      if (a.causal && k0 + S::kKeys - 1 > group_first) {
+        bool bad = false;
+        for (int i = threadIdx.x; i < S::kBlock / 16; i += kAttThreads) {
+          const i32x4 w = *reinterpret_cast<const i32x4*>(values + i * 16);
+          bad = bad || not_finite<T>(w[0]) || not_finite<T>(w[1]) || not_finite<T>(w[2]) || not_finite<T>(w[3]);
+        }
+        if (bad) odd = 1;
+      }
     }
     if (k0 > wave_last) continue;
-    f32x16 st[S::kGroups];
+    f32x4 st[2][2 * S::kGroups];
 #pragma unroll
-    for (int t = 0; t < S::kGroups; ++t)
+    for (int i = 0; i < 2; ++i)
 #pragma unroll
-      for (int r = 0; r < 16; ++r) st[t][r] = 0.f;
+      for (int t = 0; t < 2 * S::kGroups; ++t) st[i][t] = f32x4{0.f, 0.f, 0.f, 0.f};
 #pragma unroll
     for (int s = 0; s < S::kSteps; ++s)
 #pragma unroll
-      for (int t = 0; t < S::kGroups; ++t)
-        st[t] = Attn<T>::mma32(*reinterpret_cast<const vec8*>(buffer + k_at[s & 3] + (s >> 2) * 128 + t * 32 * S::kRow), q[s], st[t]);
-    if (k0 + S::kKeys - 1 > wave_first) {
-      const int mine = limit - k0 - 4 * half;
+      for (int t = 0; t < 2 * S::kGroups; ++t) {
+        const vec8 k = *reinterpret_cast<const vec8*>(buffer + k_at[s % S::kKeyBases] + s / S::kKeyBases * (S::kKeyBases * 64) + t * 16 * S::kRow);
 #pragma unroll
-      for (int t = 0; t < S::kGroups; ++t)
-#pragma unroll
-        for (int r = 0; r < 16; ++r)
-          if (t * 32 + 8 * (r / 4) + r % 4 > mine) st[t][r] = -INFINITY;
-    }
-    float high = st[0][0];
-#pragma unroll
-    for (int t = 0; t < S::kGroups; ++t)
-#pragma unroll
-      for (int r = 0; r < 16; ++r) high = fmaxf(high, st[t][r]);
-    if (__any(high > top + lag)) {
-      high = max_over_32(high);
-      const float now = fmaxf(top, high), by = top == -INFINITY ? 0.f : exp2_of((top - now) * scale);
-      sum *= by;
-#pragma unroll
-      for (int t = 0; t < S::kTiles; ++t)
-#pragma unroll
-        for (int r = 0; r < 16; ++r) o[t][r] *= by;
-      top = now;
-    }
-    const float from = top == -INFINITY ? 0.f : top * scale;
-    vec8 p[2 * S::kGroups];  // 16 keys each, to 8 or 11 bits: the second product's operand
-#pragma unroll
-    for (int t = 0; t < S::kGroups; ++t)
-#pragma unroll
-      for (int r = 0; r < 16; ++r) {
-        const float e = exp2_of(__builtin_fmaf(st[t][r], scale, -from));
-        sum += e;
-        p[t * 2 + r / 8][r % 8] = static_cast<T>(e);
+        for (int i = 0; i < 2; ++i) st[i][t] = Attn<T>::mma16(k, q[i][s], st[i][t]);
       }
+    if (k0 + S::kKeys - 1 > wave_first) {
 #pragma unroll
-    for (int s = 0; s < 2 * S::kGroups; ++s)
+      for (int i = 0; i < 2; ++i) {
+        const int mine = limit[i] - k0 - 4 * quarter;
+#pragma unroll
+        for (int t = 0; t < 2 * S::kGroups; ++t)
+#pragma unroll
+          for (int r = 0; r < 4; ++r)
+            if (t * 16 + r > mine) st[i][t][r] = -INFINITY;
+      }
+    }
+    float high[2];
+#pragma unroll
+    for (int i = 0; i < 2; ++i) {
+      high[i] = st[i][0][0];
+#pragma unroll
+      for (int t = 0; t < 2 * S::kGroups; ++t)
+#pragma unroll
+        for (int r = 0; r < 4; ++r) high[i] = fmaxf(high[i], st[i][t][r]);
+    }
+    if (__any(high[0] > top[0] + lag || high[1] > top[1] + lag)) {
+#pragma unroll
+      for (int i = 0; i < 2; ++i) {
+        const float now = fmaxf(top[i], max_over_32(max_over_16(high[i]))), by = top[i] == -INFINITY ? 0.f : exp2_of((top[i] - now) * scale);
+        sum[i] *= by;
+#pragma unroll
+        for (int t = 0; t < S::kTiles; ++t) o[i][t] *= by;
+        top[i] = now;
+      }
+    }
+    vec8 p[2][S::kGroups];  // 32 keys each, to 8 or 11 bits: the second product's operand
+#pragma unroll
+    for (int i = 0; i < 2; ++i) {
+      const float from = top[i] == -INFINITY ? 0.f : top[i] * scale;
+#pragma unroll
+      for (int t = 0; t < 2 * S::kGroups; ++t)
+#pragma unroll
+        for (int r = 0; r < 4; ++r) {
+          const float e = exp2_of(__builtin_fmaf(st[i][t][r], scale, -from));
+          sum[i] += e;
+          p[i][t / 2][t % 2 * 4 + r] = static_cast<T>(e);
+        }
+    }
+#pragma unroll
+    for (int s = 0; s < S::kGroups; ++s)
 #pragma unroll
       for (int t = 0; t < S::kTiles; ++t) {
-        const char* const at = buffer + v_at[t % S::kValueBases] + t / S::kValueBases * (S::kValueBases * 64) + s * 16 * S::kRow;
-        const vec8 v = join8(read_transposed<T>(reinterpret_cast<const T*>(at)), read_transposed<T>(reinterpret_cast<const T*>(at + 8 * S::kRow)));
-        o[t] = Attn<T>::mma32(v, p[s], o[t]);
+        const char* const at = buffer + v_at[t % S::kValueBases] + t / S::kValueBases * (S::kValueBases * 32) + s * 32 * S::kRow;
+        const vec8 v = join8(read_transposed<T>(reinterpret_cast<const T*>(at)), read_transposed<T>(reinterpret_cast<const T*>(at + 16 * S::kRow)));
+#pragma unroll
+        for (int i = 0; i < 2; ++i) o[i][t] = Attn<T>::mma16(v, p[i][s], o[i][t]);
       }
   }
 
@@ -363,32 +414,34 @@ __global__ __launch_bounds__(kAttThreads, 2) void attention_kernel(fr_attention_
     attention_rows<T, DP>(a, kc, vc, wave_row0, rows, at, kv, share, part, first * S::kKeys, blocks * S::kKeys < m ? blocks * S::kKeys : m);
     return;
   }
-  sum = sum_over_32(sum);
-  if (parts > 1) {
-    if (live) {
-      const AttPart<DP> to(a, part, q_begin + token, head);
 #pragma unroll
-      for (int t = 0; t < S::kTiles; ++t)
+  for (int i = 0; i < 2; ++i) {
+    const float all = sum_over_32(sum_over_16(sum[i]));
+    if (parts > 1) {
+      if (live[i]) {
+        const AttPart<DP> to(a, part, q_begin + token[i], head[i]);
 #pragma unroll
-        for (int r = 0; r < 4; ++r)
-          *reinterpret_cast<f32x4*>(to.rows + t * 32 + r * 8 + half * 4) = f32x4{o[t][r * 4], o[t][r * 4 + 1], o[t][r * 4 + 2], o[t][r * 4 + 3]};
-      if (half == 0) to.tops[0] = top * scale, to.sums[0] = sum;
-    }
-    return;
-  }
-  const float by = sum == 0.f ? 0.f : 1.f / sum;  // a row that sees no key: zeros
-  if (live) {
-    T* const to = reinterpret_cast<T*>(a.out) + (q_begin + token) * a.out_row + head * a.out_head + half * 4;
-#pragma unroll
-    for (int t = 0; t < S::kTiles; ++t)
-#pragma unroll
-      for (int r = 0; r < 4; ++r) {
-        const int d = t * 32 + r * 8;
-        vec4 y;
-#pragma unroll
-        for (int e = 0; e < 4; ++e) y[e] = static_cast<T>(o[t][r * 4 + e] * by);
-        if (d < dim) *reinterpret_cast<vec4*>(to + d) = y;
+        for (int t = 0; t < S::kTiles; ++t) *reinterpret_cast<f32x4*>(to.rows + t * 16 + quarter * 4) = o[i][t];
+        if (quarter == 0) to.tops[0] = top[i] * scale, to.sums[0] = all;
       }
+      continue;
+    }
+    const float by = all == 0.f ? 0.f : 1.f / all;  // a row that sees no key: zeros
+    T* const to = reinterpret_cast<T*>(a.out) + (q_begin + token[i]) * a.out_row + head[i] * a.out_head + (quarter & 1) * 16 + (quarter >> 1) * 8;
+#pragma unroll
+    for (int t = 0; t < S::kTiles; t += 2) {
+      // four dimensions of two tiles to eight of one: lanes of odd quarters exchange with those of even ones
+      typedef unsigned u32x2 __attribute__((ext_vector_type(2)));
+      vec4 y[2];
+#pragma unroll
+      for (int j = 0; j < 2; ++j)
+#pragma unroll
+        for (int e = 0; e < 4; ++e) y[j][e] = static_cast<T>(o[i][t + j][e] * by);
+      const u32x2 lo = __builtin_bit_cast(u32x2, y[0]), hi = __builtin_bit_cast(u32x2, y[1]);
+      const auto w0 = __builtin_amdgcn_permlane16_swap(lo[0], hi[0], false, false), w1 = __builtin_amdgcn_permlane16_swap(lo[1], hi[1], false, false);
+      const int d = t * 16 + (quarter & 1) * 16 + (quarter >> 1) * 8;
+      if (live[i] && d < dim) *reinterpret_cast<u32x4_t*>(to + t * 16) = u32x4_t{w0[0], w1[0], w0[1], w1[1]};
+    }
   }
 #endif
 }
@@ -461,8 +514,8 @@ int check_attention_sizes(int64_t B, int64_t rows, int64_t keys, int64_t heads, 
   FR_REQUIRE(dim >= 8 && dim <= 256 && dim % 8 == 0, FR_E_SHAPE, "fr_attention: head size %lld: a multiple of 8 up to 256", (long long)dim);
   FR_REQUIRE(rows >= 0 && rows < (int64_t(1) << 30) && keys >= 0 && keys < (int64_t(1) << 30), FR_E_SHAPE, "fr_attention: %lld rows, %lld keys: below 2^30",
              (long long)rows, (long long)keys);
-  FR_REQUIRE(B >= 0 && B <= (1 << 20) && (rows + B * kAttTile) * heads < (int64_t(1) << 37), FR_E_SHAPE, "fr_attention: %lld sequences, %lld rows of %lld heads",
-             (long long)B, (long long)rows, (long long)heads);
+  FR_REQUIRE(B >= 0 && B <= (1 << 20) && (rows + B + kAttTile) * heads < (int64_t(1) << 31), FR_E_SHAPE,
+             "fr_attention: %lld sequences, %lld rows of %lld heads: rows times heads below 2^31", (long long)B, (long long)rows, (long long)heads);
   return FR_OK;
 }
 
