@@ -314,7 +314,10 @@ __global__ __launch_bounds__(kAttThreads, 2) void attention_kernel(fr_attention_
   for (int i = 0; i < 2; ++i)
 #pragma unroll
     for (int t = 0; t < S::kTiles; ++t) o[i][t] = f32x4{0.f, 0.f, 0.f, 0.f};
-  float top[2] = {-INFINITY, -INFINITY}, sum[2] = {0.f, 0.f};  // unscaled, in all four lanes of a row, lagging; the sum of the lane's own keys
+  float top[2] = {-INFINITY, -INFINITY};  // unscaled, in all four lanes of a row, lagging
+  f32x4 sum[2] = {f32x4{0.f, 0.f, 0.f, 0.f}, f32x4{0.f, 0.f, 0.f, 0.f}};
+  const T one = static_cast<T>(1.f);
+  const vec8 ones = {one, one, one, one, one, one, one, one};
 
   for (int block = first; block < blocks; ++block) {
     const int k0 = block * S::kKeys;
@@ -342,6 +345,7 @@ __global__ __launch_bounds__(kAttThreads, 2) void attention_kernel(fr_attention_
       }
     }
     if (k0 > wave_last) continue;
+    __builtin_amdgcn_s_setprio(1);  // in front of the other workgroup's exponentials: 0.5 %
     f32x4 st[2][2 * S::kGroups];
 #pragma unroll
     for (int i = 0; i < 2; ++i)
@@ -355,6 +359,7 @@ __global__ __launch_bounds__(kAttThreads, 2) void attention_kernel(fr_attention_
 #pragma unroll
         for (int i = 0; i < 2; ++i) st[i][t] = Attn<T>::mma16(k, q[i][s], st[i][t]);
       }
+    __builtin_amdgcn_s_setprio(0);
     if (k0 + S::kKeys - 1 > wave_first) {
 #pragma unroll
       for (int i = 0; i < 2; ++i) {
@@ -394,12 +399,14 @@ __global__ __launch_bounds__(kAttThreads, 2) void attention_kernel(fr_attention_
 #pragma unroll
         for (int r = 0; r < 4; ++r) {
           const float e = exp2_of(__builtin_fmaf(st[i][t][r], scale, -from));
-          sum[i] += e;
           p[i][t / 2][t % 2 * 4 + r] = static_cast<T>(e);
         }
     }
 #pragma unroll
-    for (int s = 0; s < S::kGroups; ++s)
+    for (int s = 0; s < S::kGroups; ++s) {
+      // the terms' sum, as they are rounded, in every register of a row's lanes: on the matrix unit, which has the time the vector unit has not
+#pragma unroll
+      for (int i = 0; i < 2; ++i) sum[i] = Attn<T>::mma16(ones, p[i][s], sum[i]);
 #pragma unroll
       for (int t = 0; t < S::kTiles; ++t) {
         const char* const at = buffer + v_at[t % S::kValueBases] + t / S::kValueBases * (S::kValueBases * 32) + s * 32 * S::kRow;
@@ -407,6 +414,7 @@ __global__ __launch_bounds__(kAttThreads, 2) void attention_kernel(fr_attention_
 #pragma unroll
         for (int i = 0; i < 2; ++i) o[i][t] = Attn<T>::mma16(v, p[i][s], o[i][t]);
       }
+    }
   }
 
   __syncthreads();
@@ -416,7 +424,7 @@ __global__ __launch_bounds__(kAttThreads, 2) void attention_kernel(fr_attention_
   }
 #pragma unroll
   for (int i = 0; i < 2; ++i) {
-    const float all = sum_over_32(sum_over_16(sum[i]));
+    const float all = sum[i][0];
     if (parts > 1) {
       if (live[i]) {
         const AttPart<DP> to(a, part, q_begin + token[i], head[i]);
