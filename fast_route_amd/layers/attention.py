@@ -13,7 +13,7 @@ from .. import _native as N
 
 _FLOATS = (torch.float16, torch.bfloat16)
 _PACKED = struct.Struct("@26qd")  # fr_attention_args
-_PAGED = struct.Struct("@29qd")  # fr_paged_args
+_PAGED = struct.Struct("@30qd")  # fr_paged_args
 
 
 def _workspace(buf: torch.Tensor | None, nbytes: int, device) -> torch.Tensor | None:
@@ -110,7 +110,7 @@ def paged_attention(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tenso
     args = _PAGED.pack(q.data_ptr(), k_cache.data_ptr(), v_cache.data_ptr(), block_table.data_ptr(), seq_lens.data_ptr(), out.data_ptr(),
                        0 if ws is None else ws.data_ptr(), 0 if ws is None else ws.numel(), B, heads, kv_heads, dim, pages, page_size, table_pages,
                        block_table.stride(0), q.stride(0), q.stride(1), out.stride(0), out.stride(1), kp, ks, kh, vp, vs, vh,
-                       N.dtype_code(dtype), 0, 0, float(dim ** -0.5 if scale is None else scale))
+                       N.dtype_code(dtype), 0, 0, 0, float(dim ** -0.5 if scale is None else scale))
     with N.on(dev):
         N.check(lib.fr_paged_attention(args, N.stream_ptr(dev)))
     return out

@@ -413,15 +413,15 @@ int fr_attention(const fr_attention_args* args, void* stream);
  * sequence b in place j % page_size of page table[b, j / page_size].  lengths int32 [B], table int32 [B, table_pages] (row stride table_row).
  * A length is taken as 0 below it and as the table's end behind it; keys in a page outside [0, pages) take no part; a row without keys is
  * zeros.  Pages behind a length are not looked at.  heads a multiple of kv_heads; dim a multiple of 8 up to 256; q, out, k_cache, v_cache 16-byte
- * aligned with strides of multiples of 8 elements; any page_size, multiples of 16 are the fast case; table_pages * page_size <= 2^30; scale in [1e-20, 1e20].
+ * aligned with strides of multiples of 8 elements; any page_size, multiples of 16 are the fast case; table_pages * page_size <= 2^30, B times that below 2^36; scale in [1e-20, 1e20].
  * `workspace`: 16-byte aligned, fr_paged_attention_workspace_bytes(.., most = table_pages * page_size) bytes (0: none is needed; -1: sizes outside the
- * limits); two calls that may overlap in time need one each.  `slots` and `page_shift` are the call's own. */
+ * limits); two calls that may overlap in time need one each.  `slots`, `least` and `page_shift` are the call's own. */
 typedef struct fr_paged_args {
   const void *q, *k_cache, *v_cache, *table, *lengths;
   void *out, *workspace;
   int64_t workspace_bytes, B, heads, kv_heads, dim, pages, page_size, table_pages, table_row;
   int64_t q_row, q_head, out_row, out_head, k_cache_page, k_cache_slot, k_cache_head, v_cache_page, v_cache_slot, v_cache_head;
-  int64_t dtype, slots, page_shift;
+  int64_t dtype, slots, least, page_shift;
   double scale;
 } fr_paged_args;
 int64_t fr_paged_attention_workspace_bytes(int64_t B, int64_t heads, int64_t kv_heads, int64_t dim, int64_t most);
