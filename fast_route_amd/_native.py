@@ -139,3 +139,22 @@ _HERE = contextlib.nullcontext()
 def on(device: torch.device):
     """The device of a call's tensors as the current one, where it is another."""
     return _HERE if device.index == torch.cuda.current_device() else torch.cuda.device(device)
+
+
+def run(index: int, fn, *args) -> None:
+    """fn(*args, stream) on the current stream of device `index`, which is made the current device where another is."""
+    if index == torch._C._cuda_getDevice():
+        check(fn(*args, torch._C._cuda_getCurrentRawStream(index)))
+    else:
+        with torch.cuda.device(index):
+            check(fn(*args, torch._C._cuda_getCurrentRawStream(index)))
+
+
+def device_of(*tensors) -> int:
+    """Index of the device that all of them are on.  (An index instead of device objects: 5 us of a call with eight tensors.)"""
+    index = tensors[0].get_device()
+    assert index >= 0, "fast_route_amd operators need tensors on an MI355X device (no CPU path)"
+    for t in tensors:
+        assert t.get_device() == index, "operands on different devices" if t.is_cuda else \
+            "fast_route_amd operators need tensors on an MI355X device (no CPU path)"
+    return index

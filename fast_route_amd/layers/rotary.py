@@ -56,57 +56,56 @@ def prepare_rotary(frequencies: torch.Tensor, interleaved: bool = False, factor:
     return Rotary(turns.to(device), bool(interleaved), float(factor))
 
 
-def _check_heads(x: torch.Tensor, what: str) -> None:
-    assert x.dim() == 3 and x.dtype in _FLOATS, "%s must be [tokens, heads, head size] in float16 or bfloat16" % what
-    assert x.shape[2] == 1 or x.stride(2) == 1, "%s must be contiguous along a head" % what
+def _heads(x: torch.Tensor, what: str):
+    """Shape and strides of [tokens, heads, head size]."""
+    shape, strides = x.shape, x.stride()
+    assert len(shape) == 3 and (strides[2] == 1 or shape[2] == 1), "%s must be [tokens, heads, head size], contiguous along a head" % what
+    return shape, strides
 
 
-def _check_cache(cache: torch.Tensor, like: torch.Tensor, what: str) -> None:
-    assert cache.dim() == 4 and cache.dtype == like.dtype and cache.device == like.device, \
-        "%s must be [pages, page size, heads, head size], in the keys' type and on their device" % what
-    assert cache.shape[2:] == like.shape[1:], "%s: other heads than the keys" % what
-    assert cache.shape[3] == 1 or cache.stride(3) == 1, "%s must be contiguous along a head" % what
-    assert 0 not in cache.stride(), "%s: places that share memory" % what
+def _cache(cache: torch.Tensor, dtype: torch.dtype, heads: int, dim: int, what: str):
+    shape, strides = cache.shape, cache.stride()
+    assert len(shape) == 4 and cache.dtype == dtype, "%s must be [pages, page size, heads, head size] in the keys' type" % what
+    assert shape[2] == heads and shape[3] == dim, "%s: other heads than the keys" % what
+    assert strides[3] == 1 or dim == 1, "%s must be contiguous along a head" % what
+    assert 0 not in strides, "%s: places that share memory" % what
+    return shape, strides
 
 
 def _call(q, k, positions, rotary: Rotary, inplace: bool, cached=None):
-    N.require_cuda(q, k, positions)
-    _check_heads(q, "q")
-    _check_heads(k, "k")
-    T, heads, dim = q.shape
-    kv_heads, dev, turned = k.shape[1], q.device, 2 * rotary.turns.numel()
-    assert k.shape == (T, kv_heads, dim) and k.dtype == q.dtype, "q and k differ in tokens, head size or type"
+    turns, interleaved, factor = rotary
+    ((T, heads, dim), q_strides), (k_shape, k_strides), dtype = _heads(q, "q"), _heads(k, "k"), q.dtype
+    kv_heads, turned, at_type = k_shape[1], 2 * turns.shape[0], positions.dtype
+    assert dtype in _FLOATS, "q must be float16 or bfloat16"
+    assert k_shape[0] == T and k_shape[2] == dim and k.dtype == dtype, "q and k differ in tokens, head size or type"
     assert turned <= dim, "more dimensions are turned than a head has"
-    assert positions.shape == (T,) and positions.dtype in _INTS and positions.is_contiguous(), "positions must be contiguous int32 or int64 [tokens]"
-    assert k.device == dev and positions.device == dev and rotary.turns.device == dev, "operands on different devices"
-    v_ptr = kc_ptr = vc_ptr = slots_ptr = pages = slots_i64 = v_token = v_head = 0
-    page_size, cache_strides = 1, (0, 0, 0, 0, 0, 0)
-    if cached is not None:
-        v, k_cache, v_cache, slots = cached
-        _check_heads(v, "v")
-        assert v.shape == k.shape and v.dtype == k.dtype and v.device == dev, "v must be like k"
-        _check_cache(k_cache, k, "k_cache")
-        _check_cache(v_cache, k, "v_cache")
-        assert k_cache.shape == v_cache.shape, "k_cache and v_cache differ in shape"
-        assert slots.shape == (T,) and slots.dtype in _INTS and slots.is_contiguous() and slots.device == dev, \
-            "slots must be contiguous int32 or int64 [tokens]"
-        v_ptr, kc_ptr, vc_ptr, slots_ptr = v.data_ptr(), k_cache.data_ptr(), v_cache.data_ptr(), slots.data_ptr()
-        (v_token, v_head, _), (pages, page_size, _, _) = v.stride(), k_cache.shape
-        cache_strides = k_cache.stride()[:3] + v_cache.stride()[:3]
-        slots_i64 = int(slots.dtype == torch.int64)
-    if inplace:
-        assert 0 not in q.stride() and 0 not in k.stride(), "inplace: rows that share memory"
-        q_out, k_out = q, k
+    assert positions.shape == (T,) and at_type in _INTS and positions.is_contiguous(), "positions must be contiguous int32 or int64 [tokens]"
+    if cached is None:
+        dev = N.device_of(q, k, positions, turns)
+        v_ptr = kc_ptr = vc_ptr = slots_ptr = pages = slots_i64 = v_token = v_head = 0
+        page_size, cache_strides = 1, (0, 0, 0, 0, 0, 0)
     else:
-        q_out, k_out = (torch.empty((T, h, dim), dtype=q.dtype, device=dev) for h in (heads, kv_heads))
+        v, k_cache, v_cache, slots = cached
+        dev, slot_type = N.device_of(q, k, positions, turns, v, k_cache, v_cache, slots), slots.dtype
+        v_shape, (v_token, v_head, _) = _heads(v, "v")
+        assert v_shape == k_shape and v.dtype == dtype, "v must be like k"
+        (shape, kc), (v_cache_shape, vc) = _cache(k_cache, dtype, kv_heads, dim, "k_cache"), _cache(v_cache, dtype, kv_heads, dim, "v_cache")
+        assert shape == v_cache_shape, "k_cache and v_cache differ in shape"
+        assert slots.shape == (T,) and slot_type in _INTS and slots.is_contiguous(), "slots must be contiguous int32 or int64 [tokens]"
+        v_ptr, kc_ptr, vc_ptr, slots_ptr = v.data_ptr(), k_cache.data_ptr(), v_cache.data_ptr(), slots.data_ptr()
+        pages, page_size, cache_strides, slots_i64 = shape[0], shape[1], kc[:3] + vc[:3], int(slot_type == torch.int64)
+    if inplace:
+        assert 0 not in q_strides and 0 not in k_strides, "inplace: rows that share memory"
+        q_out, k_out, out_strides = q, k, q_strides[:2] + k_strides[:2]
+    else:
+        q_out, k_out = q.new_empty((T, heads, dim)), k.new_empty(k_shape)
+        out_strides = (heads * dim, dim, kv_heads * dim, dim)
     if T == 0:
         return q_out, k_out
     args = _ARGS.pack(q.data_ptr(), k.data_ptr(), v_ptr, q_out.data_ptr(), k_out.data_ptr(), kc_ptr, vc_ptr, positions.data_ptr(), slots_ptr,
-                      rotary.turns.data_ptr(), T, heads, kv_heads, dim, turned, pages, page_size, *q.stride()[:2], *k.stride()[:2], v_token, v_head,
-                      *q_out.stride()[:2], *k_out.stride()[:2], *cache_strides, N.dtype_code(q.dtype), int(rotary.interleaved),
-                      int(positions.dtype == torch.int64), slots_i64, rotary.factor)
-    with N.on(dev):
-        N.check(N.lib().fr_rotary(args, N.stream_ptr(dev)))
+                      turns.data_ptr(), T, heads, kv_heads, dim, turned, pages, page_size, q_strides[0], q_strides[1], k_strides[0], k_strides[1],
+                      v_token, v_head, *out_strides, *cache_strides, N.dtype_code(dtype), interleaved, at_type == torch.int64, slots_i64, factor)
+    N.run(dev, N.lib().fr_rotary, args)
     return q_out, k_out
 
 

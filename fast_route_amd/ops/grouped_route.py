@@ -7,7 +7,7 @@ import torch
 from .. import _native as N
 
 _SCORES = {"softmax": 0, "sigmoid": 1}
-_LOGITS = (torch.float32, torch.bfloat16, torch.float16)
+_DTYPES = {t: N.dtype_code(t) for t in (torch.float32, torch.bfloat16, torch.float16)}
 
 
 def grouped_topk(gating_output: torch.Tensor, topk: int, num_groups: int = 1, topk_groups: int = 1, scoring: str = "softmax",
@@ -23,22 +23,20 @@ def grouped_topk(gating_output: torch.Tensor, topk: int, num_groups: int = 1, to
 
     With a bias, scores and choices are computed in 64 bits: the order of two experts does not depend on a rounding.  A NaN counts
     as -infinity.  Limits: E <= 1024, num_groups <= 64, topk <= 64."""
-    N.require_cuda(gating_output)
-    assert gating_output.dim() == 2 and gating_output.dtype in _LOGITS, "gating_output must be [M, E] in float16, bfloat16 or float32"
-    M, E = gating_output.shape
-    assert E == 1 or gating_output.stride(1) == 1, "router logits must be contiguous along experts"
+    shape, strides, dtype = gating_output.shape, gating_output.stride(), gating_output.dtype
+    assert len(shape) == 2 and dtype in _DTYPES, "gating_output must be [M, E] in float16, bfloat16 or float32"
+    M, E = shape
+    assert E == 1 or strides[1] == 1, "router logits must be contiguous along experts"
     assert scoring in _SCORES, "scoring must be 'softmax' or 'sigmoid'"
-    dev, bias_ptr = gating_output.device, 0
-    if bias is not None:
-        assert bias.device == dev, "bias and gating_output on different devices"
+    if bias is None:
+        dev, bias_ptr = N.device_of(gating_output), 0
+    else:
+        dev, bias_ptr = N.device_of(gating_output, bias), bias.data_ptr()
         assert bias.dtype == torch.float32 and bias.shape == (E,) and bias.is_contiguous(), "bias must be contiguous float32 [E]"
-        bias_ptr = bias.data_ptr()
     topk = int(topk)
     assert 1 <= topk <= 64, "topk outside [1, 64]"
-    topk_weights = torch.empty((M, topk), dtype=torch.float32, device=dev)
-    topk_ids = torch.empty((M, topk), dtype=torch.int32, device=dev)
-    with N.on(dev):
-        N.check(N.lib().fr_gating_grouped(gating_output.data_ptr(), N.dtype_code(gating_output.dtype), M, E, gating_output.stride(0) if M > 1 else E,
-                                          bias_ptr, int(num_groups), int(topk_groups), topk, _SCORES[scoring], int(bool(renormalize)),
-                                          float(scale), topk_weights.data_ptr(), topk_ids.data_ptr(), N.stream_ptr(dev)))
+    topk_weights = gating_output.new_empty((M, topk), dtype=torch.float32)
+    topk_ids = gating_output.new_empty((M, topk), dtype=torch.int32)
+    N.run(dev, N.lib().fr_gating_grouped, gating_output.data_ptr(), _DTYPES[dtype], M, E, strides[0] if M > 1 else E, bias_ptr, int(num_groups),
+          int(topk_groups), topk, _SCORES[scoring], bool(renormalize), float(scale), topk_weights.data_ptr(), topk_ids.data_ptr())
     return topk_weights, topk_ids
