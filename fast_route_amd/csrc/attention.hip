@@ -454,29 +454,17 @@ __global__ __launch_bounds__(kAttThreads, 2) void attention_kernel(fr_attention_
 #endif
 }
 
-// Joins the parts of the keys: four dimensions of a row's head to a thread.
 template <typename T, int DP>
-__global__ __launch_bounds__(kAttThreads) void attention_join_kernel(fr_attention_args a) {
-  constexpr int kLanes = DP / 4;
-  const int64_t i = static_cast<int64_t>(blockIdx.x) * kAttThreads + threadIdx.x, at = i / kLanes, row = at / a.heads;
-  const int d = static_cast<int>(i % kLanes) * 4, head = static_cast<int>(at - row * a.heads), parts = static_cast<int>(a.parts);
+__global__ __launch_bounds__(kAttThreads) void attention_join_kernel(fr_attention_args a, int wide) {
+  typedef JoinShape<DP> J;
+  const int64_t all = a.rows * a.heads, at = wide ? blockIdx.x : static_cast<int64_t>(blockIdx.x) * J::kGroups + threadIdx.x / J::kLanes;
+  const int64_t row = (at < all ? at : all - 1) / a.heads, head = (at < all ? at : all - 1) - row * a.heads;
   const int32_t* const cu = reinterpret_cast<const int32_t*>(a.cu_q);
-  if (row >= (a.fill ? a.rows : att_clamp(cu[a.B], 0, a.rows)) || row < cu[0] || d >= a.dim) return;  // of no sequence
-  const int64_t all = a.rows * a.heads;
-  const AttPart<DP> from(a, 0, row, head);
-  float top = -INFINITY, sum = 0.f;
-  for (int p = 0; p < parts; ++p) top = fmaxf(top, from.tops[p * all]);
-  f32x4 x = {0.f, 0.f, 0.f, 0.f};
-#pragma unroll 4
-  for (int p = 0; p < parts; ++p) {
-    const float mine = from.tops[p * all], by = mine == -INFINITY ? 0.f : exp2_of(mine - top);
-    sum += by * from.sums[p * all];
-    x += *reinterpret_cast<const f32x4*>(from.rows + p * all * DP + d) * by;
-  }
-  typename Attn<T>::vec4 y;
-#pragma unroll
-  for (int e = 0; e < 4; ++e) y[e] = static_cast<T>(sum == 0.f ? 0.f : x[e] / sum);
-  *reinterpret_cast<typename Attn<T>::vec4*>(reinterpret_cast<T*>(a.out) + row * a.out_row + head * a.out_head + d) = y;
+  const bool live = at < all && row < (a.fill ? a.rows : att_clamp(cu[a.B], 0, a.rows)) && row >= cu[0];  // of a sequence
+  if (wide && !live) return;
+  const AttPart<DP> from(a, 0, row, static_cast<int>(head));
+  join_parts<T, DP>(wide, live, static_cast<int>(a.parts), from.rows, all * DP, from.tops, from.sums, all,
+                    reinterpret_cast<T*>(a.out) + row * a.out_row + head * a.out_head, static_cast<int>(a.dim));
 }
 
 int att_dim(int64_t dim) { return dim <= 64 ? 64 : dim <= 128 ? 128 : dim <= 192 ? 192 : 256; }
@@ -502,7 +490,10 @@ int launch_attention(const fr_attention_args& a, hipStream_t st) {
   hipLaunchKernelGGL((attention_kernel<T, DP>), dim3(static_cast<unsigned>(tiles * a.parts * a.kv_heads)), dim3(kAttThreads), 0, st, a);
   const int rc = check_launch("attention_kernel");
   if (rc != FR_OK || a.parts == 1) return rc;
-  hipLaunchKernelGGL((attention_join_kernel<T, DP>), dim3(static_cast<unsigned>(ceil_div(a.rows * a.heads * (DP / 4), kAttThreads))), dim3(kAttThreads), 0, st, a);
+  typedef JoinShape<DP> J;
+  static_assert(J::kThreads == kAttThreads, "join_parts' workgroups");
+  const bool wide = a.rows * a.heads <= 4096;
+  hipLaunchKernelGGL((attention_join_kernel<T, DP>), dim3(static_cast<unsigned>(J::blocks(a.rows * a.heads, wide))), dim3(kAttThreads), 0, st, a, wide);
   return check_launch("attention_join_kernel");
 }
 

@@ -69,5 +69,61 @@ constexpr float kLog2e = 1.4426950408889634f;
 // inside fp16, and keep their relative precision; the sums are fp32.
 constexpr float kLag = 8.f;
 
+// Joins the parts of a head's keys: rows of DP sums, the softmax's maxima (in units of a factor 2) and sums, each `pitch` floats from part to part.  The
+// workgroup's 256 threads are groups of DP / 4, four dimensions to a thread.  Not wide: a head to a group.  wide: one head for all groups, which share its
+// parts - for few heads, where a part after the other is a round trip to memory each (one row of 32 heads, 31 parts: 21 -> 5 us).
+template <int DP>
+struct JoinShape {
+  static constexpr int kThreads = 256, kLanes = DP / 4, kGroups = kThreads / kLanes;
+  static int64_t blocks(int64_t heads, bool wide) { return wide ? heads : (heads + kGroups - 1) / kGroups; }
+};
+template <typename T, int DP>
+__device__ __forceinline__ void join_parts(bool wide, bool live, int parts, const float* rows, int64_t row_pitch, const float* tops, const float* sums,
+                                           int64_t pitch, T* out, int dim) {
+  typedef JoinShape<DP> S;
+  __shared__ float joined[S::kGroups][DP];
+  __shared__ float weight_of[S::kGroups];
+  const int group = threadIdx.x / S::kLanes, d = threadIdx.x % S::kLanes * 4;
+  live = live && group < S::kGroups;
+  float top = -INFINITY, weight = 0.f;
+  if (wide) {
+    for (int p = threadIdx.x & 63; p < parts; p += kWave) top = fmaxf(top, tops[p * pitch]);
+#pragma unroll
+    for (int s = 1; s < kWave; s <<= 1) top = fmaxf(top, __shfl_xor(top, s, kWave));
+  } else if (live) {
+#pragma unroll 8
+    for (int p = 0; p < parts; ++p) top = fmaxf(top, tops[p * pitch]);
+  }
+  f32x4 x = {0.f, 0.f, 0.f, 0.f};
+  if (live) {
+#pragma unroll 8
+    for (int p = wide ? group : 0; p < parts; p += wide ? S::kGroups : 1) {
+      const float t = tops[p * pitch], by = t == -INFINITY ? 0.f : exp2_of(t - top);
+      weight += by * sums[p * pitch];
+      x += *reinterpret_cast<const f32x4*>(rows + p * row_pitch + d) * by;
+    }
+  }
+  if (!wide) {
+    if (live && d < dim) {
+      typename Attn<T>::vec4 y;
+#pragma unroll
+      for (int e = 0; e < 4; ++e) y[e] = static_cast<T>(weight == 0.f ? 0.f : x[e] / weight);
+      *reinterpret_cast<typename Attn<T>::vec4*>(out + d) = y;
+    }
+    return;
+  }
+  if (live) {
+    *reinterpret_cast<f32x4*>(&joined[group][d]) = x;
+    if (d == 0) weight_of[group] = weight;
+  }
+  __syncthreads();
+  for (int i = threadIdx.x; i < dim; i += S::kThreads) {
+    float sum = 0.f, total = 0.f;
+#pragma unroll
+    for (int r = 0; r < S::kGroups; ++r) sum += joined[r][i], total += weight_of[r];
+    out[i] = static_cast<T>(total == 0.f ? 0.f : sum / total);  // no key at all: zeros
+  }
+}
+
 }  // namespace
 }  // namespace fr

@@ -359,63 +359,25 @@ __global__ __launch_bounds__(kPagThreads, DP <= 128 ? 2 : 1) void paged_attentio
   }
 }
 
-// Joins the parts of a sequence's heads: DP / 4 threads to a head, four dimensions each; `wide`: a head to a workgroup, whose threads share its parts.
 template <typename T, int DP>
 __global__ __launch_bounds__(kPagThreads) void paged_join_kernel(fr_paged_args a, int unit, int wide) {
-  constexpr int kLanes = DP / 4, kAtOnce = kPagThreads / kLanes;
-  __shared__ float rows[kAtOnce][DP];
-  __shared__ float weight_of[kAtOnce];
-  const int share = static_cast<int>(a.heads / a.kv_heads), tiles = (share + kPagHeads - 1) / kPagHeads, all_heads = static_cast<int>(a.heads);
-  const int groups = (all_heads + kAtOnce - 1) / kAtOnce;  // of heads of a sequence to a workgroup
-  const int seq = wide ? blockIdx.x / all_heads : blockIdx.x / groups;
+  typedef JoinShape<DP> J;
+  const int share = static_cast<int>(a.heads / a.kv_heads), tiles = (share + kPagHeads - 1) / kPagHeads;
+  const int64_t at = wide ? blockIdx.x : static_cast<int64_t>(blockIdx.x) * J::kGroups + threadIdx.x / J::kLanes, all = a.B * a.heads;
+  const int seq = static_cast<int>((at < all ? at : all - 1) / a.heads), head = static_cast<int>((at < all ? at : all - 1) - seq * a.heads);
   const PagPlan plan(a, unit);
-  const int mine = threadIdx.x / kLanes, d = threadIdx.x % kLanes * 4, head = wide ? blockIdx.x % all_heads : blockIdx.x % groups * kAtOnce + mine;
   const int parts = plan.parts(plan.length(seq));
-  if (parts == 1) return;
-  const int64_t pitch = static_cast<int64_t>(a.kv_heads) * tiles * PagShape<DP>::kPart;
   const int kv = head / share, in = head - kv * share;
-  const float* const from = reinterpret_cast<const float*>(a.workspace) + plan.in_front(seq) * pitch + (kv * tiles + in / kPagHeads) * PagShape<DP>::kPart;
-  const float *const tops = from + kPagHeads * DP + in % kPagHeads, *const row = from + in % kPagHeads * DP + d;
-  const bool live = mine < kAtOnce && head < all_heads;
-  float top = -INFINITY, weight = 0.f;
-  if (wide) {
-    for (int p = threadIdx.x & 63; p < parts; p += kWave) top = fmaxf(top, tops[p * pitch]);
-#pragma unroll
-    for (int s = 1; s < kWave; s <<= 1) top = fmaxf(top, __shfl_xor(top, s, kWave));
-  } else if (live) {
-#pragma unroll 4
-    for (int p = 0; p < parts; ++p) top = fmaxf(top, tops[p * pitch]);
-  }
-  f32x4 x = {0.f, 0.f, 0.f, 0.f};
-  if (live) {
-#pragma unroll 8
-    for (int p = wide ? mine : 0; p < parts; p += wide ? kAtOnce : 1) {
-      const float t = tops[p * pitch], by = t == -INFINITY ? 0.f : exp2_of(t - top);
-      weight += by * tops[p * pitch + kPagHeads];
-      x += *reinterpret_cast<const f32x4*>(row + p * pitch) * by;
-    }
-  }
-  T* const to = reinterpret_cast<T*>(a.out) + seq * a.out_row + head * a.out_head;
-  if (!wide) {
-    if (live && d < a.dim) {
-      typename Attn<T>::vec4 y;
-#pragma unroll
-      for (int e = 0; e < 4; ++e) y[e] = static_cast<T>(weight == 0.f ? 0.f : x[e] / weight);
-      *reinterpret_cast<typename Attn<T>::vec4*>(to + d) = y;
-    }
-    return;
-  }
-  if (live) {
-    *reinterpret_cast<f32x4*>(&rows[mine][d]) = x;
-    if (d == 0) weight_of[mine] = weight;
-  }
-  __syncthreads();
-  for (int i = threadIdx.x; i < a.dim; i += kPagThreads) {
-    float sum = 0.f, total = 0.f;
-#pragma unroll
-    for (int r = 0; r < kAtOnce; ++r) sum += rows[r][i], total += weight_of[r];
-    to[i] = static_cast<T>(total == 0.f ? 0.f : sum / total);
-  }
+  const int64_t pitch = static_cast<int64_t>(a.kv_heads) * tiles * PagShape<DP>::kPart;
+  // the places in front of a group's sequence: of the workgroup's first one, and from there on one by one
+  const int first = __builtin_amdgcn_readfirstlane(seq);
+  int slot = plan.in_front(first);
+  for (int b = first; __any(b < seq); ++b) slot += b < seq ? plan.parts(plan.length(b)) : 0;
+  const float* const from = reinterpret_cast<const float*>(a.workspace) + slot * pitch + (kv * tiles + in / kPagHeads) * PagShape<DP>::kPart;
+  const float* const tops = from + kPagHeads * DP + in % kPagHeads;
+  if (wide && parts == 1) return;
+  join_parts<T, DP>(wide, at < all && parts > 1, parts, from + in % kPagHeads * DP, pitch, tops, tops + kPagHeads, pitch,
+                    reinterpret_cast<T*>(a.out) + seq * a.out_row + head * a.out_head, static_cast<int>(a.dim));
 }
 
 int pag_dim(int64_t dim) { return dim <= 64 ? 64 : dim <= 128 ? 128 : dim <= 192 ? 192 : 256; }
@@ -461,9 +423,10 @@ int launch_paged(const fr_paged_args& a, const PagCut& c, hipStream_t st) {
   else hipLaunchKernelGGL((paged_attention_kernel<T, DP, ALIGNED, 4, NT>), grid, block, 0, st, a);
   int rc = check_launch("paged_attention_kernel");
   if (rc != FR_OK || a.slots == a.B) return rc;
-  const int wide = a.B * a.heads <= 1024;
-  const int64_t joins = wide ? a.B * a.heads : a.B * ceil_div(a.heads, kPagThreads / (DP / 4));
-  hipLaunchKernelGGL((paged_join_kernel<T, DP>), dim3(static_cast<unsigned>(joins)), block, 0, st, a, kPagRun * c.shared, wide);
+  typedef JoinShape<DP> J;
+  static_assert(J::kThreads == kPagThreads, "join_parts' workgroups");
+  const bool wide = a.B * a.heads <= 1024;  // (more sequences have few parts each, most often one)
+  hipLaunchKernelGGL((paged_join_kernel<T, DP>), dim3(static_cast<unsigned>(J::blocks(a.B * a.heads, wide))), block, 0, st, a, kPagRun * c.shared, wide);
   return check_launch("paged_join_kernel");
 }
 
