@@ -1,0 +1,6 @@
+// Attention of single tokens over a paged cache, bf16.
+#include "paged_attention_kernel.h"
+
+namespace fr {
+template int paged_attention_run<bf16_t>(const fr_paged_args&, int64_t, int, hipStream_t);
+}  // namespace fr

@@ -1,0 +1,463 @@
+// Attention of one query row per sequence over its pages: every key and value is read once, 4 flops per byte and query head that
+// shares it, so the cache's way from memory bounds it.
+//
+// A wavefront takes the query heads of one key head (up to 16, the columns of a matrix instruction: a "column") and a part of one sequence's keys,
+// in runs of 32 with a running maximum and sum:
+//   S^T [32 keys, 16 heads] = K Q^T: rows of K are the first operand as they lie in memory, straight to registers.
+//   O^T [dim, 16 heads] += V^T P^T: S^T's accumulators hold, per lane, 2 x 4 consecutive keys of one head, which is the second
+//   operand's place for them if V^T's keys are taken in the same order: V goes through LDS (of the wavefront's own, no barrier), where
+//   transposed reads give 4 consecutive keys of a dimension.
+// A run's 16 KB (128 dimensions) are asked for before the run in front is worked on, in registers.  The four wavefronts of a workgroup take the same keys of
+// four columns where there are so many, whose rows lie next to each other in memory (64 rows of up to 16384 keys, 8 key heads: 492 us with a key head to a
+// workgroup, where a cache whose heads come first took 461); with fewer columns they share a part's keys and join their rows in LDS.
+//
+// The keys of all sequences are cut into parts of equal length on the device, since the lengths are there (every wavefront adds them up, the first 256 in its
+// lanes), and the workgroups, as many as the chip holds at a time, take the parts in turn.  Parts of a sequence that has one go to the output,
+// others to fp32 rows with their maxima and sums, which a second launch joins.
+#pragma once
+#include "attention_core.h"
+
+namespace fr {
+namespace {
+
+constexpr int kPagThreads = 256, kPagWaves = 4, kPagRun = 32, kPagHeads = 16;
+constexpr int kPagHeld = 4;  // times 64 lengths stay in the lanes
+
+__device__ __forceinline__ int pag_total(int v) {  // over the wavefront, in every lane
+  v += partner_i32<1>(v);
+  v += partner_i32<2>(v);
+  v += partner_i32<4>(v);
+  v += partner_i32<8>(v);
+  return (__builtin_amdgcn_readlane(v, 0) + __builtin_amdgcn_readlane(v, 16)) + (__builtin_amdgcn_readlane(v, 32) + __builtin_amdgcn_readlane(v, 48));
+}
+__device__ __forceinline__ int pag_up_to(int v) {  // of the lanes up to this one
+  v += __builtin_amdgcn_update_dpp(0, v, 0x111, 0xF, 0xF, true);  // row_shr 1, 2, 4, 8
+  v += __builtin_amdgcn_update_dpp(0, v, 0x112, 0xF, 0xF, true);
+  v += __builtin_amdgcn_update_dpp(0, v, 0x114, 0xF, 0xF, true);
+  v += __builtin_amdgcn_update_dpp(0, v, 0x118, 0xF, 0xF, true);
+  const int lane = threadIdx.x & 63;
+  const int r0 = __builtin_amdgcn_readlane(v, 15), r1 = __builtin_amdgcn_readlane(v, 31), r2 = __builtin_amdgcn_readlane(v, 47);
+  return v + (lane >= 16 ? r0 : 0) + (lane >= 32 ? r1 : 0) + (lane >= 48 ? r2 : 0);
+}
+
+// The parts of all sequences, counted in units of `unit` keys.
+struct PagPlan {
+  const fr_paged_args& a;
+  int lane, count, unit, per;  // units of a part
+  int held[kPagHeld];          // lengths of sequences lane + 64 j
+  __device__ __forceinline__ int length(int b) const {
+    const int64_t cap = a.table_pages * a.page_size;
+    const int n = b < count ? reinterpret_cast<const int32_t*>(a.lengths)[b] : 0;
+    return n < 0 ? 0 : (n > cap ? static_cast<int>(cap) : n);
+  }
+  __device__ __forceinline__ int units(int n) const { return static_cast<int>((static_cast<unsigned>(n) + unit - 1) / unit); }
+  __device__ __forceinline__ int parts(int n) const {
+    const int u = units(n);
+    return u <= per ? 1 : static_cast<int>((static_cast<unsigned>(u) + per - 1) / per);
+  }
+  __device__ __forceinline__ int held_length(int b0) const {  // of sequence b0 + lane, b0 a multiple of 64
+    return b0 == 0 ? held[0] : b0 == kWave ? held[1] : b0 == 2 * kWave ? held[2] : b0 == 3 * kWave ? held[3] : length(b0 + lane);
+  }
+  // With `slots` places a part has as many units as give every sequence its parts: sum over b of max(1, ceil(units / per)) <= total / per + B <= slots; and
+  // `least` units where there are more places than that takes.
+  __device__ __forceinline__ PagPlan(const fr_paged_args& args, int keys) : a(args), lane(threadIdx.x & 63), count(static_cast<int>(args.B)), unit(keys) {
+#pragma unroll
+    for (int j = 0; j < kPagHeld; ++j) held[j] = j == 0 || j * kWave < count ? length(lane + j * kWave) : 0;
+    const int spare = static_cast<int>(a.slots - a.B);
+    per = 0x7fffffff;
+    if (spare <= 0) return;  // a part each
+    int sum = 0;
+#pragma unroll
+    for (int j = 0; j < kPagHeld; ++j) sum += units(held[j]);
+    for (int b = lane + kPagHeld * kWave; b < count; b += kWave) sum += units(length(b));
+    const int total = pag_total(sum), need = static_cast<int>((static_cast<unsigned>(total) + spare - 1) / spare);
+    per = need < static_cast<int>(a.least) ? static_cast<int>(a.least) : need;
+  }
+  // Sequence, part and number of parts of place `slot`; false behind the last one.
+  __device__ __forceinline__ bool place(int slot, int* seq, int* nth, int* of, int* n) const {
+    int before = 0;
+    for (int b0 = 0; b0 < count; b0 += kWave) {
+      const int len = held_length(b0), mine = b0 + lane < count ? parts(len) : 0, sum = before + pag_up_to(mine);
+      const uint64_t hit = __ballot(slot < sum && slot >= sum - mine);
+      if (hit) {
+        const int l = __builtin_amdgcn_readfirstlane(__ffsll(static_cast<unsigned long long>(hit)) - 1);
+        *seq = b0 + l;
+        *of = __builtin_amdgcn_readlane(mine, l);
+        *nth = slot - (__builtin_amdgcn_readlane(sum, l) - *of);
+        *n = __builtin_amdgcn_readlane(len, l);
+        return true;
+      }
+      before = __builtin_amdgcn_readlane(sum, 63);
+    }
+    return false;
+  }
+  // Places of the sequences in front of `seq`.
+  __device__ __forceinline__ int in_front(int seq) const {
+    int sum = 0;
+    for (int b0 = 0; b0 < seq; b0 += kWave) sum += b0 + lane < seq ? parts(held_length(b0)) : 0;
+    return pag_total(sum);
+  }
+};
+
+// Loads of a cache that the memory-side cache does not hold go past the caches (pag_past).
+template <bool NT, typename V>
+__device__ __forceinline__ V pag_load(const V* p) {
+  if constexpr (NT) return __builtin_nontemporal_load(p);
+  else return *p;
+}
+
+template <int DP>
+struct PagShape {
+  static constexpr int kChunks = DP / 8;                  // 16-byte pieces of a row
+  static constexpr int kLoads = kPagRun * kChunks / kWave;  // of a run's V rows
+  static constexpr int kSteps = DP / 32, kTiles = DP / 16;
+  // Rows of V lie in LDS with their pieces exchanged in pairs, so that a transposed read's four rows, 16 elements each, meet in no bank.
+  static constexpr int kMask = DP % 128 == 0 ? 7 : 3;
+  static constexpr int kPart = kPagHeads * (DP + 2);      // floats of a part's column: rows of 16 heads, maxima, sums
+  // K through LDS too: a load instruction then takes whole rows, where the product's operand takes 64 bytes of 16 (64 rows of up to 16384 keys: 476 us
+  // against 460, past the caches 500 against 415; with 64 dimensions, a row being 128 bytes, 82 against 92, registers for three workgroups in place of four).
+  static constexpr bool kKeysToo = DP == 128;
+  static __device__ __forceinline__ int k_at(int row, int chunk) { return kPagRun * DP + row * DP + (chunk ^ (row & 15)) * 8; }
+  static __device__ __forceinline__ int at(int row, int chunk) { return row * DP + (chunk ^ ((row & kMask) << 1)) * 8; }
+};
+
+// ALIGNED: pages are multiples of 16 keys, so 16 consecutive keys from a multiple of 16 on share a page.  SHARED: wavefronts that share a part's keys;
+// 4 / SHARED columns to a workgroup.
+template <typename T, int DP, bool ALIGNED, int SHARED, bool NT>
+__global__ __launch_bounds__(kPagThreads, DP <= 128 ? 2 : 1) void paged_attention_kernel(fr_paged_args a) {
+  typedef typename Attn<T>::vec8 vec8;
+  typedef typename Attn<T>::vec4 vec4;
+  typedef PagShape<DP> S;
+  constexpr int kStep = kPagRun * SHARED, kColumns = kPagWaves / SHARED, kSlice = (S::kKeysToo ? 2 : 1) * kPagRun * DP;
+  __shared__ __attribute__((aligned(16))) char shared[kPagWaves * kSlice * sizeof(T)];
+  __shared__ float max_of[kPagWaves][kPagHeads], sum_of[kPagWaves][kPagHeads];
+  const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const int share = static_cast<int>(a.heads / a.kv_heads), tiles = (share + kPagHeads - 1) / kPagHeads, columns = static_cast<int>(a.kv_heads) * tiles;
+  const int groups = columns / kColumns;
+  const PagPlan plan(a, kStep);
+  const int dim = static_cast<int>(a.dim), quarter = lane >> 4, low = lane & 15;
+  const float scale = static_cast<float>(a.scale) * kLog2e;
+  T* const vl = reinterpret_cast<T*>(shared) + wave * kSlice;  // the wavefront's V rows, and K rows
+  for (int item = blockIdx.x;; item += gridDim.x) {
+  const int slot = item / groups, column = (item - slot * groups) * kColumns + wave / SHARED;
+  const int kv = column / tiles, head0 = (column - kv * tiles) * kPagHeads;
+  const int heads = share - head0 < kPagHeads ? share - head0 : kPagHeads;  // of the columns of the matrix instruction, in use
+  int seq, nth, parts, length;
+  if (!plan.place(slot, &seq, &nth, &parts, &length)) return;
+  const int first = parts > 1 ? nth * plan.per * kStep : 0;
+  const int last = parts > 1 && length - first > plan.per * kStep ? first + plan.per * kStep : length;
+  const int32_t* table = reinterpret_cast<const int32_t*>(a.table) + seq * a.table_row;
+  const T* kc = reinterpret_cast<const T*>(a.k_cache) + kv * a.k_cache_head;
+  const T* vc = reinterpret_cast<const T*>(a.v_cache) + kv * a.v_cache_head;
+
+  // Q^T, the second operand: column = lane % 16
+  vec8 q[S::kSteps];
+#pragma unroll
+  for (int s = 0; s < S::kSteps; ++s) {
+    q[s] = vec8{0, 0, 0, 0, 0, 0, 0, 0};
+    const int d = s * 32 + quarter * 8;
+    if (low < heads && d < dim)
+      q[s] = *reinterpret_cast<const vec8*>(reinterpret_cast<const T*>(a.q) + seq * a.q_row + (kv * share + head0 + low) * a.q_head + d);
+  }
+
+  auto page_of = [&](int key) { return a.page_shift >= 0 ? key >> static_cast<int>(a.page_shift) : key / static_cast<int>(a.page_size); };
+  // Where key `key`'s row lies, -1 behind the last key and in a page that there is not: such keys take no part, their rows are zeros.
+  auto row_of = [&](int key, int64_t page_stride, int64_t slot_stride) -> int64_t {
+    if (key >= last) return -1;
+    const int p = page_of(key);
+    const int64_t page = table[p];
+    if (page < 0 || page >= a.pages) return -1;
+    return page * page_stride + (key - p * static_cast<int>(a.page_size)) * slot_stride;
+  };
+  vec8 k[S::kLoads], v[S::kLoads];  // K: in the order of V's rows, or as the product takes them, 16 keys after the other
+  static_assert(S::kLoads == 2 * S::kSteps, "as many registers either way");
+  bool whole = false;  // the run in the registers: no key of it is left out
+  auto load = [&](int base) {
+    if (ALIGNED && base + kPagRun <= last) {
+      int64_t page[2];
+      int in[2];
+      whole = true;
+#pragma unroll
+      for (int t = 0; t < 2; ++t) {
+        const int p = page_of(base + 16 * t);
+        page[t] = table[p];
+        in[t] = base + 16 * t - p * static_cast<int>(a.page_size);
+        whole = whole && page[t] >= 0 && page[t] < a.pages;
+      }
+      if (whole) {
+        const vec8 none = {0, 0, 0, 0, 0, 0, 0, 0};
+        if constexpr (!S::kKeysToo) {
+#pragma unroll
+          for (int t = 0; t < 2; ++t) {
+            const T* from = kc + page[t] * a.k_cache_page + in[t] * a.k_cache_slot + (low * a.k_cache_slot + quarter * 8);
+#pragma unroll
+            for (int s = 0; s < S::kSteps; ++s) k[t * S::kSteps + s] = dim == DP || s * 32 + quarter * 8 < dim ? pag_load<NT>(reinterpret_cast<const vec8*>(from + s * 32)) : none;
+          }
+        }
+#pragma unroll
+        for (int i = 0; i < S::kLoads; ++i) {
+          const int at = i * kWave + lane, row = at / S::kChunks, d = at % S::kChunks * 8, t = i * kWave / S::kChunks >= 16 ? 1 : 0;  // a load's rows are in one half
+          const bool in_row = dim == DP || d < dim;
+          if constexpr (S::kKeysToo) {
+            const T* from = kc + page[t] * a.k_cache_page + in[t] * a.k_cache_slot + ((row - 16 * t) * a.k_cache_slot + d);
+            k[i] = in_row ? pag_load<NT>(reinterpret_cast<const vec8*>(from)) : none;
+          }
+          const T* from = vc + page[t] * a.v_cache_page + in[t] * a.v_cache_slot + ((row - 16 * t) * a.v_cache_slot + d);
+          v[i] = in_row ? pag_load<NT>(reinterpret_cast<const vec8*>(from)) : none;
+        }
+        return;
+      }
+    }
+    whole = false;
+    if constexpr (!S::kKeysToo) {
+#pragma unroll
+      for (int t = 0; t < 2; ++t) {
+        const int64_t from = row_of(base + 16 * t + low, a.k_cache_page, a.k_cache_slot);
+#pragma unroll
+        for (int s = 0; s < S::kSteps; ++s) {
+          const int d = s * 32 + quarter * 8;
+          k[t * S::kSteps + s] = vec8{0, 0, 0, 0, 0, 0, 0, 0};
+          if (from >= 0 && d < dim) k[t * S::kSteps + s] = *reinterpret_cast<const vec8*>(kc + from + d);
+        }
+      }
+    }
+#pragma unroll
+    for (int i = 0; i < S::kLoads; ++i) {
+      const int at = i * kWave + lane, row = at / S::kChunks, d = at % S::kChunks * 8;
+      if constexpr (S::kKeysToo) {
+        const int64_t from = row_of(base + row, a.k_cache_page, a.k_cache_slot);
+        k[i] = vec8{0, 0, 0, 0, 0, 0, 0, 0};
+        if (from >= 0 && d < dim) k[i] = *reinterpret_cast<const vec8*>(kc + from + d);
+      }
+      const int64_t from = row_of(base + row, a.v_cache_page, a.v_cache_slot);
+      v[i] = vec8{0, 0, 0, 0, 0, 0, 0, 0};
+      if (from >= 0 && d < dim) v[i] = *reinterpret_cast<const vec8*>(vc + from + d);
+    }
+  };
+
+  f32x4 o[S::kTiles];
+#pragma unroll
+  for (int t = 0; t < S::kTiles; ++t) o[t] = f32x4{0.f, 0.f, 0.f, 0.f};
+  float top = -INFINITY, sum = 0.f;  // of column lane % 16: the maximum (lagging) in all four lanes, the sum of the lane's own keys
+  int base = first + wave % SHARED * kPagRun;
+  if (base < last) load(base);
+  for (; base < last; base += kStep) {
+    f32x4 st[2] = {f32x4{0.f, 0.f, 0.f, 0.f}, f32x4{0.f, 0.f, 0.f, 0.f}};
+    if constexpr (!S::kKeysToo) {
+#pragma unroll
+      for (int s = 0; s < S::kSteps; ++s)
+#pragma unroll
+        for (int t = 0; t < 2; ++t) st[t] = Attn<T>::mma16(k[t * S::kSteps + s], q[s], st[t]);
+    }
+#pragma unroll
+    for (int i = 0; i < S::kLoads; ++i) {
+      const int at = i * kWave + lane;
+      if constexpr (S::kKeysToo) *reinterpret_cast<vec8*>(vl + S::k_at(at / S::kChunks, at % S::kChunks)) = k[i];
+      *reinterpret_cast<vec8*>(vl + S::at(at / S::kChunks, at % S::kChunks)) = v[i];
+    }
+    const bool all_seen = whole;
+    if (base + kStep < last) load(base + kStep);
+    if constexpr (S::kKeysToo) {
+#pragma unroll
+      for (int s = 0; s < S::kSteps; ++s)
+#pragma unroll
+        for (int t = 0; t < 2; ++t) st[t] = Attn<T>::mma16(*reinterpret_cast<const vec8*>(vl + S::k_at(t * 16 + low, s * 4 + quarter)), q[s], st[t]);
+    }
+    float p[2][4], high = -INFINITY;
+#pragma unroll
+    for (int t = 0; t < 2; ++t)
+#pragma unroll
+      for (int r = 0; r < 4; ++r) p[t][r] = st[t][r] * scale;
+    if (!all_seen) {
+#pragma unroll
+      for (int t = 0; t < 2; ++t)
+#pragma unroll
+        for (int r = 0; r < 4; ++r)
+          if (row_of(base + 16 * t + quarter * 4 + r, 0, 0) < 0) p[t][r] = -INFINITY;
+    }
+#pragma unroll
+    for (int t = 0; t < 2; ++t)
+#pragma unroll
+      for (int r = 0; r < 4; ++r) high = fmaxf(high, p[t][r]);
+    if (__any(high > top + kLag)) {
+      high = max_over_32(max_over_16(high));
+      const float now = fmaxf(top, high), by = top == -INFINITY ? 0.f : exp2_of(top - now);
+      sum *= by;
+#pragma unroll
+      for (int t = 0; t < S::kTiles; ++t) o[t] *= by;
+      top = now;
+    }
+    const float from = top == -INFINITY ? 0.f : top;
+    vec8 pt;
+#pragma unroll
+    for (int t = 0; t < 2; ++t)
+#pragma unroll
+      for (int r = 0; r < 4; ++r) {
+        const float e = exp2_of(p[t][r] - from);
+        sum += e;
+        pt[t * 4 + r] = static_cast<T>(e);  // to 8 or 11 bits: the second product's operand
+      }
+#pragma unroll
+    for (int t = 0; t < S::kTiles; ++t) {
+      const int chunk = 2 * t + ((lane & 3) >> 1), rest = (lane & 1) * 4, row = quarter * 4 + (low >> 2);
+      const auto lo = read_transposed<T>(vl + S::at(row, chunk) + rest), hi = read_transposed<T>(vl + S::at(row + 16, chunk) + rest);
+      o[t] = Attn<T>::mma16(join8(lo, hi), pt, o[t]);
+    }
+  }
+  sum = sum_over_32(sum_over_16(sum));
+
+  float* const to_part = reinterpret_cast<float*>(a.workspace) + (static_cast<int64_t>(slot) * columns + column) * S::kPart;
+  T* const to_out = reinterpret_cast<T*>(a.out) + seq * a.out_row + (kv * share + head0) * a.out_head;
+  auto put = [&](int h, int d, const f32x4& x) {  // four dimensions of a head of the column
+    if (parts > 1) {
+      *reinterpret_cast<f32x4*>(to_part + h * DP + d) = x;
+    } else if (d < dim) {
+      vec4 y;
+#pragma unroll
+      for (int e = 0; e < 4; ++e) y[e] = static_cast<T>(x[e]);
+      *reinterpret_cast<vec4*>(to_out + h * a.out_head + d) = y;
+    }
+  };
+  auto put_sums = [&](float all, float total) {
+    if (parts > 1 && quarter == 0) {
+      to_part[kPagHeads * DP + low] = all;
+      to_part[kPagHeads * (DP + 1) + low] = total;
+    }
+  };
+  if constexpr (SHARED == 1) {
+    put_sums(top, sum);
+    const float by = parts > 1 ? 1.f : (sum == 0.f ? 0.f : 1.f / sum);  // no key at all: zeros
+    if (low < heads) {
+#pragma unroll
+      for (int t = 0; t < S::kTiles; ++t) put(low, t * 16 + quarter * 4, o[t] * by);
+    }
+  } else {
+    // The wavefronts' rows in one: fp32, over V's place in LDS.
+    const int mate = wave / SHARED * SHARED;
+    if (quarter == 0) max_of[wave][low] = top, sum_of[wave][low] = sum;
+    __syncthreads();
+    float all = -INFINITY, total = 0.f;
+#pragma unroll
+    for (int w = 0; w < SHARED; ++w) all = fmaxf(all, max_of[mate + w][low]);
+#pragma unroll
+    for (int w = 0; w < SHARED; ++w) total += max_of[mate + w][low] == -INFINITY ? 0.f : sum_of[mate + w][low] * exp2_of(max_of[mate + w][low] - all);
+    float by = top == -INFINITY ? 0.f : exp2_of(top - all);
+    if (parts == 1) by = total == 0.f ? 0.f : by / total;
+    float* const rows = reinterpret_cast<float*>(shared);  // [wave][head][dimension]
+#pragma unroll
+    for (int t = 0; t < S::kTiles; ++t) *reinterpret_cast<f32x4*>(&rows[(wave * kPagHeads + low) * DP + t * 16 + quarter * 4]) = o[t] * by;
+    if (wave == mate) put_sums(all, total);
+    __syncthreads();
+    for (int i = (wave - mate) * kWave + lane; i < heads * (DP / 4); i += SHARED * kWave) {
+      const int h = i / (DP / 4), d = i % (DP / 4) * 4;
+      f32x4 x = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+      for (int w = 0; w < SHARED; ++w) x += *reinterpret_cast<const f32x4*>(&rows[((mate + w) * kPagHeads + h) * DP + d]);
+      put(h, d, x);
+    }
+    __syncthreads();  // the next part's values come after this one's rows have been read
+  }
+  }
+}
+
+template <typename T, int DP>
+__global__ __launch_bounds__(kPagThreads) void paged_join_kernel(fr_paged_args a, int unit, int wide) {
+  typedef JoinShape<DP> J;
+  const int share = static_cast<int>(a.heads / a.kv_heads), tiles = (share + kPagHeads - 1) / kPagHeads;
+  const int64_t at = wide ? blockIdx.x : static_cast<int64_t>(blockIdx.x) * J::kGroups + threadIdx.x / J::kLanes, all = a.B * a.heads;
+  const int seq = static_cast<int>((at < all ? at : all - 1) / a.heads), head = static_cast<int>((at < all ? at : all - 1) - seq * a.heads);
+  const PagPlan plan(a, unit);
+  const int parts = plan.parts(plan.length(seq));
+  const int kv = head / share, in = head - kv * share;
+  const int64_t pitch = static_cast<int64_t>(a.kv_heads) * tiles * PagShape<DP>::kPart;
+  // the places in front of a group's sequence: of the workgroup's first one, and from there on one by one
+  const int first = __builtin_amdgcn_readfirstlane(seq);
+  int slot = plan.in_front(first);
+  for (int b = first; __any(b < seq); ++b) slot += b < seq ? plan.parts(plan.length(b)) : 0;
+  const float* const from = reinterpret_cast<const float*>(a.workspace) + slot * pitch + (kv * tiles + in / kPagHeads) * PagShape<DP>::kPart;
+  const float* const tops = from + kPagHeads * DP + in % kPagHeads;
+  if (wide && parts == 1) return;
+  join_parts<T, DP>(wide, at < all && parts > 1, parts, from + in % kPagHeads * DP, pitch, tops, tops + kPagHeads, pitch,
+                    reinterpret_cast<T*>(a.out) + seq * a.out_row + head * a.out_head, static_cast<int>(a.dim));
+}
+
+int pag_dim(int64_t dim) { return dim <= 64 ? 64 : dim <= 128 ? 128 : dim <= 192 ? 192 : 256; }
+
+int64_t pag_columns(int64_t heads, int64_t kv_heads) { return kv_heads * ceil_div(heads / kv_heads, kPagHeads); }
+
+// How a call is cut: wavefronts that share a part's keys, places for parts (per group of columns), the least units of a part.
+struct PagCut {
+  int shared;
+  int64_t groups, slots, least;
+};
+int64_t pag_places(int64_t dim) { return dim <= 64 ? 1024 : dim <= 128 ? 512 : 256; }  // workgroups that the chip holds, by their registers: four, two or one to a CU
+PagCut pag_cut(int64_t B, int64_t heads, int64_t kv_heads, int64_t dim, int64_t most) {
+  const int64_t columns = pag_columns(heads, kv_heads);
+  PagCut c;
+  c.shared = columns % 4 == 0 ? 1 : columns % 2 == 0 ? 2 : 4;
+  c.groups = columns * c.shared / kPagWaves;
+  const int64_t unit = kPagRun * c.shared, useful = B * ceil_div(most, unit), once = pag_places(dim) / c.groups;
+  c.slots = B;
+  c.least = 1;
+  if (most <= 256) return c;  // a part each: a second launch takes longer
+  int64_t spare;
+  if (4 * B <= once) {
+    spare = once - B;  // few sequences: every workgroup one part
+  } else {
+    spare = ceil_div(8 * pag_places(dim), c.groups);  // many: parts to take in turn, of 512 keys at least
+    c.least = (B * c.groups < pag_places(dim) ? 256 : 512) / unit;
+  }
+  c.slots = B + (spare < useful ? spare : useful);
+  return c;
+}
+
+// Whether keys and values are read past the caches: where the pages are more than the memory-side cache's 256 MB, so that a step of all layers leaves nothing of
+// them there.
+bool pag_past(const fr_paged_args& a) { return a.pages * a.page_size * a.kv_heads * a.dim * 2 * 2 > (int64_t(256) << 20); }
+
+template <typename T, int DP, bool ALIGNED, bool NT>
+int launch_paged(const fr_paged_args& a, const PagCut& c, hipStream_t st) {
+  const int64_t items = a.slots * c.groups;
+  const dim3 grid(static_cast<unsigned>(items < pag_places(DP) ? items : pag_places(DP))), block(kPagThreads);
+  if (c.shared == 1) hipLaunchKernelGGL((paged_attention_kernel<T, DP, ALIGNED, 1, NT>), grid, block, 0, st, a);
+  else if (c.shared == 2) hipLaunchKernelGGL((paged_attention_kernel<T, DP, ALIGNED, 2, NT>), grid, block, 0, st, a);
+  else hipLaunchKernelGGL((paged_attention_kernel<T, DP, ALIGNED, 4, NT>), grid, block, 0, st, a);
+  int rc = check_launch("paged_attention_kernel");
+  if (rc != FR_OK || a.slots == a.B) return rc;
+  typedef JoinShape<DP> J;
+  static_assert(J::kThreads == kPagThreads, "join_parts' workgroups");
+  const bool wide = a.B * a.heads <= 1024;  // (more sequences have few parts each, most often one)
+  hipLaunchKernelGGL((paged_join_kernel<T, DP>), dim3(static_cast<unsigned>(J::blocks(a.B * a.heads, wide))), block, 0, st, a, kPagRun * c.shared, wide);
+  return check_launch("paged_join_kernel");
+}
+
+template <typename T, int DP>
+int launch_paged_pages(const fr_paged_args& a, const PagCut& c, hipStream_t st) {
+  if (a.page_size % 16 != 0) return launch_paged<T, DP, false, false>(a, c, st);
+  return pag_past(a) ? launch_paged<T, DP, true, true>(a, c, st) : launch_paged<T, DP, true, false>(a, c, st);
+}
+
+template <typename T>
+int dispatch_paged(const fr_paged_args& a, const PagCut& c, hipStream_t st) {
+  switch (pag_dim(a.dim)) {
+    case 64: return launch_paged_pages<T, 64>(a, c, st);
+    case 128: return launch_paged_pages<T, 128>(a, c, st);
+    case 192: return launch_paged_pages<T, 192>(a, c, st);
+    default: return launch_paged_pages<T, 256>(a, c, st);
+  }
+}
+
+}  // namespace
+
+// A call of checked arguments on rows of T; in a translation unit per type (paged_attention_inst_*.hip).
+template <typename T>
+int paged_attention_run(const fr_paged_args& a, int64_t groups, int shared, hipStream_t st) {
+  PagCut c;
+  c.groups = groups;
+  c.shared = shared;
+  return dispatch_paged<T>(a, c, st);
+}
+extern template int paged_attention_run<bf16_t>(const fr_paged_args&, int64_t, int, hipStream_t);
+extern template int paged_attention_run<f16_t>(const fr_paged_args&, int64_t, int, hipStream_t);
+
+}  // namespace fr

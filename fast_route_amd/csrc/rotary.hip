@@ -121,7 +121,11 @@ __global__ __launch_bounds__(kRotThreads) void rotary_kernel(fr_rotary_args a, i
 
 template <typename T>
 int launch_rotary(const fr_rotary_args& a, bool wide, hipStream_t st) {
-  const int tokens = a.T >= 4096 ? kRotTokens : 1;
+  // As many tokens as give every thread an item, where there are tokens enough for every CU: 8192 tokens of 12 and 4 heads of 64 dimensions 14.5 us one by one,
+  // 11.7 four together; 32 and 8 heads of 128, which have 448 items a token, 39.6 and 43.5; 64 tokens 4.3 and 7.1.
+  const int64_t vec = wide ? 8 : 1, items = ((a.heads + a.kv_heads) * (a.dim - a.turned / 2) + (a.slots ? a.kv_heads * a.dim : 0)) / vec;
+  const int64_t fill = items < kRotThreads ? kRotThreads / (items > 0 ? items : 1) : 1;
+  const int tokens = a.T < 2048 ? 1 : static_cast<int>(fill < kRotTokens ? fill : kRotTokens);
   const dim3 grid(static_cast<unsigned>(ceil_div(a.T, tokens))), block(kRotThreads);
   if (wide && a.interleaved) hipLaunchKernelGGL((rotary_kernel<T, 8, true>), grid, block, 0, st, a, tokens);
   else if (wide) hipLaunchKernelGGL((rotary_kernel<T, 8, false>), grid, block, 0, st, a, tokens);
