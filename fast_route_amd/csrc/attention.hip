@@ -2,14 +2,20 @@
 //
 // A workgroup takes 128 rows of one sequence and key head, a row being a token's query head that shares the key head: the heads of a token lie next
 // to each other, so a tile of few tokens is still a whole one and its keys are read once for all of them.  Four wavefronts of 32 rows; keys in
-// blocks of 64, through LDS in two buffers, the next block's loads in flight while one is worked on.
-//   S^T [64 keys, 32 rows] = K Q^T on 32x32x16 matrix instructions: Q stays in registers.  A lane's accumulators are 32 scores of one row: maximum
-//   and sum need one exchange with the lane that has the other 32, and rescaling is a factor per lane.
-//   O^T [dim, 32 rows] += V^T P^T: the accumulators, rounded, are the second operand as they are, if the keys of V^T are taken in the same
+// blocks of 64 (32 from 129 dimensions on), straight to LDS in two buffers, the next block's loads in flight while one is worked on, one barrier a block.
+//   S^T [keys, rows] = K Q^T on 16x16x32 matrix instructions: Q stays in registers.  A lane's accumulators are the scores of two rows with every
+//   fourth run of four keys: the maximum needs no exchange until it moves (kLag), and rescaling is a factor per lane.
+//   O^T [dim, rows] += V^T P^T: the accumulators, rounded, are the second operand as they are, if the keys of V^T are taken in the same
 //   order; transposed reads of LDS give four keys of a dimension at a time.
-// Bound by the matrix instructions and, nearly as long, the exponentials beside them; two workgroups to a CU cover for one another.
+// 16x16x32 and not 32x32x16 (a register of accumulators read per 32 flops more): the part runs under its power limit, and the clock is 1.92 in place of 1.72 GHz; 8192
+// rows without a mask 993 us against 1033.  A prompt of 16384 rows, 32 heads over 8 of 128 dimensions: 2.0 ms, 1.09 PFLOP/s (a matrix product 8192^3 reaches 1.47); 64
+// dimensions 0.92, 192 1.05, 256 1.03.  Bound by the matrix instructions (48 % of the cycles) and the vector instructions between them (an exponential, a
+// multiply-add, half a maximum and half a conversion per score: as many cycles at 128 dimensions), which two workgroups to a CU overlap only in part.  Tried and taken back: the
+// next block's scores computed beside this one's exponentials in one wavefront (256 registers, 3 % slower, and no faster with the order fixed by hand).
 //
-// Tiles of all sequences are taken in the order of their place in the sequence, last ones first: with a causal mask these have the most keys.
+// Short sequences: about 6 us of a workgroup go by before its first product (lengths, search, first loads), 24 prompts of 512 rows 119 us, 0.43 PFLOP/s.  Tiles of all
+// sequences are taken in the order of their place in the sequence, last ones first: with a causal mask these have the most keys.  Few tiles over many
+// keys are split along the keys as well and joined by a second launch.
 #include "attention_core.h"
 
 namespace fr {
@@ -473,7 +479,8 @@ int att_dim(int64_t dim) { return dim <= 64 ? 64 : dim <= 128 ? 128 : dim <= 192
 int64_t att_tiles(int64_t B, int64_t rows, int64_t share, bool fill) { return ceil_div(rows * share, kAttTile) + B + (fill ? 1 : 0) - 1; }
 
 // Parts that the keys are split into: as many as fill the chip's 512 places for workgroups where the tiles do not, none of less than kAttPartKeys keys
-// of a sequence of average length (the lengths themselves are on the device).
+// of a sequence of average length (the lengths themselves are on the device).  509 rows over 8192 keys, 16 heads over 2 of 64: one part 117 us, eight 44.  At 768
+// places 512 rows over 8704 keys take 109 us for 88; parts of 512 keys and more: a row over 8000 keys 22.5 us for 17.3.
 constexpr int64_t kAttPlaces = 512, kAttPartKeys = 256, kAttMostParts = 32;
 int64_t att_parts(int64_t B, int64_t rows, int64_t keys, int64_t heads, int64_t kv_heads) {
   if (B < 1 || rows < 1) return 1;

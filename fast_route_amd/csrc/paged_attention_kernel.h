@@ -73,10 +73,10 @@ struct PagPlan {
     const int total = pag_total(sum), need = static_cast<int>((static_cast<unsigned>(total) + spare - 1) / spare);
     per = need < static_cast<int>(a.least) ? static_cast<int>(a.least) : need;
   }
-  // Sequence, part and number of parts of place `slot`; false behind the last one.
-  __device__ __forceinline__ bool place(int slot, int* seq, int* nth, int* of, int* n) const {
-    int before = 0;
-    for (int b0 = 0; b0 < count; b0 += kWave) {
+  // Sequence, part and number of parts of place `slot`, which is not in front of the last call's; false behind the last one.
+  int b0 = 0, before = 0;  // the 64 sequences that the last call ended at, the places in front of them
+  __device__ __forceinline__ bool place(int slot, int* seq, int* nth, int* of, int* n) {
+    for (; b0 < count; b0 += kWave) {
       const int len = held_length(b0), mine = b0 + lane < count ? parts(len) : 0, sum = before + pag_up_to(mine);
       const uint64_t hit = __ballot(slot < sum && slot >= sum - mine);
       if (hit) {
@@ -134,232 +134,233 @@ __global__ __launch_bounds__(kPagThreads, DP <= 128 ? 2 : 1) void paged_attentio
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int share = static_cast<int>(a.heads / a.kv_heads), tiles = (share + kPagHeads - 1) / kPagHeads, columns = static_cast<int>(a.kv_heads) * tiles;
   const int groups = columns / kColumns;
-  const PagPlan plan(a, kStep);
+  PagPlan plan(a, kStep);
   const int dim = static_cast<int>(a.dim), quarter = lane >> 4, low = lane & 15;
   const float scale = static_cast<float>(a.scale) * kLog2e;
   T* const vl = reinterpret_cast<T*>(shared) + wave * kSlice;  // the wavefront's V rows, and K rows
   for (int item = blockIdx.x;; item += gridDim.x) {
-  const int slot = item / groups, column = (item - slot * groups) * kColumns + wave / SHARED;
-  const int kv = column / tiles, head0 = (column - kv * tiles) * kPagHeads;
-  const int heads = share - head0 < kPagHeads ? share - head0 : kPagHeads;  // of the columns of the matrix instruction, in use
-  int seq, nth, parts, length;
-  if (!plan.place(slot, &seq, &nth, &parts, &length)) return;
-  const int first = parts > 1 ? nth * plan.per * kStep : 0;
-  const int last = parts > 1 && length - first > plan.per * kStep ? first + plan.per * kStep : length;
-  const int32_t* table = reinterpret_cast<const int32_t*>(a.table) + seq * a.table_row;
-  const T* kc = reinterpret_cast<const T*>(a.k_cache) + kv * a.k_cache_head;
-  const T* vc = reinterpret_cast<const T*>(a.v_cache) + kv * a.v_cache_head;
+    const int slot = item / groups, column = (item - slot * groups) * kColumns + wave / SHARED;
+    const int kv = column / tiles, head0 = (column - kv * tiles) * kPagHeads;
+    const int heads = share - head0 < kPagHeads ? share - head0 : kPagHeads;  // of the columns of the matrix instruction, in use
+    int seq, nth, parts, length;
+    if (!plan.place(slot, &seq, &nth, &parts, &length)) return;
+    const int first = parts > 1 ? nth * plan.per * kStep : 0;
+    const int last = parts > 1 && length - first > plan.per * kStep ? first + plan.per * kStep : length;
+    const int32_t* table = reinterpret_cast<const int32_t*>(a.table) + seq * a.table_row;
+    const T* kc = reinterpret_cast<const T*>(a.k_cache) + kv * a.k_cache_head;
+    const T* vc = reinterpret_cast<const T*>(a.v_cache) + kv * a.v_cache_head;
 
-  // Q^T, the second operand: column = lane % 16
-  vec8 q[S::kSteps];
+    // Q^T, the second operand: column = lane % 16
+    vec8 q[S::kSteps];
 #pragma unroll
-  for (int s = 0; s < S::kSteps; ++s) {
-    q[s] = vec8{0, 0, 0, 0, 0, 0, 0, 0};
-    const int d = s * 32 + quarter * 8;
-    if (low < heads && d < dim)
-      q[s] = *reinterpret_cast<const vec8*>(reinterpret_cast<const T*>(a.q) + seq * a.q_row + (kv * share + head0 + low) * a.q_head + d);
-  }
+    for (int s = 0; s < S::kSteps; ++s) {
+      q[s] = vec8{0, 0, 0, 0, 0, 0, 0, 0};
+      const int d = s * 32 + quarter * 8;
+      if (low < heads && d < dim)
+        q[s] = *reinterpret_cast<const vec8*>(reinterpret_cast<const T*>(a.q) + seq * a.q_row + (kv * share + head0 + low) * a.q_head + d);
+    }
 
-  auto page_of = [&](int key) { return a.page_shift >= 0 ? key >> static_cast<int>(a.page_shift) : key / static_cast<int>(a.page_size); };
-  // Where key `key`'s row lies, -1 behind the last key and in a page that there is not: such keys take no part, their rows are zeros.
-  auto row_of = [&](int key, int64_t page_stride, int64_t slot_stride) -> int64_t {
-    if (key >= last) return -1;
-    const int p = page_of(key);
-    const int64_t page = table[p];
-    if (page < 0 || page >= a.pages) return -1;
-    return page * page_stride + (key - p * static_cast<int>(a.page_size)) * slot_stride;
-  };
-  vec8 k[S::kLoads], v[S::kLoads];  // K: in the order of V's rows, or as the product takes them, 16 keys after the other
-  static_assert(S::kLoads == 2 * S::kSteps, "as many registers either way");
-  bool whole = false;  // the run in the registers: no key of it is left out
-  auto load = [&](int base) {
-    if (ALIGNED && base + kPagRun <= last) {
-      int64_t page[2];
-      int in[2];
-      whole = true;
+    auto page_of = [&](int key) { return a.page_shift >= 0 ? key >> static_cast<int>(a.page_shift) : key / static_cast<int>(a.page_size); };
+    // Where key `key`'s row lies, -1 behind the last key and in a page that there is not: such keys take no part, their rows are zeros.
+    auto row_of = [&](int key, int64_t page_stride, int64_t slot_stride) -> int64_t {
+      if (key >= last) return -1;
+      const int p = page_of(key);
+      const int64_t page = table[p];
+      if (page < 0 || page >= a.pages) return -1;
+      return page * page_stride + (key - p * static_cast<int>(a.page_size)) * slot_stride;
+    };
+    vec8 k[S::kLoads], v[S::kLoads];  // K: in the order of V's rows, or as the product takes them, 16 keys after the other
+    static_assert(S::kLoads == 2 * S::kSteps, "as many registers either way");
+    bool whole = false;  // the run in the registers: no key of it is left out
+    auto load = [&](int base) {
+      if (ALIGNED && base + kPagRun <= last) {
+        int64_t page[2];
+        int in[2];
+        whole = true;
 #pragma unroll
-      for (int t = 0; t < 2; ++t) {
-        const int p = page_of(base + 16 * t);
-        page[t] = table[p];
-        in[t] = base + 16 * t - p * static_cast<int>(a.page_size);
-        whole = whole && page[t] >= 0 && page[t] < a.pages;
+        for (int t = 0; t < 2; ++t) {
+          const int p = page_of(base + 16 * t);
+          page[t] = table[p];
+          in[t] = base + 16 * t - p * static_cast<int>(a.page_size);
+          whole = whole && page[t] >= 0 && page[t] < a.pages;
+        }
+        if (whole) {
+          const vec8 none = {0, 0, 0, 0, 0, 0, 0, 0};
+          if constexpr (!S::kKeysToo) {
+#pragma unroll
+            for (int t = 0; t < 2; ++t) {
+              const T* from = kc + page[t] * a.k_cache_page + in[t] * a.k_cache_slot + (low * a.k_cache_slot + quarter * 8);
+#pragma unroll
+              for (int s = 0; s < S::kSteps; ++s) k[t * S::kSteps + s] = dim == DP || s * 32 + quarter * 8 < dim ? pag_load<NT>(reinterpret_cast<const vec8*>(from + s * 32)) : none;
+            }
+          }
+#pragma unroll
+          for (int i = 0; i < S::kLoads; ++i) {
+            const int at = i * kWave + lane, row = at / S::kChunks, d = at % S::kChunks * 8, t = i * kWave / S::kChunks >= 16 ? 1 : 0;  // a load's rows are in one half
+            const bool in_row = dim == DP || d < dim;
+            if constexpr (S::kKeysToo) {
+              const T* from = kc + page[t] * a.k_cache_page + in[t] * a.k_cache_slot + ((row - 16 * t) * a.k_cache_slot + d);
+              k[i] = in_row ? pag_load<NT>(reinterpret_cast<const vec8*>(from)) : none;
+            }
+            const T* from = vc + page[t] * a.v_cache_page + in[t] * a.v_cache_slot + ((row - 16 * t) * a.v_cache_slot + d);
+            v[i] = in_row ? pag_load<NT>(reinterpret_cast<const vec8*>(from)) : none;
+          }
+          return;
+        }
       }
-      if (whole) {
-        const vec8 none = {0, 0, 0, 0, 0, 0, 0, 0};
-        if constexpr (!S::kKeysToo) {
+      whole = false;
+      if constexpr (!S::kKeysToo) {
 #pragma unroll
-          for (int t = 0; t < 2; ++t) {
-            const T* from = kc + page[t] * a.k_cache_page + in[t] * a.k_cache_slot + (low * a.k_cache_slot + quarter * 8);
+        for (int t = 0; t < 2; ++t) {
+          const int64_t from = row_of(base + 16 * t + low, a.k_cache_page, a.k_cache_slot);
 #pragma unroll
-            for (int s = 0; s < S::kSteps; ++s) k[t * S::kSteps + s] = dim == DP || s * 32 + quarter * 8 < dim ? pag_load<NT>(reinterpret_cast<const vec8*>(from + s * 32)) : none;
+          for (int s = 0; s < S::kSteps; ++s) {
+            const int d = s * 32 + quarter * 8;
+            k[t * S::kSteps + s] = vec8{0, 0, 0, 0, 0, 0, 0, 0};
+            if (from >= 0 && d < dim) k[t * S::kSteps + s] = *reinterpret_cast<const vec8*>(kc + from + d);
           }
         }
-#pragma unroll
-        for (int i = 0; i < S::kLoads; ++i) {
-          const int at = i * kWave + lane, row = at / S::kChunks, d = at % S::kChunks * 8, t = i * kWave / S::kChunks >= 16 ? 1 : 0;  // a load's rows are in one half
-          const bool in_row = dim == DP || d < dim;
-          if constexpr (S::kKeysToo) {
-            const T* from = kc + page[t] * a.k_cache_page + in[t] * a.k_cache_slot + ((row - 16 * t) * a.k_cache_slot + d);
-            k[i] = in_row ? pag_load<NT>(reinterpret_cast<const vec8*>(from)) : none;
-          }
-          const T* from = vc + page[t] * a.v_cache_page + in[t] * a.v_cache_slot + ((row - 16 * t) * a.v_cache_slot + d);
-          v[i] = in_row ? pag_load<NT>(reinterpret_cast<const vec8*>(from)) : none;
-        }
-        return;
       }
-    }
-    whole = false;
-    if constexpr (!S::kKeysToo) {
 #pragma unroll
-      for (int t = 0; t < 2; ++t) {
-        const int64_t from = row_of(base + 16 * t + low, a.k_cache_page, a.k_cache_slot);
-#pragma unroll
-        for (int s = 0; s < S::kSteps; ++s) {
-          const int d = s * 32 + quarter * 8;
-          k[t * S::kSteps + s] = vec8{0, 0, 0, 0, 0, 0, 0, 0};
-          if (from >= 0 && d < dim) k[t * S::kSteps + s] = *reinterpret_cast<const vec8*>(kc + from + d);
+      for (int i = 0; i < S::kLoads; ++i) {
+        const int at = i * kWave + lane, row = at / S::kChunks, d = at % S::kChunks * 8;
+        if constexpr (S::kKeysToo) {
+          const int64_t from = row_of(base + row, a.k_cache_page, a.k_cache_slot);
+          k[i] = vec8{0, 0, 0, 0, 0, 0, 0, 0};
+          if (from >= 0 && d < dim) k[i] = *reinterpret_cast<const vec8*>(kc + from + d);
         }
+        const int64_t from = row_of(base + row, a.v_cache_page, a.v_cache_slot);
+        v[i] = vec8{0, 0, 0, 0, 0, 0, 0, 0};
+        if (from >= 0 && d < dim) v[i] = *reinterpret_cast<const vec8*>(vc + from + d);
       }
-    }
+    };
+
+    f32x4 o[S::kTiles];
 #pragma unroll
-    for (int i = 0; i < S::kLoads; ++i) {
-      const int at = i * kWave + lane, row = at / S::kChunks, d = at % S::kChunks * 8;
+    for (int t = 0; t < S::kTiles; ++t) o[t] = f32x4{0.f, 0.f, 0.f, 0.f};
+    float top = -INFINITY, sum = 0.f;  // of column lane % 16: the maximum (lagging) in all four lanes, the sum of the lane's own keys
+    int base = first + wave % SHARED * kPagRun;
+    if (base < last) load(base);
+    for (; base < last; base += kStep) {
+      f32x4 st[2] = {f32x4{0.f, 0.f, 0.f, 0.f}, f32x4{0.f, 0.f, 0.f, 0.f}};
+      if constexpr (!S::kKeysToo) {
+#pragma unroll
+        for (int s = 0; s < S::kSteps; ++s)
+#pragma unroll
+          for (int t = 0; t < 2; ++t) st[t] = Attn<T>::mma16(k[t * S::kSteps + s], q[s], st[t]);
+      }
+#pragma unroll
+      for (int i = 0; i < S::kLoads; ++i) {
+        const int at = i * kWave + lane;
+        if constexpr (S::kKeysToo) *reinterpret_cast<vec8*>(vl + S::k_at(at / S::kChunks, at % S::kChunks)) = k[i];
+        *reinterpret_cast<vec8*>(vl + S::at(at / S::kChunks, at % S::kChunks)) = v[i];
+      }
+      const bool all_seen = whole;
+      if (base + kStep < last) load(base + kStep);
       if constexpr (S::kKeysToo) {
-        const int64_t from = row_of(base + row, a.k_cache_page, a.k_cache_slot);
-        k[i] = vec8{0, 0, 0, 0, 0, 0, 0, 0};
-        if (from >= 0 && d < dim) k[i] = *reinterpret_cast<const vec8*>(kc + from + d);
+#pragma unroll
+        for (int s = 0; s < S::kSteps; ++s)
+#pragma unroll
+          for (int t = 0; t < 2; ++t) st[t] = Attn<T>::mma16(*reinterpret_cast<const vec8*>(vl + S::k_at(t * 16 + low, s * 4 + quarter)), q[s], st[t]);
       }
-      const int64_t from = row_of(base + row, a.v_cache_page, a.v_cache_slot);
-      v[i] = vec8{0, 0, 0, 0, 0, 0, 0, 0};
-      if (from >= 0 && d < dim) v[i] = *reinterpret_cast<const vec8*>(vc + from + d);
-    }
-  };
-
-  f32x4 o[S::kTiles];
-#pragma unroll
-  for (int t = 0; t < S::kTiles; ++t) o[t] = f32x4{0.f, 0.f, 0.f, 0.f};
-  float top = -INFINITY, sum = 0.f;  // of column lane % 16: the maximum (lagging) in all four lanes, the sum of the lane's own keys
-  int base = first + wave % SHARED * kPagRun;
-  if (base < last) load(base);
-  for (; base < last; base += kStep) {
-    f32x4 st[2] = {f32x4{0.f, 0.f, 0.f, 0.f}, f32x4{0.f, 0.f, 0.f, 0.f}};
-    if constexpr (!S::kKeysToo) {
-#pragma unroll
-      for (int s = 0; s < S::kSteps; ++s)
-#pragma unroll
-        for (int t = 0; t < 2; ++t) st[t] = Attn<T>::mma16(k[t * S::kSteps + s], q[s], st[t]);
-    }
-#pragma unroll
-    for (int i = 0; i < S::kLoads; ++i) {
-      const int at = i * kWave + lane;
-      if constexpr (S::kKeysToo) *reinterpret_cast<vec8*>(vl + S::k_at(at / S::kChunks, at % S::kChunks)) = k[i];
-      *reinterpret_cast<vec8*>(vl + S::at(at / S::kChunks, at % S::kChunks)) = v[i];
-    }
-    const bool all_seen = whole;
-    if (base + kStep < last) load(base + kStep);
-    if constexpr (S::kKeysToo) {
-#pragma unroll
-      for (int s = 0; s < S::kSteps; ++s)
-#pragma unroll
-        for (int t = 0; t < 2; ++t) st[t] = Attn<T>::mma16(*reinterpret_cast<const vec8*>(vl + S::k_at(t * 16 + low, s * 4 + quarter)), q[s], st[t]);
-    }
-    float p[2][4], high = -INFINITY;
-#pragma unroll
-    for (int t = 0; t < 2; ++t)
-#pragma unroll
-      for (int r = 0; r < 4; ++r) p[t][r] = st[t][r] * scale;
-    if (!all_seen) {
+      float p[2][4], high = -INFINITY;
 #pragma unroll
       for (int t = 0; t < 2; ++t)
 #pragma unroll
-        for (int r = 0; r < 4; ++r)
-          if (row_of(base + 16 * t + quarter * 4 + r, 0, 0) < 0) p[t][r] = -INFINITY;
-    }
+        for (int r = 0; r < 4; ++r) p[t][r] = st[t][r] * scale;
+      if (!all_seen) {
 #pragma unroll
-    for (int t = 0; t < 2; ++t)
+        for (int t = 0; t < 2; ++t)
 #pragma unroll
-      for (int r = 0; r < 4; ++r) high = fmaxf(high, p[t][r]);
-    if (__any(high > top + kLag)) {
-      high = max_over_32(max_over_16(high));
-      const float now = fmaxf(top, high), by = top == -INFINITY ? 0.f : exp2_of(top - now);
-      sum *= by;
-#pragma unroll
-      for (int t = 0; t < S::kTiles; ++t) o[t] *= by;
-      top = now;
-    }
-    const float from = top == -INFINITY ? 0.f : top;
-    vec8 pt;
-#pragma unroll
-    for (int t = 0; t < 2; ++t)
-#pragma unroll
-      for (int r = 0; r < 4; ++r) {
-        const float e = exp2_of(p[t][r] - from);
-        sum += e;
-        pt[t * 4 + r] = static_cast<T>(e);  // to 8 or 11 bits: the second product's operand
+          for (int r = 0; r < 4; ++r)
+            if (row_of(base + 16 * t + quarter * 4 + r, 0, 0) < 0) p[t][r] = -INFINITY;
       }
 #pragma unroll
-    for (int t = 0; t < S::kTiles; ++t) {
-      const int chunk = 2 * t + ((lane & 3) >> 1), rest = (lane & 1) * 4, row = quarter * 4 + (low >> 2);
-      const auto lo = read_transposed<T>(vl + S::at(row, chunk) + rest), hi = read_transposed<T>(vl + S::at(row + 16, chunk) + rest);
-      o[t] = Attn<T>::mma16(join8(lo, hi), pt, o[t]);
+      for (int t = 0; t < 2; ++t)
+#pragma unroll
+        for (int r = 0; r < 4; ++r) high = fmaxf(high, p[t][r]);
+      if (__any(high > top + kLag)) {
+        high = max_over_32(max_over_16(high));
+        const float now = fmaxf(top, high), by = top == -INFINITY ? 0.f : exp2_of(top - now);
+        sum *= by;
+#pragma unroll
+        for (int t = 0; t < S::kTiles; ++t) o[t] *= by;
+        top = now;
+      }
+      const float from = top == -INFINITY ? 0.f : top;
+      vec8 pt;
+#pragma unroll
+      for (int t = 0; t < 2; ++t)
+#pragma unroll
+        for (int r = 0; r < 4; ++r) {
+          const float e = exp2_of(p[t][r] - from);
+          sum += e;
+          pt[t * 4 + r] = static_cast<T>(e);  // to 8 or 11 bits: the second product's operand
+        }
+#pragma unroll
+      for (int t = 0; t < S::kTiles; ++t) {
+        const int chunk = 2 * t + ((lane & 3) >> 1), rest = (lane & 1) * 4, row = quarter * 4 + (low >> 2);
+        const auto lo = read_transposed<T>(vl + S::at(row, chunk) + rest), hi = read_transposed<T>(vl + S::at(row + 16, chunk) + rest);
+        o[t] = Attn<T>::mma16(join8(lo, hi), pt, o[t]);
+      }
     }
-  }
-  sum = sum_over_32(sum_over_16(sum));
+    sum = sum_over_32(sum_over_16(sum));
 
-  float* const to_part = reinterpret_cast<float*>(a.workspace) + (static_cast<int64_t>(slot) * columns + column) * S::kPart;
-  T* const to_out = reinterpret_cast<T*>(a.out) + seq * a.out_row + (kv * share + head0) * a.out_head;
-  auto put = [&](int h, int d, const f32x4& x) {  // four dimensions of a head of the column
-    if (parts > 1) {
-      *reinterpret_cast<f32x4*>(to_part + h * DP + d) = x;
-    } else if (d < dim) {
-      vec4 y;
+    float* const to_part = reinterpret_cast<float*>(a.workspace) + (static_cast<int64_t>(slot) * columns + column) * S::kPart;
+    T* const to_out = reinterpret_cast<T*>(a.out) + seq * a.out_row + (kv * share + head0) * a.out_head;
+    auto put = [&](int h, int d, const f32x4& x) {  // four dimensions of a head of the column
+      if (parts > 1) {
+        *reinterpret_cast<f32x4*>(to_part + h * DP + d) = x;
+      } else if (d < dim) {
+        vec4 y;
 #pragma unroll
-      for (int e = 0; e < 4; ++e) y[e] = static_cast<T>(x[e]);
-      *reinterpret_cast<vec4*>(to_out + h * a.out_head + d) = y;
+        for (int e = 0; e < 4; ++e) y[e] = static_cast<T>(x[e]);
+        *reinterpret_cast<vec4*>(to_out + h * a.out_head + d) = y;
+      }
+    };
+    auto put_sums = [&](float all, float total) {
+      if (parts > 1 && quarter == 0) {
+        to_part[kPagHeads * DP + low] = all;
+        to_part[kPagHeads * (DP + 1) + low] = total;
+      }
+    };
+    if constexpr (SHARED == 1) {
+      put_sums(top, sum);
+      const float by = parts > 1 ? 1.f : (sum == 0.f ? 0.f : 1.f / sum);  // no key at all: zeros
+      if (low < heads) {
+#pragma unroll
+        for (int t = 0; t < S::kTiles; ++t) put(low, t * 16 + quarter * 4, o[t] * by);
+      }
+    } else {
+      // The wavefronts' rows in one: fp32, over V's place in LDS.
+      const int mate = wave / SHARED * SHARED;
+      if (quarter == 0) max_of[wave][low] = top, sum_of[wave][low] = sum;
+      __syncthreads();
+      float all = -INFINITY, total = 0.f;
+#pragma unroll
+      for (int w = 0; w < SHARED; ++w) all = fmaxf(all, max_of[mate + w][low]);
+#pragma unroll
+      for (int w = 0; w < SHARED; ++w) total += max_of[mate + w][low] == -INFINITY ? 0.f : sum_of[mate + w][low] * exp2_of(max_of[mate + w][low] - all);
+      float by = top == -INFINITY ? 0.f : exp2_of(top - all);
+      if (parts == 1) by = total == 0.f ? 0.f : by / total;
+      float* const rows = reinterpret_cast<float*>(shared);  // [wave][head][dimension]
+#pragma unroll
+      for (int t = 0; t < S::kTiles; ++t) *reinterpret_cast<f32x4*>(&rows[(wave * kPagHeads + low) * DP + t * 16 + quarter * 4]) = o[t] * by;
+      if (wave == mate) put_sums(all, total);
+      __syncthreads();
+      for (int i = (wave - mate) * kWave + lane; i < heads * (DP / 4); i += SHARED * kWave) {
+        const int h = i / (DP / 4), d = i % (DP / 4) * 4;
+        f32x4 x = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+        for (int w = 0; w < SHARED; ++w) x += *reinterpret_cast<const f32x4*>(&rows[((mate + w) * kPagHeads + h) * DP + d]);
+        put(h, d, x);
+      }
+      __syncthreads();  // the next part's values come after this one's rows have been read
     }
-  };
-  auto put_sums = [&](float all, float total) {
-    if (parts > 1 && quarter == 0) {
-      to_part[kPagHeads * DP + low] = all;
-      to_part[kPagHeads * (DP + 1) + low] = total;
-    }
-  };
-  if constexpr (SHARED == 1) {
-    put_sums(top, sum);
-    const float by = parts > 1 ? 1.f : (sum == 0.f ? 0.f : 1.f / sum);  // no key at all: zeros
-    if (low < heads) {
-#pragma unroll
-      for (int t = 0; t < S::kTiles; ++t) put(low, t * 16 + quarter * 4, o[t] * by);
-    }
-  } else {
-    // The wavefronts' rows in one: fp32, over V's place in LDS.
-    const int mate = wave / SHARED * SHARED;
-    if (quarter == 0) max_of[wave][low] = top, sum_of[wave][low] = sum;
-    __syncthreads();
-    float all = -INFINITY, total = 0.f;
-#pragma unroll
-    for (int w = 0; w < SHARED; ++w) all = fmaxf(all, max_of[mate + w][low]);
-#pragma unroll
-    for (int w = 0; w < SHARED; ++w) total += max_of[mate + w][low] == -INFINITY ? 0.f : sum_of[mate + w][low] * exp2_of(max_of[mate + w][low] - all);
-    float by = top == -INFINITY ? 0.f : exp2_of(top - all);
-    if (parts == 1) by = total == 0.f ? 0.f : by / total;
-    float* const rows = reinterpret_cast<float*>(shared);  // [wave][head][dimension]
-#pragma unroll
-    for (int t = 0; t < S::kTiles; ++t) *reinterpret_cast<f32x4*>(&rows[(wave * kPagHeads + low) * DP + t * 16 + quarter * 4]) = o[t] * by;
-    if (wave == mate) put_sums(all, total);
-    __syncthreads();
-    for (int i = (wave - mate) * kWave + lane; i < heads * (DP / 4); i += SHARED * kWave) {
-      const int h = i / (DP / 4), d = i % (DP / 4) * 4;
-      f32x4 x = {0.f, 0.f, 0.f, 0.f};
-#pragma unroll
-      for (int w = 0; w < SHARED; ++w) x += *reinterpret_cast<const f32x4*>(&rows[((mate + w) * kPagHeads + h) * DP + d]);
-      put(h, d, x);
-    }
-    __syncthreads();  // the next part's values come after this one's rows have been read
-  }
   }
 }
 
+// Joins the parts of a sequence's heads (join_parts); `unit`: the keys that the parts were counted in.
 template <typename T, int DP>
 __global__ __launch_bounds__(kPagThreads) void paged_join_kernel(fr_paged_args a, int unit, int wide) {
   typedef JoinShape<DP> J;
@@ -399,20 +400,26 @@ PagCut pag_cut(int64_t B, int64_t heads, int64_t kv_heads, int64_t dim, int64_t 
   const int64_t unit = kPagRun * c.shared, useful = B * ceil_div(most, unit), once = pag_places(dim) / c.groups;
   c.slots = B;
   c.least = 1;
-  if (most <= 256) return c;  // a part each: a second launch takes longer
+  // A part each where a second launch takes longer: a run after the other is 1.9 us, joining 4 us.  us, a part each / split: one row of 128 keys 12.1 / 10.5, of 256
+  // 19.6 / 10.5; 32 rows of 256 20.6 / 16.0; but 128 rows of 256 26.5 / 29.9, of 512 45.6 / 50.2.
+  if (most <= 64 || (most <= 512 && B * c.groups >= 256)) return c;
+  // Few sequences: a part to each workgroup that the chip holds.  Many: eight times as many, taken in turn, none of less than 256 or 512 keys (32 rows of up to
+  // 2048 keys, 32 key heads: 512 keys 122 us, 256 92, 128 97; 256 rows of up to 300, which fill the chip by themselves: 42, 57, 46).  64 rows of up to 16384
+  // keys, parts for one / two / four / eight times the places: 591, 515, 494, 487 us.
   int64_t spare;
   if (4 * B <= once) {
-    spare = once - B;  // few sequences: every workgroup one part
+    spare = once - B;
   } else {
-    spare = ceil_div(8 * pag_places(dim), c.groups);  // many: parts to take in turn, of 512 keys at least
+    spare = ceil_div(8 * pag_places(dim), c.groups);
     c.least = (B * c.groups < pag_places(dim) ? 256 : 512) / unit;
   }
   c.slots = B + (spare < useful ? spare : useful);
   return c;
 }
 
-// Whether keys and values are read past the caches: where the pages are more than the memory-side cache's 256 MB, so that a step of all layers leaves nothing of
-// them there.
+// Whether keys and values are read past the caches: where the pages are more than the memory-side cache's 256 MB, so that nothing of them is left there from the last
+// step.  us, past them / not: 64 rows of up to 16384 keys (2.6 GB) 421 / 462, three of 131071 (0.4 GB) 82 / 88, 32 rows (0.45 GB) 85 / 95; but pages of 139 MB read
+// again and again 43 / 40 and 34 / 32.
 bool pag_past(const fr_paged_args& a) { return a.pages * a.page_size * a.kv_heads * a.dim * 2 * 2 > (int64_t(256) << 20); }
 
 template <typename T, int DP, bool ALIGNED, bool NT>

@@ -155,6 +155,52 @@ def test_parts_of_a_joint_projection(native, dtype):
     assert torch.equal(shared, attention_varlen(q, k[:, :1], v[:, :1], _cu([50, 27]).cuda()))
 
 
+@pytest.mark.parametrize("causal", [True, False])
+def test_keys_split_along_their_length(native, causal):
+    """Few rows over many keys: parts that are joined, values that are not finite among the last ones, rows behind the sequences, a workspace's end."""
+    from fast_route_amd import attention_varlen
+    for lengths, keys, H, G, D in (([40], [3000], 8, 2, 128), ([3, 0, 9], [1500, 20, 2900], 4, 1, 64), ([1], [5000], 28, 4, 96), ([20], [2000], 2, 2, 256)):
+        _say(f"split {lengths} {keys} {causal}")
+        q, k, v = _packed(lengths, keys, H, G, D, torch.bfloat16, sum(keys))
+        ref, error = _want(q, k, v, lengths, keys, causal, D ** -0.5)
+        rows = torch.cat([q, q[:2]])
+        need = native.fr_attention_workspace_bytes(len(lengths), len(rows), sum(keys), H, G, D)
+        assert need > 0
+        guard = torch.full((need + 256,), 0xA5, dtype=torch.uint8, device="cuda")
+        args = rows.cuda(), k.cuda(), v.cuda(), _cu(lengths).cuda(), _cu(keys).cuda()
+        got = attention_varlen(*args, causal=causal, workspace_buf=guard[:need])
+        _close(got[:len(q)], ref, error)
+        assert (got[len(q):] == 0).all() and (guard[need:] == 0xA5).all()
+        out = torch.full_like(args[0], 5.0)
+        attention_varlen(*args, causal=causal, out=out)
+        assert torch.equal(out[:len(q)], got[:len(q)]) and (out[len(q):] == 5).all()
+        with pytest.raises(AssertionError):
+            attention_varlen(*args, causal=causal, workspace_buf=guard[:need - 1])
+        if causal and lengths[-1] > 1:
+            bad = v.clone()
+            bad[-1] = NAN  # the last row alone sees it
+            got = attention_varlen(args[0][:len(q)], args[1], bad.cuda(), *args[3:])
+            _close(got[:-1], ref[:-1], error[:-1])
+            assert got[-1].isnan().all()
+
+
+@pytest.mark.parametrize("count", [65, 300, 1100])
+def test_many_sequences(native, count):
+    """More sequences than a wavefront holds the lengths of."""
+    from fast_route_amd import attention_varlen, paged_attention
+    _say(f"{count} sequences")
+    g = torch.Generator().manual_seed(count)
+    lengths = torch.randint(0, 9, (count,), generator=g).tolist()
+    lengths[count // 2], lengths[-1] = 150, 70
+    q, k, v = _packed(lengths, lengths, 2, 1, 64, torch.bfloat16, count)
+    ref, error = _want(q, k, v, lengths, lengths, True, 0.125)
+    _close(attention_varlen(q.cuda(), k.cuda(), v.cuda(), _cu(lengths).cuda()), ref, error)
+    lengths[3] = 1300
+    for page in (16, 6):
+        q, kc, vc, table, n = _paged(lengths, 2, 1, 64, page, torch.bfloat16, count)
+        _close(paged_attention(q.cuda(), kc.cuda(), vc.cuda(), table.cuda(), n.cuda()), *_want_paged(q, kc, vc, table, n, 0.125))
+
+
 def test_long_prompt_and_chunks_of_it(native):
     """A prompt of several thousand rows against fp32 on the GPU, and the same one in chunks with the keys in front of them."""
     from fast_route_amd import attention_varlen

@@ -142,6 +142,49 @@ def test_no_tokens_and_one(native):
     assert torch.equal(grouped_topk(one, 6)[1].cpu(), oracle.grouped_topk(row.t(), 6)[1])
 
 
+@pytest.mark.parametrize("E,groups,kept,topk", [(256, 8, 4, 8), (64, 1, 1, 6), (128, 16, 5, 16), (512, 16, 4, 10), (384, 1, 1, 8)])
+def test_order_of_many_tokens(native, E, groups, kept, topk):
+    """16384 tokens' choices in the order of 64 bits: random logits, and logits whose choices crowd together around the last place, so that more than topk
+    have to be told apart (and for some tokens more than a lane each can)."""
+    from fast_route_amd import grouped_topk
+    _say(f"order E={E} groups={groups}")
+    g = torch.Generator(device="cuda").manual_seed(E)
+    M = 16384
+    logits = torch.randn(M, E, device="cuda", generator=g) * 1.5
+    logits[M // 2:] = 0.5 + 2.0 ** -22 * torch.randint(0, 40, (M // 2, E), device="cuda", generator=g).float()
+    logits[M // 2::2, : topk - 1] += 1.0  # the first places clear, the others crowded
+    bias = torch.randn(E, device="cuda", generator=g) * 0.1
+    near = torch.zeros(E, device="cuda")
+    near[::3] = 2.0 ** -24
+    for scoring in ("sigmoid", "softmax"):
+        for b in (None, bias, near):
+            x = logits.double()
+            score = torch.sigmoid(x) if scoring == "sigmoid" else torch.softmax(x, dim=1)
+            choice = x if b is None else score + b.double()
+            # distances that 64-bit sums in another order could turn: none of the tokens that are compared
+            if groups > 1:
+                best = choice.view(M, groups, -1).topk(2, dim=2).values
+                worth = best[:, :, 0] if b is None else best.sum(dim=2)
+                top = torch.sort(worth, dim=1, descending=True, stable=True)
+                out = torch.ones_like(worth, dtype=torch.bool).scatter_(1, top.indices[:, :kept], False)
+                choice = choice.masked_fill(out.repeat_interleave(E // groups, dim=1), float("-inf"))
+                edge = top.values[:, kept - 1] - top.values[:, kept]
+            order = torch.sort(choice, dim=1, descending=True, stable=True)
+            clear = torch.ones(M, dtype=torch.bool, device="cuda")
+            if b is not None:
+                step = order.values[:, :topk] - order.values[:, 1: topk + 1]
+                clear = ((step == 0) & (scoring == "sigmoid") | (step > 1e-14)).all(dim=1)
+                if groups > 1:
+                    clear &= edge > 1e-14
+            assert clear[: M // 2].float().mean() > 0.99
+            w, ids = grouped_topk(logits, topk, num_groups=groups, topk_groups=kept, scoring=scoring, bias=b)
+            same = (ids == order.indices[:, :topk]).all(dim=1)
+            assert same[clear].all(), (scoring, b is None, (~same & clear).nonzero()[:3, 0].tolist())
+            want = score.gather(1, ids.long())
+            want = want / want.sum(dim=1, keepdim=True)
+            assert ((w.double() - want).abs() <= 2.0 ** -14 * want).all()
+
+
 def test_captured_and_replayed(native):
     from fast_route_amd import grouped_topk
     _say("graph")
