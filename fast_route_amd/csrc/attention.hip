@@ -9,9 +9,10 @@
 //   order; transposed reads of LDS give four keys of a dimension at a time.
 // 16x16x32 and not 32x32x16 (a register of accumulators read per 32 flops more): the part runs under its power limit, and the clock is 1.92 in place of 1.72 GHz; 8192
 // rows without a mask 993 us against 1033.  A prompt of 16384 rows, 32 heads over 8 of 128 dimensions: 2.0 ms, 1.09 PFLOP/s (a matrix product 8192^3 reaches 1.47); 64
-// dimensions 0.92, 192 1.05, 256 1.03.  Bound by the matrix instructions (48 % of the cycles) and the vector instructions between them (an exponential, a
-// multiply-add, half a maximum and half a conversion per score: as many cycles at 128 dimensions), which two workgroups to a CU overlap only in part.  Tried and taken back: the
-// next block's scores computed beside this one's exponentials in one wavefront (256 registers, 3 % slower, and no faster with the order fixed by hand).
+// dimensions 0.92, 192 1.05, 256 1.03.  Bound by the matrix instructions (48 % of the cycles) and the vector instructions between them (an exponential, a multiply-add, half
+// a maximum and half a conversion per score: 770 cycles beside 1090 in a wavefront's block of 128 dimensions, and a block takes 1880): a SIMD hardly runs the two at once.
+// Tried and taken back: the next block's scores computed beside this one's exponentials in one wavefront (3 % slower, and no faster with the order fixed by hand);
+// eight wavefronts whose halves take turns, products beside exponentials, with a barrier between the turns (10 % slower, 64 dimensions 27 %).
 //
 // Short sequences: about 6 us of a workgroup go by before its first product (lengths, search, first loads), 24 prompts of 512 rows 119 us, 0.43 PFLOP/s.  Tiles of all
 // sequences are taken in the order of their place in the sequence, last ones first: with a causal mask these have the most keys.  Few tiles over many
