@@ -31,95 +31,107 @@ __device__ __forceinline__ void att_range(const int32_t* cu, int64_t b, int64_t 
   *end = b == B ? all : att_clamp(cu[b + 1], *begin, all);
 }
 
-__device__ __forceinline__ int att_total(int v) {  // over the wavefront, in every lane
-  v += partner_i32<1>(v);
-  v += partner_i32<2>(v);
-  v += partner_i32<4>(v);
-  v += partner_i32<8>(v);
-  return (__builtin_amdgcn_readlane(v, 0) + __builtin_amdgcn_readlane(v, 16)) + (__builtin_amdgcn_readlane(v, 32) + __builtin_amdgcn_readlane(v, 48));
-}
-
 struct AttPlace {
   int tile;                  // of the sequence, -1: none
   int q_begin, n, k_begin, m;  // its rows and keys
 };
 
-// Tile `nth` of the tiles in descending order of their place.  The first 256 sequences' tiles stay in the lanes: a search step is a
-// handful of instructions there and a round trip to L2 beyond (96 sequences of 128 rows: 6.7 us of a workgroup's 16 when only 64 did).
-constexpr int kAttHeld = 4;
+__device__ __forceinline__ int att_tiles_of(const fr_attention_args& a, int b) {
+  int64_t begin, end;
+  att_range(reinterpret_cast<const int32_t*>(a.cu_q), b, a.B, a.rows, &begin, &end);
+  return (static_cast<int>(end - begin) * static_cast<int>(a.heads / a.kv_heads) + kAttTile - 1) / kAttTile;
+}
+
+// Tile `nth` of the tiles in descending order of their place.  The sequences' tiles stay in the lanes, four times 64: a search step is a
+// handful of instructions there and a round trip to L2 beyond (96 sequences of 128 rows: 6.7 us of a workgroup's 16 when only 64 did).  More sequences: one after the
+// other, found in what attention_plan_kernel wrote.
+constexpr int kAttHeld = kHeldLengths / kWave;
 __device__ __forceinline__ AttPlace att_place(const fr_attention_args& a, int nth) {
   const int lane = threadIdx.x & 63;
-  const int share = static_cast<int>(a.heads / a.kv_heads), count = static_cast<int>(a.B + (a.fill ? 1 : 0));
-  const int32_t* const cu_q = reinterpret_cast<const int32_t*>(a.cu_q);
-  const int32_t* const cu_k = reinterpret_cast<const int32_t*>(a.cu_k);
-  struct Rows { int begin, n; };
-  auto range = [](const int32_t* cu, int64_t b, int64_t B, int64_t all) -> Rows {
-    int64_t begin, end;
-    att_range(cu, b, B, all, &begin, &end);
-    return Rows{static_cast<int>(begin), static_cast<int>(end - begin)};
-  };
-  auto tiles_in = [&](int n) { return (n * share + kAttTile - 1) / kAttTile; };
-  auto tiles_of = [&](int b) { return b < count ? tiles_in(range(cu_q, b, a.B, a.rows).n) : 0; };
-  Rows mine_q = {0, 0}, mine_k = {0, 0};  // of sequence `lane`
-  if (lane < count) mine_q = range(cu_q, lane, a.B, a.rows);
-  if (lane < a.B) mine_k = range(cu_k, lane, a.B, a.keys);
-  int mine[kAttHeld];  // tiles of sequences lane + 64 j
-#pragma unroll
-  for (int j = 0; j < kAttHeld; ++j) mine[j] = j == 0 ? tiles_in(mine_q.n) : (j * kWave < count ? tiles_of(lane + j * kWave) : 0);
-  auto total = [&](auto f) {
-    int v = f(mine[0]);
-    if (count > kWave) {
-#pragma unroll
-      for (int j = 1; j < kAttHeld; ++j) v += f(mine[j]);
-      for (int b = lane + kAttHeld * kWave; b < count; b += kWave) v += f(tiles_of(b));
-    }
-    return att_total(v);
-  };
+  const int count = static_cast<int>(a.B + (a.fill ? 1 : 0));
   AttPlace p = {-1, 0, 0, 0, 0};
   int seq = 0, lo = 0;
-  if (count == 1) {
-    lo = __builtin_amdgcn_readfirstlane(mine[0]) - 1 - nth;
-    if (lo < 0) return p;
-  } else {
-    if (total([](int t) { return t; }) <= nth) return p;
-    int hi = tiles_in(static_cast<int>(a.rows));  // tiles at places >= lo: more than nth; >= hi: not
-    for (int step = 1; lo + step < hi; step <<= 1) {  // most sequences are short beside all of them
-      if (total([&](int t) { return t > lo + step ? t - lo - step : 0; }) <= nth) {
-        hi = lo + step;
-        break;
-      }
-      lo += step;
-    }
-    while (hi - lo > 1) {
-      const int mid = (lo + hi) >> 1;
-      if (total([&](int t) { return t > mid ? t - mid : 0; }) > nth) lo = mid;
-      else hi = mid;
-    }
-    int left = nth - total([&](int t) { return t > lo + 1 ? t - lo - 1 : 0; });  // which of the sequences with a tile there
-    seq = -1;
-    for (int b0 = 0; b0 < count && seq < 0; b0 += kWave) {
-      const uint64_t has = __ballot((b0 ? tiles_of(b0 + lane) : mine[0]) > lo);
-      const int there = __popcll(has);
-      if (left < there) {
-        const uint64_t hit = __ballot(((has >> lane) & 1) && __popcll(has & ((1ull << lane) - 1)) == left);
-        if (!hit) return p;
-        seq = b0 + __ffsll(static_cast<unsigned long long>(hit)) - 1;
-      }
-      left -= there;
-    }
+  struct Rows { int begin, n; };
+  auto range = [](const void* cu, int b, int64_t B, int64_t all) -> Rows {
+    int64_t begin, end;
+    att_range(reinterpret_cast<const int32_t*>(cu), b, B, all, &begin, &end);
+    return Rows{static_cast<int>(begin), static_cast<int>(end - begin)};
+  };
+  Rows mine_q = {0, 0}, mine_k = {0, 0};  // of sequence `lane`
+  if (a.plan) {
+    const int* const plan = reinterpret_cast<const int*>(a.plan);
+    seq = place_in(plan, count, nth);
     if (seq < 0) return p;
+    lo = plan[seq + 1] - 1 - nth;
+    mine_q = range(a.cu_q, seq, a.B, a.rows);
+    if (seq < a.B) mine_k = range(a.cu_k, seq, a.B, a.keys);
+  } else {
+    if (lane < count) mine_q = range(a.cu_q, lane, a.B, a.rows);
+    if (lane < a.B) mine_k = range(a.cu_k, lane, a.B, a.keys);
+    const int share = static_cast<int>(a.heads / a.kv_heads);
+    int mine[kAttHeld];  // tiles of sequences lane + 64 j
+#pragma unroll
+    for (int j = 0; j < kAttHeld; ++j) {
+      const int b = lane + j * kWave;
+      mine[j] = j == 0 ? (mine_q.n * share + kAttTile - 1) / kAttTile : (b < count ? att_tiles_of(a, b) : 0);
+    }
+    auto total = [&](auto f) {
+      int v = f(mine[0]);
+      if (count > kWave) {
+#pragma unroll
+        for (int j = 1; j < kAttHeld; ++j) v += f(mine[j]);
+      }
+      return sum_of_all(v);
+    };
+    if (count == 1) {
+      lo = __builtin_amdgcn_readfirstlane(mine[0]) - 1 - nth;
+      if (lo < 0) return p;
+    } else {
+      if (total([](int t) { return t; }) <= nth) return p;
+      int hi = (static_cast<int>(a.rows) * share + kAttTile - 1) / kAttTile;  // tiles at places >= lo: more than nth; >= hi: not
+      for (int step = 1; lo + step < hi; step <<= 1) {                        // most sequences are short beside all of them
+        if (total([&](int t) { return t > lo + step ? t - lo - step : 0; }) <= nth) {
+          hi = lo + step;
+          break;
+        }
+        lo += step;
+      }
+      while (hi - lo > 1) {
+        const int mid = (lo + hi) >> 1;
+        if (total([&](int t) { return t > mid ? t - mid : 0; }) > nth) lo = mid;
+        else hi = mid;
+      }
+      int left = nth - total([&](int t) { return t > lo + 1 ? t - lo - 1 : 0; });  // which of the sequences with a tile there
+      seq = -1;
+#pragma unroll
+      for (int j = 0; j < kAttHeld; ++j) {
+        const uint64_t has = __ballot(mine[j] > lo);
+        const int there = __popcll(has);
+        if (seq < 0 && left < there) {
+          const uint64_t hit = __ballot(((has >> lane) & 1) && __popcll(has & ((1ull << lane) - 1)) == left);
+          if (!hit) return p;
+          seq = j * kWave + __ffsll(static_cast<unsigned long long>(hit)) - 1;
+        }
+        left -= there;
+      }
+      if (seq < 0) return p;
+      if (seq >= kWave) {
+        mine_q = range(a.cu_q, seq, a.B, a.rows);
+        mine_k = seq < a.B ? range(a.cu_k, seq, a.B, a.keys) : Rows{0, 0};
+      }
+    }
   }
   p.tile = __builtin_amdgcn_readfirstlane(lo);
   const int l = __builtin_amdgcn_readfirstlane(seq & 63);
-  if (seq >= kWave) {
-    mine_q = range(cu_q, seq, a.B, a.rows);
-    mine_k = seq < a.B ? range(cu_k, seq, a.B, a.keys) : Rows{0, 0};
-  }
   p.q_begin = __builtin_amdgcn_readlane(mine_q.begin, l);
   p.n = __builtin_amdgcn_readlane(mine_q.n, l);
   p.k_begin = __builtin_amdgcn_readlane(mine_k.begin, l);
   p.m = __builtin_amdgcn_readlane(mine_k.n, l);
   return p;
+}
+
+__global__ __launch_bounds__(kPlanThreads) void attention_plan_kernel(fr_attention_args a) {
+  prefix_of(static_cast<int>(a.B + (a.fill ? 1 : 0)), [&](int b) { return att_tiles_of(a, b); }, reinterpret_cast<int*>(a.plan));
 }
 
 template <int DP>
@@ -239,7 +251,7 @@ __global__ __launch_bounds__(kAttThreads, 2) void attention_kernel(fr_attention_
   if (at.tile < 0) return;
   const int n = at.n, m = at.m, q_begin = at.q_begin;
   const int rows = n * share, row0 = at.tile * kAttTile, wave_row0 = row0 + wave * kAttRows;
-  if (row0 >= rows) return;
+  if (row0 < 0 || row0 >= rows) return;
   // the lane's two rows, 16 apart: token and query head; keys up to `limit` are seen
   int token[2], head[2], limit[2];
   bool live[2];
@@ -492,8 +504,16 @@ int64_t att_parts(int64_t B, int64_t rows, int64_t keys, int64_t heads, int64_t 
   return parts < 1 ? 1 : (parts > kAttMostParts ? kAttMostParts : parts);
 }
 
+int64_t att_part_bytes(int64_t parts, int64_t rows, int64_t heads, int64_t dim) { return parts == 1 ? 0 : round_up(parts * rows * heads * (att_dim(dim) + 2) * 4, 16); }
+int64_t att_plan_bytes(int64_t B) { return B + 1 <= kHeldLengths ? 0 : round_up((B + 2) * 4, 16); }
+
 template <typename T, int DP>
 int launch_attention(const fr_attention_args& a, hipStream_t st) {
+  if (a.plan) {
+    hipLaunchKernelGGL(attention_plan_kernel, dim3(1), dim3(kPlanThreads), 0, st, a);
+    const int rc = check_launch("attention_plan_kernel");
+    if (rc != FR_OK) return rc;
+  }
   const int64_t tiles = att_tiles(a.B, a.rows, a.heads / a.kv_heads, a.fill != 0);
   hipLaunchKernelGGL((attention_kernel<T, DP>), dim3(static_cast<unsigned>(tiles * a.parts * a.kv_heads)), dim3(kAttThreads), 0, st, a);
   const int rc = check_launch("attention_kernel");
@@ -532,8 +552,7 @@ int check_attention_sizes(int64_t B, int64_t rows, int64_t keys, int64_t heads, 
 extern "C" int64_t fr_attention_workspace_bytes(int64_t B, int64_t rows, int64_t keys, int64_t heads, int64_t kv_heads, int64_t dim) {
   using namespace fr;
   if (check_attention_sizes(B, rows, keys, heads, kv_heads, dim) != FR_OK) return -1;
-  const int64_t parts = att_parts(B, rows, keys, heads, kv_heads);
-  return parts == 1 ? 0 : parts * rows * heads * (att_dim(dim) + 2) * 4;
+  return att_part_bytes(att_parts(B, rows, keys, heads, kv_heads), rows, heads, dim) + att_plan_bytes(B);
 }
 
 extern "C" int fr_attention(const fr_attention_args* args, void* stream) {
@@ -555,6 +574,7 @@ extern "C" int fr_attention(const fr_attention_args* args, void* stream) {
   FR_REQUIRE(need == 0 || (a.workspace && aligned16(a.workspace) && a.workspace_bytes >= need), FR_E_WORKSPACE,
              "fr_attention: workspace of %lld bytes, %lld needed", (long long)a.workspace_bytes, (long long)need);
   a.parts = att_parts(a.B, a.rows, a.keys, a.heads, a.kv_heads);
+  a.plan = att_plan_bytes(a.B) ? static_cast<char*>(a.workspace) + att_part_bytes(a.parts, a.rows, a.heads, a.dim) : nullptr;
   hipStream_t st = static_cast<hipStream_t>(stream);
   return a.dtype == FR_BF16 ? dispatch_attention<bf16_t>(a, st) : dispatch_attention<f16_t>(a, st);
 }

@@ -60,6 +60,59 @@ __device__ __forceinline__ float sum_over_32(float v) {
   return __uint_as_float(x[0]) + __uint_as_float(x[1]);
 }
 
+// Of the lanes up to this one; over the wavefront, in every lane.
+__device__ __forceinline__ int sum_up_to(int v) {
+  v += __builtin_amdgcn_update_dpp(0, v, 0x111, 0xF, 0xF, true);  // row_shr 1, 2, 4, 8
+  v += __builtin_amdgcn_update_dpp(0, v, 0x112, 0xF, 0xF, true);
+  v += __builtin_amdgcn_update_dpp(0, v, 0x114, 0xF, 0xF, true);
+  v += __builtin_amdgcn_update_dpp(0, v, 0x118, 0xF, 0xF, true);
+  const int lane = threadIdx.x & 63;
+  const int r0 = __builtin_amdgcn_readlane(v, 15), r1 = __builtin_amdgcn_readlane(v, 31), r2 = __builtin_amdgcn_readlane(v, 47);
+  return v + (lane >= 16 ? r0 : 0) + (lane >= 32 ? r1 : 0) + (lane >= 48 ? r2 : 0);
+}
+__device__ __forceinline__ int sum_of_all(int v) {
+  v += partner_i32<1>(v);
+  v += partner_i32<2>(v);
+  v += partner_i32<4>(v);
+  v += partner_i32<8>(v);
+  return (__builtin_amdgcn_readlane(v, 0) + __builtin_amdgcn_readlane(v, 16)) + (__builtin_amdgcn_readlane(v, 32) + __builtin_amdgcn_readlane(v, 48));
+}
+
+// The lengths of up to kHeldLengths sequences stay in a wavefront's lanes; of more, a launch of one workgroup writes what lies in front of each (prefix_of) to the
+// workspace first, where place_in finds a place again.  us, with that launch / every wavefront going over all lengths: packed, 300 sequences of 8 rows 23 / 27, 1100 of
+// 64 205 / 609, 4000 of 20 306 / 2492; paged, 300 of up to 2000 keys 143 / 139, 1100 of up to 600 190 / 199, 4000 of up to 600 549 / 681.
+constexpr int kHeldLengths = 256, kPlanThreads = 1024;
+
+// to[i] = the sum of value(0) .. value(i - 1), to[count] of all; by one workgroup of kPlanThreads.
+template <typename F>
+__device__ __forceinline__ void prefix_of(int count, F value, int* to) {
+  __shared__ int of_wave[kPlanThreads / kWave];
+  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+  int before = 0;
+  for (int b0 = 0; b0 < count; b0 += kPlanThreads) {
+    const int b = b0 + threadIdx.x, mine = b < count ? value(b) : 0, sum = sum_up_to(mine);
+    if (lane == 63) of_wave[wave] = sum;
+    __syncthreads();
+    int front = before, all = 0;
+#pragma unroll
+    for (int w = 0; w < kPlanThreads / kWave; ++w) front += w < wave ? of_wave[w] : 0, all += of_wave[w];
+    if (b < count) to[b] = front + sum - mine;
+    before += all;
+    __syncthreads();
+  }
+  if (threadIdx.x == 0) to[count] = before;
+}
+// The i with to[i] <= place < to[i + 1], -1: none.
+__device__ __forceinline__ int place_in(const int* to, int count, int place) {
+  int lo = 0, hi = count;
+  while (hi - lo > 1) {
+    const int mid = (lo + hi) >> 1;
+    if (to[mid] <= place) lo = mid;
+    else hi = mid;
+  }
+  return count > 0 && to[lo] <= place && place < to[lo + 1] ? lo : -1;
+}
+
 __device__ __forceinline__ float exp2_of(float v) { return __builtin_amdgcn_exp2f(v); }
 
 constexpr float kLog2e = 1.4426950408889634f;

@@ -21,7 +21,7 @@ extern "C" int64_t fr_paged_attention_workspace_bytes(int64_t B, int64_t heads, 
   using namespace fr;
   if (check_paged_sizes(B, heads, kv_heads, dim, most) != FR_OK) return -1;
   const int64_t slots = pag_cut(B, heads, kv_heads, dim, most).slots;
-  return slots == B ? 0 : slots * pag_columns(heads, kv_heads) * kPagHeads * (pag_dim(dim) + 2) * 4;
+  return pag_part_bytes(B, slots, heads, kv_heads, dim) + pag_plan_bytes(B, slots);
 }
 
 extern "C" int fr_paged_attention(const fr_paged_args* args, void* stream) {
@@ -43,9 +43,11 @@ extern "C" int fr_paged_attention(const fr_paged_args* args, void* stream) {
   const PagCut cut = pag_cut(a.B, a.heads, a.kv_heads, a.dim, most);
   a.slots = cut.slots;
   a.least = cut.least;
+  a.plan = nullptr;
   const int64_t need = fr_paged_attention_workspace_bytes(a.B, a.heads, a.kv_heads, a.dim, most);
   FR_REQUIRE(need == 0 || (a.workspace && aligned16(a.workspace) && a.workspace_bytes >= need), FR_E_WORKSPACE,
              "fr_paged_attention: workspace of %lld bytes, %lld needed", (long long)a.workspace_bytes, (long long)need);
+  if (pag_plan_bytes(a.B, a.slots)) a.plan = static_cast<char*>(a.workspace) + pag_part_bytes(a.B, a.slots, a.heads, a.kv_heads, a.dim);
   a.page_shift = (a.page_size & (a.page_size - 1)) == 0 ? __builtin_ctzll(a.page_size) : -1;
   hipStream_t st = static_cast<hipStream_t>(stream);
   return a.dtype == FR_BF16 ? paged_attention_run<bf16_t>(a, cut.groups, cut.shared, st) : paged_attention_run<f16_t>(a, cut.groups, cut.shared, st);

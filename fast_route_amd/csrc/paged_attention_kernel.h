@@ -11,8 +11,8 @@
 // four columns where there are so many, whose rows lie next to each other in memory (64 rows of up to 16384 keys, 8 key heads: 492 us with a key head to a
 // workgroup, where a cache whose heads come first took 461); with fewer columns they share a part's keys and join their rows in LDS.
 //
-// The keys of all sequences are cut into parts of equal length on the device, since the lengths are there (every wavefront adds them up, the first 256 in its
-// lanes), and the workgroups, as many as the chip holds at a time, take the parts in turn.  Parts of a sequence that has one go to the output,
+// The keys of all sequences are cut into parts of equal length on the device, since the lengths are there (every wavefront adds them up in its lanes, of more than 256 sequences a
+// launch in front), and the workgroups, as many as the chip holds at a time, take the parts in turn.  Parts of a sequence that has one go to the output,
 // others to fp32 rows with their maxima and sums, which a second launch joins.
 #pragma once
 #include "attention_core.h"
@@ -21,81 +21,87 @@ namespace fr {
 namespace {
 
 constexpr int kPagThreads = 256, kPagWaves = 4, kPagRun = 32, kPagHeads = 16;
-constexpr int kPagHeld = 4;  // times 64 lengths stay in the lanes
+constexpr int kPagHeld = kHeldLengths / kWave;  // times 64 lengths stay in the lanes
 
-__device__ __forceinline__ int pag_total(int v) {  // over the wavefront, in every lane
-  v += partner_i32<1>(v);
-  v += partner_i32<2>(v);
-  v += partner_i32<4>(v);
-  v += partner_i32<8>(v);
-  return (__builtin_amdgcn_readlane(v, 0) + __builtin_amdgcn_readlane(v, 16)) + (__builtin_amdgcn_readlane(v, 32) + __builtin_amdgcn_readlane(v, 48));
+__device__ __forceinline__ int pag_length(const fr_paged_args& a, int b) {
+  const int64_t cap = a.table_pages * a.page_size;
+  const int n = reinterpret_cast<const int32_t*>(a.lengths)[b];
+  return n < 0 ? 0 : (n > cap ? static_cast<int>(cap) : n);
 }
-__device__ __forceinline__ int pag_up_to(int v) {  // of the lanes up to this one
-  v += __builtin_amdgcn_update_dpp(0, v, 0x111, 0xF, 0xF, true);  // row_shr 1, 2, 4, 8
-  v += __builtin_amdgcn_update_dpp(0, v, 0x112, 0xF, 0xF, true);
-  v += __builtin_amdgcn_update_dpp(0, v, 0x114, 0xF, 0xF, true);
-  v += __builtin_amdgcn_update_dpp(0, v, 0x118, 0xF, 0xF, true);
-  const int lane = threadIdx.x & 63;
-  const int r0 = __builtin_amdgcn_readlane(v, 15), r1 = __builtin_amdgcn_readlane(v, 31), r2 = __builtin_amdgcn_readlane(v, 47);
-  return v + (lane >= 16 ? r0 : 0) + (lane >= 32 ? r1 : 0) + (lane >= 48 ? r2 : 0);
+__device__ __forceinline__ int pag_units(int n, int unit) { return static_cast<int>((static_cast<unsigned>(n) + unit - 1) / unit); }
+// Parts of `per` units each, one at least.
+__device__ __forceinline__ int pag_parts(int units, int per) { return units <= per ? 1 : static_cast<int>((static_cast<unsigned>(units) + per - 1) / per); }
+// Units of a part where all sequences have `total`: with `slots` places as many as give every sequence its parts - the sum over b of max(1, ceil(units / per)) is at most
+// total / per + B <= slots -, and `least` where there are more places than that takes.
+__device__ __forceinline__ int pag_per(const fr_paged_args& a, int total) {
+  const int spare = static_cast<int>(a.slots - a.B), need = static_cast<int>((static_cast<unsigned>(total) + spare - 1) / spare);
+  return need < static_cast<int>(a.least) ? static_cast<int>(a.least) : need;
 }
 
-// The parts of all sequences, counted in units of `unit` keys.
+// The parts of all sequences, counted in units of `unit` keys.  Three forms: a part each (slots == B); the lengths in the lanes; what paged_plan_kernel wrote: the
+// places in front of each sequence and, behind them, the units of a part.
 struct PagPlan {
   const fr_paged_args& a;
   int lane, count, unit, per;  // units of a part
-  int held[kPagHeld];          // lengths of sequences lane + 64 j
-  __device__ __forceinline__ int length(int b) const {
-    const int64_t cap = a.table_pages * a.page_size;
-    const int n = b < count ? reinterpret_cast<const int32_t*>(a.lengths)[b] : 0;
-    return n < 0 ? 0 : (n > cap ? static_cast<int>(cap) : n);
-  }
-  __device__ __forceinline__ int units(int n) const { return static_cast<int>((static_cast<unsigned>(n) + unit - 1) / unit); }
-  __device__ __forceinline__ int parts(int n) const {
-    const int u = units(n);
-    return u <= per ? 1 : static_cast<int>((static_cast<unsigned>(u) + per - 1) / per);
-  }
-  __device__ __forceinline__ int held_length(int b0) const {  // of sequence b0 + lane, b0 a multiple of 64
-    return b0 == 0 ? held[0] : b0 == kWave ? held[1] : b0 == 2 * kWave ? held[2] : b0 == 3 * kWave ? held[3] : length(b0 + lane);
-  }
-  // With `slots` places a part has as many units as give every sequence its parts: sum over b of max(1, ceil(units / per)) <= total / per + B <= slots; and
-  // `least` units where there are more places than that takes.
-  __device__ __forceinline__ PagPlan(const fr_paged_args& args, int keys) : a(args), lane(threadIdx.x & 63), count(static_cast<int>(args.B)), unit(keys) {
-#pragma unroll
-    for (int j = 0; j < kPagHeld; ++j) held[j] = j == 0 || j * kWave < count ? length(lane + j * kWave) : 0;
-    const int spare = static_cast<int>(a.slots - a.B);
-    per = 0x7fffffff;
-    if (spare <= 0) return;  // a part each
+  bool each;
+  int held[kPagHeld];  // lengths of sequences lane + 64 j
+  __device__ __forceinline__ const int* plan() const { return reinterpret_cast<const int*>(a.plan); }
+  __device__ __forceinline__ int parts(int n) const { return each ? 1 : pag_parts(pag_units(n, unit), per); }
+  __device__ __forceinline__ PagPlan(const fr_paged_args& args, int keys) : a(args), lane(threadIdx.x & 63), count(static_cast<int>(args.B)), unit(keys), per(1) {
+    each = a.slots == a.B;
+    if (each) return;
+    if (a.plan) {
+      per = plan()[count + 1];
+      return;
+    }
     int sum = 0;
 #pragma unroll
-    for (int j = 0; j < kPagHeld; ++j) sum += units(held[j]);
-    for (int b = lane + kPagHeld * kWave; b < count; b += kWave) sum += units(length(b));
-    const int total = pag_total(sum), need = static_cast<int>((static_cast<unsigned>(total) + spare - 1) / spare);
-    per = need < static_cast<int>(a.least) ? static_cast<int>(a.least) : need;
+    for (int j = 0; j < kPagHeld; ++j) {
+      const int b = lane + j * kWave;
+      held[j] = b < count ? pag_length(a, b) : 0;
+      sum += pag_units(held[j], unit);
+    }
+    per = pag_per(a, sum_of_all(sum));
   }
-  // Sequence, part and number of parts of place `slot`, which is not in front of the last call's; false behind the last one.
-  int b0 = 0, before = 0;  // the 64 sequences that the last call ended at, the places in front of them
-  __device__ __forceinline__ bool place(int slot, int* seq, int* nth, int* of, int* n) {
-    for (; b0 < count; b0 += kWave) {
-      const int len = held_length(b0), mine = b0 + lane < count ? parts(len) : 0, sum = before + pag_up_to(mine);
+  // Sequence, part, number of parts and length of place `slot`; false behind the last one.
+  __device__ __forceinline__ bool place(int slot, int* seq, int* nth, int* of, int* n) const {
+    if (each || a.plan) {
+      const int b = each ? (slot < count ? slot : -1) : place_in(plan(), count, slot);
+      if (b < 0) return false;
+      *seq = __builtin_amdgcn_readfirstlane(b);
+      *n = __builtin_amdgcn_readfirstlane(pag_length(a, b));
+      *of = parts(*n);
+      *nth = each ? 0 : __builtin_amdgcn_readfirstlane(slot - plan()[b]);
+      return true;
+    }
+    int before = 0;
+#pragma unroll
+    for (int j = 0; j < kPagHeld; ++j) {
+      if (j * kWave >= count) break;
+      const int mine = lane + j * kWave < count ? parts(held[j]) : 0, sum = before + sum_up_to(mine);
       const uint64_t hit = __ballot(slot < sum && slot >= sum - mine);
       if (hit) {
         const int l = __builtin_amdgcn_readfirstlane(__ffsll(static_cast<unsigned long long>(hit)) - 1);
-        *seq = b0 + l;
+        *seq = j * kWave + l;
         *of = __builtin_amdgcn_readlane(mine, l);
         *nth = slot - (__builtin_amdgcn_readlane(sum, l) - *of);
-        *n = __builtin_amdgcn_readlane(len, l);
+        *n = __builtin_amdgcn_readlane(held[j], l);
         return true;
       }
       before = __builtin_amdgcn_readlane(sum, 63);
     }
     return false;
   }
-  // Places of the sequences in front of `seq`.
+  // Places of the sequences in front of `seq`, which the lanes may differ in.
   __device__ __forceinline__ int in_front(int seq) const {
+    if (a.plan) return plan()[seq];
+    const int first = __builtin_amdgcn_readfirstlane(seq);  // the lowest
     int sum = 0;
-    for (int b0 = 0; b0 < seq; b0 += kWave) sum += b0 + lane < seq ? parts(held_length(b0)) : 0;
-    return pag_total(sum);
+#pragma unroll
+    for (int j = 0; j < kPagHeld; ++j) sum += lane + j * kWave < first ? parts(held[j]) : 0;
+    sum = sum_of_all(sum);
+    for (int b = first; __any(b < seq); ++b) sum += b < seq ? parts(pag_length(a, b)) : 0;
+    return sum;
   }
 };
 
@@ -134,7 +140,7 @@ __global__ __launch_bounds__(kPagThreads, DP <= 128 ? 2 : 1) void paged_attentio
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int share = static_cast<int>(a.heads / a.kv_heads), tiles = (share + kPagHeads - 1) / kPagHeads, columns = static_cast<int>(a.kv_heads) * tiles;
   const int groups = columns / kColumns;
-  PagPlan plan(a, kStep);
+  const PagPlan plan(a, kStep);
   const int dim = static_cast<int>(a.dim), quarter = lane >> 4, low = lane & 15;
   const float scale = static_cast<float>(a.scale) * kLog2e;
   T* const vl = reinterpret_cast<T*>(shared) + wave * kSlice;  // the wavefront's V rows, and K rows
@@ -360,6 +366,23 @@ __global__ __launch_bounds__(kPagThreads, DP <= 128 ? 2 : 1) void paged_attentio
   }
 }
 
+__global__ __launch_bounds__(kPlanThreads) void paged_plan_kernel(fr_paged_args a, int unit) {
+  __shared__ int of_wave[kPlanThreads / kWave];
+  const int count = static_cast<int>(a.B);
+  int sum = 0;
+  for (int b = threadIdx.x; b < count; b += kPlanThreads) sum += pag_units(pag_length(a, b), unit);
+  sum = sum_of_all(sum);
+  if ((threadIdx.x & 63) == 0) of_wave[threadIdx.x >> 6] = sum;
+  __syncthreads();
+  int total = 0;
+#pragma unroll
+  for (int w = 0; w < kPlanThreads / kWave; ++w) total += of_wave[w];
+  const int per = pag_per(a, total);
+  int* const to = reinterpret_cast<int*>(a.plan);
+  prefix_of(count, [&](int b) { return pag_parts(pag_units(pag_length(a, b), unit), per); }, to);
+  if (threadIdx.x == 0) to[count + 1] = per;
+}
+
 // Joins the parts of a sequence's heads (join_parts); `unit`: the keys that the parts were counted in.
 template <typename T, int DP>
 __global__ __launch_bounds__(kPagThreads) void paged_join_kernel(fr_paged_args a, int unit, int wide) {
@@ -368,13 +391,10 @@ __global__ __launch_bounds__(kPagThreads) void paged_join_kernel(fr_paged_args a
   const int64_t at = wide ? blockIdx.x : static_cast<int64_t>(blockIdx.x) * J::kGroups + threadIdx.x / J::kLanes, all = a.B * a.heads;
   const int seq = static_cast<int>((at < all ? at : all - 1) / a.heads), head = static_cast<int>((at < all ? at : all - 1) - seq * a.heads);
   const PagPlan plan(a, unit);
-  const int parts = plan.parts(plan.length(seq));
+  const int parts = plan.parts(pag_length(a, seq));
   const int kv = head / share, in = head - kv * share;
   const int64_t pitch = static_cast<int64_t>(a.kv_heads) * tiles * PagShape<DP>::kPart;
-  // the places in front of a group's sequence: of the workgroup's first one, and from there on one by one
-  const int first = __builtin_amdgcn_readfirstlane(seq);
-  int slot = plan.in_front(first);
-  for (int b = first; __any(b < seq); ++b) slot += b < seq ? plan.parts(plan.length(b)) : 0;
+  const int slot = plan.in_front(seq);
   const float* const from = reinterpret_cast<const float*>(a.workspace) + slot * pitch + (kv * tiles + in / kPagHeads) * PagShape<DP>::kPart;
   const float* const tops = from + kPagHeads * DP + in % kPagHeads;
   if (wide && parts == 1) return;
@@ -417,6 +437,11 @@ PagCut pag_cut(int64_t B, int64_t heads, int64_t kv_heads, int64_t dim, int64_t 
   return c;
 }
 
+int64_t pag_part_bytes(int64_t B, int64_t slots, int64_t heads, int64_t kv_heads, int64_t dim) {
+  return slots == B ? 0 : slots * pag_columns(heads, kv_heads) * kPagHeads * (pag_dim(dim) + 2) * 4;
+}
+int64_t pag_plan_bytes(int64_t B, int64_t slots) { return slots == B || B <= kHeldLengths ? 0 : round_up((B + 2) * 4, 16); }
+
 // Whether keys and values are read past the caches: where the pages are more than the memory-side cache's 256 MB, so that nothing of them is left there from the last
 // step.  us, past them / not: 64 rows of up to 16384 keys (2.6 GB) 421 / 462, three of 131071 (0.4 GB) 82 / 88, 32 rows (0.45 GB) 85 / 95; but pages of 139 MB read
 // again and again 43 / 40 and 34 / 32.
@@ -424,6 +449,11 @@ bool pag_past(const fr_paged_args& a) { return a.pages * a.page_size * a.kv_head
 
 template <typename T, int DP, bool ALIGNED, bool NT>
 int launch_paged(const fr_paged_args& a, const PagCut& c, hipStream_t st) {
+  if (a.plan) {
+    hipLaunchKernelGGL(paged_plan_kernel, dim3(1), dim3(kPlanThreads), 0, st, a, kPagRun * c.shared);
+    const int rc = check_launch("paged_plan_kernel");
+    if (rc != FR_OK) return rc;
+  }
   const int64_t items = a.slots * c.groups;
   const dim3 grid(static_cast<unsigned>(items < pag_places(DP) ? items : pag_places(DP))), block(kPagThreads);
   if (c.shared == 1) hipLaunchKernelGGL((paged_attention_kernel<T, DP, ALIGNED, 1, NT>), grid, block, 0, st, a);

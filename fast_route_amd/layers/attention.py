@@ -12,8 +12,8 @@ import torch
 from .. import _native as N
 
 _FLOATS = (torch.float16, torch.bfloat16)
-_PACKED = struct.Struct("@26qd")  # fr_attention_args
-_PAGED = struct.Struct("@30qd")  # fr_paged_args
+_PACKED = struct.Struct("@26qdq")  # fr_attention_args
+_PAGED = struct.Struct("@30qdq")  # fr_paged_args
 
 
 def _workspace(buf: torch.Tensor | None, nbytes: int, device) -> torch.Tensor | None:
@@ -74,7 +74,7 @@ def attention_varlen(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, cu_seqle
         ws_ptr, ws_bytes = ws.data_ptr(), ws.numel()
     args = _PACKED.pack(q.data_ptr(), k.data_ptr(), v.data_ptr(), cu_seqlens_q.data_ptr(), cu_k.data_ptr(), out.data_ptr(), ws_ptr, ws_bytes,
                         B, rows, keys, heads, kv_heads, dim, q_strides[0], q_strides[1], k_strides[0], k_strides[1], v_strides[0], v_strides[1],
-                        out_strides[0], out_strides[1], N.dtype_code(dtype), bool(causal), fill, 0, float(dim ** -0.5 if scale is None else scale))
+                        out_strides[0], out_strides[1], N.dtype_code(dtype), bool(causal), fill, 0, float(dim ** -0.5 if scale is None else scale), 0)
     N.run(dev, lib.fr_attention, args)
     return out
 
@@ -112,6 +112,6 @@ def paged_attention(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tenso
     args = _PAGED.pack(q.data_ptr(), k_cache.data_ptr(), v_cache.data_ptr(), block_table.data_ptr(), seq_lens.data_ptr(), out.data_ptr(),
                        ws_ptr, ws_bytes, B, heads, kv_heads, dim, pages, page_size, table[1], table_strides[0], q_strides[0], q_strides[1],
                        out_strides[0], out_strides[1], kc[0], kc[1], kc[2], vc[0], vc[1], vc[2], N.dtype_code(dtype), 0, 0, 0,
-                       float(dim ** -0.5 if scale is None else scale))
+                       float(dim ** -0.5 if scale is None else scale), 0)
     N.run(dev, lib.fr_paged_attention, args)
     return out

@@ -397,7 +397,7 @@ int fr_rotary(const fr_rotary_args* args, void* stream);
  * the first) are left as they were; with `fill` those behind it are set to zero.  heads a multiple of kv_heads; dim a multiple of 8 up to
  * 256; q, k, v, out 16-byte aligned with strides of multiples of 8 elements; keys below 2^30 and less than 2^23 elements apart; rows times heads below 2^31;
  * scale in [1e-20, 1e20].  `out` may be q itself.  `workspace`: 16-byte aligned, fr_attention_workspace_bytes bytes (0: none is needed; -1: sizes outside the
- * limits): few rows over many keys are split along the keys; two calls that may overlap in time need one each.  `parts` is the call's own. */
+ * limits): few rows over many keys are split along the keys; two calls that may overlap in time need one each.  `parts` and `plan` are the call's own. */
 typedef struct fr_attention_args {
   const void *q, *k, *v, *cu_q, *cu_k;
   void *out, *workspace;
@@ -405,6 +405,7 @@ typedef struct fr_attention_args {
   int64_t q_row, q_head, k_row, k_head, v_row, v_head, out_row, out_head;
   int64_t dtype, causal, fill, parts;
   double scale;
+  void* plan;
 } fr_attention_args;
 int64_t fr_attention_workspace_bytes(int64_t B, int64_t rows, int64_t keys, int64_t heads, int64_t kv_heads, int64_t dim);
 int fr_attention(const fr_attention_args* args, void* stream);
@@ -415,7 +416,7 @@ int fr_attention(const fr_attention_args* args, void* stream);
  * zeros.  Pages behind a length are not looked at.  heads a multiple of kv_heads; dim a multiple of 8 up to 256; q, out, k_cache, v_cache 16-byte
  * aligned with strides of multiples of 8 elements; any page_size, multiples of 16 are the fast case; table_pages * page_size <= 2^30, B times that below 2^36; scale in [1e-20, 1e20].
  * `workspace`: 16-byte aligned, fr_paged_attention_workspace_bytes(.., most = table_pages * page_size) bytes (0: none is needed; -1: sizes outside the
- * limits); two calls that may overlap in time need one each.  `slots`, `least` and `page_shift` are the call's own. */
+ * limits); two calls that may overlap in time need one each.  `slots`, `least`, `page_shift` and `plan` are the call's own. */
 typedef struct fr_paged_args {
   const void *q, *k_cache, *v_cache, *table, *lengths;
   void *out, *workspace;
@@ -423,6 +424,7 @@ typedef struct fr_paged_args {
   int64_t q_row, q_head, out_row, out_head, k_cache_page, k_cache_slot, k_cache_head, v_cache_page, v_cache_slot, v_cache_head;
   int64_t dtype, slots, least, page_shift;
   double scale;
+  void* plan;
 } fr_paged_args;
 int64_t fr_paged_attention_workspace_bytes(int64_t B, int64_t heads, int64_t kv_heads, int64_t dim, int64_t most);
 int fr_paged_attention(const fr_paged_args* args, void* stream);

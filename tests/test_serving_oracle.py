@@ -84,7 +84,7 @@ def _attention(scale=1.0, **change):
     f = dict(q=16, k=16, v=16, cu_q=16, cu_k=16, out=16, workspace=0, workspace_bytes=0, B=1, rows=4, keys=4, heads=4, kv_heads=2, dim=64, q_row=256, q_head=64, k_row=128, k_head=64,
              v_row=128, v_head=64, out_row=256, out_head=64, dtype=1, causal=1, fill=0, parts=0)
     f.update(change)
-    return struct.pack("@26qd", *f.values(), scale)
+    return struct.pack("@26qdq", *f.values(), scale, 0)
 
 
 def _paged(scale=1.0, **change):
@@ -92,7 +92,7 @@ def _paged(scale=1.0, **change):
              table_row=2, q_row=256, q_head=64, out_row=256, out_head=64, k_cache_page=2048, k_cache_slot=128, k_cache_head=64, v_cache_page=2048, v_cache_slot=128,
              v_cache_head=64, dtype=1, slots=0, least=0, page_shift=0)
     f.update(change)
-    return struct.pack("@30qd", *f.values(), scale)
+    return struct.pack("@30qdq", *f.values(), scale, 0)
 
 
 def test_refusals_come_before_any_launch():
@@ -136,7 +136,8 @@ def test_workspace_sizes():
     for B, heads, kv, dim, most in ((1, 32, 8, 128, 1024), (3, 16, 4, 64, 131072), (64, 32, 8, 128, 16384), (700, 32, 8, 128, 16384), (16, 66, 2, 256, 5000)):
         n = paged(B, heads, kv, dim, most)
         padded = 64 if dim <= 64 else 128 if dim <= 128 else 192 if dim <= 192 else 256
-        assert 0 < n < 1 << 30 and n % (16 * (padded + 2) * 4) == 0
+        plan = 0 if B <= 256 else -(-(B + 2) * 4 // 16) * 16
+        assert 0 < n < 1 << 30 and (n - plan) % (16 * (padded + 2) * 4) == 0
     whole = lib.fr_attention_workspace_bytes
     assert whole(1, 16384, 16384, 32, 8, 128) == 0 and whole(1, 37, 37, 32, 8, 128) == 0 and whole(1, 37, 37, 32, 5, 128) == -1
-    assert whole(1, 509, 8192, 16, 2, 64) == 8 * 509 * 16 * 66 * 4
+    assert whole(1, 509, 8192, 16, 2, 64) == 8 * 509 * 16 * 66 * 4 and whole(255, 4000, 4000, 8, 2, 64) == 0 and whole(256, 4000, 4000, 8, 2, 64) == 258 * 4 + 8
