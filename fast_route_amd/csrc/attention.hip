@@ -25,11 +25,13 @@ namespace {
 constexpr int kAttThreads = 256, kAttWaves = 4, kAttRows = 32, kAttTile = kAttWaves * kAttRows;
 
 __device__ __forceinline__ int64_t att_clamp(int64_t v, int64_t lo, int64_t hi) { return v < lo ? lo : (v > hi ? hi : v); }
-// Rows [*begin, *end) of sequence b of the cumulative lengths cu, inside [0, all] whatever they say; b = B: the rows behind the last one.
+// Rows [*begin, *end) of sequence b of the cumulative lengths cu, inside [0, all] whatever they say; b = B: the rows behind the last one, B + 1: in front of
+// the first.
 __device__ __forceinline__ void att_range(const int32_t* cu, int64_t b, int64_t B, int64_t all, int64_t* begin, int64_t* end) {
-  *begin = att_clamp(cu[b], 0, all);
-  *end = b == B ? all : att_clamp(cu[b + 1], *begin, all);
+  *begin = b > B ? 0 : att_clamp(cu[b], 0, all);
+  *end = b > B ? att_clamp(cu[0], 0, all) : b == B ? all : att_clamp(cu[b + 1], *begin, all);
 }
+constexpr int kAttOutside = 2;  // of those two
 
 struct AttPlace {
   int tile;                  // of the sequence, -1: none
@@ -48,7 +50,7 @@ __device__ __forceinline__ int att_tiles_of(const fr_attention_args& a, int b) {
 constexpr int kAttHeld = kHeldLengths / kWave;
 __device__ __forceinline__ AttPlace att_place(const fr_attention_args& a, int nth) {
   const int lane = threadIdx.x & 63;
-  const int count = static_cast<int>(a.B + (a.fill ? 1 : 0));
+  const int count = static_cast<int>(a.B + (a.fill ? kAttOutside : 0));
   AttPlace p = {-1, 0, 0, 0, 0};
   int seq = 0, lo = 0;
   struct Rows { int begin, n; };
@@ -131,7 +133,7 @@ __device__ __forceinline__ AttPlace att_place(const fr_attention_args& a, int nt
 }
 
 __global__ __launch_bounds__(kPlanThreads) void attention_plan_kernel(fr_attention_args a) {
-  prefix_of(static_cast<int>(a.B + (a.fill ? 1 : 0)), [&](int b) { return att_tiles_of(a, b); }, reinterpret_cast<int*>(a.plan));
+  prefix_of(static_cast<int>(a.B + (a.fill ? kAttOutside : 0)), [&](int b) { return att_tiles_of(a, b); }, reinterpret_cast<int*>(a.plan));
 }
 
 template <int DP>
@@ -479,7 +481,7 @@ __global__ __launch_bounds__(kAttThreads) void attention_join_kernel(fr_attentio
   const int64_t all = a.rows * a.heads, at = wide ? blockIdx.x : static_cast<int64_t>(blockIdx.x) * J::kGroups + threadIdx.x / J::kLanes;
   const int64_t row = (at < all ? at : all - 1) / a.heads, head = (at < all ? at : all - 1) - row * a.heads;
   const int32_t* const cu = reinterpret_cast<const int32_t*>(a.cu_q);
-  const bool live = at < all && row < (a.fill ? a.rows : att_clamp(cu[a.B], 0, a.rows)) && row >= cu[0];  // of a sequence
+  const bool live = at < all && (a.fill || (row < att_clamp(cu[a.B], 0, a.rows) && row >= cu[0]));  // of a sequence
   if (wide && !live) return;
   const AttPart<DP> from(a, 0, row, static_cast<int>(head));
   join_parts<T, DP>(wide, live, static_cast<int>(a.parts), from.rows, all * DP, from.tops, from.sums, all,
@@ -488,8 +490,8 @@ __global__ __launch_bounds__(kAttThreads) void attention_join_kernel(fr_attentio
 
 int att_dim(int64_t dim) { return dim <= 64 ? 64 : dim <= 128 ? 128 : dim <= 192 ? 192 : 256; }
 
-// Workgroups of a part: every sequence's last tile may be a part of one; the rows behind the last sequence are one more.
-int64_t att_tiles(int64_t B, int64_t rows, int64_t share, bool fill) { return ceil_div(rows * share, kAttTile) + B + (fill ? 1 : 0) - 1; }
+// Workgroups of a part: every sequence's last tile may be a part of one; the rows in front of the first sequence and behind the last one are two more.
+int64_t att_tiles(int64_t B, int64_t rows, int64_t share, bool fill) { return ceil_div(rows * share, kAttTile) + B + (fill ? kAttOutside : 0) - 1; }
 
 // Parts that the keys are split into: as many as fill the chip's 512 places for workgroups where the tiles do not, none of less than kAttPartKeys keys
 // of a sequence of average length (the lengths themselves are on the device).  509 rows over 8192 keys, 16 heads over 2 of 64: one part 117 us, eight 44.  At 768
@@ -505,7 +507,7 @@ int64_t att_parts(int64_t B, int64_t rows, int64_t keys, int64_t heads, int64_t 
 }
 
 int64_t att_part_bytes(int64_t parts, int64_t rows, int64_t heads, int64_t dim) { return parts == 1 ? 0 : round_up(parts * rows * heads * (att_dim(dim) + 2) * 4, 16); }
-int64_t att_plan_bytes(int64_t B) { return B + 1 <= kHeldLengths ? 0 : round_up((B + 2) * 4, 16); }
+int64_t att_plan_bytes(int64_t B) { return B + kAttOutside <= kHeldLengths ? 0 : round_up((B + kAttOutside + 1) * 4, 16); }
 
 template <typename T, int DP>
 int launch_attention(const fr_attention_args& a, hipStream_t st) {

@@ -10,13 +10,11 @@ template <> struct Attn<bf16_t> {
   typedef bf16x4 vec4;
   typedef bf16x8 vec8;
   static __device__ __forceinline__ f32x4 mma16(vec8 a, vec8 b, f32x4 c) { return __builtin_amdgcn_mfma_f32_16x16x32_bf16(a, b, c, 0, 0, 0); }
-  static __device__ __forceinline__ f32x16 mma32(vec8 a, vec8 b, f32x16 c) { return __builtin_amdgcn_mfma_f32_32x32x16_bf16(a, b, c, 0, 0, 0); }
 };
 template <> struct Attn<f16_t> {
   typedef f16x4 vec4;
   typedef f16x8 vec8;
   static __device__ __forceinline__ f32x4 mma16(vec8 a, vec8 b, f32x4 c) { return __builtin_amdgcn_mfma_f32_16x16x32_f16(a, b, c, 0, 0, 0); }
-  static __device__ __forceinline__ f32x16 mma32(vec8 a, vec8 b, f32x16 c) { return __builtin_amdgcn_mfma_f32_32x32x16_f16(a, b, c, 0, 0, 0); }
 };
 
 typedef short i16x4 __attribute__((ext_vector_type(4)));

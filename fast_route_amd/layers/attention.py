@@ -52,8 +52,8 @@ def attention_varlen(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, cu_seqle
     (head size ** -0.5) on the products.  causal: the last row of a sequence sees all its keys, each row before it one less - a chunk of a
     prompt brings the keys in front of it along.  Scores, softmax and sums in fp32, the softmax's terms rounded to q's type for the product with the values.
 
-    A row that sees no key is zeros.  What a row does not see does not reach it, NaN included.  Rows behind the last sequence: zeros, in an `out` given
-    left as they were (out may be q).  Head size a multiple of 8 up to 256; strides (but 1 along a head) multiples of 8 elements, 16-byte aligned.  Forward only."""
+    A row that sees no key is zeros.  What a row does not see does not reach it, NaN included.  Rows of no sequence, in front of the first or behind the last: zeros, in an
+    `out` given left as they were (out may be q).  Head size a multiple of 8 up to 256; strides (but 1 along a head) multiples of 8 elements, 16-byte aligned.  Forward only."""
     cu_k = cu_seqlens_q if cu_seqlens_k is None else cu_seqlens_k
     dev, dtype = N.device_of(q, k, v, cu_seqlens_q, cu_k), q.dtype
     ((rows, heads, dim), q_strides), (k_shape, k_strides), (v_shape, v_strides) = _rows(q, "q"), _rows(k, "k"), _rows(v, "v")

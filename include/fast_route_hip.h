@@ -393,8 +393,8 @@ int fr_rotary(const fr_rotary_args* args, void* stream);
 /* Packed prompts: sequence b's rows are cu_q[b] .. cu_q[b + 1] - 1 of q [rows, heads, dim], its keys cu_k[b] .. cu_k[b + 1] - 1 of k and v
  * [keys, kv_heads, dim] (cu_* int32 [B + 1], device, not falling; taken inside [0, rows] and [0, keys]); out[r, h] = sum_j p_j v_j, p = softmax of
  * scale * q[r, h] . k_j over the sequence's keys or, causal, those up to its row's place counted from the end: row i of n sees keys 0 .. m - n + i of m.
- * A row that sees no key is zeros.  Keys that a row does not see do not reach it, whatever they hold.  Rows behind the last sequence (and in front of
- * the first) are left as they were; with `fill` those behind it are set to zero.  heads a multiple of kv_heads; dim a multiple of 8 up to
+ * A row that sees no key is zeros.  Keys that a row does not see do not reach it, whatever they hold.  Rows of no sequence, in front of the
+ * first or behind the last, are left as they were, with `fill` set to zero.  heads a multiple of kv_heads; dim a multiple of 8 up to
  * 256; q, k, v, out 16-byte aligned with strides of multiples of 8 elements; keys below 2^30 and less than 2^23 elements apart; rows times heads below 2^31;
  * scale in [1e-20, 1e20].  `out` may be q itself.  `workspace`: 16-byte aligned, fr_attention_workspace_bytes bytes (0: none is needed; -1: sizes outside the
  * limits): few rows over many keys are split along the keys; two calls that may overlap in time need one each.  `parts` and `plan` are the call's own. */

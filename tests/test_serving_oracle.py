@@ -140,4 +140,4 @@ def test_workspace_sizes():
         assert 0 < n < 1 << 30 and (n - plan) % (16 * (padded + 2) * 4) == 0
     whole = lib.fr_attention_workspace_bytes
     assert whole(1, 16384, 16384, 32, 8, 128) == 0 and whole(1, 37, 37, 32, 8, 128) == 0 and whole(1, 37, 37, 32, 5, 128) == -1
-    assert whole(1, 509, 8192, 16, 2, 64) == 8 * 509 * 16 * 66 * 4 and whole(255, 4000, 4000, 8, 2, 64) == 0 and whole(256, 4000, 4000, 8, 2, 64) == 258 * 4 + 8
+    assert whole(1, 509, 8192, 16, 2, 64) == 8 * 509 * 16 * 66 * 4 and whole(254, 4000, 4000, 8, 2, 64) == 0 and whole(256, 4000, 4000, 8, 2, 64) == 259 * 4 + 4
