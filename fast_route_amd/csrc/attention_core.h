@@ -78,7 +78,7 @@ __device__ __forceinline__ int sum_of_all(int v) {
 
 // The lengths of up to kHeldLengths sequences stay in a wavefront's lanes; of more, a launch of one workgroup writes what lies in front of each (prefix_of) to the
 // workspace first, where place_in finds a place again.  us, with that launch / every wavefront going over all lengths: packed, 300 sequences of 8 rows 23 / 27, 1100 of
-// 64 205 / 609, 4000 of 20 306 / 2492; paged, 300 of up to 2000 keys 143 / 139, 1100 of up to 600 190 / 199, 4000 of up to 600 549 / 681.
+// 64 205 / 609, 4000 of 20 306 / 2492; paged, 300 of up to 2000 keys 143 / 138, 1100 of up to 600 190 / 199, 4000 of up to 600 549 / 681.
 constexpr int kHeldLengths = 256, kPlanThreads = 1024;
 
 // to[i] = the sum of value(0) .. value(i - 1), to[count] of all; by one workgroup of kPlanThreads.

@@ -48,19 +48,18 @@ struct PagPlan {
   __device__ __forceinline__ const int* plan() const { return reinterpret_cast<const int*>(a.plan); }
   __device__ __forceinline__ int parts(int n) const { return each ? 1 : pag_parts(pag_units(n, unit), per); }
   __device__ __forceinline__ PagPlan(const fr_paged_args& args, int keys) : a(args), lane(threadIdx.x & 63), count(static_cast<int>(args.B)), unit(keys), per(1) {
+    // (In front of the branches, which would put a wait for arguments before it: a launch's first loads are 0.3 us each.  Few sequences: one load.)
+#pragma unroll
+    for (int j = 0; j < kPagHeld; ++j) held[j] = j == 0 || j * kWave < count ? (lane + j * kWave < count ? pag_length(a, lane + j * kWave) : 0) : 0;
     each = a.slots == a.B;
     if (each) return;
     if (a.plan) {
-      per = plan()[count + 1];
+      per = __builtin_amdgcn_readfirstlane(plan()[count + 1]);
       return;
     }
     int sum = 0;
 #pragma unroll
-    for (int j = 0; j < kPagHeld; ++j) {
-      const int b = lane + j * kWave;
-      held[j] = b < count ? pag_length(a, b) : 0;
-      sum += pag_units(held[j], unit);
-    }
+    for (int j = 0; j < kPagHeld; ++j) sum += pag_units(held[j], unit);
     per = pag_per(a, sum_of_all(sum));
   }
   // Sequence, part, number of parts and length of place `slot`; false behind the last one.
@@ -75,17 +74,17 @@ struct PagPlan {
       return true;
     }
     int before = 0;
-#pragma unroll
-    for (int j = 0; j < kPagHeld; ++j) {
-      if (j * kWave >= count) break;
-      const int mine = lane + j * kWave < count ? parts(held[j]) : 0, sum = before + sum_up_to(mine);
+#pragma unroll 1  // unrolled, 64 dimensions take 138 registers: three workgroups to a CU for four, 103 us for 82 (three rows of 131071 keys)
+    for (int j = 0; j * kWave < count; ++j) {
+      const int len = j == 0 ? held[0] : j == 1 ? held[1] : j == 2 ? held[2] : held[3];
+      const int mine = lane + j * kWave < count ? parts(len) : 0, sum = before + sum_up_to(mine);
       const uint64_t hit = __ballot(slot < sum && slot >= sum - mine);
       if (hit) {
         const int l = __builtin_amdgcn_readfirstlane(__ffsll(static_cast<unsigned long long>(hit)) - 1);
         *seq = j * kWave + l;
         *of = __builtin_amdgcn_readlane(mine, l);
         *nth = slot - (__builtin_amdgcn_readlane(sum, l) - *of);
-        *n = __builtin_amdgcn_readlane(held[j], l);
+        *n = __builtin_amdgcn_readlane(len, l);
         return true;
       }
       before = __builtin_amdgcn_readlane(sum, 63);
@@ -98,7 +97,8 @@ struct PagPlan {
     const int first = __builtin_amdgcn_readfirstlane(seq);  // the lowest
     int sum = 0;
 #pragma unroll
-    for (int j = 0; j < kPagHeld; ++j) sum += lane + j * kWave < first ? parts(held[j]) : 0;
+    for (int j = 0; j < kPagHeld; ++j)
+      if (j == 0 || j * kWave < first) sum += lane + j * kWave < first ? parts(held[j]) : 0;
     sum = sum_of_all(sum);
     for (int b = first; __any(b < seq); ++b) sum += b < seq ? parts(pag_length(a, b)) : 0;
     return sum;
@@ -130,7 +130,7 @@ struct PagShape {
 // ALIGNED: pages are multiples of 16 keys, so 16 consecutive keys from a multiple of 16 on share a page.  SHARED: wavefronts that share a part's keys;
 // 4 / SHARED columns to a workgroup.
 template <typename T, int DP, bool ALIGNED, int SHARED, bool NT>
-__global__ __launch_bounds__(kPagThreads, DP <= 128 ? 2 : 1) void paged_attention_kernel(fr_paged_args a) {
+__global__ __launch_bounds__(kPagThreads, DP <= 64 ? 4 : DP <= 128 ? 2 : 1) void paged_attention_kernel(fr_paged_args a) {
   typedef typename Attn<T>::vec8 vec8;
   typedef typename Attn<T>::vec4 vec4;
   typedef PagShape<DP> S;
