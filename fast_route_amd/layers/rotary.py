@@ -95,7 +95,7 @@ def _call(q, k, positions, rotary: Rotary, inplace: bool, cached=None):
         v_ptr, kc_ptr, vc_ptr, slots_ptr = v.data_ptr(), k_cache.data_ptr(), v_cache.data_ptr(), slots.data_ptr()
         pages, page_size, cache_strides, slots_i64 = shape[0], shape[1], kc[:3] + vc[:3], int(slot_type == torch.int64)
     if inplace:
-        assert 0 not in q_strides and 0 not in k_strides, "inplace: rows that share memory"
+        assert 0 not in q_strides and 0 not in k_strides and (T == 0 or q.data_ptr() != k.data_ptr()), "inplace: rows that share memory"
         q_out, k_out, out_strides = q, k, q_strides[:2] + k_strides[:2]
     else:
         q_out, k_out = q.new_empty((T, heads, dim)), k.new_empty(k_shape)
@@ -111,8 +111,8 @@ def _call(q, k, positions, rotary: Rotary, inplace: bool, cached=None):
 
 def rotary_embed(q: torch.Tensor, k: torch.Tensor, positions: torch.Tensor, rotary: Rotary, inplace: bool = False):
     """Queries q [tokens, heads, head size] and keys k [tokens, kv heads, head size] (f16/bf16, any strides but 1 along a head, such as
-    parts of a joint projection's result) turned by their positions (int32/int64 [tokens], any value): new tensors, or with inplace q and k themselves.
-    Computed in fp32, angles in 64-bit integers, rounded once."""
+    parts of a joint projection's result) turned by their positions (int32/int64 [tokens], any value): new tensors, or with inplace q and k themselves,
+    which share no memory then.  Computed in fp32, angles in 64-bit integers, rounded once."""
     return _call(q, k, positions, rotary, inplace)
 
 

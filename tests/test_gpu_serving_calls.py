@@ -200,3 +200,17 @@ def test_no_tables_and_no_pages(native):
         out = torch.full_like(q, 5.0)
         assert paged_attention(*call, out=out) is out and (out == 0).all()
     assert paged_attention(q[:0], kc, vc, table[:0], n[:0]).shape == (0, 4, 64)
+
+
+def test_results_over_what_is_still_read(native):
+    from fast_route_amd import attention_varlen, prepare_rotary, rotary_embed, rotary_frequencies
+    _say("shared memory")
+    rotary = prepare_rotary(rotary_frequencies(64), device="cuda")
+    x, other, at = torch.zeros(9, 2, 64, device="cuda").half(), torch.zeros(9, 2, 64, device="cuda").half(), torch.arange(9, device="cuda")
+    cu = _cu([9]).cuda()
+    for call in (lambda: rotary_embed(x, x, at, rotary, inplace=True), lambda: attention_varlen(x, other, x, cu, out=x), lambda: attention_varlen(x, other, x.clone(), cu, out=other),
+                 lambda: attention_varlen(x, x, x, cu, out=x)):
+        with pytest.raises(AssertionError, match="memory"):
+            call()
+    rotary_embed(x, x, at, rotary), attention_varlen(x, x, x, cu)
+    rotary_embed(x[:0], x[:0], at[:0], rotary, inplace=True), attention_varlen(x[:0], x[:0], x[:0], cu, out=x[:0])
