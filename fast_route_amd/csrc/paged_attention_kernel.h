@@ -346,7 +346,8 @@ __global__ __launch_bounds__(kPagThreads, DP <= 64 ? 4 : DP <= 128 ? 2 : 1) void
 #pragma unroll
       for (int w = 0; w < SHARED; ++w) all = fmaxf(all, max_of[mate + w][low]);
 #pragma unroll
-      for (int w = 0; w < SHARED; ++w) total += max_of[mate + w][low] == -INFINITY ? 0.f : sum_of[mate + w][low] * exp2_of(max_of[mate + w][low] - all);
+      for (int w = 0; w < SHARED; ++w)  // (a wavefront without a key has the sum 0, one whose scores are no numbers a NaN, which stays)
+        total += sum_of[mate + w][low] * (max_of[mate + w][low] == -INFINITY ? 0.f : exp2_of(max_of[mate + w][low] - all));
       float by = top == -INFINITY ? 0.f : exp2_of(top - all);
       if (parts == 1) by = total == 0.f ? 0.f : by / total;
       float* const rows = reinterpret_cast<float*>(shared);  // [wave][head][dimension]
