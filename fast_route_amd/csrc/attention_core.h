@@ -115,12 +115,14 @@ __device__ __forceinline__ float exp2_of(float v) { return __builtin_amdgcn_exp2
 
 constexpr float kLog2e = 1.4426950408889634f;
 
-// Scores are kept in units of a factor 2.  A running maximum that lags behind the scores by up to kLag of them leaves the results as they
-// are - every term and the sum carry the same 2^lag - and the output rows need not be rescaled for each new maximum.  Terms reach 2^kLag, far
+// A term is exp2((score - maximum) * scale), scale with log2(e) in it.  A running maximum that lags behind the scores by up to kLag factors of 2 leaves the results as
+// they are - every term and the sum carry the same 2^lag - and the output rows need not be rescaled for each new maximum.  Terms reach 2^kLag, far
 // inside fp16, and keep their relative precision; the sums are fp32.
+// The difference comes first, or the maximum's product is known not to be large: score * scale - maximum * scale is off by 2^-24 of the products, which
+// makes a term of any size of scores beyond 2^25 factors of 2.
 constexpr float kLag = 8.f;
 
-// Joins the parts of a head's keys: rows of DP sums, the softmax's maxima (in units of a factor 2) and sums, each `pitch` floats from part to part.  The
+// Joins the parts of a head's keys: rows of DP sums, the softmax's maxima and sums, each `pitch` floats from part to part.  The
 // workgroup's 256 threads are groups of DP / 4, four dimensions to a thread.  Not wide: a head to a group.  wide: one head for all groups, which share its
 // parts - for few heads, where a part after the other is a round trip to memory each (one row of 32 heads, 31 parts: 21 -> 5 us).
 template <int DP>
@@ -130,7 +132,7 @@ struct JoinShape {
 };
 template <typename T, int DP>
 __device__ __forceinline__ void join_parts(bool wide, bool live, int parts, const float* rows, int64_t row_pitch, const float* tops, const float* sums,
-                                           int64_t pitch, T* out, int dim) {
+                                           int64_t pitch, float scale, T* out, int dim) {
   typedef JoinShape<DP> S;
   __shared__ float joined[S::kGroups][DP];
   __shared__ float weight_of[S::kGroups];
@@ -149,7 +151,7 @@ __device__ __forceinline__ void join_parts(bool wide, bool live, int parts, cons
   if (live) {
 #pragma unroll 8
     for (int p = wide ? group : 0; p < parts; p += wide ? S::kGroups : 1) {
-      const float t = tops[p * pitch], by = t == -INFINITY ? 0.f : exp2_of(t - top);
+      const float t = tops[p * pitch], by = t == -INFINITY ? 0.f : exp2_of((t - top) * scale);
       weight += by * sums[p * pitch];
       x += *reinterpret_cast<const f32x4*>(rows + p * row_pitch + d) * by;
     }

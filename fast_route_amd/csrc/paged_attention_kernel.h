@@ -273,7 +273,7 @@ __global__ __launch_bounds__(kPagThreads, DP <= 64 ? 4 : DP <= 128 ? 2 : 1) void
 #pragma unroll
       for (int t = 0; t < 2; ++t)
 #pragma unroll
-        for (int r = 0; r < 4; ++r) p[t][r] = st[t][r] * scale;
+        for (int r = 0; r < 4; ++r) p[t][r] = st[t][r];
       if (!all_seen) {
 #pragma unroll
         for (int t = 0; t < 2; ++t)
@@ -285,9 +285,9 @@ __global__ __launch_bounds__(kPagThreads, DP <= 64 ? 4 : DP <= 128 ? 2 : 1) void
       for (int t = 0; t < 2; ++t)
 #pragma unroll
         for (int r = 0; r < 4; ++r) high = fmaxf(high, p[t][r]);
-      if (__any(high > top + kLag)) {
+      if (__any((high - top) * scale > kLag)) {
         high = max_over_32(max_over_16(high));
-        const float now = fmaxf(top, high), by = top == -INFINITY ? 0.f : exp2_of(top - now);
+        const float now = fmaxf(top, high), by = top == -INFINITY ? 0.f : exp2_of((top - now) * scale);
         sum *= by;
 #pragma unroll
         for (int t = 0; t < S::kTiles; ++t) o[t] *= by;
@@ -299,7 +299,7 @@ __global__ __launch_bounds__(kPagThreads, DP <= 64 ? 4 : DP <= 128 ? 2 : 1) void
       for (int t = 0; t < 2; ++t)
 #pragma unroll
         for (int r = 0; r < 4; ++r) {
-          const float e = exp2_of(p[t][r] - from);
+          const float e = exp2_of((p[t][r] - from) * scale);
           sum += e;
           pt[t * 4 + r] = static_cast<T>(e);  // to 8 or 11 bits: the second product's operand
         }
@@ -347,8 +347,8 @@ __global__ __launch_bounds__(kPagThreads, DP <= 64 ? 4 : DP <= 128 ? 2 : 1) void
       for (int w = 0; w < SHARED; ++w) all = fmaxf(all, max_of[mate + w][low]);
 #pragma unroll
       for (int w = 0; w < SHARED; ++w)  // (a wavefront without a key has the sum 0, one whose scores are no numbers a NaN, which stays)
-        total += sum_of[mate + w][low] * (max_of[mate + w][low] == -INFINITY ? 0.f : exp2_of(max_of[mate + w][low] - all));
-      float by = top == -INFINITY ? 0.f : exp2_of(top - all);
+        total += sum_of[mate + w][low] * (max_of[mate + w][low] == -INFINITY ? 0.f : exp2_of((max_of[mate + w][low] - all) * scale));
+      float by = top == -INFINITY ? 0.f : exp2_of((top - all) * scale);
       if (parts == 1) by = total == 0.f ? 0.f : by / total;
       float* const rows = reinterpret_cast<float*>(shared);  // [wave][head][dimension]
 #pragma unroll
@@ -399,7 +399,7 @@ __global__ __launch_bounds__(kPagThreads) void paged_join_kernel(fr_paged_args a
   const float* const from = reinterpret_cast<const float*>(a.workspace) + slot * pitch + (kv * tiles + in / kPagHeads) * PagShape<DP>::kPart;
   const float* const tops = from + kPagHeads * DP + in % kPagHeads;
   if (wide && parts == 1) return;
-  join_parts<T, DP>(wide, at < all && parts > 1, parts, from + in % kPagHeads * DP, pitch, tops, tops + kPagHeads, pitch,
+  join_parts<T, DP>(wide, at < all && parts > 1, parts, from + in % kPagHeads * DP, pitch, tops, tops + kPagHeads, pitch, static_cast<float>(a.scale) * kLog2e,
                     reinterpret_cast<T*>(a.out) + seq * a.out_row + head * a.out_head, static_cast<int>(a.dim));
 }
 
