@@ -207,7 +207,7 @@ __device__ void attention_rows(const fr_attention_args& a, const T* kc, const T*
 #pragma unroll
     for (int d = 0; d < DP / kWave; ++d) acc[d] = 0.f;
     for (int k0 = k_first; k0 < count; k0 += kWave) {
-      const float p = k0 + lane < count ? exp2_of((score(k0 + lane) - from) * scale) : 0.f;
+      const float p = k0 + lane < count ? exp2_of(__builtin_fmaf(score(k0 + lane) - from, scale, Attn<T>::kRaise)) : 0.f;
       sum += p;
       for (int j = 0; j < kWave && k0 + j < count; ++j) {
         const float pj = __shfl(p, j, kWave);
@@ -420,7 +420,7 @@ __global__ __launch_bounds__(kAttThreads, 2) void attention_kernel(fr_attention_
     vec8 p[2][S::kGroups];  // 32 keys each, to 8 or 11 bits: the second product's operand
 #pragma unroll
     for (int i = 0; i < 2; ++i) {
-      const float from = top[i] == -INFINITY ? 0.f : top[i] * scale;
+      const float from = top[i] == -INFINITY ? 0.f : __builtin_fmaf(top[i], scale, -Attn<T>::kRaise);
 #pragma unroll
       for (int t = 0; t < 2 * S::kGroups; ++t)
 #pragma unroll

@@ -9,11 +9,13 @@ template <typename T> struct Attn;
 template <> struct Attn<bf16_t> {
   typedef bf16x4 vec4;
   typedef bf16x8 vec8;
+  static constexpr float kRaise = 0.f;
   static __device__ __forceinline__ f32x4 mma16(vec8 a, vec8 b, f32x4 c) { return __builtin_amdgcn_mfma_f32_16x16x32_bf16(a, b, c, 0, 0, 0); }
 };
 template <> struct Attn<f16_t> {
   typedef f16x4 vec4;
   typedef f16x8 vec8;
+  static constexpr float kRaise = 7.f;
   static __device__ __forceinline__ f32x4 mma16(vec8 a, vec8 b, f32x4 c) { return __builtin_amdgcn_mfma_f32_16x16x32_f16(a, b, c, 0, 0, 0); }
 };
 
@@ -115,9 +117,11 @@ __device__ __forceinline__ float exp2_of(float v) { return __builtin_amdgcn_exp2
 
 constexpr float kLog2e = 1.4426950408889634f;
 
-// A term is exp2((score - maximum) * scale), scale with log2(e) in it.  A running maximum that lags behind the scores by up to kLag factors of 2 leaves the results as
-// they are - every term and the sum carry the same 2^lag - and the output rows need not be rescaled for each new maximum.  Terms reach 2^kLag, far
-// inside fp16, and keep their relative precision; the sums are fp32.
+// A term is exp2((score - maximum) * scale + kRaise), scale with log2(e) in it.  A running maximum that lags behind the scores by up to kLag factors of 2 leaves the results
+// as they are - every term and the sum carry the same 2^(lag + kRaise) - and the output rows need not be rescaled for each new maximum.  The terms, rounded to the inputs' type, are the
+// second product's operand, and the sum is theirs, in fp32.  bf16 has fp32's range.  In fp16 terms may reach 2^15, which kRaise makes use of: with the largest term at 2^7 or above,
+// those from 2^-21 of it on keep 11 bits, and smaller ones, subnormal, are off by 2^-32 of it at most.  Without the raise that was 2^-25: of 131071 keys 25 octaves below
+// another nothing was left, 0.4 % of the result.
 // The difference comes first, or the maximum's product is known not to be large: score * scale - maximum * scale is off by 2^-24 of the products, which
 // makes a term of any size of scores beyond 2^25 factors of 2.
 constexpr float kLag = 8.f;

@@ -299,9 +299,9 @@ __global__ __launch_bounds__(kPagThreads, DP <= 64 ? 4 : DP <= 128 ? 2 : 1) void
       for (int t = 0; t < 2; ++t)
 #pragma unroll
         for (int r = 0; r < 4; ++r) {
-          const float e = exp2_of((p[t][r] - from) * scale);
-          sum += e;
-          pt[t * 4 + r] = static_cast<T>(e);  // to 8 or 11 bits: the second product's operand
+          const T e = static_cast<T>(exp2_of(__builtin_fmaf(p[t][r] - from, scale, Attn<T>::kRaise)));  // to 8 or 11 bits: the second product's operand
+          sum += static_cast<float>(e);
+          pt[t * 4 + r] = e;
         }
 #pragma unroll
       for (int t = 0; t < S::kTiles; ++t) {
