@@ -18,6 +18,7 @@
 // sequences are taken in the order of their place in the sequence, last ones first: with a causal mask these have the most keys.  Few tiles over many
 // keys are split along the keys as well and joined by a second launch.
 #include "attention_core.h"
+#include "fr_memory.h"
 
 namespace fr {
 namespace {
@@ -581,6 +582,11 @@ extern "C" int fr_attention(const fr_attention_args* args, void* stream) {
   const int64_t need = fr_attention_workspace_bytes(a.B, a.rows, a.keys, a.heads, a.kv_heads, a.dim);
   FR_REQUIRE(need == 0 || (a.workspace && aligned16(a.workspace) && a.workspace_bytes >= need), FR_E_WORKSPACE,
              "fr_attention: workspace of %lld bytes, %lld needed", (long long)a.workspace_bytes, (long long)need);
+  const Box q(a.q, a.rows, a.q_row, a.heads, a.q_head, a.dim), out(a.out, a.rows, a.out_row, a.heads, a.out_head, a.dim);
+  FR_REQUIRE(!meets_itself(out), FR_E_SHAPE, "fr_attention: out: rows that share memory");
+  FR_REQUIRE(is_same(out, q) || !meets(out, q), FR_E_SHAPE, "fr_attention: out shares memory with q, and is not q itself");
+  FR_REQUIRE(!meets(out, Box(a.k, a.keys, a.k_row, a.kv_heads, a.k_head, a.dim)) && !meets(out, Box(a.v, a.keys, a.v_row, a.kv_heads, a.v_head, a.dim)), FR_E_SHAPE,
+             "fr_attention: out shares memory with k or v");
   a.parts = att_parts(a.B, a.rows, a.keys, a.heads, a.kv_heads);
   a.plan = att_plan_bytes(a.B) ? static_cast<char*>(a.workspace) + att_part_bytes(a.parts, a.rows, a.heads, a.dim) : nullptr;
   hipStream_t st = static_cast<hipStream_t>(stream);

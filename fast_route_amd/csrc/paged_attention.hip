@@ -1,5 +1,6 @@
 // Attention of single tokens over a paged cache: sizes, checks and the entry points.  The kernels: paged_attention_kernel.h.
 #include "paged_attention_kernel.h"
+#include "fr_memory.h"
 
 namespace fr {
 namespace {
@@ -47,6 +48,12 @@ extern "C" int fr_paged_attention(const fr_paged_args* args, void* stream) {
   const int64_t need = fr_paged_attention_workspace_bytes(a.B, a.heads, a.kv_heads, a.dim, most);
   FR_REQUIRE(need == 0 || (a.workspace && aligned16(a.workspace) && a.workspace_bytes >= need), FR_E_WORKSPACE,
              "fr_paged_attention: workspace of %lld bytes, %lld needed", (long long)a.workspace_bytes, (long long)need);
+  const Box q(a.q, a.B, a.q_row, a.heads, a.q_head, a.dim), out(a.out, a.B, a.out_row, a.heads, a.out_head, a.dim);
+  FR_REQUIRE(!meets_itself(out), FR_E_SHAPE, "fr_paged_attention: out: rows that share memory");
+  FR_REQUIRE(is_same(out, q) || !meets(out, q), FR_E_SHAPE, "fr_paged_attention: out shares memory with q, and is not q itself");
+  FR_REQUIRE(!meets(out, Box(a.k_cache, a.pages, a.k_cache_page, a.page_size, a.k_cache_slot, a.kv_heads, a.k_cache_head, a.dim, 1)) &&
+                 !meets(out, Box(a.v_cache, a.pages, a.v_cache_page, a.page_size, a.v_cache_slot, a.kv_heads, a.v_cache_head, a.dim, 1)),
+             FR_E_SHAPE, "fr_paged_attention: out shares memory with the cache");
   if (pag_plan_bytes(a.B, a.slots)) a.plan = static_cast<char*>(a.workspace) + pag_part_bytes(a.B, a.slots, a.heads, a.kv_heads, a.dim);
   a.page_shift = (a.page_size & (a.page_size - 1)) == 0 ? __builtin_ctzll(a.page_size) : -1;
   hipStream_t st = static_cast<hipStream_t>(stream);

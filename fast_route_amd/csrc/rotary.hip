@@ -8,7 +8,7 @@
 //
 // Bound by memory: everything is read once and written once (keys twice with a cache): 8192 tokens of 32 and 8 heads of 128 dimensions into a cache 39.6 us, 5.5 TB/s.  The
 // angles of a token are computed once, by one thread each, and shared by its heads through LDS.  Rows that 16-byte accesses cannot read go element by element.
-#include "fr_common.h"
+#include "fr_memory.h"
 
 namespace fr {
 namespace {
@@ -139,6 +139,25 @@ bool rot_wide(const void* p, int64_t s0, int64_t s1, int64_t s2 = 0) {
   return aligned16(p) && s0 % 8 == 0 && s1 % 8 == 0 && s2 % 8 == 0;
 }
 
+// Results that lie where another workgroup, or another thread, still reads or writes: all but queries and keys turned in place.
+int check_rotary_memory(const fr_rotary_args& a) {
+  const Box in[3] = {Box(a.q, a.T, a.q_token, a.heads, a.q_head, a.dim), Box(a.k, a.T, a.k_token, a.kv_heads, a.k_head, a.dim),
+                     Box(a.v, a.slots ? a.T : 0, a.v_token, a.kv_heads, a.v_head, a.dim)};
+  const int64_t pages = a.slots ? a.pages : 0;
+  const Box out[4] = {Box(a.q_out, a.T, a.q_out_token, a.heads, a.q_out_head, a.dim), Box(a.k_out, a.T, a.k_out_token, a.kv_heads, a.k_out_head, a.dim),
+                      Box(a.k_cache, pages, a.k_cache_page, a.page_size, a.k_cache_slot, a.kv_heads, a.k_cache_head, a.dim, 1),
+                      Box(a.v_cache, pages, a.v_cache_page, a.page_size, a.v_cache_slot, a.kv_heads, a.v_cache_head, a.dim, 1)};
+  static const char* const in_name[3] = {"q", "k", "v"};
+  static const char* const out_name[4] = {"turned q", "turned k", "k_cache", "v_cache"};
+  for (int i = 0; i < 4; ++i) {
+    FR_REQUIRE(!meets_itself(out[i]), FR_E_SHAPE, "fr_rotary: %s: places that share memory", out_name[i]);
+    for (int j = 0; j < 3; ++j)
+      FR_REQUIRE((i == j && is_same(out[i], in[j])) || !meets(out[i], in[j]), FR_E_SHAPE, "fr_rotary: %s and %s share memory", out_name[i], in_name[j]);
+    for (int j = 0; j < i; ++j) FR_REQUIRE(!meets(out[i], out[j]), FR_E_SHAPE, "fr_rotary: %s and %s share memory", out_name[i], out_name[j]);
+  }
+  return FR_OK;
+}
+
 }  // namespace
 }  // namespace fr
 
@@ -163,6 +182,8 @@ extern "C" int fr_rotary(const fr_rotary_args* args, void* stream) {
   if (a.slots)
     wide = wide && rot_wide(a.v, a.v_token, a.v_head) && rot_wide(a.k_cache, a.k_cache_page, a.k_cache_slot, a.k_cache_head) &&
            rot_wide(a.v_cache, a.v_cache_page, a.v_cache_slot, a.v_cache_head);
+  const int rc = check_rotary_memory(a);
+  if (rc != FR_OK) return rc;
   hipStream_t st = static_cast<hipStream_t>(stream);
   return a.dtype == FR_BF16 ? launch_rotary<bf16_t>(a, wide, st) : launch_rotary<f16_t>(a, wide, st);
 }

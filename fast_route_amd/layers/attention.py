@@ -39,7 +39,6 @@ def _output(out: torch.Tensor | None, q: torch.Tensor):
     assert out.shape == q.shape and out.dtype == q.dtype and out.device == q.device, "out must be like q"
     strides = out.stride()
     assert strides[2] == 1, "out must be contiguous along a head"
-    assert 0 not in strides, "out: rows that share memory"
     return out, strides
 
 
@@ -53,7 +52,7 @@ def attention_varlen(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, cu_seqle
     prompt brings the keys in front of it along.  Scores, softmax and sums in fp32, the softmax's terms rounded to q's type for the product with the values.
 
     A row that sees no key is zeros.  What a row does not see does not reach it, NaN included.  Rows of no sequence, in front of the first or behind the last: zeros, in an
-    `out` given left as they were (out may be q, but shares no memory with k and v).  Head size a multiple of 8 up to 256; strides (but 1 along a head) multiples of 8 elements, 16-byte aligned.  Forward only."""
+    `out` given left as they were (out may be q, of the same strides, and lies beside q, k and v otherwise).  Head size a multiple of 8 up to 256; strides (but 1 along a head) multiples of 8 elements, 16-byte aligned.  Forward only."""
     cu_k = cu_seqlens_q if cu_seqlens_k is None else cu_seqlens_k
     dev, dtype = N.device_of(q, k, v, cu_seqlens_q, cu_k), q.dtype
     ((rows, heads, dim), q_strides), (k_shape, k_strides), (v_shape, v_strides) = _rows(q, "q"), _rows(k, "k"), _rows(v, "v")
@@ -66,7 +65,6 @@ def attention_varlen(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, cu_seqle
     assert B >= 0 and cu_k.shape[0] == B + 1, "cu_seqlens_q and cu_seqlens_k differ in length, or are empty"
     fill = out is None
     out, out_strides = _output(out, q)
-    assert fill or rows == 0 or out.data_ptr() not in (k.data_ptr(), v.data_ptr()), "out must share no memory with k and v"
     need = lib.fr_attention_workspace_bytes(B, rows, keys, heads, kv_heads, dim)
     assert need >= 0, lib.fr_last_error_string().decode()
     ws_ptr = ws_bytes = 0
@@ -87,7 +85,7 @@ def paged_attention(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tenso
     (int32 [B, pages of a sequence at most]).  f16/bf16; heads a multiple of kv heads, consecutive ones share a key head; `scale`
     (head size ** -0.5) on the products.  Scores, softmax and sums in fp32, the softmax's terms rounded to q's type for the product with the values.
 
-    A row without keys is zeros; a length behind the table's end is the table's end; keys in a page outside the cache take no part; what lies
+    `out` may be q, of the same strides, and lies beside q and the cache otherwise.  A row without keys is zeros; a length behind the table's end is the table's end; keys in a page outside the cache take no part; what lies
     behind a length, NaN included, is not read.  Head size a multiple of 8 up to 256; strides (but 1 along a head) multiples of 8 elements, 16-byte aligned;
     page sizes of multiples of 16 are the fast case."""
     dev, dtype = N.device_of(q, k_cache, v_cache, block_table, seq_lens), q.dtype

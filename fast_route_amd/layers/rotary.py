@@ -68,7 +68,6 @@ def _cache(cache: torch.Tensor, dtype: torch.dtype, heads: int, dim: int, what: 
     assert len(shape) == 4 and cache.dtype == dtype, "%s must be [pages, page size, heads, head size] in the keys' type" % what
     assert shape[2] == heads and shape[3] == dim, "%s: other heads than the keys" % what
     assert strides[3] == 1 or dim == 1, "%s must be contiguous along a head" % what
-    assert 0 not in strides, "%s: places that share memory" % what
     return shape, strides
 
 
@@ -95,7 +94,6 @@ def _call(q, k, positions, rotary: Rotary, inplace: bool, cached=None):
         v_ptr, kc_ptr, vc_ptr, slots_ptr = v.data_ptr(), k_cache.data_ptr(), v_cache.data_ptr(), slots.data_ptr()
         pages, page_size, cache_strides, slots_i64 = shape[0], shape[1], kc[:3] + vc[:3], int(slot_type == torch.int64)
     if inplace:
-        assert 0 not in q_strides and 0 not in k_strides and (T == 0 or q.data_ptr() != k.data_ptr()), "inplace: rows that share memory"
         q_out, k_out, out_strides = q, k, q_strides[:2] + k_strides[:2]
     else:
         q_out, k_out = q.new_empty((T, heads, dim)), k.new_empty(k_shape)
@@ -112,7 +110,7 @@ def _call(q, k, positions, rotary: Rotary, inplace: bool, cached=None):
 def rotary_embed(q: torch.Tensor, k: torch.Tensor, positions: torch.Tensor, rotary: Rotary, inplace: bool = False):
     """Queries q [tokens, heads, head size] and keys k [tokens, kv heads, head size] (f16/bf16, any strides but 1 along a head, such as
     parts of a joint projection's result) turned by their positions (int32/int64 [tokens], any value): new tensors, or with inplace q and k themselves,
-    which share no memory then.  Computed in fp32, angles in 64-bit integers, rounded once."""
+    which share no memory then (parts of the same rows do not).  Computed in fp32, angles in 64-bit integers, rounded once."""
     return _call(q, k, positions, rotary, inplace)
 
 
@@ -121,5 +119,6 @@ def rotary_to_cache(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, positions
     """rotary_embed, and in the same pass the turned keys and the values v [tokens, kv heads, head size] into a paged cache k_cache, v_cache
     [pages, page size, kv heads, head size] (any strides but 1 along a head): token t's into place slots[t] % page size of page
     slots[t] // page size.  A token whose slot (int32/int64) is negative or behind the last page is not kept.  Slots are of one token each: one that two
-    tokens name ends up with pieces of either.  The cache holds what paged_attention reads."""
+    tokens name ends up with pieces of either.  The cache holds what paged_attention reads; k_cache and v_cache share no memory with each other nor with q, k
+    and v; inplace, q and k share none with each other nor with v."""
     return _call(q, k, positions, rotary, inplace, (v, k_cache, v_cache, slots))

@@ -373,7 +373,8 @@ int fr_fused_moe_mxfp4(const void* x, int dtype, const void* w1_tiled, const voi
  *
  * Rotary positions.  Pair i of a head's first `turned` dimensions is turned by position * freq[i] radians and scaled by
  * `factor`: pairs (i, i + turned / 2) or, interleaved, (2 i, 2 i + 1); the other dimensions stay.  turns[i] = freq[i] / (2 pi) * 2^64,
- * rounded, modulo 2^64 (uint64, device).  q [T, heads, dim] and k [T, kv_heads, dim] to q_out and k_out, which may be q and k themselves.
+ * rounded, modulo 2^64 (uint64, device).  q [T, heads, dim] and k [T, kv_heads, dim] to q_out and k_out, which may be q and k themselves, of the same strides.  What is written
+ * shares no other element with what is read or written (FR_E_SHAPE), and no two of its places are one; parts of the same rows are fine.
  * With slots (not NULL), k_out's row and v's of token t also go to slot slots[t] of the cache: page slots[t] / page_size, place
  * slots[t] % page_size; a slot outside [0, pages * page_size) keeps nothing.  A slot that two tokens name holds pieces of either.
  * positions, slots: int64 where *_i64 is 1, else int32; any position.  turned even, <= 512; dim <= 1024.  Rows of 16-byte aligned
@@ -396,7 +397,7 @@ int fr_rotary(const fr_rotary_args* args, void* stream);
  * A row that sees no key is zeros.  Keys that a row does not see do not reach it, whatever they hold.  Rows of no sequence, in front of the
  * first or behind the last, are left as they were, with `fill` set to zero.  heads a multiple of kv_heads; dim a multiple of 8 up to
  * 256; q, k, v, out 16-byte aligned with strides of multiples of 8 elements; keys below 2^30 and less than 2^23 elements apart; rows times heads below 2^31;
- * scale in [1e-20, 1e20].  `out` may be q itself.  `workspace`: 16-byte aligned, fr_attention_workspace_bytes bytes (0: none is needed; -1: sizes outside the
+ * scale in [1e-20, 1e20].  `out` may be q itself, of the same strides, and shares no element with q, k or v otherwise.  `workspace`: 16-byte aligned, fr_attention_workspace_bytes bytes (0: none is needed; -1: sizes outside the
  * limits): few rows over many keys are split along the keys; two calls that may overlap in time need one each.  `parts` and `plan` are the call's own. */
 typedef struct fr_attention_args {
   const void *q, *k, *v, *cu_q, *cu_k;
@@ -415,6 +416,7 @@ int fr_attention(const fr_attention_args* args, void* stream);
  * A length is taken as 0 below it and as the table's end behind it; keys in a page outside [0, pages) take no part; a row without keys is
  * zeros.  Pages behind a length are not looked at.  heads a multiple of kv_heads; dim a multiple of 8 up to 256; q, out, k_cache, v_cache 16-byte
  * aligned with strides of multiples of 8 elements; any page_size, multiples of 16 are the fast case; table_pages * page_size <= 2^30, B times that below 2^36; scale in [1e-20, 1e20].
+ * `out` may be q itself, of the same strides, and shares no element with q or the cache otherwise.
  * `workspace`: 16-byte aligned, fr_paged_attention_workspace_bytes(.., most = table_pages * page_size) bytes (0: none is needed; -1: sizes outside the
  * limits); two calls that may overlap in time need one each.  `slots`, `least`, `page_shift` and `plan` are the call's own. */
 typedef struct fr_paged_args {
