@@ -2,9 +2,9 @@
 //
 // Pair i of the first `turned` dimensions of a head, at position p, is turned by the angle p * freq[i]:
 //   (a, b) -> (a cos - b sin, b cos + a sin) * factor,  pairs (i, i + turned / 2) or, interleaved, (2 i, 2 i + 1); the rest of a head stays.
-// A frequency comes as turns per position in units of 2^-64 turn: position * frequency in wrapping 64-bit integers is the angle's part
-// within a turn to position * 2^-64 turn, at any position, where a 32-bit product of position and radians is off by half a radian at
-// 10^7.  The part, signed, is rounded to 32 bits (1.9e-7 radian at most) and goes to sincospi.
+// A frequency comes as turns per position in units of 2^-64 turn, rounded: position * frequency in wrapping 64-bit integers is the angle's part
+// within a turn, off by |position| * 2^-65 turn at most (2^-25, what the next rounding takes, at 2^40), where a 32-bit product of position and radians is off by
+// half a radian at 10^7.  The part, signed, is rounded to 32 bits (1.9e-7 radian at most) and goes to sincospi.
 //
 // Bound by memory: everything is read once and written once (keys twice with a cache): 8192 tokens of 32 and 8 heads of 128 dimensions into a cache 39.6 us, 5.5 TB/s.  The
 // angles of a token are computed once, by one thread each, and shared by its heads through LDS.  Rows that 16-byte accesses cannot read go element by element.

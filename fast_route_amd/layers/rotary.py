@@ -42,6 +42,28 @@ def rotary_frequencies(turned: int, base: float = 10000.0, scale: float = 1.0, o
     return freq * keep + freq / scale * (1.0 - keep)
 
 
+def _pi(bits: int) -> int:
+    """pi * 2^bits, to a few units: 16 arctan(1/5) - 4 arctan(1/239) (Machin 1706) in whole numbers."""
+    def arctan(x):
+        term, total, n = (1 << bits + 16) // x, 0, 1
+        while term:
+            total += term // n if n % 4 == 1 else -(term // n)
+            term, n = term // (x * x), n + 2
+        return total
+    return (16 * arctan(5) - 4 * arctan(239)) >> 16
+
+
+_PI_BITS = 192
+_PI = _pi(_PI_BITS)
+
+
+def _turn(frequency: float) -> int:
+    """frequency / (2 pi) * 2^64, rounded: in whole numbers, since 64 bits are more than a product of floats has."""
+    over, under = frequency.as_integer_ratio()
+    over, under = over << 64 + _PI_BITS, 2 * _PI * under
+    return (2 * over + under) // (2 * under)
+
+
 def prepare_rotary(frequencies: torch.Tensor, interleaved: bool = False, factor: float = 1.0, device=None) -> Rotary:
     """The handle that rotary_embed and rotary_to_cache take, made once: frequencies in radians per position (fp64 or fp32, one per
     pair, of less than half a turn each, for instance from rotary_frequencies), pairs (2 i, 2 i + 1) if interleaved, else (i, i + n), a factor on what is turned.
@@ -51,8 +73,7 @@ def prepare_rotary(frequencies: torch.Tensor, interleaved: bool = False, factor:
     values = frequencies.detach().double().cpu()
     assert bool((values.abs() < math.pi).all()), "a frequency is below half a turn (pi) per position"
     device = frequencies.device if device is None else torch.device(device)
-    # 2^64 / (2 pi), below 2^63 in magnitude: rounded to 53 bits, like the frequencies
-    turns = torch.round(values * (2.0 ** 63 / math.pi)).clamp(-2.0 ** 63 + 1024, 2.0 ** 63 - 1024).to(torch.int64)
+    turns = torch.tensor([_turn(f) for f in values.tolist()], dtype=torch.int64)  # below half a turn, 2^63, in magnitude
     return Rotary(turns.to(device), bool(interleaved), float(factor))
 
 
@@ -110,7 +131,8 @@ def _call(q, k, positions, rotary: Rotary, inplace: bool, cached=None):
 def rotary_embed(q: torch.Tensor, k: torch.Tensor, positions: torch.Tensor, rotary: Rotary, inplace: bool = False):
     """Queries q [tokens, heads, head size] and keys k [tokens, kv heads, head size] (f16/bf16, any strides but 1 along a head, such as
     parts of a joint projection's result) turned by their positions (int32/int64 [tokens], any value): new tensors, or with inplace q and k themselves,
-    which share no memory then (parts of the same rows do not).  Computed in fp32, angles in 64-bit integers, rounded once."""
+    which share no memory then (parts of the same rows do not).  Computed in fp32, rounded once; angles in 64-bit integers, off by |position| * 2^-65 turn at
+    most and by 2^-25 turn."""
     return _call(q, k, positions, rotary, inplace)
 
 
