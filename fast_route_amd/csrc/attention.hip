@@ -551,7 +551,10 @@ int check_attention_sizes(int64_t B, int64_t rows, int64_t keys, int64_t heads, 
   FR_REQUIRE(rows >= 0 && rows < (int64_t(1) << 30) && keys >= 0 && keys < (int64_t(1) << 30), FR_E_SHAPE, "fr_attention: %lld rows, %lld keys: below 2^30",
              (long long)rows, (long long)keys);
   FR_REQUIRE(B >= 0 && B <= (1 << 20) && (rows + B + kAttTile) * heads < (int64_t(1) << 31), FR_E_SHAPE,
-             "fr_attention: %lld sequences, %lld rows of %lld heads: rows times heads below 2^31", (long long)B, (long long)rows, (long long)heads);
+             "fr_attention: %lld sequences, %lld rows of %lld heads: up to 2^20 sequences, (rows + sequences + 128) times heads below 2^31", (long long)B, (long long)rows, (long long)heads);
+  FR_REQUIRE(att_tiles(B, rows, heads / kv_heads, true) * kv_heads <= kMostBlocks256, FR_E_SHAPE,
+             "fr_attention: %lld sequences, %lld rows of %lld heads over %lld: rows times heads / 128 and sequences times key heads, together, up to 2^24", (long long)B, (long long)rows,
+             (long long)heads, (long long)kv_heads);
   return FR_OK;
 }
 

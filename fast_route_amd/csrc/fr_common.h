@@ -97,6 +97,8 @@ int down_impl(const void* act, const float* act_scale, const void* w2, const flo
     if (!(cond)) return ::fr::fail((code), __VA_ARGS__); \
   } while (0)
 
+// A launch has fewer than 2^32 threads (one of more ran as many as the rest modulo 2^32, without an error): of workgroups of 256.
+constexpr int64_t kMostBlocks256 = (int64_t(1) << 24) - 1;
 static inline bool aligned16(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 15u) == 0; }
 static inline int64_t ceil_div(int64_t a, int64_t b) { return (a + b - 1) / b; }
 static inline int64_t round_up(int64_t a, int64_t b) { return ceil_div(a, b) * b; }

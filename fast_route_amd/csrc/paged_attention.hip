@@ -10,8 +10,9 @@ int check_paged_sizes(int64_t B, int64_t heads, int64_t kv_heads, int64_t dim, i
              (long long)heads, (long long)kv_heads);
   FR_REQUIRE(dim >= 8 && dim <= 256 && dim % 8 == 0, FR_E_SHAPE, "fr_paged_attention: head size %lld: a multiple of 8 up to 256", (long long)dim);
   FR_REQUIRE(most >= 0 && most <= (int64_t(1) << 30), FR_E_SHAPE, "fr_paged_attention: a table of %lld keys: up to 2^30", (long long)most);
-  FR_REQUIRE(B >= 0 && B <= (1 << 20) && B * heads <= (1 << 26) && B * ceil_div(most, kPagRun) < (int64_t(1) << 31), FR_E_SHAPE,
-             "fr_paged_attention: %lld rows of %lld heads, %lld keys each: rows times heads up to 2^26, rows times keys below 2^36", (long long)B, (long long)heads, (long long)most);
+  // (256 dimensions: four heads to a workgroup of the joining launch, kMostBlocks256 of them)
+  FR_REQUIRE(B >= 0 && B <= (1 << 20) && B * heads <= 4 * kMostBlocks256 && B * ceil_div(most, kPagRun) < (int64_t(1) << 31), FR_E_SHAPE,
+             "fr_paged_attention: %lld rows of %lld heads, %lld keys each: up to 2^20 rows, rows times heads below 2^26 - 3, rows times keys below 2^36", (long long)B, (long long)heads, (long long)most);
   return FR_OK;
 }
 

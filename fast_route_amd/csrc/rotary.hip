@@ -119,6 +119,17 @@ __global__ __launch_bounds__(kRotThreads) void rotary_kernel(fr_rotary_args a, i
   }
 }
 
+// The call on its tokens from the t-th on.
+fr_rotary_args tokens_from(fr_rotary_args a, int64_t t) {
+  auto on = [](const void* p, int64_t bytes) { return p ? static_cast<const char*>(p) + bytes : nullptr; };
+  auto on_out = [](void* p, int64_t bytes) { return p ? static_cast<char*>(p) + bytes : nullptr; };
+  a.q = on(a.q, t * a.q_token * 2), a.k = on(a.k, t * a.k_token * 2), a.v = on(a.v, t * a.v_token * 2);
+  a.q_out = on_out(a.q_out, t * a.q_out_token * 2), a.k_out = on_out(a.k_out, t * a.k_out_token * 2);
+  a.positions = on(a.positions, t * (a.positions_i64 ? 8 : 4)), a.slots = on(a.slots, t * (a.slots_i64 ? 8 : 4));
+  a.T -= t;
+  return a;
+}
+
 template <typename T>
 int launch_rotary(const fr_rotary_args& a, bool wide, hipStream_t st) {
   // As many tokens as give every thread an item, where there are tokens enough for every CU: 8192 tokens of 12 and 4 heads of 64 dimensions 14.5 us one by one,
@@ -126,12 +137,20 @@ int launch_rotary(const fr_rotary_args& a, bool wide, hipStream_t st) {
   const int64_t vec = wide ? 8 : 1, items = ((a.heads + a.kv_heads) * (a.dim - a.turned / 2) + (a.slots ? a.kv_heads * a.dim : 0)) / vec;
   const int64_t fill = items < kRotThreads ? kRotThreads / (items > 0 ? items : 1) : 1;
   const int tokens = a.T < 2048 ? 1 : static_cast<int>(fill < kRotTokens ? fill : kRotTokens);
-  const dim3 grid(static_cast<unsigned>(ceil_div(a.T, tokens))), block(kRotThreads);
-  if (wide && a.interleaved) hipLaunchKernelGGL((rotary_kernel<T, 8, true>), grid, block, 0, st, a, tokens);
-  else if (wide) hipLaunchKernelGGL((rotary_kernel<T, 8, false>), grid, block, 0, st, a, tokens);
-  else if (a.interleaved) hipLaunchKernelGGL((rotary_kernel<T, 1, true>), grid, block, 0, st, a, tokens);
-  else hipLaunchKernelGGL((rotary_kernel<T, 1, false>), grid, block, 0, st, a, tokens);
-  return check_launch("rotary_kernel");
+  // More tokens than the workgroups of a launch take: one launch after the other.
+  const int64_t most = kMostBlocks256 * tokens;
+  for (int64_t t = 0; t < a.T; t += most) {
+    const fr_rotary_args b = t == 0 ? a : tokens_from(a, t);
+    const int64_t count = b.T < most ? b.T : most;
+    const dim3 grid(static_cast<unsigned>(ceil_div(count, tokens))), block(kRotThreads);
+    if (wide && a.interleaved) hipLaunchKernelGGL((rotary_kernel<T, 8, true>), grid, block, 0, st, b, tokens);
+    else if (wide) hipLaunchKernelGGL((rotary_kernel<T, 8, false>), grid, block, 0, st, b, tokens);
+    else if (a.interleaved) hipLaunchKernelGGL((rotary_kernel<T, 1, true>), grid, block, 0, st, b, tokens);
+    else hipLaunchKernelGGL((rotary_kernel<T, 1, false>), grid, block, 0, st, b, tokens);
+    const int rc = check_launch("rotary_kernel");
+    if (rc != FR_OK) return rc;
+  }
+  return FR_OK;
 }
 
 // Rows of heads that 16-byte accesses can read: address and strides.

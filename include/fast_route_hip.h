@@ -377,7 +377,7 @@ int fr_fused_moe_mxfp4(const void* x, int dtype, const void* w1_tiled, const voi
  * shares no other element with what is read or written (FR_E_SHAPE), and no two of its places are one; parts of the same rows are fine.
  * With slots (not NULL), k_out's row and v's of token t also go to slot slots[t] of the cache: page slots[t] / page_size, place
  * slots[t] % page_size; a slot outside [0, pages * page_size) keeps nothing.  A slot that two tokens name holds pieces of either.
- * positions, slots: int64 where *_i64 is 1, else int32; any position.  turned even, <= 512; dim <= 1024.  Rows of 16-byte aligned
+ * positions, slots: int64 where *_i64 is 1, else int32; any position.  T < 2^31; heads <= 4096; turned even, <= 512; dim <= 1024.  Rows of 16-byte aligned
  * addresses and strides, turned % 16 == 0 and dim % 8 == 0 are the fast case. */
 typedef struct fr_rotary_args {
   const void *q, *k, *v;
@@ -396,7 +396,8 @@ int fr_rotary(const fr_rotary_args* args, void* stream);
  * scale * q[r, h] . k_j over the sequence's keys or, causal, those up to its row's place counted from the end: row i of n sees keys 0 .. m - n + i of m.
  * A row that sees no key is zeros.  Keys that a row does not see do not reach it, whatever they hold.  Rows of no sequence, in front of the
  * first or behind the last, are left as they were, with `fill` set to zero.  heads a multiple of kv_heads; dim a multiple of 8 up to
- * 256; q, k, v, out 16-byte aligned with strides of multiples of 8 elements; keys below 2^30 and less than 2^23 elements apart; rows times heads below 2^31;
+ * 256; q, k, v, out 16-byte aligned with strides of multiples of 8 elements; keys below 2^30 and less than 2^23 elements apart; B up to 2^20; heads up to 65536;
+ * (rows + B + 128) * heads below 2^31 and (ceil(rows * heads / kv_heads / 128) + B + 1) * kv_heads below 2^24, the workgroups of a launch;
  * scale in [1e-20, 1e20].  `out` may be q itself, of the same strides, and shares no element with q, k or v otherwise.  `workspace`: 16-byte aligned, fr_attention_workspace_bytes bytes (0: none is needed; -1: sizes outside the
  * limits): few rows over many keys are split along the keys; two calls that may overlap in time need one each.  `parts` and `plan` are the call's own. */
 typedef struct fr_attention_args {
@@ -415,7 +416,7 @@ int fr_attention(const fr_attention_args* args, void* stream);
  * sequence b in place j % page_size of page table[b, j / page_size].  lengths int32 [B], table int32 [B, table_pages] (row stride table_row).
  * A length is taken as 0 below it and as the table's end behind it; keys in a page outside [0, pages) take no part; a row without keys is
  * zeros.  Pages behind a length are not looked at.  heads a multiple of kv_heads; dim a multiple of 8 up to 256; q, out, k_cache, v_cache 16-byte
- * aligned with strides of multiples of 8 elements; any page_size, multiples of 16 are the fast case; table_pages * page_size <= 2^30, B times that below 2^36; scale in [1e-20, 1e20].
+ * aligned with strides of multiples of 8 elements; any page_size, multiples of 16 are the fast case; table_pages * page_size <= 2^30, B times that below 2^36; B up to 2^20; heads up to 65536, B * heads up to 2^26 - 4; scale in [1e-20, 1e20].
  * `out` may be q itself, of the same strides, and shares no element with q or the cache otherwise.
  * `workspace`: 16-byte aligned, fr_paged_attention_workspace_bytes(.., most = table_pages * page_size) bytes (0: none is needed; -1: sizes outside the
  * limits); two calls that may overlap in time need one each.  `slots`, `least`, `page_shift` and `plan` are the call's own. */

@@ -1,0 +1,54 @@
+"""Sizes that are taken can be launched; others are refused with the sizes' error, before anything is launched."""
+import pytest
+import torch
+
+
+def test_sizes_of_a_launch():
+    """A launch has fewer than 2^32 threads, 256 to a workgroup."""
+    from fast_route_amd import _native
+    lib = _native.lib()
+    whole, paged = lib.fr_attention_workspace_bytes, lib.fr_paged_attention_workspace_bytes
+    # sequences times key heads and rows times heads / 128: B + 1 tiles of a key head for B sequences that may be empty, and what the rows fill
+    for B, rows, heads, kv, good in ((1 << 20, 0, 16, 16, False), (1 << 20, 0, 15, 15, True), ((1 << 20) + 1, 0, 1, 1, False), (1, (1 << 26) - 65536, 32, 32, True),
+                                     (1, (1 << 26) - 300, 32, 32, False), (1, (1 << 26) - 1500, 32, 1, True), (1, 1 << 26, 32, 1, False), (65535, (1 << 25), 32, 32, True),
+                                     (1 << 18, (1 << 25), 32, 32, False)):
+        blocks = (-(-rows * (heads // kv) // 128) + B + 1) * kv
+        if good:
+            assert blocks < 1 << 24 and whole(B, rows, 100, heads, kv, 64) >= 0, (B, rows, heads, kv)
+        else:
+            assert whole(B, rows, 100, heads, kv, 64) == -1 and b"2^" in lib.fr_last_error_string(), (B, rows, heads, kv)
+    # four heads of 256 dimensions to a workgroup of the joining launch
+    assert paged(1 << 20, 63, 1, 256, 600) > 0 and paged(1 << 20, 64, 1, 256, 600) == -1 and paged(16777215, 4, 1, 256, 64) == -1
+    assert paged((1 << 20) - 1, 64, 1, 256, 600) > 0 and -(-((1 << 20) - 1) * 64 // 4) < 1 << 24
+
+
+@pytest.mark.gpu
+def test_more_tokens_than_a_launch_takes(native):
+    """2^26 + 7 tokens, four to a workgroup, two dimensions: against the definition by groups of positions."""
+    from fast_route_amd import prepare_rotary, rotary_to_cache
+    print("[case] 2^26 tokens", flush=True)
+    T, page = (1 << 26) + 7, 64
+    assert (T + 3) // 4 > (1 << 24) - 1
+    g = torch.Generator("cuda").manual_seed(1)
+    q, k, v = (torch.empty(T, 1, 2, dtype=torch.half, device="cuda").normal_(generator=g) for _ in range(3))
+    at = torch.arange(T, dtype=torch.int32, device="cuda") % 1000
+    slots = (torch.arange(T, dtype=torch.int32, device="cuda") + 5) % T
+    kc, vc = (torch.zeros(T // page + 1, page, 1, 2, dtype=torch.half, device="cuda") for _ in range(2))
+    q2, k2 = rotary_to_cache(q, k, v, at, prepare_rotary(torch.tensor([0.37], dtype=torch.float64), device="cuda"), kc, vc, slots)
+    for lo in (0, (1 << 25) - 99, T - (1 << 20)):  # the middle, and on either side of the second launch
+        part = slice(lo, lo + (1 << 20))
+        angle = at[part].double() * 0.37
+        cos, sin = angle.cos(), angle.sin()
+        for x, y in ((q, q2), (k, k2)):
+            a, b = x[part, 0, 0].double(), x[part, 0, 1].double()
+            for got, want in ((y[part, 0, 0], a * cos - b * sin), (y[part, 0, 1], b * cos + a * sin)):
+                # the result's rounding, and the angle's, sine's and cosine's and three operations' together: 2^-20 of the pair's size
+                tol = 2.0 ** -11 * want.abs() * (1 + 2.0 ** -10) + 2.0 ** -20 * (a.abs() + b.abs()) + 2.0 ** -24
+                assert ((got.double() - want).abs() <= tol).all()
+        assert torch.equal(kc.view(-1, 1, 2)[slots[part].long()], k2[part]) and torch.equal(vc.view(-1, 1, 2)[slots[part].long()], v[part])
+    # every token, by what a turn leaves: a pair's length
+    for x, y in ((q, q2), (k, k2)):
+        for part in torch.arange(0, T, 1 << 24).tolist():
+            a, b = (t[part:part + (1 << 24), 0].float().norm(dim=1) for t in (x, y))
+            assert ((a - b).abs() <= 2.0 ** -9 * a + 2.0 ** -20).all(), part
+    assert torch.equal(vc.view(-1, 1, 2)[5:T], v[:T - 5]) and torch.equal(kc.view(-1, 1, 2)[5:T], k2[:T - 5])
