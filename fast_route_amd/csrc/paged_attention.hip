@@ -30,7 +30,7 @@ extern "C" int fr_paged_attention(const fr_paged_args* args, void* stream) {
   using namespace fr;
   FR_REQUIRE(args, FR_E_NULL, "fr_paged_attention: null pointer");
   fr_paged_args a = *args;
-  FR_REQUIRE(a.page_size >= 1 && a.page_size <= (1 << 20) && a.table_pages >= 0 && a.table_pages <= (1 << 30) && a.pages >= 0, FR_E_SHAPE,
+  FR_REQUIRE(a.page_size >= 1 && a.page_size <= (1 << 30) && a.table_pages >= 0 && a.table_pages <= (1 << 30) && a.pages >= 0, FR_E_SHAPE,
              "fr_paged_attention: tables of %lld pages of %lld keys", (long long)a.table_pages, (long long)a.page_size);
   const int64_t most = a.table_pages * a.page_size;
   const int rc = check_paged_sizes(a.B, a.heads, a.kv_heads, a.dim, most);

@@ -52,3 +52,35 @@ def test_more_tokens_than_a_launch_takes(native):
             a, b = (t[part:part + (1 << 24), 0].float().norm(dim=1) for t in (x, y))
             assert ((a - b).abs() <= 2.0 ** -9 * a + 2.0 ** -20).all(), part
     assert torch.equal(vc.view(-1, 1, 2)[5:T], v[:T - 5]) and torch.equal(kc.view(-1, 1, 2)[5:T], k2[:T - 5])
+
+
+def test_pages_of_any_size():
+    """A page of more than 2^20 keys is one: what stops this call is the address behind it."""
+    import struct
+    from fast_route_amd import _native
+    lib = _native.lib()
+
+    def call(page_size, table_pages):
+        return lib.fr_paged_attention(struct.pack("@30qdq", 16, 24, 16, 16, 16, 16, 0, 0, 2, 4, 2, 64, 4, page_size, table_pages, 2, 256, 64, 256, 64, 2048, 128, 64, 2048, 128, 64, 1,
+                                                  0, 0, 0, 1.0, 0), None)
+    assert call(16, 2) == -4
+    for page_size, table_pages in ((1 << 20, 3), ((1 << 20) + 1, 3), (1 << 21, 1), (1 << 30, 1)):
+        assert call(page_size, table_pages) == -4, lib.fr_last_error_string()
+    assert call(1 << 30, 2) == -2 and call((1 << 30) + 1, 1) == -2 and call(0, 1) == -2
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("page", [1 << 21, (1 << 21) - 5])
+def test_one_large_page(native, page):
+    import oracle
+    from fast_route_amd import paged_attention
+    print("[case] page of", page, flush=True)
+    g = torch.Generator().manual_seed(page)
+    kc, vc = (torch.randn(2, page, 1, 8, generator=g).bfloat16() for _ in range(2))
+    q, lengths = torch.randn(3, 2, 8, generator=g).bfloat16(), [2 * page - 70, 5, page + 33]
+    got = paged_attention(q.cuda(), kc.cuda(), vc.cuda(), torch.tensor([[1, 0]] * 3, dtype=torch.int32).cuda(), torch.tensor(lengths, dtype=torch.int32).cuda()).cpu()
+    k, v = (torch.cat([c[1], c[0]]) for c in (kc, vc))
+    for b, n in enumerate(lengths):
+        ref, error = oracle.attention(q[b:b + 1], k[:n], v[:n], torch.ones(1, n, dtype=torch.bool), 8 ** -0.5)
+        tol = error + 2.0 ** -8 * (ref.abs() + error)
+        assert ((got[b:b + 1].double() - ref).abs() <= tol).all()
