@@ -105,6 +105,17 @@ struct PagPlan {
   }
 };
 
+// Results of a part of the keys, by place and column: for the heads that a column has, rows of DP sums and behind them the softmax's maxima and sums (next to the rows: in
+// arrays of their own 8 rows of up to 8192 keys, 256 dimensions, took 36.2 us for 35.3), whole 16 bytes together.
+__host__ __device__ __forceinline__ int pag_column_heads(int share) { return share < kPagHeads ? share : kPagHeads; }
+__host__ __device__ __forceinline__ int pag_column_floats(int share, int padded) { return pag_column_heads(share) * padded + (2 * pag_column_heads(share) + 3) / 4 * 4; }
+template <int DP>
+struct PagPart {
+  float *rows, *tops, *sums;
+  __device__ __forceinline__ PagPart(const fr_paged_args& a, int64_t at, int share)  // at: place * columns + column
+      : rows(reinterpret_cast<float*>(a.workspace) + at * pag_column_floats(share, DP)), tops(rows + pag_column_heads(share) * DP), sums(tops + pag_column_heads(share)) {}
+};
+
 // Loads of a cache that the memory-side cache does not hold go past the caches (pag_past).
 template <bool NT, typename V>
 __device__ __forceinline__ V pag_load(const V* p) {
@@ -119,7 +130,6 @@ struct PagShape {
   static constexpr int kSteps = DP / 32, kTiles = DP / 16;
   // Rows of V lie in LDS with their pieces exchanged in pairs, so that a transposed read's four rows, 16 elements each, meet in no bank.
   static constexpr int kMask = DP % 128 == 0 ? 7 : 3;
-  static constexpr int kPart = kPagHeads * (DP + 2);      // floats of a part's column: rows of 16 heads, maxima, sums
   // K through LDS too: a load instruction then takes whole rows, where the product's operand takes 64 bytes of 16 (64 rows of up to 16384 keys: 476 us
   // against 460, past the caches 500 against 415; with 64 dimensions, a row being 128 bytes, 82 against 92, registers for three workgroups in place of four).
   static constexpr bool kKeysToo = DP == 128;
@@ -312,11 +322,11 @@ __global__ __launch_bounds__(kPagThreads, DP <= 64 ? 4 : DP <= 128 ? 2 : 1) void
     }
     sum = sum_over_32(sum_over_16(sum));
 
-    float* const to_part = reinterpret_cast<float*>(a.workspace) + (static_cast<int64_t>(slot) * columns + column) * S::kPart;
+    const PagPart<DP> to_part(a, static_cast<int64_t>(slot) * columns + column, share);
     T* const to_out = reinterpret_cast<T*>(a.out) + seq * a.out_row + (kv * share + head0) * a.out_head;
     auto put = [&](int h, int d, const f32x4& x) {  // four dimensions of a head of the column
       if (parts > 1) {
-        *reinterpret_cast<f32x4*>(to_part + h * DP + d) = x;
+        *reinterpret_cast<f32x4*>(to_part.rows + h * DP + d) = x;
       } else if (d < dim) {
         vec4 y;
 #pragma unroll
@@ -325,9 +335,9 @@ __global__ __launch_bounds__(kPagThreads, DP <= 64 ? 4 : DP <= 128 ? 2 : 1) void
       }
     };
     auto put_sums = [&](float all, float total) {
-      if (parts > 1 && quarter == 0) {
-        to_part[kPagHeads * DP + low] = all;
-        to_part[kPagHeads * (DP + 1) + low] = total;
+      if (parts > 1 && quarter == 0 && low < heads) {
+        to_part.tops[low] = all;
+        to_part.sums[low] = total;
       }
     };
     if constexpr (SHARED == 1) {
@@ -393,13 +403,12 @@ __global__ __launch_bounds__(kPagThreads) void paged_join_kernel(fr_paged_args a
   const int seq = static_cast<int>((at < all ? at : all - 1) / a.heads), head = static_cast<int>((at < all ? at : all - 1) - seq * a.heads);
   const PagPlan plan(a, unit);
   const int parts = plan.parts(pag_length(a, seq));
-  const int kv = head / share, in = head - kv * share;
-  const int64_t pitch = static_cast<int64_t>(a.kv_heads) * tiles * PagShape<DP>::kPart;
-  const int slot = plan.in_front(seq);
-  const float* const from = reinterpret_cast<const float*>(a.workspace) + slot * pitch + (kv * tiles + in / kPagHeads) * PagShape<DP>::kPart;
-  const float* const tops = from + kPagHeads * DP + in % kPagHeads;
+  const int kv = head / share, in = head - kv * share, columns = static_cast<int>(a.kv_heads) * tiles;
+  const int64_t pitch = static_cast<int64_t>(columns) * pag_column_floats(share, DP);
+  const PagPart<DP> from(a, static_cast<int64_t>(plan.in_front(seq)) * columns + kv * tiles + in / kPagHeads, share);
+  const int at_head = in % kPagHeads;
   if (wide && parts == 1) return;
-  join_parts<T, DP>(wide, at < all && parts > 1, parts, from + in % kPagHeads * DP, pitch, tops, tops + kPagHeads, pitch, static_cast<float>(a.scale) * kLog2e,
+  join_parts<T, DP>(wide, at < all && parts > 1, parts, from.rows + at_head * DP, pitch, from.tops + at_head, from.sums + at_head, pitch, static_cast<float>(a.scale) * kLog2e,
                     reinterpret_cast<T*>(a.out) + seq * a.out_row + head * a.out_head, static_cast<int>(a.dim));
 }
 
@@ -439,7 +448,7 @@ PagCut pag_cut(int64_t B, int64_t heads, int64_t kv_heads, int64_t dim, int64_t 
 }
 
 int64_t pag_part_bytes(int64_t B, int64_t slots, int64_t heads, int64_t kv_heads, int64_t dim) {
-  return slots == B ? 0 : slots * pag_columns(heads, kv_heads) * kPagHeads * (pag_dim(dim) + 2) * 4;
+  return slots == B ? 0 : slots * pag_columns(heads, kv_heads) * pag_column_floats(static_cast<int>(heads / kv_heads), static_cast<int>(pag_dim(dim))) * 4;
 }
 int64_t pag_plan_bytes(int64_t B, int64_t slots) { return slots == B || B <= kHeldLengths ? 0 : round_up((B + 2) * 4, 16); }
 

@@ -84,3 +84,44 @@ def test_one_large_page(native, page):
         ref, error = oracle.attention(q[b:b + 1], k[:n], v[:n], torch.ones(1, n, dtype=torch.bool), 8 ** -0.5)
         tol = error + 2.0 ** -8 * (ref.abs() + error)
         assert ((got[b:b + 1].double() - ref).abs() <= tol).all()
+
+
+def test_workspace_holds_the_heads_that_there_are():
+    """A place of a key head of up to 16 query heads: a row for each of them, and two numbers, whole 16 bytes together."""
+    from fast_route_amd import _native
+    need = _native.lib().fr_paged_attention_workspace_bytes
+    for B, heads, kv, dim, most in ((256, 32, 32, 128, 2048), (2048, 32, 32, 128, 2048), (64, 32, 8, 128, 16384), (3, 12, 4, 64, 131072), (5, 7, 7, 80, 3000)):
+        share, padded = heads // kv, 64 if dim <= 64 else 128
+        plan = 0 if B <= 256 else -(-(B + 2) * 4 // 16) * 16
+        of_place = lambda share: kv * (share * padded + -(-2 * share // 4) * 4) * 4
+        places, rest = divmod(need(B, heads, kv, dim, most) - plan, of_place(share))
+        assert rest == 0 and places > B and need(B, heads * 16 // share, kv, dim, most) - plan == places * of_place(16), (B, heads, kv)
+    assert need(256, 32, 32, 128, 2048) < 16 << 20
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("H,G,D", [(7, 7, 64), (12, 4, 64), (5, 1, 80), (34, 2, 64), (3, 1, 128), (32, 32, 128), (40, 2, 192)])
+def test_workspace_of_any_share(native, H, G, D):
+    """Exactly as many bytes as are asked for, with what lies on either side of them."""
+    import oracle
+    from fast_route_amd import paged_attention
+    print("[case] workspace", H, G, D, flush=True)
+    g = torch.Generator().manual_seed(H + D)
+    lengths, page = [900, 33, 1500], 16
+    pages = [-(-n // page) for n in lengths]
+    table = torch.zeros(3, max(pages), dtype=torch.int32)
+    order = torch.randperm(sum(pages), generator=g).to(torch.int32).split(pages)
+    for b, o in enumerate(order):
+        table[b, :len(o)] = o
+    kc, vc = (torch.randn(sum(pages), page, G, D, generator=g).half() for _ in range(2))
+    q, need = torch.randn(3, H, D, generator=g).half(), native.fr_paged_attention_workspace_bytes(3, H, G, D, table.shape[1] * page)
+    assert need > 0
+    held = torch.full((256 + need + 4096,), 0xA5, dtype=torch.uint8, device="cuda")
+    got = paged_attention(q.cuda(), kc.cuda(), vc.cuda(), table.cuda(), torch.tensor(lengths, dtype=torch.int32).cuda(), workspace_buf=held[256:256 + need]).cpu()
+    assert (held[:256] == 0xA5).all() and (held[256 + need:] == 0xA5).all()
+    for b, n in enumerate(lengths):
+        at = torch.arange(n)
+        where = table[b].long()[at // page]
+        ref, error = oracle.attention(q[b:b + 1], kc[where, at % page], vc[where, at % page], torch.ones(1, n, dtype=torch.bool), D ** -0.5)
+        tol = error + 2.0 ** -11 * (ref.abs() + error) + 2.0 ** -24
+        assert ((got[b:b + 1].double() - ref).abs() <= tol).all(), b
