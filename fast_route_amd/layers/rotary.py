@@ -53,15 +53,15 @@ def _pi(bits: int) -> int:
     return (16 * arctan(5) - 4 * arctan(239)) >> 16
 
 
-_PI_BITS = 192
-_PI = _pi(_PI_BITS)
+_TURN_BITS = 160
+_TURN = (1 << _TURN_BITS + 199) // _pi(200)  # 2^_TURN_BITS / (2 pi)
 
 
 def _turn(frequency: float) -> int:
     """frequency / (2 pi) * 2^64, rounded: in whole numbers, since 64 bits are more than a product of floats has."""
-    over, under = frequency.as_integer_ratio()
-    over, under = over << 64 + _PI_BITS, 2 * _PI * under
-    return (2 * over + under) // (2 * under)
+    digits, exponent = math.frexp(frequency)
+    behind = _TURN_BITS + 53 - 64 - exponent  # binary places of the product below 2^-64 turn
+    return (int(digits * 2.0 ** 53) * _TURN + (1 << behind - 1)) >> behind
 
 
 def prepare_rotary(frequencies: torch.Tensor, interleaved: bool = False, factor: float = 1.0, device=None) -> Rotary:
