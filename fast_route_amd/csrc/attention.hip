@@ -8,8 +8,9 @@
 //   O^T [dim, rows] += V^T P^T: the accumulators, rounded, are the second operand as they are, if the keys of V^T are taken in the same
 //   order; transposed reads of LDS give four keys of a dimension at a time.
 // 16x16x32 and not 32x32x16 (a register of accumulators read per 32 flops more): the part runs under its power limit, and the clock is 1.92 in place of 1.72 GHz; 8192
-// rows without a mask 993 us against 1033.  A prompt of 16384 rows, 32 heads over 8 of 128 dimensions: 2.0 ms, 1.09 PFLOP/s (a matrix product 8192^3 reaches 1.47); 64
-// dimensions 0.92, 192 1.05, 256 1.03.  Bound by the matrix instructions (48 % of the cycles) and the vector instructions between them (an exponential, a multiply-add, half
+// rows without a mask 993 us against 1033.  A prompt of 16384 rows, 32 heads over 8 of 128 dimensions: 2.0 ms, 1.08 to 1.12 PFLOP/s (a matrix product 8192^3 reaches 1.47); 64
+// dimensions 0.98, 192 1.14, 256 1.04; 80 and 96, which are computed as 128, 0.74 and 0.88.
+// Bound by the matrix instructions (48 % of the cycles) and the vector instructions between them (an exponential, a multiply-add, half
 // a maximum and half a conversion per score: 770 cycles beside 1090 in a wavefront's block of 128 dimensions, and a block takes 1880): a SIMD hardly runs the two at once.
 // Tried and taken back: the next block's scores computed beside this one's exponentials in one wavefront (3 % slower, and no faster with the order fixed by hand);
 // eight wavefronts whose halves take turns, products beside exponentials, with a barrier between the turns (10 % slower, 64 dimensions 27 %).
@@ -502,7 +503,8 @@ int64_t att_tiles(int64_t B, int64_t rows, int64_t share, bool fill) { return ce
 
 // Parts that the keys are split into: as many as fill the chip's 512 places for workgroups where the tiles do not, none of less than kAttPartKeys keys
 // of a sequence of average length (the lengths themselves are on the device).  509 rows over 8192 keys, 16 heads over 2 of 64: one part 117 us, eight 44.  At 768
-// places 512 rows over 8704 keys take 109 us for 88; parts of 512 keys and more: a row over 8000 keys 22.5 us for 17.3.
+// places 512 rows over 8704 keys take 109 us for 88; parts of 512 keys and more: a row over 8000 keys 22.5 us for 17.3.  All of these are of equal sequences: the average says
+// little where one has most of the keys (512 rows over 66048 keys, 32 heads over 8: 620 us; beside seven prompts of 100 rows, which take 13 alone, 1960).
 constexpr int64_t kAttPlaces = 512, kAttPartKeys = 256, kAttMostParts = 32;
 int64_t att_parts(int64_t B, int64_t rows, int64_t keys, int64_t heads, int64_t kv_heads) {
   if (B < 1 || rows < 1) return 1;

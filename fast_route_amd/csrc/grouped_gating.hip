@@ -408,7 +408,9 @@ __global__ __launch_bounds__(kGroupWaves * kWave) void gating_grouped_rows_kerne
 
 // Whether the calls' sizes and addresses suit gating_grouped_rows_kernel, with VPL logits to a lane.  us, a wavefront per token / this: 16384 tokens, 256 experts in 8 groups,
 // sigmoid and bias 32.1 / 15.4, 7 tokens 6.8 / 6.2; 16384 of 64 experts, softmax and bias 17.8 / 10.7, of 512 60.6 / 30.6, of 256 without bias 18.6 / 10.7; but 7 of 64
-// experts in 8 groups 4.2 / 4.6.
+// experts in 8 groups 4.2 / 4.6.  Other sizes, a wavefront per token, us for 7, 1031 and 16384 tokens: 8 or 16 experts 2.9, 3.2, 8.7; 60 in 4 groups 4.1, 4.6, 14.4; 160 in 8 groups 6.3,
+// 7.2, 27.7; the best 32 of 256 13.1, 15.2, 62.7 (sigmoid and bias).  Without a bias and groups topk_softmax does the softmax's job too: 16384 tokens of 8 experts 2.6 us for 7.8 here, of
+// 64 4.3 / 5.4, of 256 7.1 / 7.9, but 64 tokens of 128 5.2 / 3.9 and of 256 6.4 / 4.6 (bf16).
 template <typename T, int VPL>
 bool rows_fit(const void* logits, int64_t M, int E, int64_t ld, const float* bias, int groups, int kept, int topk, int sigmoid, int renorm) {
   constexpr int piece = VPL * sizeof(T) < 16 ? VPL : 16 / sizeof(T);

@@ -1,5 +1,5 @@
-// Attention of one query row per sequence over its pages: every key and value is read once, 4 flops per byte and query head that
-// shares it, so the cache's way from memory bounds it.
+// Attention of one query row per sequence over its pages: every key and value is read once, a flop per byte and query head that
+// shares it (4 D of each for a key, its value and a head), so the cache's way from memory bounds it.
 //
 // A wavefront takes the query heads of one key head (up to 16, the columns of a matrix instruction: a "column") and a part of one sequence's keys,
 // in runs of 32 with a running maximum and sum:
@@ -452,9 +452,11 @@ int64_t pag_part_bytes(int64_t B, int64_t slots, int64_t heads, int64_t kv_heads
 }
 int64_t pag_plan_bytes(int64_t B, int64_t slots) { return slots == B || B <= kHeldLengths ? 0 : round_up((B + 2) * 4, 16); }
 
-// Whether keys and values are read past the caches: where the pages are more than the memory-side cache's 256 MB, so that nothing of them is left there from the last
-// step.  us, past them / not: 64 rows of up to 16384 keys (2.6 GB) 421 / 462, three of 131071 (0.4 GB) 82 / 88, 32 rows (0.45 GB) 85 / 95; but pages of 139 MB read
-// again and again 43 / 40 and 34 / 32.
+// Whether keys and values are read past the caches: where the pages are more than the memory-side cache's 256 MB, so that what a call reads is most likely no longer there
+// from the last step, however little it is.  us, past them / not: 64 rows of up to 16384 keys (2.6 GB) 421 / 462, three of 131071 (0.4 GB) 82 / 88, 32 rows (0.45 GB) 85 / 95.
+// Small reads of a pool of 2.6 GB, other pages each time (16 sets in turn): 134 MB 36.7 / 39.0 and 36.2 / 39.9, 34 MB 19.9 / 20.8 and 17.9 / 18.8, 268 MB 58.2 / 63.4; the same
+// pages again and again, which a layer among others does not do: 134 MB 34.8 / 32.7 and 34.3 / 32.0, 34 MB 17.0 / 16.9 and 16.4 / 15.5, 268 MB 56.5 / 53.4.  Pages of 139 MB in
+// all, again and again: 35.4 / 32.5.
 bool pag_past(const fr_paged_args& a) { return a.pages * a.page_size * a.kv_heads * a.dim * 2 * 2 > (int64_t(256) << 20); }
 
 template <typename T, int DP, bool ALIGNED, bool NT>
