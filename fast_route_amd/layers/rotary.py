@@ -94,6 +94,7 @@ def _cache(cache: torch.Tensor, dtype: torch.dtype, heads: int, dim: int, what: 
 
 def _call(q, k, positions, rotary: Rotary, inplace: bool, cached=None):
     turns, interleaved, factor = rotary
+    assert turns.dtype == torch.int64 and turns.dim() == 1 and turns.is_contiguous(), "rotary: turns must be as prepare_rotary lays them out, contiguous int64"
     ((T, heads, dim), q_strides), (k_shape, k_strides), dtype = _heads(q, "q"), _heads(k, "k"), q.dtype
     kv_heads, turned, at_type = k_shape[1], 2 * turns.shape[0], positions.dtype
     assert dtype in _FLOATS, "q must be float16 or bfloat16"

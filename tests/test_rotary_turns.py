@@ -24,6 +24,17 @@ def test_turns_are_exact():
             assert abs(Fraction(f) * 2 ** 63 / PI - t) <= Fraction(1, 2) + Fraction(1, 1000), (name, f, t)
 
 
+def test_handle_of_another_kind():
+    """The kernel reads 64-bit whole numbers, one after the other: a handle that was cast or sliced is refused, before the tensors' device is asked for."""
+    from fast_route_amd import Rotary, prepare_rotary, rotary_embed, rotary_frequencies
+    x, at, whole = torch.zeros(4, 2, 64, dtype=torch.half), torch.arange(4), prepare_rotary(rotary_frequencies(64))
+    for turns in (whole.turns.int(), whole.turns.double(), whole.turns.float(), whole.turns[::2], whole.turns[None], whole.turns[0], torch.zeros(1, dtype=torch.int64).expand(32)):
+        with pytest.raises(AssertionError, match="turns"):
+            rotary_embed(x, x, at, Rotary(turns, False, 1.0))
+    with pytest.raises(AssertionError, match="MI355X"):
+        rotary_embed(x, x, at, whole)
+
+
 @pytest.mark.gpu
 @pytest.mark.parametrize("interleaved", [False, True])
 def test_far_positions(native, interleaved):
