@@ -35,3 +35,37 @@ def test_any_scale(native, scale, dtype):
             kc, vc = (torch.cat([t, t[:pages * 16 - m]]).view(pages, 16, G, D) for t in (k, v))
             got = paged_attention(q, kc, vc, torch.arange(pages, dtype=torch.int32)[None].cuda(), cu[1][1:], scale=scale)
             assert ((got.cpu().double() - want).abs() <= tol).all(), ("paged", m, H, G, D)
+
+
+@pytest.mark.parametrize("dtype", [torch.float16, torch.bfloat16])
+def test_parts_of_different_kinds(native, dtype):
+    """Keys split along their length, where some parts are done row by row - a value that is not finite among keys that the tile's first rows do not see, or scores far from
+    zero in some of the parts only - and the others are not: they are joined as if all were of one kind."""
+    import oracle
+    from fast_route_amd import attention_varlen
+    _say(f"parts {dtype}")
+    n, m, H, G, D = 20, 3000, 4, 2, 64
+    g = torch.Generator().manual_seed(2)
+    q, (k, v) = torch.randn(n, H, D, generator=g).to(dtype), (torch.randn(m, G, D, generator=g).to(dtype) for _ in range(2))
+    cu = [torch.tensor([0, c], dtype=torch.int32).cuda() for c in (n, m)]
+    assert native.fr_attention_workspace_bytes(1, n, m, H, G, D) > 0
+    seen = torch.arange(m)[None, :] <= torch.arange(n)[:, None] + (m - n)
+    ref, error = oracle.attention(q, k, v, seen, 0.125)
+    tol = error + torch.finfo(dtype).eps / 2 * (ref.abs() + error) + 2.0 ** -24
+    bad = v.clone()
+    bad[-1] = float("inf")  # the last row alone sees it
+    got = attention_varlen(q.cuda(), k.cuda(), bad.cuda(), *cu).cpu()
+    assert ((got[:-1].double() - ref[:-1]).abs() <= tol[:-1]).all() and not got[-1].isfinite().any()
+    # whole numbers: scores are exact.  The first keys' scores are up to 4096 times the others', at a scale that makes these alone too large for one product.
+    q = torch.randint(1, 5, (n, H, D), generator=g)
+    k, v = torch.randint(-4, 5, (m, G, D), generator=g), torch.randint(-4, 5, (m, G, D), generator=g)
+    for sign in (1, -1):
+        far = k.clone()
+        far[:300] = sign * 512 * torch.randint(4, 9, (300, G, D), generator=g)
+        want = torch.zeros(n, H, D, dtype=torch.float64)
+        for h in range(H):
+            s = (q[:, h] @ far[:, h // 2].t()).masked_fill(~seen, -1 << 40)
+            p = (s == s.amax(dim=1, keepdim=True)).double()
+            want[:, h] = p @ v[:, h // 2].double() / p.sum(dim=1, keepdim=True)
+        got = attention_varlen(*(t.to(dtype).cuda() for t in (q, far, v)), *cu, scale=64.0).cpu()
+        assert ((got.double() - want).abs() <= 4 * 2.0 ** -18 + torch.finfo(dtype).eps / 2 * want.abs()).all(), sign
